@@ -60,6 +60,8 @@ EXPORTED = (
     "aspire_linear_splits",
     "aspire_linear_partials",
     "aspire_add_rms_norm_partials",
+    "aspire_rotary",
+    "aspire_rotary_append",
     "aspire_bandwidth_probe",
 )
 
@@ -184,6 +186,27 @@ class RopeArgs(ctypes.Structure):
     ]
 
 
+class RotaryArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", ctypes.c_void_p), ("q_stride_t", ctypes.c_int64), ("q_stride_h", ctypes.c_int64),
+        ("q_out", ctypes.c_void_p), ("q_out_stride_t", ctypes.c_int64), ("q_out_stride_h", ctypes.c_int64),
+        ("k", ctypes.c_void_p), ("k_stride_t", ctypes.c_int64), ("k_stride_h", ctypes.c_int64),
+        ("k_out", ctypes.c_void_p), ("k_out_stride_t", ctypes.c_int64), ("k_out_stride_h", ctypes.c_int64),
+        ("v", ctypes.c_void_p), ("v_stride_t", ctypes.c_int64), ("v_stride_h", ctypes.c_int64),
+        ("num_qo_heads", ctypes.c_int32), ("num_kv_heads", ctypes.c_int32), ("total_tokens", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32), ("rotary_dim", ctypes.c_int32), ("interleaved", ctypes.c_int32),
+        ("dtype", ctypes.c_int32), ("inverse", ctypes.c_int32),
+        ("turns", ctypes.c_void_p), ("amplitude", ctypes.c_float), ("positions_64", ctypes.c_int32),
+        ("positions", ctypes.c_void_p),
+        ("kv_cache", ctypes.c_void_p), ("cache_stride_p", ctypes.c_int64), ("cache_stride_kv", ctypes.c_int64),
+        ("cache_stride_t", ctypes.c_int64), ("cache_stride_h", ctypes.c_int64),
+        ("num_pages", ctypes.c_int64), ("num_page_indices", ctypes.c_int64),
+        ("page_size", ctypes.c_int32), ("num_seq", ctypes.c_int32),
+        ("append_indptr", ctypes.c_void_p), ("kv_page_indices", ctypes.c_void_p),
+        ("kv_page_indptr", ctypes.c_void_p), ("kv_last_page_len", ctypes.c_void_p),
+    ]
+
+
 _lib = None
 
 
@@ -233,6 +256,8 @@ def _declare(lib):
         "aspire_linear_splits": [i32, i32, i32],
         "aspire_linear_partials": [vp, i64, vp, i64, vp, i64, i32, i32, i32, vp],
         "aspire_add_rms_norm_partials": [vp, i64, vp, i32, vp, vp, i64, i32, i32, f32, vp],
+        "aspire_rotary": [ctypes.POINTER(RotaryArgs), vp],
+        "aspire_rotary_append": [ctypes.POINTER(RotaryArgs), vp],
         "aspire_bandwidth_probe": [i32, vp, i64, vp, i64, i32, i32, vp],
     }
     for name, argtypes in sigs.items():

@@ -422,6 +422,49 @@ int aspire_rope_frequencies(int32_t head_dim, float rope_theta, float rope_scale
                             float low_freq_factor, float high_freq_factor, float old_context_len,
                             float* out);
 
+/* ------------------------------------------------ rotary positions, with or without the append
+ * Pair i of a token's head turns by position * f_i: y_a = A (a cos - b sin), y_b = A (b cos + a sin), of
+ * dims (i, i + rotary_dim / 2), or (2i, 2i + 1) with interleaved; dims from rotary_dim on are copied (in place:
+ * left). inverse turns back (times A): the transpose, i.e. the gradient. Tokens at negative positions are
+ * copied. f_i comes as turns[i] = f_i / (2 pi) * 2^64 modulo 2^64 (device memory), so angles are exact at any
+ * position. Any strides of tokens and heads (elements), head dims contiguous; out equal to in, or apart from it.
+ *
+ * aspire_rotary: q and k to q_out and k_out at positions (32- or 64-bit).
+ * aspire_rotary_append (bf16, fp16): q to q_out, the turned k and v to the page pool, where aspire_paged_kv_append
+ * puts them; a token's position is its place in its row's sequence unless positions is given. q of tokens of no
+ * row is copied; tokens whose page lies outside the lists or the pool are not written. */
+#define ASPIRE_ROTARY_BF16 0
+#define ASPIRE_ROTARY_FP16 1
+#define ASPIRE_ROTARY_FP32 2
+typedef struct aspire_rotary_args {
+  const void* q;                /* [T, Hq, head_dim] */
+  int64_t q_stride_t, q_stride_h;
+  void* q_out;
+  int64_t q_out_stride_t, q_out_stride_h;
+  const void* k;                /* [T, Hkv, head_dim] */
+  int64_t k_stride_t, k_stride_h;
+  void* k_out;                  /* not used by the append */
+  int64_t k_out_stride_t, k_out_stride_h;
+  const void* v;                /* append only */
+  int64_t v_stride_t, v_stride_h;
+  int32_t num_qo_heads, num_kv_heads, total_tokens, head_dim, rotary_dim, interleaved, dtype, inverse;
+  const uint64_t* turns;        /* [rotary_dim / 2] */
+  float amplitude;
+  int32_t positions_64;
+  const void* positions;        /* [T]; NULL (append): the places in the sequences */
+  void* kv_cache;               /* append only, from here */
+  int64_t cache_stride_p, cache_stride_kv, cache_stride_t, cache_stride_h;
+  int64_t num_pages, num_page_indices;
+  int32_t page_size, num_seq;
+  const int32_t* append_indptr;     /* [num_seq + 1] */
+  const int32_t* kv_page_indices;   /* [num_page_indices] */
+  const int32_t* kv_page_indptr;    /* [num_seq + 1] */
+  const int32_t* kv_last_page_len;  /* [num_seq] */
+} aspire_rotary_args;
+
+int aspire_rotary(const aspire_rotary_args* args, void* stream);
+int aspire_rotary_append(const aspire_rotary_args* args, void* stream);
+
 /* ------------------------------------------------ decode-step row operations
  * The per-token steps a decode step runs between the GEMMs, used by the full
  * decode step. One workgroup per row, no scratch memory.

@@ -1,0 +1,97 @@
+"""Rotary configurations and the host-side checks of the rotary entry points (no GPU)."""
+
+import ctypes
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from aspire_amd import _lib
+from aspire_amd.attention.rope import RopeConfig, rope_frequencies
+from aspire_amd.attention.rotary import RotaryConfig, RotaryEmbedding
+
+
+def test_frequencies_equal_the_fused_kernels_where_both_exist():
+    """Plain, divided and llama3 frequencies against aspire_rope_frequencies, whose fp32 values are the 64-bit ones rounded."""
+    for mine, theirs in ((RotaryConfig(theta=1e6), RopeConfig(1e6)),
+                         (RotaryConfig(theta=1e4, scaling="linear", factor=2.0), RopeConfig(1e4, 2.0)),
+                         (RotaryConfig(theta=5e5, scaling="llama3", factor=8.0, original_max_position=8192),
+                          RopeConfig(5e5, 8.0, 1.0, 4.0, 8192))):
+        f, g = np.array(mine.frequencies()), rope_frequencies(128, theirs).double().numpy()
+        assert np.all(np.abs(f - g) <= 2.0 ** -23 * g)
+
+
+def test_yarn_regions():
+    """Pairs that turn more than beta_fast times over the trained context keep their frequency, those below beta_slow
+    are divided, the ones between lie between and never rise back."""
+    c = RotaryConfig(theta=1e6, scaling="yarn", factor=4.0, original_max_position=32768)
+    base = np.array(RotaryConfig(theta=1e6).frequencies())
+    f, turns = np.array(c.frequencies()), 32768 * base / (2 * math.pi)
+    keep = (f / base - 0.25) / 0.75
+    assert np.allclose(keep[turns > 32 * 1.3], 1) and np.allclose(keep[turns < 1 / 1.3], 0, atol=1e-12)
+    assert np.all(np.diff(keep) <= 1e-12) and ((keep > 0.01) & (keep < 0.99)).any()
+    assert c.scale == 0.1 * math.log(4.0) + 1 and RotaryConfig().scale == 1
+    assert RotaryConfig(scaling="yarn", original_max_position=4096).scale == 1     # nothing stretched
+    assert RotaryConfig(amplitude=0.5).scale == 0.5
+
+
+def test_partial_heads_use_the_rotated_width():
+    whole, part = RotaryConfig(head_dim=64, theta=1e4), RotaryConfig(head_dim=256, rotary_dim=64, theta=1e4)
+    assert whole.frequencies() == part.frequencies() and len(part.frequencies()) == 32
+
+
+def test_turns_are_fractions_of_a_turn():
+    c = RotaryConfig(head_dim=64, pair_factors=(0.01,) + (1.0,) * 31)  # 100 radians a position: many whole turns
+    t = [x % (1 << 64) for x in RotaryEmbedding(c, "cpu").turns.tolist()]
+    for x, f in zip(t, c.frequencies()):
+        want = f / (2 * math.pi) % 1.0
+        assert abs(x / 2.0 ** 64 - want) < 1e-13
+
+
+@pytest.mark.parametrize("kw", [
+    dict(head_dim=0), dict(head_dim=257), dict(rotary_dim=0), dict(rotary_dim=33), dict(rotary_dim=130), dict(head_dim=75),
+    dict(layout="neox"), dict(scaling="dynamic"), dict(theta=0.0), dict(theta=float("nan")), dict(factor=-1.0),
+    dict(scaling="yarn"), dict(scaling="llama3"), dict(scaling="yarn", original_max_position=4096, theta=1.0),
+    dict(scaling="llama3", original_max_position=8192, high_freq_factor=1.0), dict(amplitude=float("inf")),
+    dict(pair_factors=(1.0,)), dict(pair_factors=(1.0,) * 64, scaling="linear"),
+])
+def test_refused_configurations(kw):
+    with pytest.raises(ValueError):
+        RotaryConfig(**kw)
+
+
+@pytest.mark.skipif(not _lib.LIB_PATH.exists(), reason="libaspire_hip.so not built")
+def test_entry_points_refuse_on_the_host():
+    """Everything that the C entries can see to be wrong is refused before a launch (so this runs without a GPU)."""
+    L = _lib.lib()
+
+    def args(**kw):
+        a = _lib.RotaryArgs(q=4096, q_out=8192, k=12288, k_out=16384, v=20480, num_qo_heads=4, num_kv_heads=2,
+                            total_tokens=3, head_dim=64, rotary_dim=32, turns=4096, amplitude=1.0, positions=4096,
+                            kv_cache=4096, num_pages=4, num_page_indices=4, page_size=16, num_seq=1, append_indptr=4096,
+                            kv_page_indices=4096, kv_page_indptr=4096, kv_last_page_len=4096)
+        for name, value in kw.items():
+            setattr(a, name, value)
+        return ctypes.byref(a)
+
+    both = [dict(dtype=3), dict(dtype=-1), dict(head_dim=257), dict(rotary_dim=31), dict(rotary_dim=66), dict(rotary_dim=0),
+            dict(total_tokens=-1), dict(num_qo_heads=-1), dict(num_kv_heads=1025), dict(turns=None), dict(q=None), dict(q_out=None),
+            dict(k=None)]
+    for kw in both:
+        for entry in (L.aspire_rotary, L.aspire_rotary_append):
+            assert entry(args(**kw), None) == _lib.ASPIRE_ERR_INVALID, kw
+    for kw in (dict(positions=None), dict(k_out=None)):
+        assert L.aspire_rotary(args(**kw), None) == _lib.ASPIRE_ERR_INVALID, kw
+    for kw in (dict(dtype=2), dict(v=None), dict(kv_cache=None), dict(page_size=0), dict(num_pages=-1), dict(num_seq=-1),
+               dict(append_indptr=None), dict(kv_page_indptr=None), dict(kv_last_page_len=None), dict(kv_page_indices=None)):
+        assert L.aspire_rotary_append(args(**kw), None) == _lib.ASPIRE_ERR_INVALID, kw
+    assert "aspire_rotary_append" in _lib.lib().aspire_last_error().decode()
+    assert L.aspire_rotary(args(total_tokens=0), None) == _lib.ASPIRE_OK
+    assert L.aspire_rotary(None, None) == _lib.ASPIRE_ERR_INVALID
+
+
+def test_cpu_tensors_are_refused():
+    rot = RotaryEmbedding(RotaryConfig(head_dim=64), "cpu")
+    with pytest.raises(RuntimeError):
+        rot.apply(torch.zeros(1, 1, 64), None, torch.zeros(1, dtype=torch.int32))
