@@ -60,6 +60,7 @@ EXPORTED = (
     "aspire_linear_splits",
     "aspire_linear_partials",
     "aspire_add_rms_norm_partials",
+    "aspire_linear_int4",
     "aspire_rotary",
     "aspire_rotary_append",
     "aspire_bandwidth_probe",
@@ -186,6 +187,16 @@ class RopeArgs(ctypes.Structure):
     ]
 
 
+class Int4Args(ctypes.Structure):
+    _fields_ = [
+        ("x", ctypes.c_void_p), ("x_stride", ctypes.c_int64), ("weights", ctypes.c_void_p),
+        ("scales", ctypes.c_void_p), ("zeros", ctypes.c_void_p), ("out", ctypes.c_void_p),
+        ("out_stride", ctypes.c_int64),
+        ("rows", ctypes.c_int32), ("n", ctypes.c_int32), ("k", ctypes.c_int32), ("group", ctypes.c_int32),
+        ("swiglu", ctypes.c_int32), ("fp16", ctypes.c_int32), ("scales_fp16", ctypes.c_int32),
+    ]
+
+
 class RotaryArgs(ctypes.Structure):
     _fields_ = [
         ("q", ctypes.c_void_p), ("q_stride_t", ctypes.c_int64), ("q_stride_h", ctypes.c_int64),
@@ -256,6 +267,7 @@ def _declare(lib):
         "aspire_linear_splits": [i32, i32, i32],
         "aspire_linear_partials": [vp, i64, vp, i64, vp, i64, i32, i32, i32, vp],
         "aspire_add_rms_norm_partials": [vp, i64, vp, i32, vp, vp, i64, i32, i32, f32, vp],
+        "aspire_linear_int4": [ctypes.POINTER(Int4Args), vp],
         "aspire_rotary": [ctypes.POINTER(RotaryArgs), vp],
         "aspire_rotary_append": [ctypes.POINTER(RotaryArgs), vp],
         "aspire_bandwidth_probe": [i32, vp, i64, vp, i64, i32, i32, vp],

@@ -1,0 +1,142 @@
+"""Linear layers with 4-bit weights on the HIP path (``aspire_linear_int4``).
+
+The projections of ``aspire_amd.linear`` for checkpoints whose weights are 4-bit codes in groups along K, each with a
+scale and, where the checkpoint has them, a zero point: ``w[n, k] = scales[n, k // group] * (codes[n, k] - zeros[n,
+k // group])``. The weights are read as they are (an eighth of fp32's bytes) and never rounded to 16 bits: codes are
+multiplied exactly, sums are fp32, and the output is rounded once. Any number of token rows, bf16 or fp16.
+
+``Int4Weight`` holds a matrix in the kernels' layout, made once from a checkpoint's packed codes
+(``from_packed``) or from a bf16 matrix (``quantize``).
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from aspire_amd import _lib
+from aspire_amd.attention.rotary import _on
+
+GROUPS = (32, 64, 128)
+
+
+class Int4Weight:
+    """``[N, K]`` 4-bit weights on a GPU, laid out in blocks of 16 rows x 128 columns."""
+
+    def __init__(self, shape, group, codes, scales, zeros):
+        self.shape, self.group = tuple(shape), group
+        self.codes, self.scales, self.zeros = codes, scales, zeros  # see aspire_hip.h for the layouts
+
+    @classmethod
+    def from_packed(cls, packed: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None = None, *,
+                    group: int) -> "Int4Weight":
+        """``packed`` uint8 ``[N, K / 2]`` (column 2j in the low half of byte j), ``scales`` bf16 or fp16
+        ``[N, K / group]``, ``zeros`` uint8 ``[N, K / group]`` of 0 to 15 (None: 8 everywhere)."""
+        n, k = packed.shape[0], packed.shape[1] * 2 if packed.dim() == 2 else 0
+        if packed.dim() != 2 or packed.dtype != torch.uint8 or n == 0 or group not in GROUPS or k == 0 or k % group:
+            raise ValueError(f"Int4Weight: packed must be uint8 [N, K / 2], group one of {GROUPS} and K a multiple of it")
+        if scales.shape != (n, k // group) or scales.dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError("Int4Weight: scales must be bf16 or fp16 [N, K / group]")
+        if zeros is not None and (zeros.shape != scales.shape or zeros.dtype != torch.uint8):
+            raise ValueError("Int4Weight: zeros must be uint8 [N, K / group]")
+        if any(t is not None and t.device != packed.device for t in (scales, zeros)):
+            raise ValueError("Int4Weight: packed, scales and zeros must be on one device")
+        if zeros is not None and int(zeros.max()) > 15:
+            raise ValueError("Int4Weight: zeros must be 0 to 15")
+        tiles, blocks = (n + 15) // 16, (k + 127) // 128
+
+        def fill(t, rows, cols):  # zeros behind the matrix' end
+            if t.shape == (rows, cols):
+                return t
+            out = torch.zeros(rows, cols, dtype=t.dtype, device=t.device)
+            out[: t.shape[0], : t.shape[1]] = t
+            return out
+
+        # bytes of a lane's word: [tile, row, block, word, lane / 16, byte] -> [tile, block, lane / 16, row, word, byte]
+        b = fill(packed, tiles * 16, blocks * 64).view(tiles, 16, blocks, 4, 4, 4).permute(0, 2, 4, 1, 3, 5)
+        even, odd = torch.empty_like(b, memory_format=torch.contiguous_format), None
+        even.copy_(b)
+        # nibble e of 8 goes to place e / 2 + 4 (e % 2): bytes (e1 e0)(e3 e2)(e5 e4)(e7 e6) -> (e2 e0)(e6 e4)(e3 e1)(e7 e5)
+        lo, hi = even & 15, even >> 4
+        codes = torch.empty_like(even)
+        codes[..., 0] = lo[..., 0] | (lo[..., 1] << 4)
+        codes[..., 1] = lo[..., 2] | (lo[..., 3] << 4)
+        codes[..., 2] = hi[..., 0] | (hi[..., 1] << 4)
+        codes[..., 3] = hi[..., 2] | (hi[..., 3] << 4)
+        groups = blocks * 128 // group
+        flat = lambda t: None if t is None else fill(t, tiles * 16, groups).t().contiguous()
+        return cls((n, k), group, codes.view(tiles, blocks, 64, 16), flat(scales), flat(zeros))
+
+    @classmethod
+    def quantize(cls, w: torch.Tensor, *, group: int = 128, symmetric: bool = False) -> "Int4Weight":
+        """The nearest 4-bit form of a matrix ``[N, K]``: each group's range (with 0 in it) in 15 steps, or with ``symmetric``
+        its largest magnitude in 7."""
+        if w.dim() != 2 or group not in GROUPS or w.shape[1] % group:
+            raise ValueError(f"Int4Weight: w must be [N, K], group one of {GROUPS} and K a multiple of it")
+        dtype = w.dtype if w.dtype in (torch.bfloat16, torch.float16) else torch.bfloat16
+        v = w.float().view(w.shape[0], -1, group)
+        if symmetric:
+            scale, zero = v.abs().amax(-1) / 7, None
+        else:
+            lo, hi = v.amin(-1).clamp(max=0), v.amax(-1).clamp(min=0)
+            scale = (hi - lo) / 15
+        scale = scale.to(dtype)
+        step = scale.float().clamp(min=torch.finfo(torch.float32).tiny)[..., None]
+        if not symmetric:
+            zero = (-lo[..., None] / step).round_().clamp_(0, 15)
+        codes = ((v / step).round_() + (8 if zero is None else zero)).clamp_(0, 15).to(torch.uint8).view(w.shape)
+        packed = codes[:, 0::2] | (codes[:, 1::2] << 4)
+        return cls.from_packed(packed, scale, None if zero is None else zero[..., 0].to(torch.uint8), group=group)
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    def nbytes(self) -> int:
+        return sum(t.numel() * t.element_size() for t in (self.codes, self.scales, self.zeros) if t is not None)
+
+    def to(self, device) -> "Int4Weight":
+        move = lambda t: None if t is None else t.to(device)
+        return Int4Weight(self.shape, self.group, move(self.codes), move(self.scales), move(self.zeros))
+
+    def dequantize(self, dtype=torch.float32) -> torch.Tensor:
+        """The matrix ``[N, K]`` that the codes stand for."""
+        (n, k), (tiles, blocks) = self.shape, self.codes.shape[:2]
+        c = self.codes.view(tiles, blocks, 4, 16, 4, 4)
+        nib = torch.stack([c & 15, c >> 4], dim=-1).flatten(-2)              # places 0 .. 7 of a word
+        nib = nib[..., [0, 4, 1, 5, 2, 6, 3, 7]]                              # in k's order
+        codes = nib.permute(0, 3, 1, 4, 2, 5).reshape(tiles * 16, blocks * 128)
+        spread = lambda t: t.t().float().repeat_interleave(self.group, dim=1)
+        w = (codes.float() - (8.0 if self.zeros is None else spread(self.zeros))) * spread(self.scales)
+        return w[:n, :k].to(dtype)
+
+
+def linear_int4(x: torch.Tensor, w: Int4Weight, out: torch.Tensor, *, swiglu: bool = False) -> torch.Tensor:
+    """``out = x @ w.T`` (``[rows, N]``), or with ``swiglu`` ``silu(x @ w[:N/2].T) * (x @ w[N/2:].T)`` (``[rows, N/2]``, N a
+    multiple of 32), for bf16 or fp16 ``x`` with 16-byte aligned rows; ``out`` of ``x``'s type with contiguous rows, apart from x."""
+    what = "linear_int4"
+    _lib.require_cuda(x, out, w.codes, what=what)
+    n, k = w.shape
+    if x.dim() != 2 or x.dtype not in (torch.bfloat16, torch.float16) or x.shape[1] != k or x.stride(1) != 1 \
+            or x.stride(0) % 8 or x.data_ptr() % 16:
+        raise ValueError(f"{what}: x must be bf16 or fp16 [rows, {k}] with 16-byte aligned rows")
+    if swiglu and n % 32:
+        raise ValueError(f"{what}: swiglu needs N a multiple of 32")
+    cols = n // 2 if swiglu else n
+    if out.dtype != x.dtype or out.shape != (x.shape[0], cols) or out.stride(1) != 1:
+        raise ValueError(f"{what}: out must be {x.dtype} [{x.shape[0]}, {cols}] with contiguous rows")
+    if x.device != w.device or out.device != w.device:
+        raise ValueError(f"{what}: x, out and the weights must be on one device")
+    if torch.is_grad_enabled() and x.requires_grad:
+        raise ValueError(f"{what}: not differentiable")
+    a = _lib.Int4Args(x=x.data_ptr(), x_stride=x.stride(0), weights=w.codes.data_ptr(), scales=w.scales.data_ptr(),
+                      zeros=_lib.ptr(w.zeros), out=out.data_ptr(), out_stride=out.stride(0), rows=x.shape[0], n=n, k=k,
+                      group=w.group, swiglu=int(swiglu), fp16=int(x.dtype == torch.float16),
+                      scales_fp16=int(w.scales.dtype == torch.float16))
+    with _on(w.device):
+        _lib.check(_lib.lib().aspire_linear_int4(ctypes.byref(a), _lib.stream_of(x)), what)
+    return out
+
+
+__all__ = ["GROUPS", "Int4Weight", "linear_int4"]

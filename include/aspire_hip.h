@@ -499,6 +499,26 @@ int32_t aspire_linear_splits(int32_t rows, int32_t n, int32_t k);
 int aspire_linear_partials(const void* x, int64_t x_stride, const void* w, int64_t w_stride, float* partials,
                            int64_t partials_size, int32_t rows, int32_t n, int32_t k, void* stream);
 
+/* Products with 4-bit weights: out[m, n] = sum_k x[m, k] * scales[n, k / group] * (code[n, k] - zeros[n, k / group]),
+ * exact weights, fp32 sums, one rounding to x's type (bf16, or fp16 with fp16 set). With swiglu, n counts n / 2 gate
+ * rows, then n / 2 up rows, and out[m, :n / 2] = silu(gate) * up, rounded once.
+ * weights: blocks of 16 rows x 128 k in 1 KiB, [n / 16, up][k / 128, up][64][4] words: word c of lane l holds row
+ * l % 16, k 32 c + 8 (l / 16) + e in bits 4 (e / 2) + 16 (e % 2), e = 0 .. 7. scales ([k / group][n up to a multiple
+ * of 16], bf16 or fp16) and zeros (the same in bytes, 0 .. 15, NULL: 8) cover whole blocks: their groups past k and rows past n are
+ * there and 0. group 32, 64 or 128, k a multiple of it; 16-byte aligned x rows; out rows of any stride. */
+typedef struct aspire_int4_args {
+  const void* x;
+  int64_t x_stride;
+  const void* weights;
+  const void* scales;
+  const void* zeros;
+  void* out;
+  int64_t out_stride;
+  int32_t rows, n, k, group, swiglu, fp16, scales_fp16;
+} aspire_int4_args;
+
+int aspire_linear_int4(const aspire_int4_args* args, void* stream);
+
 /* aspire_add_rms_norm with delta = bf16(the sum of the slabs partials [splits][rows][dim]). */
 int aspire_add_rms_norm_partials(void* x, int64_t x_stride, const float* partials, int32_t splits,
                                  const void* weight, void* out, int64_t out_stride, int32_t rows, int32_t dim,

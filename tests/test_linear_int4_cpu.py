@@ -1,0 +1,74 @@
+"""The 4-bit weights' layout, and the host-side checks of the products (no GPU)."""
+
+import ctypes
+
+import pytest
+import torch
+
+from aspire_amd import _lib
+from aspire_amd.linear_int4 import Int4Weight
+
+
+@pytest.mark.parametrize("n,k,group,zeros", [(16, 128, 128, False), (40, 96, 32, True), (1, 320, 64, True)])
+def test_layout_is_the_documented_one(n, k, group, zeros):
+    g = torch.Generator().manual_seed(n + k)
+    packed = torch.randint(0, 256, (n, k // 2), dtype=torch.uint8, generator=g)
+    scales = torch.rand(n, k // group, generator=g).to(torch.float16)
+    z = torch.randint(0, 16, (n, k // group), dtype=torch.uint8, generator=g) if zeros else None
+    w = Int4Weight.from_packed(packed, scales, z, group=group)
+    tiles, blocks = (n + 15) // 16, (k + 127) // 128
+    words = w.codes.contiguous().view(torch.int32).view(tiles, blocks, 64, 4).tolist()
+    code = lambda r, c: int(packed[r, c // 2]) >> (4 * (c % 2)) & 15 if r < n and c < k else 0
+    for t in range(tiles):
+        for b in range(blocks):
+            for l in range(64):
+                for c in range(4):
+                    for e in range(8):
+                        got = words[t][b][l][c] >> (4 * (e // 2) + 16 * (e % 2)) & 15
+                        assert got == code(16 * t + l % 16, 128 * b + 32 * c + 8 * (l // 16) + e)
+    full = torch.zeros(blocks * 128 // group, tiles * 16, dtype=torch.float16)
+    full[: k // group, :n] = scales.t()
+    assert torch.equal(w.scales, full)
+    c = torch.stack([packed & 15, packed >> 4], dim=-1).view(n, k).float()
+    spread = lambda t: t.float().repeat_interleave(group, dim=1)
+    assert torch.equal(w.dequantize(), (c - (spread(z) if zeros else 8)) * spread(scales))
+    if zeros:
+        assert torch.equal(w.zeros[: k // group, :n], z.t())
+
+
+@pytest.mark.parametrize("change", [
+    dict(packed=torch.zeros(4, 64)), dict(packed=torch.zeros(64, dtype=torch.uint8)), dict(group=48), dict(group=256),
+    dict(scales=torch.zeros(4, 1, dtype=torch.bfloat16)), dict(scales=torch.zeros(4, 2)),
+    dict(zeros=torch.zeros(4, 1, dtype=torch.uint8)), dict(zeros=torch.zeros(4, 2, dtype=torch.int32)),
+    dict(zeros=torch.full((4, 2), 16, dtype=torch.uint8)), dict(packed=torch.zeros(4, 40, dtype=torch.uint8)),
+])
+def test_refused_weights(change):
+    kw = dict(packed=torch.zeros(4, 64, dtype=torch.uint8), scales=torch.zeros(4, 2, dtype=torch.bfloat16), zeros=None, group=64)
+    Int4Weight.from_packed(**kw)
+    with pytest.raises(ValueError):
+        Int4Weight.from_packed(**{**kw, **change})
+
+
+def test_refused_matrices():
+    for w, group in ((torch.zeros(4, 100), 64), (torch.zeros(64), 64), (torch.zeros(4, 128), 16)):
+        with pytest.raises(ValueError):
+            Int4Weight.quantize(w, group=group)
+
+
+@pytest.mark.skipif(not _lib.LIB_PATH.exists(), reason="libaspire_hip.so not built")
+def test_entry_point_refuses_on_the_host():
+    L = _lib.lib()
+
+    def call(**kw):
+        a = _lib.Int4Args(x=4096, x_stride=256, weights=4096, scales=4096, zeros=4096, out=4096, out_stride=64, rows=4, n=64,
+                          k=256, group=64)
+        for name, value in kw.items():
+            setattr(a, name, value)
+        return L.aspire_linear_int4(ctypes.byref(a), None)
+
+    for kw in (dict(rows=-1), dict(rows=1 << 22), dict(n=-1), dict(k=0), dict(k=250), dict(group=16), dict(group=0), dict(x=None),
+               dict(weights=None), dict(scales=None), dict(out=None), dict(x=4104), dict(x_stride=260), dict(x_stride=248),
+               dict(out_stride=63), dict(n=48, swiglu=1), dict(scales=4100), dict(zeros=4097)):
+        assert call(**kw) == _lib.ASPIRE_ERR_INVALID, kw
+    assert call(rows=0) == _lib.ASPIRE_OK and call(n=0) == _lib.ASPIRE_OK
+    assert L.aspire_linear_int4(None, None) == _lib.ASPIRE_ERR_INVALID
