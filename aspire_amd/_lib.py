@@ -61,6 +61,7 @@ EXPORTED = (
     "aspire_linear_partials",
     "aspire_add_rms_norm_partials",
     "aspire_linear_int4",
+    "aspire_linear_int4_workspace",
     "aspire_rotary",
     "aspire_rotary_append",
     "aspire_bandwidth_probe",
@@ -194,6 +195,7 @@ class Int4Args(ctypes.Structure):
         ("out_stride", ctypes.c_int64),
         ("rows", ctypes.c_int32), ("n", ctypes.c_int32), ("k", ctypes.c_int32), ("group", ctypes.c_int32),
         ("swiglu", ctypes.c_int32), ("fp16", ctypes.c_int32), ("scales_fp16", ctypes.c_int32),
+        ("workspace", ctypes.c_void_p), ("workspace_floats", ctypes.c_int64),
     ]
 
 
@@ -268,6 +270,7 @@ def _declare(lib):
         "aspire_linear_partials": [vp, i64, vp, i64, vp, i64, i32, i32, i32, vp],
         "aspire_add_rms_norm_partials": [vp, i64, vp, i32, vp, vp, i64, i32, i32, f32, vp],
         "aspire_linear_int4": [ctypes.POINTER(Int4Args), vp],
+        "aspire_linear_int4_workspace": [i32, i32, i32, i32, i32],
         "aspire_rotary": [ctypes.POINTER(RotaryArgs), vp],
         "aspire_rotary_append": [ctypes.POINTER(RotaryArgs), vp],
         "aspire_bandwidth_probe": [i32, vp, i64, vp, i64, i32, i32, vp],
@@ -276,6 +279,7 @@ def _declare(lib):
         fn = getattr(lib, name)
         fn.argtypes = argtypes
         fn.restype = ctypes.c_int
+    lib.aspire_linear_int4_workspace.restype = i64
 
 
 def lib():

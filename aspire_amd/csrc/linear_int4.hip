@@ -1,14 +1,13 @@
 // Products with 4-bit weights: y[m, n] = sum_k x[m, k] s[n, g(k)] (c[n, k] - z[n, g(k)]), codes c of 4 bits,
 // a 16-bit scale s and a whole-numbered zero point z (8 without) for each group of 32, 64 or 128 k.
 //
-// Nothing is rounded on the way: a code becomes the 16-bit float kOffset + c (exact: bf16 128 + c, fp16 1024 + c)
-// by putting its bits into the constant's mantissa, MFMAs sum it against x in fp32, and what the offset adds is
-// taken off for each group before the scale goes on,
-//     y += s (sum (kOffset + c) x - (kOffset + z) sum x),
-// the sums of x from one more MFMA with ones in the weights' place. fp16 has packed subtraction, so there
-// kOffset + z comes off the weights themselves, exactly, and no sums of x are needed.
+// Weights are never rounded. fp16: a code's bits in the mantissa of 1024 give 1024 + c, and a packed subtraction of 1024 + z
+// leaves c - z exactly. bf16 has no packed arithmetic, but the bits of 192 + d are those of 192 (0x4340) plus d for every
+// d = c - z from -15 to 15 (one binade, steps of 1), so bytes 0x40 + d, four to an addition, get their upper byte 0x43 from a
+// byte permutation, and the sum over a group starts from -192 sum x, which one MFMA with -192 in the weights' place gives for all of them:
+//     part = sum (192 + d) x - 192 sum x (fp32),  y += s part  for each group.
 //
-// Weights are laid out once (aspire_int4_pack's order): 16 rows x 128 k make a block of 1 KiB in which lane l of a
+// Weights are laid out once (aspire_hip.h): 16 rows x 128 k make a block of 1 KiB in which lane l of a
 // wave finds its 32 codes (row l % 16, and for each 32 k the 8 from 8 (l / 16) on) in one 16-byte load; blocks of 16
 // rows follow each other along k. A word's nibbles are ordered so that shifts by 0, 4, 8, 12 leave neighbours in
 // the low and high half.
@@ -24,234 +23,579 @@ struct Int4Params {
   const uint16_t* x;
   int64_t x_st;
   const uint4* w;
-  const uint16_t* scales;    // [groups][n_pad]
-  const uint8_t* zeros;      // [groups][n_pad], or null: 8
+  const uint8_t* scales;     // [tiles][blocks][4][128 / group][4] 16-bit floats
+  const uint8_t* zeros;      // [tiles][blocks][16][128 / group] bytes, or null: 8
   uint16_t* out;
   int64_t o_st;
   int32_t rows, n, n_pad, k, blocks;   // n: output columns; blocks: of 128 k
-  int32_t up_tile;           // swiglu: 16-row tile where the up rows begin
-  int32_t scale_fp16;
+  int32_t swiglu;            // the up rows' first 16-row tile is n / 16
   int32_t wide_out;          // output rows take 8-byte stores
+  int32_t splits;            // of the blocks along k
+  float* partials;           // [splits][rows][n_pad]
 };
 
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
 typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
 
+// A type's MFMA, and 8 codes as its weights in k's order, with what a row's zero point makes of them (`Row`).
 struct Bf16 {
-  static constexpr uint32_t kMagic = 0x43004300u;
+  static constexpr bool kOffset = true;
   static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
   }
   static __device__ __forceinline__ uint16_t narrow(float f) { return __builtin_bit_cast(uint16_t, static_cast<__bf16>(f)); }
+  static __device__ __forceinline__ float low(uint32_t v) { return __uint_as_float(v << 16); }
+  static __device__ __forceinline__ float high(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
+  typedef uint32_t Row;             // 0x40 - z in each byte
+  static __device__ __forceinline__ Row row(uint32_t z) { return 0x40404040u - z * 0x01010101u; }
+  // bytes 0x40 + c - z, then 0x43 above each
+  static __device__ __forceinline__ u32x4 weights(uint32_t w, Row z) {
+    const uint32_t lo = (w & 0x0f0f0f0fu) + z, hi = ((w >> 4) & 0x0f0f0f0fu) + z;
+    return u32x4{__builtin_amdgcn_perm(0x43434343u, lo, 0x04020400u), __builtin_amdgcn_perm(0x43434343u, hi, 0x04020400u),
+                 __builtin_amdgcn_perm(0x43434343u, lo, 0x04030401u), __builtin_amdgcn_perm(0x43434343u, hi, 0x04030401u)};
+  }
 };
 struct Fp16 {
-  static constexpr uint32_t kMagic = 0x64006400u;
+  static constexpr bool kOffset = false;
   static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
   }
   static __device__ __forceinline__ uint16_t narrow(float f) { return __builtin_bit_cast(uint16_t, static_cast<_Float16>(f)); }
-};
-
-// 8 codes as 8 values kOffset + c, in k's order.
-template <class T>
-__device__ __forceinline__ u32x4 spread(uint32_t w) {
-  u32x4 v;
+  static __device__ __forceinline__ float low(uint32_t v) { return float(__builtin_bit_cast(_Float16, uint16_t(v))); }
+  static __device__ __forceinline__ float high(uint32_t v) { return float(__builtin_bit_cast(_Float16, uint16_t(v >> 16))); }
+  struct Row { f16x2 low, high; };  // -(1024 + z) and -(64 + z), twice
+  static __device__ __forceinline__ Row row(uint32_t z) {
+    const _Float16 f = static_cast<_Float16>(float(z));
+    const _Float16 low = _Float16(-1024) - f, high = _Float16(-64) - f;
+    return Row{f16x2{low, low}, f16x2{high, high}};
+  }
+  // a nibble in bits 4 to 7 makes 1024 + 16 c
+  static __device__ __forceinline__ u32x4 weights(uint32_t w, Row z) {
+    const f16x2 sixteenth = f16x2{_Float16(0.0625f), _Float16(0.0625f)};
+    u32x4 v;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = ((w >> (4 * i)) & 0x000f000fu) | T::kMagic;
-  return v;
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t b = w >> (8 * i);
+      v[2 * i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, (b & 0x000f000fu) | 0x64006400u) + z.low);
+      v[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(__builtin_bit_cast(f16x2, (b & 0x00f000f0u) | 0x64006400u), sixteenth, z.high));
+    }
+    return v;
+  }
+};
+constexpr uint32_t kMinusOffset = 0xc340c340u;  // -192 twice
+
+__device__ __forceinline__ float silu(float x) { return x / (1.f + expf(-x)); }
+
+// A row's zero points of a block's groups, a byte each.
+template <int kParts>
+__device__ __forceinline__ uint32_t zero_points(const uint8_t* at) {
+  if (kParts == 4) return *reinterpret_cast<const uint32_t*>(at);
+  if (kParts == 2) return *reinterpret_cast<const uint16_t*>(at);
+  return *at;
 }
 
-__device__ __forceinline__ float scale_of(uint32_t bits, int fp16) {
-  return fp16 ? float(__builtin_bit_cast(_Float16, uint16_t(bits))) : __uint_as_float(bits << 16);
+// 4 neighbouring outputs of a row.
+template <class T>
+__device__ __forceinline__ void store4(const Int4Params& p, int64_t m, int col, const float* v) {
+  uint16_t* to = p.out + m * p.o_st + col;
+  const uint16_t o[4] = {T::narrow(v[0]), T::narrow(v[1]), T::narrow(v[2]), T::narrow(v[3])};
+  if (p.wide_out && col + 4 <= p.n) {
+    *reinterpret_cast<uint2*>(to) = make_uint2(o[0] | uint32_t(o[1]) << 16, o[2] | uint32_t(o[3]) << 16);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (col + e < p.n) to[e] = o[e];
+  }
 }
 
 constexpr int kWaves = 8;
+constexpr int kAhead = 4;     // blocks of 1 KiB a wave has in flight
 
-// A workgroup takes TN tiles of 16 weight rows and TM of 16 rows of x; its waves take the blocks of 128 k in
-// turn and add up through LDS at the end, in a fixed order.
-template <class T, int G, int TM, int TN, bool kSwiglu>
-__global__ __launch_bounds__(64 * kWaves) void int4_stream_kernel(Int4Params p) {
+// Up to 16 rows: bound by the weights' stream. A workgroup walks over output tiles of 16 columns (with swiglu over pairs of a
+// gate and an up tile), for all of k or the split blockIdx.y of at most kAhead * kWaves blocks; its waves take the blocks of
+// 128 k in turn, keep their x in registers, and add up through LDS, in a fixed order. A block is asked for as soon as
+// the one before it in its registers is multiplied, across the ends of tiles, so the stream never pauses.
+template <class T, class S, int G>
+__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(G == 128 ? 4 : 3))) void int4_stream_kernel(Int4Params p) {
   constexpr int kParts = 128 / G;   // groups of a block
-  constexpr bool kIsBf16 = std::is_same<T, Bf16>::value;
-  __shared__ float4 sums[kWaves][TM * TN][64];
+  constexpr int kSteps = 4 / kParts;
+  __shared__ float4 sums[2][kWaves][64];
   const int lane = threadIdx.x & 63;
   const int wave = wave_uniform(threadIdx.x >> 6);
   const int r = lane & 15, grp = lane >> 4;
-  const int64_t m0 = int64_t(blockIdx.y) * (16 * TM);
-  int tile[TN];                     // 16-row tiles of the weights
+  const int first = wave_uniform(int(int64_t(p.blocks) * blockIdx.y / p.splits));
+  const int blocks = wave_uniform(int(int64_t(p.blocks) * (blockIdx.y + 1) / p.splits)) - first;
+  const int tiles = p.swiglu ? p.n / 16 : p.splits > 1 ? p.n_pad / 16 : (p.n + 15) / 16, halves = p.swiglu ? 2 : 1;
+
+  // No load depends on a branch (the compiler could not count the loads in flight, and would wait for all of them): past
+  // an end it reads what is there before it. Rows past the last are not stored; k past the end has codes and scales of 0.
+  struct Block {
+    uint4 w;
+    uint2 sc[kParts];
+    uint32_t zp;                    // a byte a group
+  };
+  const uint8_t* zeros = p.zeros ? p.zeros : p.scales;
+  const int64_t zero_block = p.zeros ? 16 * kParts : 0;
+  const auto fetch = [&](Block& f, int tile, int i) {
+    const int64_t at = int64_t(tile) * p.blocks + first + min(i * kWaves + wave, blocks - 1);
+    f.w = p.w[at * 64 + lane];
 #pragma unroll
-  for (int j = 0; j < TN; ++j)
-    tile[j] = kSwiglu ? (j < TN / 2 ? blockIdx.x * (TN / 2) + j : p.up_tile + blockIdx.x * (TN / 2) + j - TN / 2)
-                      : blockIdx.x * TN + j;
-  const int last_tile = p.n_pad / 16 - 1;
-  const uint16_t* xrow[TM];
-  bool live[TM];
+    for (int g = 0; g < kParts; ++g)
+      f.sc[g] = *reinterpret_cast<const uint2*>(p.scales + at * (32 * kParts) + grp * (8 * kParts) + 8 * g);
+    f.zp = zero_points<kParts>(zeros + at * zero_block + r * kParts);
+  };
+  const auto multiply = [&](const Block& f, const u32x4* x, f32x4 acc) {
+    const uint32_t words[4] = {f.w.x, f.w.y, f.w.z, f.w.w};
 #pragma unroll
-  for (int t = 0; t < TM; ++t) {
-    const int64_t m = m0 + t * 16 + r;
-    live[t] = m < p.rows;
-    xrow[t] = p.x + (live[t] ? m : 0) * p.x_st + 8 * grp;
+    for (int g = 0; g < kParts; ++g) {
+      f32x4 part = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (T::kOffset)  // -192 times the sum of x over the group, the same for all 16 weight rows
+#pragma unroll
+        for (int c = g * kSteps; c < (g + 1) * kSteps; ++c)
+          part = T::mfma(u32x4{kMinusOffset, kMinusOffset, kMinusOffset, kMinusOffset}, x[c], part);
+      const typename T::Row base = T::row(p.zeros ? (f.zp >> (8 * g)) & 15u : 8u);
+#pragma unroll
+      for (int c = g * kSteps; c < (g + 1) * kSteps; ++c) part = T::mfma(T::weights(words[c], base), x[c], part);
+      const float sc[4] = {S::low(f.sc[g].x), S::high(f.sc[g].x), S::low(f.sc[g].y), S::high(f.sc[g].y)};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[i] = fmaf(sc[i], part[i], acc[i]);
+    }
+    return acc;
+  };
+
+  int tile = blockIdx.x, half = 0;  // half 1: the up tile
+  Block ring[kAhead];
+  u32x4 x[kAhead][4];
+  const uint16_t* xrow = p.x + min(r, p.rows - 1) * p.x_st + 8 * grp;
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) {
+    fetch(ring[i], tile, i);
+    const int k = (first + min(i * kWaves + wave, blocks - 1)) * 128;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) x[i][c] = *reinterpret_cast<const u32x4*>(xrow + min(k + c * 32, p.k - 32));
   }
+  float4 gate = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int done = 0; tile < tiles; ++done) {
+    const bool last = half + 1 == halves;
+    const int next = last ? tile + int(gridDim.x) : tile, next_half = last ? 0 : half + 1;
+    f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      if (i * kWaves + wave < blocks) acc = multiply(ring[i], x[i], acc);
+      fetch(ring[i], min(next, tiles - 1) + next_half * (p.n / 16), i);
+    }
+    // a wave in turn adds up, while the others go on
+    float4 (*to)[64] = sums[done & 1];
+    to[wave][lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+    __syncthreads();
+    if (wave == (done / halves) % kWaves) {
+      float4 v = to[0][lane];
+#pragma unroll
+      for (int q = 1; q < kWaves; ++q) {
+        const float4 u = to[q][lane];
+        v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
+      }
+      if (!last) {
+        gate = v;
+      } else if (r < p.rows) {
+        if (p.swiglu) v = make_float4(silu(gate.x) * v.x, silu(gate.y) * v.y, silu(gate.z) * v.z, silu(gate.w) * v.w);
+        const float o[4] = {v.x, v.y, v.z, v.w};
+        const int col = tile * 16 + 4 * grp;
+        if (p.splits > 1)
+          *reinterpret_cast<float4*>(p.partials + (int64_t(blockIdx.y) * p.rows + r) * p.n_pad + col) = v;
+        else
+          store4<T>(p, r, col, o);
+      }
+    }
+    tile = next, half = next_half;
+  }
+}
+
+// ---------------------------------------------------------------- more rows
+constexpr uint32_t kBufferConfig = 0x00020000u;  // gfx9 raw buffer dword 3
+
+__device__ __forceinline__ u32x4 buffer_desc(const char* base, int span) {
+  const uint64_t v = reinterpret_cast<uint64_t>(base);
+  return u32x4{uint32_t(__builtin_amdgcn_readfirstlane(uint32_t(v))),
+               uint32_t(__builtin_amdgcn_readfirstlane(uint32_t(v >> 32))) & 0xffffu, uint32_t(span), kBufferConfig};
+}
+
+// 64 lanes x 16 bytes from the buffer straight into 1 KiB of LDS at address `at` (no register output); loads past the
+// buffer's span return zeros.
+__device__ __forceinline__ void load_lds(u32x4 desc, int voff, uint32_t at) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+               :: "s"(wave_uniform(int(at))), "v"(voff), "s"(desc) : "memory");
+}
+
+// Bytes of a ring stage of 128 k: x rows, weight tiles, their scales and zero points; and the stages that fit a CU.
+constexpr int stage_bytes(int bm, int tiles, int parts) { return bm * 256 + tiles * (1024 + 48 * parts); }
+constexpr int sum_bytes(int bm, int parts) { return 2 * parts * bm * 4; }
+constexpr int stages(int bm, int tiles, int parts) {
+  // two workgroups a CU where three stages each leave room for them
+  const int half = (80 * 1024 - sum_bytes(bm, parts)) / stage_bytes(bm, tiles, parts);
+  return half >= 3 ? std::min(half, 5) : std::max(3, std::min(5, (160 * 1024 - sum_bytes(bm, parts)) / stage_bytes(bm, tiles, parts)));
+}
+
+// WM x 8 / WM waves; a wave multiplies TM tiles of 16 rows of x with TN tiles of 16 weight rows. Everything travels
+// HBM -> LDS directly, into a ring of 3 to 5 stages of 128 k (chunk c of x's row q lies at c ^ (q % 16), so that a
+// fragment read covers every bank); one barrier a step. While a wave multiplies 32 k it reads the next
+// 32 k's fragments of x and makes the next weights.
+// The sums of x (bf16) are made once for all waves, a tile of rows each, a step ahead.
+template <class T, class S, int G, int WM, int TM, int TN>
+__global__ __launch_bounds__(512) void int4_tile_kernel(Int4Params p) {
+  constexpr int kWN = 8 / WM, kBM = 16 * TM * WM, kTiles = kWN * TN;
+  constexpr int kParts = 128 / G, kSteps = 4 / kParts;
+  constexpr int kDepth = stages(kBM, kTiles, kParts), kStage = stage_bytes(kBM, kTiles, kParts);
+  constexpr int kW = kBM * 256, kSc = kW + kTiles * 1024, kZp = kSc + kTiles * 32 * kParts;  // offsets in a stage
+  constexpr int kLoadX = kBM / 32, kLoadW = (kTiles + 7) / 8;   // 1 KiB loads of a wave and stage
+  static_assert(kBM % 32 == 0 && kTiles % 8 == 0, "whole loads a wave");
+  constexpr int kReady = (kDepth - 3) * (kLoadX + kLoadW + 2);  // later stages' loads that may be in flight at a barrier
+  static_assert(kReady < 64, "vmcnt has 6 bits");
+  constexpr int kWait = (kReady & 15) | ((kReady >> 4) << 14) | 0x70;  // vmcnt(kReady) lgkmcnt(0)
+  __shared__ uint4 ring[kDepth * kStage / 16];
+  __shared__ float x_sums[T::kOffset ? 2 * kParts * kBM : 1];
+  const char* lds = reinterpret_cast<const char*>(ring);
+  const uint32_t lds_at = uint32_t(reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) void*)&ring[0]));
+  const int lane = threadIdx.x & 63;
+  const int wave = wave_uniform(threadIdx.x >> 6);
+  const int r = lane & 15, grp = lane >> 4;
+  const int wm = wave % WM, wn = wave / WM;
+  const int z = wave_uniform(int(blockIdx.x) % p.splits), bx = wave_uniform(int(blockIdx.x) / p.splits);
+  const int64_t m0 = int64_t(blockIdx.y) * kBM;
+  const int s0 = wave_uniform(int(int64_t(p.blocks) * z / p.splits));
+  const int steps = wave_uniform(int(int64_t(p.blocks) * (z + 1) / p.splits)) - s0;
+  const int last_tile = p.n_pad / 16 - 1;
+  // tile i of the workgroup; with swiglu a wave's first TN / 2 tiles are gate rows, the others the same columns' up rows
+  const auto tile_of = [&](int i) {
+    const int w = i / TN, j = i % TN;
+    return p.swiglu ? (bx * kWN + w) * (TN / 2) + j % (TN / 2 + (TN == 1)) + (j < TN / 2 ? 0 : p.n / 16) : bx * kTiles + i;
+  };
+
+  // ---- loads: an eighth of x's rows and of the weight tiles; the scales and zero points of those tiles
+  const int x_row_bytes = int(p.x_st) * 2;
+  const char* x_base = reinterpret_cast<const char*>(p.x + m0 * p.x_st) + int64_t(s0) * 256;
+  const int rows = int(min(int64_t(kBM), p.rows - m0));
+  const int x_row = (lane / 16) * x_row_bytes, x_chunk = ((lane % 16) ^ (lane / 16)) * 16;
+  int at[kLoadW];                     // first block of a tile
+#pragma unroll
+  for (int i = 0; i < kLoadW; ++i) at[i] = min(tile_of(wave * kLoadW + i), last_tile) * p.blocks + s0;
+  // lane l takes 16 bytes of the scales of tile l / (2 kParts), of the zero points of tile l / kParts
+  int s_off = 0, z_off = 0;
+#pragma unroll
+  for (int i = 0; i < kLoadW; ++i) {
+    if (lane / (2 * kParts) == i) s_off = at[i] * (32 * kParts) + (lane % (2 * kParts)) * 16;
+    if (lane / kParts == i) z_off = at[i] * (16 * kParts) + (lane % kParts) * 16;
+  }
+  const auto issue = [&](int s) {
+    const uint32_t to = lds_at + uint32_t(s % kDepth) * kStage;
+    const bool real = s < steps;      // past the end: no bytes, so that every stage counts the same loads
+    const int left = (p.k - (s0 + s) * 128) * 2;
+    const u32x4 dx = buffer_desc(x_base + int64_t(s) * 256, real ? (rows - 1) * x_row_bytes + left : 0);
+#pragma unroll
+    for (int i = 0; i < kLoadX; ++i) {
+      const int n = wave * kLoadX + i, chunk = x_chunk ^ ((n & 3) * 64);
+      // k past the end: zeros (an offset past the span), whatever lies behind x's rows
+      load_lds(dx, chunk >= left ? 0x7ffffff0 : n * 4 * x_row_bytes + x_row + chunk, to + n * 1024);
+    }
+#pragma unroll
+    for (int i = 0; i < kLoadW; ++i) {
+      const u32x4 dw = buffer_desc(reinterpret_cast<const char*>(p.w) + int64_t(at[i] + s) * 1024, real ? 1024 : 0);
+      load_lds(dw, lane * 16, to + kW + (wave * kLoadW + i) * 1024);
+    }
+    const int all = p.n_pad / 16 * p.blocks * (16 * kParts);
+    const u32x4 ds = buffer_desc(reinterpret_cast<const char*>(p.scales), real ? 2 * all : 0);
+    const u32x4 dz = buffer_desc(reinterpret_cast<const char*>(p.zeros), real && p.zeros ? all : 0);
+    if (lane < kLoadW * 2 * kParts) load_lds(ds, s_off + s * (32 * kParts), to + kSc + wave * (kLoadW * 32 * kParts));
+    if (lane < kLoadW * kParts) load_lds(dz, z_off + s * (16 * kParts), to + kZp + wave * (kLoadW * 16 * kParts));
+  };
+
+  const f32x4 none = f32x4{0.f, 0.f, 0.f, 0.f};
   f32x4 acc[TM][TN];
 #pragma unroll
   for (int t = 0; t < TM; ++t)
 #pragma unroll
-    for (int j = 0; j < TN; ++j) acc[t][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const f32x4 none = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < TN; ++j) acc[t][j] = none;
+  const int x_at = r * 256 + wm * (TM * 4096);  // this lane's row of the wave's first tile
+  const int c_at = (grp ^ r) * 16;              // its chunk of 32 k number c: c_at ^ (64 c)
+  const auto meet = [&]() {
+    __builtin_amdgcn_s_waitcnt(kWait);
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+  // -192 times the sums of x's rows: each wave makes those of one tile (some twice where there are fewer than 8)
+  const int sum_tile = wave % (TM * WM);
+  const auto sum_chunk = [&](const char* stage, int c) { return *reinterpret_cast<const u32x4*>(stage + sum_tile * 4096 + r * 256 + (c_at ^ (64 * c))); };
+  const auto sum_step = [&](u32x4 x, f32x4 v) { return T::mfma(u32x4{kMinusOffset, kMinusOffset, kMinusOffset, kMinusOffset}, x, v); };
+  const auto sum_at = [&](int s, int g) { return &x_sums[T::kOffset ? ((s & 1) * kParts + g) * kBM : 0]; };
 
-  for (int kb = wave; kb < p.blocks; kb += kWaves) {
-    uint4 w[TN];
-    uint2 sc[TN][kParts];
-    uint32_t zp[TN][kParts];
-#pragma unroll
-    for (int j = 0; j < TN; ++j) {
-      const int at = min(tile[j], last_tile);
-      w[j] = p.w[(int64_t(at) * p.blocks + kb) * 64 + lane];
-#pragma unroll
-      for (int g = 0; g < kParts; ++g) {
-        const int64_t row = (int64_t(kb) * kParts + g) * p.n_pad + at * 16;
-        sc[j][g] = *reinterpret_cast<const uint2*>(p.scales + row + 4 * grp);
-        zp[j][g] = 0x08080808u;
-        if (p.zeros) zp[j][g] = kIsBf16 ? *reinterpret_cast<const uint32_t*>(p.zeros + row + 4 * grp) : p.zeros[row + r];
-      }
-    }
-    u32x4 xs[TM][4];
-#pragma unroll
-    for (int t = 0; t < TM; ++t)
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        xs[t][c] = u32x4{0, 0, 0, 0};
-        const int k = kb * 128 + c * 32;
-        if (live[t] && k < p.k) xs[t][c] = *reinterpret_cast<const u32x4*>(xrow[t] + k);
-      }
+  for (int s = 0; s < kDepth; ++s) issue(s);
+  meet();
+  if (T::kOffset) {
 #pragma unroll
     for (int g = 0; g < kParts; ++g) {
-      f32x4 part[TM][TN], ones[TM];
+      f32x4 v = none;
 #pragma unroll
-      for (int t = 0; t < TM; ++t) {
-        ones[t] = none;
+      for (int c = g * kSteps; c < (g + 1) * kSteps; ++c) v = sum_step(sum_chunk(lds, c), v);
+      if (grp == 0) sum_at(0, g)[sum_tile * 16 + r] = v[0];
+    }
+    __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  }
+
+  uint4 w[TN];
+  uint32_t zp[TN];
+  typename T::Row base[TN];
+  u32x4 xf[TM], a[2][TN];
+  const auto read_w = [&](const char* stage, int j) {
+    w[j] = *reinterpret_cast<const uint4*>(stage + kW + (wn * TN + j) * 1024 + lane * 16);
+    zp[j] = zero_points<kParts>(reinterpret_cast<const uint8_t*>(stage) + kZp + ((wn * TN + j) * 16 + r) * kParts);
+    if (!p.zeros) zp[j] = 0x08080808u;
+  };
+  const auto make_a = [&](int c, int j) {
+    const uint32_t words[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
+    if (c % kSteps == 0) base[j] = T::row((zp[j] >> (8 * (c / kSteps))) & 15u);
+    a[c & 1][j] = T::weights(words[c], base[j]);
+    asm volatile("" : "+v"(a[c & 1][j]));
+  };
+  const auto read_x = [&](const char* stage, int c, int t) {
+    xf[t] = *reinterpret_cast<const u32x4*>(stage + x_at + t * 4096 + (c_at ^ (64 * c)));
+  };
+  uint2 s4[TN];
+  const auto read_scales = [&](const char* stage, int g) {
 #pragma unroll
-        for (int j = 0; j < TN; ++j) part[t][j] = none;
-      }
+    for (int j = 0; j < TN; ++j) s4[j] = *reinterpret_cast<const uint2*>(stage + kSc + (((wn * TN + j) * 4 + grp) * kParts + g) * 8);
+  };
+  constexpr int kSoon = 4;
+  const char* stage = lds;
+  if (kSteps == 1) read_scales(stage, 0);
 #pragma unroll
-      for (int c = g * (4 / kParts); c < (g + 1) * (4 / kParts); ++c) {
-        if (kIsBf16) {
-          constexpr uint32_t one = 0x3f803f80u;
+  for (int j = 0; j < TN; ++j) read_w(stage, j), make_a(0, j);
 #pragma unroll
-          for (int t = 0; t < TM; ++t) ones[t] = T::mfma(u32x4{one, one, one, one}, xs[t][c], ones[t]);
-        }
-#pragma unroll
-        for (int j = 0; j < TN; ++j) {
-          const uint32_t word = c == 0 ? w[j].x : c == 1 ? w[j].y : c == 2 ? w[j].z : w[j].w;
-          u32x4 a = spread<T>(word);
-          if (!kIsBf16) {
-            const uint32_t off = 0x6400u | (zp[j][g] & 15u);
-            const f16x2 z = __builtin_bit_cast(f16x2, off | off << 16);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) a[i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, uint32_t(a[i])) - z);
-          }
-#pragma unroll
-          for (int t = 0; t < TM; ++t) part[t][j] = T::mfma(a, xs[t][c], part[t][j]);
-        }
-      }
+  for (int t = 0; t < TM; ++t) read_x(stage, 0, t);
+  int slot = 0;
+  for (int s = 0; s < steps; ++s) {
+    slot = slot + 1 == kDepth ? 0 : slot + 1;
+    const char* following = lds + slot * kStage;  // landed, too; past the last step its values are not used
+    f32x4 part[TM][TN], sum = none;
+    float sc[TN][4];
+    u32x4 sum_x;
+    const auto take = [&](int t) {     // a finished group of row tile t
 #pragma unroll
       for (int j = 0; j < TN; ++j) {
-        const uint32_t sw[2] = {sc[j][g].x, sc[j][g].y};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float s = scale_of((sw[i / 2] >> (16 * (i & 1))) & 0xffffu, p.scale_fp16);
-          const float z = 128.f + float((zp[j][g] >> (8 * i)) & 0xffu);
-#pragma unroll
-          for (int t = 0; t < TM; ++t)
-            acc[t][j][i] = fmaf(s, kIsBf16 ? fmaf(-z, ones[t][i], part[t][j][i]) : part[t][j][i], acc[t][j][i]);
-        }
+        for (int i = 0; i < 4; ++i) acc[t][j][i] = fmaf(sc[j][i], part[t][j][i], acc[t][j][i]);
+        asm volatile("" : "+v"(acc[t][j]));  // here: pure arithmetic would drift to the loop's end, past every fence
       }
+    };
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const int g = c / kSteps;
+      const bool begins = c % kSteps == 0, ends = c % kSteps == kSteps - 1;
+      float v[TM];                     // read kSoon slices ahead
+      if (begins)
+#pragma unroll
+        for (int t = 0; t < kSoon && t < TM; ++t) v[t] = T::kOffset ? sum_at(s, g)[(wm * TM + t) * 16 + r] : 0.f;
+      // A slice reads a row tile's next fragment and makes its share of the next weights beside a row tile's
+      // products (the fences keep that order: left alone, the compiler makes all weights first, and VALU and matrix cores take turns).
+#pragma unroll
+      for (int t = 0; t < TM; ++t) {
+        if (ends && t == 0)
+#pragma unroll
+          for (int j = 0; j < TN; ++j)
+            sc[j][0] = S::low(s4[j].x), sc[j][1] = S::high(s4[j].x), sc[j][2] = S::low(s4[j].y), sc[j][3] = S::high(s4[j].y);
+#pragma unroll
+        for (int j = t * TN / TM; j < (t + 1) * TN / TM; ++j) {
+          make_a(c < 3 ? c + 1 : 0, j);
+          if (c == 2) read_w(following, j);
+        }
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+          part[t][j] = T::mfma(a[c & 1][j], xf[t], begins ? f32x4{v[t], v[t], v[t], v[t]} : part[t][j]);
+        // (kept in vector registers, where the compiler needs 10 fewer than with part of them in accumulation registers)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) asm volatile("" : "+v"(part[t][j]));
+        if (c < 3) read_x(stage, c + 1, t);
+        else read_x(following, 0, t);
+        if (begins && t + kSoon < TM) v[t + kSoon] = T::kOffset ? sum_at(s, g)[(wm * TM + t + kSoon) * 16 + r] : 0.f;
+        // the scales of a group that ends in the next phase
+        if (t == TM - 1 && (c + 1) % kSteps == kSteps - 1) read_scales(c < 3 ? stage : following, (c + 1) % 4 / kSteps);
+        if (ends && t > 0) take(t - 1);
+        if (T::kOffset && t == (TM > 4 ? 2 : 0)) sum_x = sum_chunk(following, c);
+        if (T::kOffset && t == TM - 1) {
+          sum = sum_step(sum_x, begins ? none : sum);
+          if (ends && grp == 0) sum_at(s + 1, g)[sum_tile * 16 + r] = sum[0];
+        }
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if (ends) take(TM - 1);
     }
+    meet();          // every wave has read this stage, and the next two have landed
+    issue(s + kDepth);
+    stage = following;
   }
+  __builtin_amdgcn_s_waitcnt(0x70);  // vmcnt(0): no load may land after the ring is given up
+  asm volatile("" ::: "memory");
 
 #pragma unroll
-  for (int t = 0; t < TM; ++t)
-#pragma unroll
-    for (int j = 0; j < TN; ++j)
-      sums[wave][t * TN + j][lane] = make_float4(acc[t][j][0], acc[t][j][1], acc[t][j][2], acc[t][j][3]);
-  __syncthreads();
-  constexpr int kOuts = kSwiglu ? TN / 2 : TN;
-  for (int i = wave; i < TM * kOuts; i += kWaves) {
-    const int t = i / kOuts, j = i % kOuts;
-    const auto total = [&](int tj) {
-      float4 v = sums[0][tj][lane];
-#pragma unroll
-      for (int q = 1; q < kWaves; ++q) {
-        const float4 u = sums[q][tj][lane];
-        v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
-      }
-      return v;
-    };
-    float4 v = total(t * TN + j);
-    if (kSwiglu) {
-      const float4 u = total(t * TN + j + TN / 2);
-      v.x = v.x / (1.f + expf(-v.x)) * u.x;
-      v.y = v.y / (1.f + expf(-v.y)) * u.y;
-      v.z = v.z / (1.f + expf(-v.z)) * u.z;
-      v.w = v.w / (1.f + expf(-v.w)) * u.w;
-    }
-    const int64_t m = m0 + t * 16 + r;
-    const int col = tile[j] * 16 + 4 * grp;
+  for (int t = 0; t < TM; ++t) {
+    const int64_t m = m0 + (wm * TM + t) * 16 + r;
     if (m >= p.rows) continue;
-    uint16_t* to = p.out + m * p.o_st + col;
-    const uint16_t o[4] = {T::narrow(v.x), T::narrow(v.y), T::narrow(v.z), T::narrow(v.w)};
-    if (p.wide_out && col + 4 <= p.n) {
-      *reinterpret_cast<uint2*>(to) = make_uint2(o[0] | uint32_t(o[1]) << 16, o[2] | uint32_t(o[3]) << 16);
+    if (p.splits > 1) {
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        const int col = tile_of(wn * TN + j) * 16 + 4 * grp;
+        const f32x4 v = acc[t][j];
+        if (col < p.n_pad)
+          *reinterpret_cast<float4*>(p.partials + (int64_t(z) * p.rows + m) * p.n_pad + col) = make_float4(v[0], v[1], v[2], v[3]);
+      }
+    } else if (p.swiglu) {
+#pragma unroll
+      for (int j = 0; j < TN / 2; ++j) {
+        const f32x4 v = acc[t][j], u = acc[t][j + TN / 2];
+        const float o[4] = {silu(v[0]) * u[0], silu(v[1]) * u[1], silu(v[2]) * u[2], silu(v[3]) * u[3]};
+        const int col = tile_of(wn * TN + j) * 16 + 4 * grp;
+        if (col < p.n) store4<T>(p, m, col, o);
+      }
     } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (col + e < p.n) to[e] = o[e];
+      for (int j = 0; j < TN; ++j) {
+        const float o[4] = {acc[t][j][0], acc[t][j][1], acc[t][j][2], acc[t][j][3]};
+        store4<T>(p, m, tile_of(wn * TN + j) * 16 + 4 * grp, o);
+      }
     }
   }
 }
 
-template <class T, int G, int TM, bool kSwiglu>
-void launch(const Int4Params& p, hipStream_t s) {
-  constexpr int TN = kSwiglu ? 2 : 1, kOuts = kSwiglu ? TN / 2 : TN;
-  const dim3 grid((p.n + 16 * kOuts - 1) / (16 * kOuts), (p.rows + 16 * TM - 1) / (16 * TM));
-  hipLaunchKernelGGL((int4_stream_kernel<T, G, TM, TN, kSwiglu>), grid, dim3(64 * kWaves), 0, s, p);
-}
-
-template <class T, int G>
-void pick(const Int4Params& p, bool swiglu, hipStream_t s) {
-  const auto rows = [&](auto sw) {
-    if (p.rows <= 16) launch<T, G, 1, sw()>(p, s);
-    else if (p.rows <= 32) launch<T, G, 2, sw()>(p, s);
-    else launch<T, G, 4, sw()>(p, s);
+// The sum of the split tiles' slabs, in their order, with the epilogue.
+template <class T>
+__global__ __launch_bounds__(256) void int4_join_kernel(Int4Params p) {
+  const int quads = (p.n + 3) / 4;
+  const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= int64_t(quads) * p.rows) return;
+  const int64_t m = i / quads;
+  const int col = int(i - m * quads) * 4;
+  const auto total = [&](int at) {
+    const float* from = p.partials + m * p.n_pad + at;
+    float4 v = *reinterpret_cast<const float4*>(from);
+    for (int q = 1; q < p.splits; ++q) {
+      const float4 u = *reinterpret_cast<const float4*>(from + int64_t(q) * p.rows * p.n_pad);
+      v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
+    }
+    return v;
   };
-  if (swiglu) rows(std::true_type{});
-  else rows(std::false_type{});
+  const float4 v = total(col);
+  float o[4] = {v.x, v.y, v.z, v.w};
+  if (p.swiglu) {
+    const float4 u = total(p.n + col);
+    const float up[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = silu(o[e]) * up[e];
+  }
+  store4<T>(p, m, col, o);
 }
 
 template <class T>
-void pick_group(const Int4Params& p, int group, bool swiglu, hipStream_t s) {
-  if (group == 32) pick<T, 32>(p, swiglu, s);
-  else if (group == 64) pick<T, 64>(p, swiglu, s);
-  else pick<T, 128>(p, swiglu, s);
+void launch_join(const Int4Params& p, hipStream_t s) {
+  const int64_t quads = int64_t((p.n + 3) / 4) * p.rows;
+  hipLaunchKernelGGL((int4_join_kernel<T>), dim3(unsigned((quads + 255) / 256)), dim3(256), 0, s, p);
 }
+
+template <class T, class S, int G>
+void launch_stream(const Int4Params& p, hipStream_t s) {
+  const int tiles = p.swiglu ? p.n / 16 : p.splits > 1 ? p.n_pad / 16 : (p.n + 15) / 16;
+  // two workgroups a CU at most; the second ones take what is over of an uneven number of tiles
+  hipLaunchKernelGGL((int4_stream_kernel<T, S, G>), dim3(std::min(tiles, std::max(1, 512 / p.splits)), p.splits), dim3(64 * kWaves), 0, s, p);
+}
+
+template <class T, class S, int G, int WM, int TM, int TN>
+void launch_tile(const Int4Params& p, hipStream_t s) {
+  const int cols = 16 * (8 / WM) * TN / (p.swiglu ? 2 : 1), width = p.splits > 1 ? p.n_pad : p.n, rows = 16 * WM * TM;
+  const dim3 grid((width + cols - 1) / cols * p.splits, (p.rows + rows - 1) / rows);
+  hipLaunchKernelGGL((int4_tile_kernel<T, S, G, WM, TM, TN>), grid, dim3(512), 0, s, p);
+}
+
+// Rows and columns of a workgroup's tile, and the splits of k; 0 rows: the stream kernel.
+struct Shape {
+  int rows, cols, splits;
+};
+
+// The stream kernel up to 16 rows, its splits as many blocks as its waves hold. Above, the shortest of the tiles and splits
+// by what the kernel's parts measured: 2 us to fill the ring and store, the steps, and the slabs' join, in whole
+// rounds of one workgroup a CU. Steps of a 128-wide group in us (groups of 32: a third more):
+//   32 x 128 0.75, 32 x 256 1.05, 64 x 128 1.0, 64 x 256 1.35, 128 x 128 1.4, 128 x 256 2.05.
+// us it chooses between: 33 x 4,096 x 12,288 (128 columns in 1 / 2 / 4 / 8 splits) 91 / 51 / 30 / 22, in 256 118 / 64 / 37 / 26;
+// 208 x 24,576 x 4,096 91 / 90 / 110 / 150, 71 / 84 / 90 / 127; 2,048 x 6,144 x 4,096 147 and 139.
+Shape choose(int rows, int n_pad, int blocks, int group, bool swiglu) {
+  if (rows <= 16) return Shape{0, 0, (blocks + kAhead * kWaves - 1) / (kAhead * kWaves)};
+  const int bm = rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
+  const double mblocks = (rows + bm - 1) / bm;
+  Shape best{bm, 128, 1};
+  double least = 1e30;
+  for (int bn = 128; bn <= 256; bn += 128) {
+    // 128 columns are one tile a wave up to 64 rows: gate and up tiles do not pair there, but in the join
+    const int from = swiglu && bn == 128 && bm <= 64 ? 2 : 1;
+    const double step = (bm == 32 ? 0.45 : bm == 64 ? 0.65 : 0.75) + (bm == 32 ? 0.3 : bm == 64 ? 0.35 : 0.65) * (bn / 128);
+    for (int s = from; s <= std::max(from, std::min(16, blocks / 2)); ++s) {
+      const double rounds = std::ceil(mblocks * ((n_pad + bn - 1) / bn) * s / 256);
+      const double join = s > 1 ? 2.5 + double(s) * rows * n_pad * 8 / 4e6 : 0;
+      const double cost = rounds * (2 + std::ceil(double(blocks) / s) * step * (group == 32 ? 1.33 : 1.0)) + join;
+      if (cost < least) {
+        least = cost;
+        best = Shape{bm, bn, s};
+      }
+    }
+  }
+  return best;
+}
+
+template <class T, class S, int G>
+void pick(const Int4Params& p, const Shape& f, hipStream_t s) {
+  if (f.rows == 0) return launch_stream<T, S, G>(p, s);
+  const bool wide = f.cols == 256;
+  if (f.rows == 32) return wide ? launch_tile<T, S, G, 1, 2, 2>(p, s) : launch_tile<T, S, G, 1, 2, 1>(p, s);
+  if (f.rows == 64) return wide ? launch_tile<T, S, G, 1, 4, 2>(p, s) : launch_tile<T, S, G, 1, 4, 1>(p, s);
+  return wide ? launch_tile<T, S, G, 1, 8, 2>(p, s) : launch_tile<T, S, G, 2, 4, 2>(p, s);
+}
+
+template <class T, class S>
+void pick_group(const Int4Params& p, int group, const Shape& f, hipStream_t s) {
+  if (group == 32) pick<T, S, 32>(p, f, s);
+  else if (group == 64) pick<T, S, 64>(p, f, s);
+  else pick<T, S, 128>(p, f, s);
+}
+
+int64_t partial_floats(const Shape& f, int rows, int n_pad) { return f.splits > 1 ? int64_t(f.splits) * rows * n_pad : 0; }
 
 inline bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 
 }  // namespace
 }  // namespace aspire
 
+extern "C" int64_t aspire_linear_int4_workspace(int32_t rows, int32_t n, int32_t k, int32_t group, int32_t swiglu) {
+  using namespace aspire;
+  if (rows <= 0 || n <= 0 || k <= 0 || n > (1 << 30)) return 0;
+  const int n_pad = (n + 15) / 16 * 16;
+  return partial_floats(choose(rows, n_pad, (k + 127) / 128, group, swiglu != 0), rows, n_pad);
+}
+
 extern "C" int aspire_linear_int4(const aspire_int4_args* a, void* stream) {
   using namespace aspire;
   ASPIRE_CHECK_ARG(a != nullptr, "null arguments");
-  ASPIRE_CHECK_ARG(a->rows >= 0 && a->n >= 0 && a->k > 0, "bad sizes");
+  ASPIRE_CHECK_ARG(a->rows >= 0 && a->n >= 0 && a->n <= (1 << 30) && a->k > 0 && a->k < (1 << 22), "bad sizes");
+  ASPIRE_CHECK_ARG((int64_t(a->n) + 15) / 16 * ((a->k + 127) / 128) < (1 << 23), "weights of 2^34 values or more");
   ASPIRE_CHECK_ARG(a->rows <= (1 << 22) - 64, "at most 4,194,240 rows");
   ASPIRE_CHECK_ARG(a->group == 32 || a->group == 64 || a->group == 128, "groups of 32, 64 or 128");
   ASPIRE_CHECK_ARG(a->k % a->group == 0, "k must be a multiple of the group");
   ASPIRE_CHECK_ARG(!a->swiglu || a->n % 32 == 0, "swiglu needs whole 16-row tiles of gate and up rows");
   if (a->rows == 0 || a->n == 0) return ASPIRE_OK;
   ASPIRE_CHECK_ARG(a->x && a->weights && a->scales && a->out, "null pointer");
-  ASPIRE_CHECK_ARG(aligned(a->x, 16) && a->x_stride % 8 == 0 && a->x_stride >= a->k, "x rows must be 16-byte aligned");
+  ASPIRE_CHECK_ARG(aligned(a->x, 16) && a->x_stride % 8 == 0 && a->x_stride >= a->k && a->x_stride < (1 << 22),
+                   "x rows must be 16-byte aligned, of less than 2^22 elements");
   ASPIRE_CHECK_ARG(aligned(a->weights, 16) && aligned(a->scales, 16) && aligned(a->zeros, 16),
                    "weights, scales and zeros must be 16-byte aligned");
   const int outs = a->swiglu ? a->n / 2 : a->n;
@@ -260,7 +604,7 @@ extern "C" int aspire_linear_int4(const aspire_int4_args* a, void* stream) {
   p.x = static_cast<const uint16_t*>(a->x);
   p.x_st = a->x_stride;
   p.w = static_cast<const uint4*>(a->weights);
-  p.scales = static_cast<const uint16_t*>(a->scales);
+  p.scales = static_cast<const uint8_t*>(a->scales);
   p.zeros = static_cast<const uint8_t*>(a->zeros);
   p.out = static_cast<uint16_t*>(a->out);
   p.o_st = a->out_stride;
@@ -269,12 +613,24 @@ extern "C" int aspire_linear_int4(const aspire_int4_args* a, void* stream) {
   p.n_pad = (a->n + 15) / 16 * 16;
   p.k = a->k;
   p.blocks = (a->k + 127) / 128;
-  p.up_tile = outs / 16;
-  p.scale_fp16 = a->scales_fp16;
+  p.swiglu = a->swiglu != 0;
   p.wide_out = aligned(a->out, 8) && a->out_stride % 4 == 0;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (a->fp16) pick_group<Fp16>(p, a->group, a->swiglu != 0, s);
-  else pick_group<Bf16>(p, a->group, a->swiglu != 0, s);
+  const Shape f = choose(p.rows, p.n_pad, p.blocks, a->group, a->swiglu != 0);
+  p.splits = f.splits;
+  p.partials = static_cast<float*>(a->workspace);
+  ASPIRE_CHECK_ARG(f.splits == 1 || (a->workspace && aligned(a->workspace, 16) && a->workspace_floats >= partial_floats(f, p.rows, p.n_pad)),
+                   "workspace must be 16-byte aligned and hold aspire_linear_int4_workspace floats");
+  if (f.splits > 1) p.swiglu = 0;  // slabs hold gate and up columns; the join pairs them
+  if (a->fp16 && a->scales_fp16) pick_group<Fp16, Fp16>(p, a->group, f, s);
+  else if (a->fp16) pick_group<Fp16, Bf16>(p, a->group, f, s);
+  else if (a->scales_fp16) pick_group<Bf16, Fp16>(p, a->group, f, s);
+  else pick_group<Bf16, Bf16>(p, a->group, f, s);
+  if (f.splits > 1) {
+    p.swiglu = a->swiglu != 0;
+    if (a->fp16) launch_join<Fp16>(p, s);
+    else launch_join<Bf16>(p, s);
+  }
   ASPIRE_CHECK_LAUNCH();
   return ASPIRE_OK;
 }

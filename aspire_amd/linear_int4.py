@@ -64,9 +64,12 @@ class Int4Weight:
         codes[..., 1] = lo[..., 2] | (lo[..., 3] << 4)
         codes[..., 2] = hi[..., 0] | (hi[..., 1] << 4)
         codes[..., 3] = hi[..., 2] | (hi[..., 3] << 4)
-        groups = blocks * 128 // group
-        flat = lambda t: None if t is None else fill(t, tiles * 16, groups).t().contiguous()
-        return cls((n, k), group, codes.view(tiles, blocks, 64, 16), flat(scales), flat(zeros))
+        parts = 128 // group
+        # [tile, row, block, group of it] -> [tile, block, row / 4, group, row % 4] and [tile, block, row, group]
+        scales = fill(scales, tiles * 16, blocks * parts).view(tiles, 4, 4, blocks, parts).permute(0, 3, 1, 4, 2).contiguous()
+        if zeros is not None:
+            zeros = fill(zeros, tiles * 16, blocks * parts).view(tiles, 16, blocks, parts).transpose(1, 2).contiguous()
+        return cls((n, k), group, codes.view(tiles, blocks, 64, 16), scales, zeros)
 
     @classmethod
     def quantize(cls, w: torch.Tensor, *, group: int = 128, symmetric: bool = False) -> "Int4Weight":
@@ -107,8 +110,9 @@ class Int4Weight:
         nib = torch.stack([c & 15, c >> 4], dim=-1).flatten(-2)              # places 0 .. 7 of a word
         nib = nib[..., [0, 4, 1, 5, 2, 6, 3, 7]]                              # in k's order
         codes = nib.permute(0, 3, 1, 4, 2, 5).reshape(tiles * 16, blocks * 128)
-        spread = lambda t: t.t().float().repeat_interleave(self.group, dim=1)
-        w = (codes.float() - (8.0 if self.zeros is None else spread(self.zeros))) * spread(self.scales)
+        spread = lambda t: t.reshape(tiles * 16, -1).float().repeat_interleave(self.group, dim=1)
+        zeros = 8.0 if self.zeros is None else spread(self.zeros.transpose(1, 2))
+        w = (codes.float() - zeros) * spread(self.scales.permute(0, 2, 4, 1, 3))
         return w[:n, :k].to(dtype)
 
 
@@ -130,12 +134,17 @@ def linear_int4(x: torch.Tensor, w: Int4Weight, out: torch.Tensor, *, swiglu: bo
         raise ValueError(f"{what}: x, out and the weights must be on one device")
     if torch.is_grad_enabled() and x.requires_grad:
         raise ValueError(f"{what}: not differentiable")
+    L = _lib.lib()
+    floats = L.aspire_linear_int4_workspace(x.shape[0], n, k, w.group, int(swiglu))
     a = _lib.Int4Args(x=x.data_ptr(), x_stride=x.stride(0), weights=w.codes.data_ptr(), scales=w.scales.data_ptr(),
                       zeros=_lib.ptr(w.zeros), out=out.data_ptr(), out_stride=out.stride(0), rows=x.shape[0], n=n, k=k,
                       group=w.group, swiglu=int(swiglu), fp16=int(x.dtype == torch.float16),
                       scales_fp16=int(w.scales.dtype == torch.float16))
+    if floats:
+        ws = torch.empty(floats, dtype=torch.float32, device=x.device)
+        a.workspace, a.workspace_floats = ws.data_ptr(), floats
     with _on(w.device):
-        _lib.check(_lib.lib().aspire_linear_int4(ctypes.byref(a), _lib.stream_of(x)), what)
+        _lib.check(L.aspire_linear_int4(ctypes.byref(a), _lib.stream_of(x)), what)
     return out
 
 

@@ -503,9 +503,10 @@ int aspire_linear_partials(const void* x, int64_t x_stride, const void* w, int64
  * exact weights, fp32 sums, one rounding to x's type (bf16, or fp16 with fp16 set). With swiglu, n counts n / 2 gate
  * rows, then n / 2 up rows, and out[m, :n / 2] = silu(gate) * up, rounded once.
  * weights: blocks of 16 rows x 128 k in 1 KiB, [n / 16, up][k / 128, up][64][4] words: word c of lane l holds row
- * l % 16, k 32 c + 8 (l / 16) + e in bits 4 (e / 2) + 16 (e % 2), e = 0 .. 7. scales ([k / group][n up to a multiple
- * of 16], bf16 or fp16) and zeros (the same in bytes, 0 .. 15, NULL: 8) cover whole blocks: their groups past k and rows past n are
- * there and 0. group 32, 64 or 128, k a multiple of it; 16-byte aligned x rows; out rows of any stride. */
+ * l % 16, k 32 c + 8 (l / 16) + e in bits 4 (e / 2) + 16 (e % 2), e = 0 .. 7. For each block, scales (bf16 or fp16) are
+ * [4][128 / group][4], row 4 a + b of the tile and group g at [a][g][b], and zeros (bytes of 0 .. 15, NULL: 8) [16][128 / group].
+ * Codes and scales of rows past n and columns past k are there and 0. group 32, 64 or 128, k a multiple of it; 16-byte aligned
+ * x rows; out rows of any stride, apart from x. */
 typedef struct aspire_int4_args {
   const void* x;
   int64_t x_stride;
@@ -515,7 +516,12 @@ typedef struct aspire_int4_args {
   void* out;
   int64_t out_stride;
   int32_t rows, n, k, group, swiglu, fp16, scales_fp16;
+  float* workspace;             /* 16-byte aligned */
+  int64_t workspace_floats;
 } aspire_int4_args;
+
+/* Floats of workspace that a product needs (0: none): partial sums of k splits, until the call's launches have run. */
+int64_t aspire_linear_int4_workspace(int32_t rows, int32_t n, int32_t k, int32_t group, int32_t swiglu);
 
 int aspire_linear_int4(const aspire_int4_args* args, void* stream);
 

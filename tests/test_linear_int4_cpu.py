@@ -26,14 +26,20 @@ def test_layout_is_the_documented_one(n, k, group, zeros):
                     for e in range(8):
                         got = words[t][b][l][c] >> (4 * (e // 2) + 16 * (e % 2)) & 15
                         assert got == code(16 * t + l % 16, 128 * b + 32 * c + 8 * (l // 16) + e)
-    full = torch.zeros(blocks * 128 // group, tiles * 16, dtype=torch.float16)
-    full[: k // group, :n] = scales.t()
-    assert torch.equal(w.scales, full)
+    parts = 128 // group
+    assert w.scales.shape == (tiles, blocks, 4, parts, 4) and w.scales.is_contiguous()
+    for t in range(tiles):
+        for b in range(blocks):
+            for row in range(16):
+                for g in range(parts):
+                    inside = 16 * t + row < n and b * parts + g < k // group
+                    want = scales[16 * t + row, b * parts + g] if inside else 0
+                    assert w.scales[t, b, row // 4, g, row % 4] == want
+                    if zeros and inside:
+                        assert w.zeros[t, b, row, g] == z[16 * t + row, b * parts + g]
     c = torch.stack([packed & 15, packed >> 4], dim=-1).view(n, k).float()
     spread = lambda t: t.float().repeat_interleave(group, dim=1)
     assert torch.equal(w.dequantize(), (c - (spread(z) if zeros else 8)) * spread(scales))
-    if zeros:
-        assert torch.equal(w.zeros[: k // group, :n], z.t())
 
 
 @pytest.mark.parametrize("change", [
@@ -66,7 +72,7 @@ def test_entry_point_refuses_on_the_host():
             setattr(a, name, value)
         return L.aspire_linear_int4(ctypes.byref(a), None)
 
-    for kw in (dict(rows=-1), dict(rows=1 << 22), dict(n=-1), dict(k=0), dict(k=250), dict(group=16), dict(group=0), dict(x=None),
+    for kw in (dict(rows=-1), dict(rows=1 << 22), dict(n=-1), dict(k=0), dict(k=250), dict(k=1 << 22, x_stride=1 << 22), dict(x_stride=1 << 22), dict(group=16), dict(group=0), dict(x=None),
                dict(weights=None), dict(scales=None), dict(out=None), dict(x=4104), dict(x_stride=260), dict(x_stride=248),
                dict(out_stride=63), dict(n=48, swiglu=1), dict(scales=4100), dict(zeros=4097)):
         assert call(**kw) == _lib.ASPIRE_ERR_INVALID, kw
