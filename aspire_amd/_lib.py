@@ -269,10 +269,11 @@ def _declare(lib):
         "aspire_linear_splits": [i32, i32, i32],
         "aspire_linear_partials": [vp, i64, vp, i64, vp, i64, i32, i32, i32, vp],
         "aspire_add_rms_norm_partials": [vp, i64, vp, i32, vp, vp, i64, i32, i32, f32, vp],
-        "aspire_linear_int4": [ctypes.POINTER(Int4Args), vp],
+        # the address of the arguments, or the structure's bytes
+        "aspire_linear_int4": [vp, vp],
         "aspire_linear_int4_workspace": [i32, i32, i32, i32, i32],
-        "aspire_rotary": [ctypes.POINTER(RotaryArgs), vp],
-        "aspire_rotary_append": [ctypes.POINTER(RotaryArgs), vp],
+        "aspire_rotary": [vp, vp],
+        "aspire_rotary_append": [vp, vp],
         "aspire_bandwidth_probe": [i32, vp, i64, vp, i64, i32, i32, vp],
     }
     for name, argtypes in sigs.items():

@@ -18,9 +18,8 @@
 
 from __future__ import annotations
 
-import contextlib
-import ctypes
 import math
+import struct
 from dataclasses import dataclass
 
 import torch
@@ -118,11 +117,13 @@ def _same_place(a: torch.Tensor, b: torch.Tensor) -> bool:
     return a.data_ptr() != b.data_ptr() or all(n == 1 or x == y for n, x, y in zip(a.shape, a.stride(), b.stride()))
 
 
-def _on(device: torch.device):
-    """The tensors' device as the current one for a launch."""
-    if device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+# aspire_rotary_args as one packed string: filling a ctypes structure field by field takes longer than the launch.
+# q .. v (pointer and strides), eight counts, turns, amplitude, positions; then the cache, its strides and lists.
+_HEAD = struct.Struct("PqqPqqPqqPqqPqq8iPfiP")
+_ARGS = struct.Struct(_HEAD.format + "P4q2q2i4P")
+_NO_CACHE = bytes(_ARGS.size - _HEAD.size)
+_NONE = (0, 0, 0)
+_INTS = (torch.int32, torch.int64)
 
 
 class RotaryEmbedding:
@@ -132,79 +133,87 @@ class RotaryEmbedding:
         self.config = config
         self.turns = _turns(config.frequencies()).to(device)
         self.device = self.turns.device
-        self._args = dict(head_dim=config.head_dim, rotary_dim=config.rotated,
-                          interleaved=int(config.layout == "interleaved"), amplitude=config.scale,
-                          turns=self.turns.data_ptr())
+        self._index = self.turns.get_device()
+        self._dims = (config.head_dim, config.rotated, int(config.layout == "interleaved"))
+        self._tail = (self.turns.data_ptr(), config.scale)
 
     # ------------------------------------------------------------------ checks
-    def _check(self, what: str, **tensors) -> torch.dtype:
-        _lib.require_cuda(*tensors.values(), what=what)
-        dtype = next(t.dtype for t in tensors.values() if t is not None)
-        if dtype not in _DTYPES:
+    def _heads(self, t: torch.Tensor, dtype: torch.dtype, what: str, name: str):
+        """A head tensor's (tokens, heads), address and strides, after its checks."""
+        if not t.is_cuda:
+            _lib.require_cuda(t, what=what)
+        if t.get_device() != self._index:
+            raise ValueError(f"{what}: {name} is on {t.device}, the frequencies on {self.device}")
+        shape, strides = t.shape, t.stride()
+        if t.dtype is not dtype or len(shape) != 3 or shape[2] != self._dims[0]:
+            raise ValueError(f"{what}: {name} must be {dtype} [T, H, {self._dims[0]}]")
+        if strides[2] != 1 and t.numel():
+            raise ValueError(f"{what}: {name} must have contiguous head dims")
+        return shape, (t.data_ptr(), strides[0], strides[1])
+
+    def _dtype(self, t: torch.Tensor, what: str) -> int:
+        code = _DTYPES.get(t.dtype)
+        if code is None:
             raise ValueError(f"{what}: bf16, fp16 or fp32 tensors")
-        for name, t in tensors.items():
-            if t is None:
-                continue
-            if t.device != self.device:
-                raise ValueError(f"{what}: {name} is on {t.device}, the frequencies on {self.device}")
-            if t.dtype != dtype or t.dim() != 3 or t.shape[2] != self.config.head_dim:
-                raise ValueError(f"{what}: {name} must be {dtype} [T, H, {self.config.head_dim}]")
-            if t.stride(2) != 1 and t.numel():
-                raise ValueError(f"{what}: {name} must have contiguous head dims")
-        return dtype
+        return code
 
     def _positions(self, positions: torch.Tensor, tokens: int, what: str) -> torch.Tensor:
-        if positions.dim() != 1 or positions.shape[0] != tokens or positions.dtype not in (torch.int32, torch.int64):
+        if positions.dtype not in _INTS or positions.dim() != 1 or positions.shape[0] != tokens:
             raise ValueError(f"{what}: positions must be int32 or int64 [T]")
-        if positions.device != self.device:
+        if positions.get_device() != self._index:
             raise ValueError(f"{what}: positions are on {positions.device}, the frequencies on {self.device}")
         return positions if positions.stride(0) == 1 else positions.contiguous()
 
-    def _fill(self, dtype, tokens, inverse=False, positions=None) -> _lib.RotaryArgs:
-        a = _lib.RotaryArgs(total_tokens=tokens, dtype=_DTYPES[dtype], inverse=int(inverse), **self._args)
-        if positions is not None:
-            a.positions, a.positions_64 = positions.data_ptr(), int(positions.dtype == torch.int64)
-        return a
+    def _launch(self, entry, args: bytes, what: str) -> None:
+        stream = torch._C._cuda_getCurrentRawStream(self._index)
+        if torch._C._cuda_getDevice() == self._index:
+            rc = entry(args, stream)
+        else:
+            with torch.cuda.device(self._index):
+                rc = entry(args, stream)
+        if rc:
+            _lib.check(rc, what)
 
-    def _turn(self, q, k, q_out, k_out, positions, inverse, what) -> None:
+    def _turn(self, q, k, positions, inverse, in_place, what):
+        """q and k (either may be None) turned, in place or into new tensors, which it returns."""
         first = q if q is not None else k
-        tokens = first.shape[0]
-        if k is not None and k.shape[0] != tokens:
-            raise ValueError(f"{what}: q and k must have the same number of tokens")
-        positions = self._positions(positions, tokens, what)
-        a = self._fill(first.dtype, tokens, inverse, positions)
+        code, dtype = self._dtype(first, what), first.dtype
+        tokens, hq, hkv, qa, ka, qo, ko = first.shape[0], 0, 0, _NONE, _NONE, _NONE, _NONE
+        q_out, k_out = q, k
         if q is not None:
-            a.q, a.q_stride_t, a.q_stride_h, a.num_qo_heads = q.data_ptr(), q.stride(0), q.stride(1), q.shape[1]
-            a.q_out, a.q_out_stride_t, a.q_out_stride_h = q_out.data_ptr(), q_out.stride(0), q_out.stride(1)
+            shape, qa = self._heads(q, dtype, what, "q")
+            hq, qo = shape[1], qa
+            if not in_place:
+                q_out = q.new_empty(shape)
+                qo = (q_out.data_ptr(), hq * shape[2], shape[2])
         if k is not None:
-            a.k, a.k_stride_t, a.k_stride_h, a.num_kv_heads = k.data_ptr(), k.stride(0), k.stride(1), k.shape[1]
-            a.k_out, a.k_out_stride_t, a.k_out_stride_h = k_out.data_ptr(), k_out.stride(0), k_out.stride(1)
-        with _on(self.device):
-            _lib.check(_lib.lib().aspire_rotary(ctypes.byref(a), _lib.stream_of(first)), what)
+            shape, ka = self._heads(k, dtype, what, "k")
+            if shape[0] != tokens:
+                raise ValueError(f"{what}: q and k must have the same number of tokens")
+            hkv, ko = shape[1], ka
+            if not in_place:
+                k_out = k.new_empty(shape)
+                ko = (k_out.data_ptr(), hkv * shape[2], shape[2])
+        positions = self._positions(positions, tokens, what)
+        args = _HEAD.pack(*qa, *qo, *ka, *ko, *_NONE, hq, hkv, tokens, *self._dims, code, inverse, *self._tail,
+                          positions.dtype is torch.int64, positions.data_ptr()) + _NO_CACHE
+        self._launch(_lib.lib().aspire_rotary, args, what)
+        return q_out, k_out
 
     # -------------------------------------------------------------- operators
     def apply(self, q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor):
         """``(q, k)`` turned at ``positions`` ``[T]``, as new tensors (``k`` may be None); differentiable. Tokens at
         negative positions are copied."""
-        what = "RotaryEmbedding.apply"
-        self._check(what, q=q, k=k)
         if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-            out = _Turn.apply(q, k, positions, self, False)
-            return out if k is not None else (out[0], None)
-        return self._new(q, k, positions, False, what)
-
-    def _new(self, q, k, positions, inverse, what):
-        q_out, k_out = (None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k))
-        self._turn(q, k, q_out, k_out, positions, inverse, what)
-        return q_out, k_out
+            return _Turn.apply(q, k, positions, self, False)
+        return self._turn(q, k, positions, False, False, "RotaryEmbedding.apply")
 
     def apply_inplace(self, q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor) -> None:
         """``apply`` on q and k themselves (not differentiable; no two of their rows may share memory)."""
         what = "RotaryEmbedding.apply_inplace"
-        self._check(what, q=q, k=k)
         if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
             raise ValueError(f"{what}: not differentiable; use apply")
-        self._turn(q, k, q, k, positions, False, what)
+        self._turn(q, k, positions, False, True, what)
 
     def append(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_append_indptr: torch.Tensor,
                kv_cache: torch.Tensor, kv_page_indices: torch.Tensor, kv_page_indptr: torch.Tensor,
@@ -216,41 +225,48 @@ class RotaryEmbedding:
         padding: their q passes unchanged, and nothing is written to the cache; nor is it for a token whose
         page id or list entry lies outside the pool or the list."""
         what = "RotaryEmbedding.append"
-        dtype = self._check(what, q=q, k=k, v=v, q_out=q_out)
-        q_out = q if q_out is None else q_out
-        tokens = q.shape[0]
+        code, dtype = self._dtype(q, what), q.dtype
+        if code == 2:
+            raise ValueError(f"{what}: the cache holds bf16 or fp16")
+        shape, qa = self._heads(q, dtype, what, "q")
+        kv_shape, ka = self._heads(k, dtype, what, "k")
+        v_shape, va = self._heads(v, dtype, what, "v")
+        tokens, hkv = shape[0], kv_shape[1]
         if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
             raise ValueError(f"{what}: not differentiable")
-        if dtype == torch.float32:
-            raise ValueError(f"{what}: the cache holds bf16 or fp16")
-        if k.shape[0] != tokens or v.shape != k.shape or q_out.shape != q.shape:
-            raise ValueError(f"{what}: q, k and v must have the same tokens, k and v the same heads, q_out q's shape")
-        if not _same_place(q, q_out):
-            raise ValueError(f"{what}: q_out must be q itself or apart from it")
-        if kv_cache.device != self.device or kv_cache.dtype != dtype or kv_cache.dim() != 5 \
-                or tuple(kv_cache.shape[1:]) != (2, page_size, k.shape[1], self.config.head_dim) or kv_cache.stride(4) != 1:
-            raise ValueError(f"{what}: kv_cache must be {dtype} [P, 2, {page_size}, {k.shape[1]}, "
-                             f"{self.config.head_dim}] with contiguous head dims")
-        lists = (kv_append_indptr, kv_page_indices, kv_page_indptr, kv_last_page_len)
-        if any(t.device != self.device or t.dim() != 1 or t.dtype not in (torch.int32, torch.int64) for t in lists):
-            raise ValueError(f"{what}: the index arrays must be 1-D int32 on {self.device}")
-        num_seq = kv_last_page_len.shape[0]
-        if kv_append_indptr.shape[0] < num_seq + 1 or kv_page_indptr.shape[0] < num_seq + 1:
+        qo = qa
+        if q_out is None:
+            q_out = q
+        elif q_out is not q:
+            out_shape, qo = self._heads(q_out, dtype, what, "q_out")
+            if out_shape != shape:
+                raise ValueError(f"{what}: q_out must have q's shape")
+            if not _same_place(q, q_out):
+                raise ValueError(f"{what}: q_out must be q itself or apart from it")
+        if kv_shape[0] != tokens or v_shape != kv_shape:
+            raise ValueError(f"{what}: q, k and v must have the same tokens, k and v the same heads")
+        cache_shape, cs = kv_cache.shape, kv_cache.stride()
+        if kv_cache.get_device() != self._index or kv_cache.dtype is not dtype \
+                or cache_shape[1:] != (2, page_size, hkv, self._dims[0]) or cs[4] != 1:
+            raise ValueError(f"{what}: kv_cache must be {dtype} [P, 2, {page_size}, {hkv}, {self._dims[0]}] on "
+                             f"{self.device} with contiguous head dims")
+        ind, pages, ptr, last = kv_append_indptr, kv_page_indices, kv_page_indptr, kv_last_page_len
+        for t in (ind, pages, ptr, last):
+            if t.dtype not in _INTS or t.dim() != 1 or t.get_device() != self._index:
+                raise ValueError(f"{what}: the index arrays must be 1-D int32 on {self.device}")
+        num_seq = last.shape[0]
+        if ind.shape[0] <= num_seq or ptr.shape[0] <= num_seq:
             raise ValueError(f"{what}: kv_page_indptr and kv_append_indptr need len(kv_last_page_len) + 1 entries")
+        ind, pages, ptr, last = (_lib.dense(ind, torch.int32), _lib.dense(pages, torch.int32),
+                                 _lib.dense(ptr, torch.int32), _lib.dense(last, torch.int32))
+        at, wide = 0, False
         if positions is not None:
             positions = self._positions(positions, tokens, what)
-        ind, pages, ptr, last = (_lib.dense(t, torch.int32) for t in lists)
-        a = self._fill(dtype, tokens, False, positions)
-        a.q, a.q_stride_t, a.q_stride_h, a.num_qo_heads = q.data_ptr(), q.stride(0), q.stride(1), q.shape[1]
-        a.q_out, a.q_out_stride_t, a.q_out_stride_h = q_out.data_ptr(), q_out.stride(0), q_out.stride(1)
-        a.k, a.k_stride_t, a.k_stride_h, a.num_kv_heads = k.data_ptr(), k.stride(0), k.stride(1), k.shape[1]
-        a.v, a.v_stride_t, a.v_stride_h = v.data_ptr(), v.stride(0), v.stride(1)
-        a.kv_cache, a.num_pages, a.page_size, a.num_seq = kv_cache.data_ptr(), kv_cache.shape[0], page_size, num_seq
-        a.cache_stride_p, a.cache_stride_kv, a.cache_stride_t, a.cache_stride_h = kv_cache.stride()[:4]
-        a.append_indptr, a.kv_page_indices, a.num_page_indices = ind.data_ptr(), pages.data_ptr(), pages.shape[0]
-        a.kv_page_indptr, a.kv_last_page_len = ptr.data_ptr(), last.data_ptr()
-        with _on(self.device):
-            _lib.check(_lib.lib().aspire_rotary_append(ctypes.byref(a), _lib.stream_of(q)), what)
+            at, wide = positions.data_ptr(), positions.dtype is torch.int64
+        args = _ARGS.pack(*qa, *qo, *ka, *_NONE, *va, shape[1], hkv, tokens, *self._dims, code, 0, *self._tail, wide, at,
+                          kv_cache.data_ptr(), cs[0], cs[1], cs[2], cs[3], cache_shape[0], pages.shape[0], page_size,
+                          num_seq, ind.data_ptr(), pages.data_ptr(), ptr.data_ptr(), last.data_ptr())
+        self._launch(_lib.lib().aspire_rotary_append, args, what)
         return q_out
 
 
@@ -262,15 +278,21 @@ class _Turn(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(positions)
         ctx.rotary, ctx.inverse = rotary, inverse
-        return rotary._new(q, k, positions, inverse, "RotaryEmbedding.apply")
+        return rotary._turn(q, k, positions, inverse, False, "RotaryEmbedding.apply")
 
     @staticmethod
     def backward(ctx, dq, dk):
         (positions,) = ctx.saved_tensors
         if dq is None and dk is None:
             return None, None, None, None, None
-        dq, dk = (t if t is None or t.stride(2) == 1 else t.contiguous() for t in (dq, dk))
-        gq, gk = _Turn.apply(dq, dk, positions, ctx.rotary, not ctx.inverse)
+        if dq is not None and dq.stride(2) != 1:
+            dq = dq.contiguous()
+        if dk is not None and dk.stride(2) != 1:
+            dk = dk.contiguous()
+        if torch.is_grad_enabled():  # a second derivative is wanted
+            gq, gk = _Turn.apply(dq, dk, positions, ctx.rotary, not ctx.inverse)
+        else:
+            gq, gk = ctx.rotary._turn(dq, dk, positions, not ctx.inverse, False, "RotaryEmbedding.apply")
         return gq, gk, None, None, None
 
 

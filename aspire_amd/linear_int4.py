@@ -11,14 +11,14 @@ multiplied exactly, sums are fp32, and the output is rounded once. Any number of
 
 from __future__ import annotations
 
-import ctypes
+import struct
 
 import torch
 
 from aspire_amd import _lib
-from aspire_amd.attention.rotary import _on
 
 GROUPS = (32, 64, 128)
+_TYPES = (torch.bfloat16, torch.float16)
 
 
 class Int4Weight:
@@ -27,6 +27,8 @@ class Int4Weight:
     def __init__(self, shape, group, codes, scales, zeros):
         self.shape, self.group = tuple(shape), group
         self.codes, self.scales, self.zeros = codes, scales, zeros  # see aspire_hip.h for the layouts
+        self._addresses = (codes.data_ptr(), scales.data_ptr(), 0 if zeros is None else zeros.data_ptr())
+        self._scales_fp16 = scales.dtype is torch.float16
 
     @classmethod
     def from_packed(cls, packed: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None = None, *,
@@ -116,35 +118,46 @@ class Int4Weight:
         return w[:n, :k].to(dtype)
 
 
+# aspire_int4_args as one packed string (filling a ctypes structure takes longer than the launch)
+_ARGS = struct.Struct("PqPPPPq7iPq")
+
+
 def linear_int4(x: torch.Tensor, w: Int4Weight, out: torch.Tensor, *, swiglu: bool = False) -> torch.Tensor:
     """``out = x @ w.T`` (``[rows, N]``), or with ``swiglu`` ``silu(x @ w[:N/2].T) * (x @ w[N/2:].T)`` (``[rows, N/2]``, N a
-    multiple of 32), for bf16 or fp16 ``x`` with 16-byte aligned rows; ``out`` of ``x``'s type with contiguous rows, apart from x."""
+    multiple of 32), for bf16 or fp16 ``x`` with 16-byte aligned rows; ``out`` of ``x``'s type with contiguous rows, apart
+    from x. A row of x with an infinity or NaN gives no finite outputs; the other rows are not touched by it."""
     what = "linear_int4"
-    _lib.require_cuda(x, out, w.codes, what=what)
+    if not (x.is_cuda and out.is_cuda and w.codes.is_cuda):
+        _lib.require_cuda(x, out, w.codes, what=what)
     n, k = w.shape
-    if x.dim() != 2 or x.dtype not in (torch.bfloat16, torch.float16) or x.shape[1] != k or x.stride(1) != 1 \
-            or x.stride(0) % 8 or x.data_ptr() % 16:
+    shape, st, dtype, at = x.shape, x.stride(), x.dtype, x.data_ptr()
+    if len(shape) != 2 or dtype not in _TYPES or shape[1] != k or st[1] != 1 or st[0] % 8 or at % 16:
         raise ValueError(f"{what}: x must be bf16 or fp16 [rows, {k}] with 16-byte aligned rows")
     if swiglu and n % 32:
         raise ValueError(f"{what}: swiglu needs N a multiple of 32")
-    cols = n // 2 if swiglu else n
-    if out.dtype != x.dtype or out.shape != (x.shape[0], cols) or out.stride(1) != 1:
-        raise ValueError(f"{what}: out must be {x.dtype} [{x.shape[0]}, {cols}] with contiguous rows")
-    if x.device != w.device or out.device != w.device:
+    rows, cols, to = shape[0], n // 2 if swiglu else n, out.stride()
+    if out.dtype is not dtype or out.shape != (rows, cols) or to[1] != 1:
+        raise ValueError(f"{what}: out must be {dtype} [{rows}, {cols}] with contiguous rows")
+    index = w.codes.get_device()
+    if x.get_device() != index or out.get_device() != index:
         raise ValueError(f"{what}: x, out and the weights must be on one device")
     if torch.is_grad_enabled() and x.requires_grad:
         raise ValueError(f"{what}: not differentiable")
     L = _lib.lib()
-    floats = L.aspire_linear_int4_workspace(x.shape[0], n, k, w.group, int(swiglu))
-    a = _lib.Int4Args(x=x.data_ptr(), x_stride=x.stride(0), weights=w.codes.data_ptr(), scales=w.scales.data_ptr(),
-                      zeros=_lib.ptr(w.zeros), out=out.data_ptr(), out_stride=out.stride(0), rows=x.shape[0], n=n, k=k,
-                      group=w.group, swiglu=int(swiglu), fp16=int(x.dtype == torch.float16),
-                      scales_fp16=int(w.scales.dtype == torch.float16))
+    floats, ws = L.aspire_linear_int4_workspace(rows, n, k, w.group, swiglu), 0
     if floats:
-        ws = torch.empty(floats, dtype=torch.float32, device=x.device)
-        a.workspace, a.workspace_floats = ws.data_ptr(), floats
-    with _on(w.device):
-        _lib.check(L.aspire_linear_int4(ctypes.byref(a), _lib.stream_of(x)), what)
+        workspace = torch.empty(floats, dtype=torch.float32, device=x.device)
+        ws = workspace.data_ptr()
+    args = _ARGS.pack(at, st[0], *w._addresses, out.data_ptr(), to[0], rows, n, k, w.group, swiglu,
+                      dtype is torch.float16, w._scales_fp16, ws, floats)
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if torch._C._cuda_getDevice() == index:
+        rc = L.aspire_linear_int4(args, stream)
+    else:
+        with torch.cuda.device(index):
+            rc = L.aspire_linear_int4(args, stream)
+    if rc:
+        _lib.check(rc, what)
     return out
 
 
