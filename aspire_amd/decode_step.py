@@ -22,6 +22,12 @@ the residual adds, norms and token pick are the row kernels of the HIP library
 (``aspire_add_rms_norm``, ``aspire_argmax_rows``), so a whole step can be
 recorded in one HIP graph.
 
+Two forms of a checkpoint take other kernels on the way. ``DecodeWeights.quantized`` holds a layer's four projections as
+4-bit codes (``aspire_amd.linear_int4``: any number of tokens, w13 with the SwiGLU step in its epilogue).
+``ModelShape.rotary`` (a ``RotaryConfig``, for models without q/k norm) prepares q, k and v with
+``RotaryEmbedding.append`` in place of ``qk_norm_rope_update_kv``: half or interleaved pairs, part of the head, scaled
+frequencies.
+
 Refresh layer, ``selector="keymean"`` (a selection per KV head): at
 ``refresh_layer`` every row attends its full context and the kernel writes the
 key-mean page scores of the single-query (draft) rows; the top-``budget`` pages
@@ -56,7 +62,9 @@ from aspire_amd import linear as lin
 from aspire_amd.attention.holistic_wrapper import HolisticAttentionWrapper, build_holistic_dump_jit_args
 from aspire_amd.attention.page_list import build_head_page_lists, build_unified_indices
 from aspire_amd.attention.rope import RopeConfig, qk_norm_rope_update_kv, qk_norm_rope_update_kv_partials
+from aspire_amd.attention.rotary import RotaryConfig, RotaryEmbedding
 from aspire_amd.backends.page_selector import KeyMeanPageSelector, PageSelectorFirstLastAvg
+from aspire_amd.linear_int4 import Int4Weight, linear_int4
 
 PAGE = 16
 DRAFT_MODE, VERIFY_MODE = 0, 1
@@ -81,6 +89,7 @@ class ModelShape:
     rope_base: float = 1e6
     norm_eps: float = 1e-6
     use_qk_norm: bool = True
+    rotary: RotaryConfig | None = None  # in place of rope_base's interleaved pairs (models without q/k norm)
 
     @property
     def q_size(self) -> int:
@@ -214,7 +223,17 @@ class DecodeWeights:
         self.output = lin(shape.vocab_size, d)
 
     def layer_bytes(self) -> int:
-        return sum(t.numel() * t.element_size() for t in self.layers[0].values() if t is not None)
+        return sum(t.nbytes() if isinstance(t, Int4Weight) else t.numel() * t.element_size()
+                   for t in self.layers[0].values() if t is not None)
+
+    def quantized(self, group: int = 128, symmetric: bool = False) -> "DecodeWeights":
+        """The same weights with every layer's four projections in 4 bits (``Int4Weight.quantize``); norms, embeddings
+        and the vocabulary projection stay."""
+        new = object.__new__(DecodeWeights)
+        new.shape, new.tok_embeddings, new.norm, new.output = self.shape, self.tok_embeddings, self.norm, self.output
+        new.layers = [{k: Int4Weight.quantize(v, group=group, symmetric=symmetric) if k in ("wqkv", "wo", "w13", "w2") else v
+                       for k, v in l.items()} for l in self.layers]
+        return new
 
     def to(self, device) -> "DecodeWeights":
         """A copy on ``device`` (test helper: the CPU restatement runs on host copies)."""
@@ -269,6 +288,8 @@ class MixedDecodeStep:
             raise ValueError("every row needs q_len >= 1 new tokens inside its context")
         if shape.head_dim != 128 or shape.n_head % shape.n_local_heads:
             raise ValueError("head_dim 128 and whole GQA groups only")
+        if shape.rotary is not None and (shape.use_qk_norm or shape.rotary.head_dim != shape.head_dim):
+            raise ValueError("rotary goes with models without q/k norm, and has their head_dim")
         if not 0 <= refresh_layer < shape.n_layer:
             raise ValueError("refresh_layer must be one of the model's layers")
         # A draft segment's length is (count - 1) * 16 + last_page_len: the row's current
@@ -381,6 +402,7 @@ class MixedDecodeStep:
         self.refresh_wrapper = HolisticAttentionWrapper(ws, "NHD", jit_args=dump_args, waves_per_cu=waves_per_cu)
         self.mixed_wrapper = HolisticAttentionWrapper(ws, "NHD", waves_per_cu=waves_per_cu)
         self.rope = RopeConfig(rope_theta=shape.rope_base)
+        self.rotary = None if shape.rotary is None else RotaryEmbedding(shape.rotary, dev)
 
         # activations
         bf = torch.bfloat16
@@ -473,8 +495,10 @@ class MixedDecodeStep:
         ``capture`` (a dict, for tests) receives each layer's fused projection
         output before the q/k preparation as ``qkv{layer}``, the attention input q
         (after RoPE) as ``q{layer}``, the attention output as ``y{layer}`` and the
-        final hidden state as ``h``."""
+        final hidden state as ``h``; also the norms' outputs ``a{layer}`` and ``f{layer}``,
+        the gated activations ``act{layer}`` and the outputs of wo and w2 as ``o{layer}`` and ``d{layer}``."""
         s, w = self.shape, self.w
+        whole = lambda t: t.clone() if t.dim() == 2 else t.sum(0).to(torch.bfloat16)
         self._full_lists()
         if self.selector_kind == "first_last":
             self.select_first_last()
@@ -482,21 +506,32 @@ class MixedDecodeStep:
         pending = None  # the previous block's output, not yet added to x
         for layer, lw in enumerate(w.layers):
             self._add_norm(lw["attention_norm"], pending)
-            qkv = self._project(self.a, lw["wqkv"])
+            if capture is not None:
+                capture[f"a{layer}"] = self.a.clone()
+            qkv = self._project(self.a, lw["wqkv"], whole=self.rotary is not None)
             if capture is not None:  # q is rewritten in place below
-                capture[f"qkv{layer}"] = qkv.clone() if qkv.dim() == 2 else qkv.sum(0).to(torch.bfloat16)
+                capture[f"qkv{layer}"] = whole(qkv)
             q = self._prepare_qkv(layer, lw, qkv)
             if capture is not None:
                 capture[f"q{layer}"] = q.clone()
             self.attention(layer, q)
             if capture is not None:
                 capture[f"y{layer}"] = self.y.clone()
-            self._add_norm(lw["ffn_norm"], self._project(self.y.view(self.T, s.q_size), lw["wo"]))
-            if lin.supported(self.a, lw["w13"]) and lin.swiglu_pays(self.T, s.intermediate_size):
+            out = self._project(self.y.view(self.T, s.q_size), lw["wo"])
+            if capture is not None:
+                capture[f"o{layer}"] = whole(out)
+            self._add_norm(lw["ffn_norm"], out)
+            if capture is not None:
+                capture[f"f{layer}"] = self.a.clone()
+            if isinstance(lw["w13"], Int4Weight):
+                self._gate_up_int4(lw["w13"])
+            elif lin.supported(self.a, lw["w13"]) and lin.swiglu_pays(self.T, s.intermediate_size):
                 lin.linear(self.a, lw["w13"], self.act, swiglu=True)
             else:
                 silu_mul(F.linear(self.a, lw["w13"]), self.act)
             pending = self._project(self.act, lw["w2"])
+            if capture is not None:
+                capture[f"act{layer}"], capture[f"d{layer}"] = self.act.clone(), whole(pending)
         self._add_norm(w.norm, pending)
         if capture is not None:
             capture["h"] = self.a.clone()
@@ -507,10 +542,24 @@ class MixedDecodeStep:
             self.logits = F.linear(self.a, w.output)
         return argmax_rows(self.logits, self.ids)
 
-    def _project(self, x: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
+    def _project(self, x: torch.Tensor, w, whole: bool = False) -> torch.Tensor:
         """``x @ w.T``: its split partial sums ``[S, T, N]`` fp32 (in ``partials``, until the next call) where
-        the library's kernels take the shape, else the bf16 ``[T, N]`` of torch's GEMM."""
-        return lin.linear_partials(x, w, self.partials) if lin.supported(x, w) else F.linear(x, w)
+        the library's kernels take the shape (and ``whole`` does not ask for their sum), else the bf16 ``[T, N]`` of torch's
+        GEMM, or of the 4-bit product."""
+        if isinstance(w, Int4Weight):
+            return linear_int4(x, w, torch.empty(x.shape[0], w.shape[0], dtype=x.dtype, device=x.device))
+        if not lin.supported(x, w):
+            return F.linear(x, w)
+        if whole:
+            return lin.linear(x, w, torch.empty(x.shape[0], w.shape[0], dtype=x.dtype, device=x.device))
+        return lin.linear_partials(x, w, self.partials)
+
+    def _gate_up_int4(self, w13: Int4Weight) -> None:
+        """``act = silu(gate) * up`` of the ffn norm's output."""
+        if w13.shape[0] % 32 == 0:
+            linear_int4(self.a, w13, self.act, swiglu=True)
+        else:
+            silu_mul(self._project(self.a, w13), self.act)
 
     def _add_norm(self, weight: torch.Tensor, delta: torch.Tensor | None) -> None:
         """``x += delta`` (a ``_project`` result), ``a = RMSNorm(x) * weight``."""
@@ -522,6 +571,10 @@ class MixedDecodeStep:
     def _prepare_qkv(self, layer: int, lw: dict, qkv: torch.Tensor) -> torch.Tensor:
         """q/k norm, RoPE and the append of a layer's fused projection; the prepared q."""
         s, T = self.shape, self.T
+        if self.rotary is not None:
+            q, k, v = (t.unflatten(1, (-1, s.head_dim)) for t in qkv.split((s.q_size, s.kv_size, s.kv_size), dim=1))
+            return self.rotary.append(q, k, v, self.qo_indptr, self.caches[layer], self.full_indices, self.full_indptr,
+                                      self.last_page_len, PAGE, q_out=self.q)
         args = (lw["q_norm"], lw["k_norm"], s.norm_eps, self.qo_indptr, self.offsets, self.caches[layer],
                 self.full_indices, self.full_indptr, self.last_page_len, PAGE)
         if qkv.dim() == 3:
