@@ -228,6 +228,14 @@ __device__ __forceinline__ void load_lds(u32x4 desc, int voff, uint32_t at) {
                :: "s"(wave_uniform(int(at))), "v"(voff), "s"(desc) : "memory");
 }
 
+// All but the newest kLoads of this wave's loads have landed, and its LDS accesses are done (gfx9's encoding of vmcnt(kLoads)
+// lgkmcnt(0): vmcnt in bits 3:0 and 15:14, expcnt 6:4 at 7).
+template <int kLoads>
+__device__ __forceinline__ void wait_for() {
+  static_assert(kLoads < 64, "vmcnt has 6 bits");
+  __builtin_amdgcn_s_waitcnt((kLoads & 15) | ((kLoads >> 4) << 14) | 0x70);
+}
+
 // Bytes of a ring stage of 128 k: x rows, weight tiles, their scales and zero points; and the stages that fit a CU.
 constexpr int stage_bytes(int bm, int tiles, int parts) { return bm * 256 + tiles * (1024 + 48 * parts); }
 constexpr int sum_bytes(int bm, int parts) { return 2 * parts * bm * 4; }
@@ -250,9 +258,7 @@ __global__ __launch_bounds__(512) void int4_tile_kernel(Int4Params p) {
   constexpr int kW = kBM * 256, kSc = kW + kTiles * 1024, kZp = kSc + kTiles * 32 * kParts;  // offsets in a stage
   constexpr int kLoadX = kBM / 32, kLoadW = (kTiles + 7) / 8;   // 1 KiB loads of a wave and stage
   static_assert(kBM % 32 == 0 && kTiles % 8 == 0, "whole loads a wave");
-  constexpr int kReady = (kDepth - 3) * (kLoadX + kLoadW + 2);  // later stages' loads that may be in flight at a barrier
-  static_assert(kReady < 64, "vmcnt has 6 bits");
-  constexpr int kWait = (kReady & 15) | ((kReady >> 4) << 14) | 0x70;  // vmcnt(kReady) lgkmcnt(0)
+  constexpr int kLater = kDepth - 3;       // stages whose loads may be in flight at a barrier
   __shared__ uint4 ring[kDepth * kStage / 16];
   __shared__ float x_sums[T::kOffset ? 2 * kParts * kBM : 1];
   const char* lds = reinterpret_cast<const char*>(ring);
@@ -280,34 +286,50 @@ __global__ __launch_bounds__(512) void int4_tile_kernel(Int4Params p) {
   int at[kLoadW];                     // first block of a tile
 #pragma unroll
   for (int i = 0; i < kLoadW; ++i) at[i] = min(tile_of(wave * kLoadW + i), last_tile) * p.blocks + s0;
-  // lane l takes 16 bytes of the scales of tile l / (2 kParts), of the zero points of tile l / kParts
-  int s_off = 0, z_off = 0;
+  // Scales and zero points of all tiles: waves 0 and 1, 16 bytes a lane. A load costs about the same however few lanes it has
+  // (with one each a wave, 16 a step, the steps of 64 x 128 tiles took 1.0 us).
+  constexpr int kLoadS = (kTiles * kParts * 2 + 63) / 64, kLoadZ = (kTiles * kParts + 63) / 64;
+  int s_off[kLoadS], z_off[kLoadZ];
 #pragma unroll
-  for (int i = 0; i < kLoadW; ++i) {
-    if (lane / (2 * kParts) == i) s_off = at[i] * (32 * kParts) + (lane % (2 * kParts)) * 16;
-    if (lane / kParts == i) z_off = at[i] * (16 * kParts) + (lane % kParts) * 16;
+  for (int i = 0; i < kLoadS; ++i) {
+    const int n = i * 64 + lane;
+    s_off[i] = (min(tile_of(min(n / (2 * kParts), kTiles - 1)), last_tile) * p.blocks + s0) * (32 * kParts) + n % (2 * kParts) * 16;
   }
-  const auto issue = [&](int s) {
-    const uint32_t to = lds_at + uint32_t(s % kDepth) * kStage;
-    const bool real = s < steps;      // past the end: no bytes, so that every stage counts the same loads
-    const int left = (p.k - (s0 + s) * 128) * 2;
-    const u32x4 dx = buffer_desc(x_base + int64_t(s) * 256, real ? (rows - 1) * x_row_bytes + left : 0);
 #pragma unroll
-    for (int i = 0; i < kLoadX; ++i) {
-      const int n = wave * kLoadX + i, chunk = x_chunk ^ ((n & 3) * 64);
+  for (int i = 0; i < kLoadZ; ++i) {
+    const int n = i * 64 + lane;
+    z_off[i] = (min(tile_of(min(n / kParts, kTiles - 1)), last_tile) * p.blocks + s0) * (16 * kParts) + n % kParts * 16;
+  }
+  constexpr int kLoads = kLoadX + kLoadW;
+  const int all = p.n_pad / 16 * p.blocks * (16 * kParts);  // bytes of zero points
+  // load number d of step s's stage; past the end no bytes, so that every stage counts the same loads
+  const auto issue = [&](int s, int d) {
+    const uint32_t to = lds_at + uint32_t(s % kDepth) * kStage;
+    const bool real = s < steps;
+    if (d < kLoadX) {
+      const int left = (p.k - (s0 + s) * 128) * 2, n = wave * kLoadX + d, chunk = x_chunk ^ ((n & 3) * 64);
+      const u32x4 dx = buffer_desc(x_base + int64_t(s) * 256, real ? (rows - 1) * x_row_bytes + left : 0);
       // k past the end: zeros (an offset past the span), whatever lies behind x's rows
       load_lds(dx, chunk >= left ? 0x7ffffff0 : n * 4 * x_row_bytes + x_row + chunk, to + n * 1024);
+    } else {
+      const u32x4 dw = buffer_desc(reinterpret_cast<const char*>(p.w) + int64_t(at[d - kLoadX] + s) * 1024, real ? 1024 : 0);
+      load_lds(dw, lane * 16, to + kW + (wave * kLoadW + d - kLoadX) * 1024);
     }
+  };
+  const auto issue_groups = [&](int s) {
+    const uint32_t to = lds_at + uint32_t(s % kDepth) * kStage;
+    const bool real = s < steps;
+    if (wave == 0) {
+      const u32x4 ds = buffer_desc(reinterpret_cast<const char*>(p.scales), real ? 2 * all : 0);
 #pragma unroll
-    for (int i = 0; i < kLoadW; ++i) {
-      const u32x4 dw = buffer_desc(reinterpret_cast<const char*>(p.w) + int64_t(at[i] + s) * 1024, real ? 1024 : 0);
-      load_lds(dw, lane * 16, to + kW + (wave * kLoadW + i) * 1024);
+      for (int i = 0; i < kLoadS; ++i)
+        if (i * 64 + lane < kTiles * kParts * 2) load_lds(ds, s_off[i] + s * (32 * kParts), to + kSc + i * 1024);
+    } else if (wave == 1) {
+      const u32x4 dz = buffer_desc(reinterpret_cast<const char*>(p.zeros), real && p.zeros ? all : 0);
+#pragma unroll
+      for (int i = 0; i < kLoadZ; ++i)
+        if (i * 64 + lane < kTiles * kParts) load_lds(dz, z_off[i] + s * (16 * kParts), to + kZp + i * 1024);
     }
-    const int all = p.n_pad / 16 * p.blocks * (16 * kParts);
-    const u32x4 ds = buffer_desc(reinterpret_cast<const char*>(p.scales), real ? 2 * all : 0);
-    const u32x4 dz = buffer_desc(reinterpret_cast<const char*>(p.zeros), real && p.zeros ? all : 0);
-    if (lane < kLoadW * 2 * kParts) load_lds(ds, s_off + s * (32 * kParts), to + kSc + wave * (kLoadW * 32 * kParts));
-    if (lane < kLoadW * kParts) load_lds(dz, z_off + s * (16 * kParts), to + kZp + wave * (kLoadW * 16 * kParts));
   };
 
   const f32x4 none = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -319,7 +341,9 @@ __global__ __launch_bounds__(512) void int4_tile_kernel(Int4Params p) {
   const int x_at = r * 256 + wm * (TM * 4096);  // this lane's row of the wave's first tile
   const int c_at = (grp ^ r) * 16;              // its chunk of 32 k number c: c_at ^ (64 c)
   const auto meet = [&]() {
-    __builtin_amdgcn_s_waitcnt(kWait);
+    if (kLater == 0 || wave >= 2) wait_for<kLater * (kLoadX + kLoadW)>();
+    else if (wave == 0) wait_for<kLater * (kLoadX + kLoadW + kLoadS)>();
+    else wait_for<kLater * (kLoadX + kLoadW + kLoadZ)>();
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
@@ -330,8 +354,15 @@ __global__ __launch_bounds__(512) void int4_tile_kernel(Int4Params p) {
   const auto sum_step = [&](u32x4 x, f32x4 v) { return T::mfma(u32x4{kMinusOffset, kMinusOffset, kMinusOffset, kMinusOffset}, x, v); };
   const auto sum_at = [&](int s, int g) { return &x_sums[T::kOffset ? ((s & 1) * kParts + g) * kBM : 0]; };
 
-  for (int s = 0; s < kDepth; ++s) issue(s);
-  meet();
+  for (int s = 0; s < kDepth - 1; ++s) {
+    issue_groups(s);
+#pragma unroll
+    for (int d = 0; d < kLoads; ++d) issue(s, d);
+  }
+  wait_for<0>();
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
   if (T::kOffset) {
 #pragma unroll
     for (int g = 0; g < kParts; ++g) {
@@ -383,6 +414,7 @@ __global__ __launch_bounds__(512) void int4_tile_kernel(Int4Params p) {
     f32x4 part[TM][TN], sum = none;
     float sc[TN][4];
     u32x4 sum_x;
+    issue_groups(s + kDepth - 1);  // into the slot that the step before read
     const auto take = [&](int t) {     // a finished group of row tile t
 #pragma unroll
       for (int j = 0; j < TN; ++j) {
@@ -415,6 +447,10 @@ __global__ __launch_bounds__(512) void int4_tile_kernel(Int4Params p) {
 #pragma unroll
         for (int j = 0; j < TN; ++j)
           part[t][j] = T::mfma(a[c & 1][j], xf[t], begins ? f32x4{v[t], v[t], v[t], v[t]} : part[t][j]);
+        // The next stage's loads are spread over the first half of the step: together after the barrier they held up every wave.
+#pragma unroll
+        for (int d = 0; d < kLoads; ++d)
+          if (d * 2 * TM / kLoads == c * TM + t) issue(s + kDepth - 1, d);
         // (kept in vector registers, where the compiler needs 10 fewer than with part of them in accumulation registers)
 #pragma unroll
         for (int j = 0; j < TN; ++j) asm volatile("" : "+v"(part[t][j]));
@@ -424,9 +460,11 @@ __global__ __launch_bounds__(512) void int4_tile_kernel(Int4Params p) {
         // the scales of a group that ends in the next phase
         if (t == TM - 1 && (c + 1) % kSteps == kSteps - 1) read_scales(c < 3 ? stage : following, (c + 1) % 4 / kSteps);
         if (ends && t > 0) take(t - 1);
-        if (T::kOffset && t == (TM > 4 ? 2 : 0)) sum_x = sum_chunk(following, c);
+        // (where a phase is short, its chunk is read a phase ahead)
+        if (T::kOffset && t == (TM > 4 ? 2 : 0) && (TM > 4 || c == 0)) sum_x = sum_chunk(following, c);
         if (T::kOffset && t == TM - 1) {
           sum = sum_step(sum_x, begins ? none : sum);
+          if (TM <= 4 && c < 3) sum_x = sum_chunk(following, c + 1);
           if (ends && grp == 0) sum_at(s + 1, g)[sum_tile * 16 + r] = sum[0];
         }
         asm volatile("" ::: "memory");
@@ -435,7 +473,6 @@ __global__ __launch_bounds__(512) void int4_tile_kernel(Int4Params p) {
       if (ends) take(TM - 1);
     }
     meet();          // every wave has read this stage, and the next two have landed
-    issue(s + kDepth);
     stage = following;
   }
   __builtin_amdgcn_s_waitcnt(0x70);  // vmcnt(0): no load may land after the ring is given up
