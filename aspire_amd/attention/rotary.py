@@ -139,17 +139,22 @@ class RotaryEmbedding:
 
     # ------------------------------------------------------------------ checks
     def _heads(self, t: torch.Tensor, dtype: torch.dtype, what: str, name: str):
-        """A head tensor's (tokens, heads), address and strides, after its checks."""
-        if not t.is_cuda:
-            _lib.require_cuda(t, what=what)
+        """A head tensor's shape, its address and strides, after its checks."""
+        shape, strides = t.shape, t.stride()
+        if t.get_device() == self._index and t.dtype is dtype and len(shape) == 3 and shape[2] == self._dims[0] \
+                and (strides[2] == 1 or not t.numel()):
+            return shape, (t.data_ptr(), strides[0], strides[1])
+        _lib.require_cuda(t, what=what)
         if t.get_device() != self._index:
             raise ValueError(f"{what}: {name} is on {t.device}, the frequencies on {self.device}")
-        shape, strides = t.shape, t.stride()
-        if t.dtype is not dtype or len(shape) != 3 or shape[2] != self._dims[0]:
-            raise ValueError(f"{what}: {name} must be {dtype} [T, H, {self._dims[0]}]")
-        if strides[2] != 1 and t.numel():
-            raise ValueError(f"{what}: {name} must have contiguous head dims")
-        return shape, (t.data_ptr(), strides[0], strides[1])
+        raise ValueError(f"{what}: {name} must be {dtype} [T, H, {self._dims[0]}] with contiguous head dims")
+
+    def _list(self, t: torch.Tensor, what: str):
+        """An index array as int32 in one piece, and its length."""
+        if t.dim() != 1 or t.get_device() != self._index or t.dtype not in _INTS:
+            raise ValueError(f"{what}: the index arrays must be 1-D int32 on {self.device}")
+        t = _lib.dense(t, torch.int32)
+        return t, t.shape[0]
 
     def _dtype(self, t: torch.Tensor, what: str) -> int:
         code = _DTYPES.get(t.dtype)
@@ -158,7 +163,7 @@ class RotaryEmbedding:
         return code
 
     def _positions(self, positions: torch.Tensor, tokens: int, what: str) -> torch.Tensor:
-        if positions.dtype not in _INTS or positions.dim() != 1 or positions.shape[0] != tokens:
+        if positions.dtype not in _INTS or positions.shape != (tokens,):
             raise ValueError(f"{what}: positions must be int32 or int64 [T]")
         if positions.get_device() != self._index:
             raise ValueError(f"{what}: positions are on {positions.device}, the frequencies on {self.device}")
@@ -184,7 +189,7 @@ class RotaryEmbedding:
             shape, qa = self._heads(q, dtype, what, "q")
             hq, qo = shape[1], qa
             if not in_place:
-                q_out = q.new_empty(shape)
+                q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
                 qo = (q_out.data_ptr(), hq * shape[2], shape[2])
         if k is not None:
             shape, ka = self._heads(k, dtype, what, "k")
@@ -192,7 +197,7 @@ class RotaryEmbedding:
                 raise ValueError(f"{what}: q and k must have the same number of tokens")
             hkv, ko = shape[1], ka
             if not in_place:
-                k_out = k.new_empty(shape)
+                k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
                 ko = (k_out.data_ptr(), hkv * shape[2], shape[2])
         positions = self._positions(positions, tokens, what)
         args = _HEAD.pack(*qa, *qo, *ka, *ko, *_NONE, hq, hkv, tokens, *self._dims, code, inverse, *self._tail,
@@ -250,21 +255,16 @@ class RotaryEmbedding:
                 or cache_shape[1:] != (2, page_size, hkv, self._dims[0]) or cs[4] != 1:
             raise ValueError(f"{what}: kv_cache must be {dtype} [P, 2, {page_size}, {hkv}, {self._dims[0]}] on "
                              f"{self.device} with contiguous head dims")
-        ind, pages, ptr, last = kv_append_indptr, kv_page_indices, kv_page_indptr, kv_last_page_len
-        for t in (ind, pages, ptr, last):
-            if t.dtype not in _INTS or t.dim() != 1 or t.get_device() != self._index:
-                raise ValueError(f"{what}: the index arrays must be 1-D int32 on {self.device}")
-        num_seq = last.shape[0]
-        if ind.shape[0] <= num_seq or ptr.shape[0] <= num_seq:
+        (ind, ind_len), (pages, num_pages) = self._list(kv_append_indptr, what), self._list(kv_page_indices, what)
+        (ptr, ptr_len), (last, num_seq) = self._list(kv_page_indptr, what), self._list(kv_last_page_len, what)
+        if ind_len <= num_seq or ptr_len <= num_seq:
             raise ValueError(f"{what}: kv_page_indptr and kv_append_indptr need len(kv_last_page_len) + 1 entries")
-        ind, pages, ptr, last = (_lib.dense(ind, torch.int32), _lib.dense(pages, torch.int32),
-                                 _lib.dense(ptr, torch.int32), _lib.dense(last, torch.int32))
         at, wide = 0, False
         if positions is not None:
             positions = self._positions(positions, tokens, what)
             at, wide = positions.data_ptr(), positions.dtype is torch.int64
         args = _ARGS.pack(*qa, *qo, *ka, *_NONE, *va, shape[1], hkv, tokens, *self._dims, code, 0, *self._tail, wide, at,
-                          kv_cache.data_ptr(), cs[0], cs[1], cs[2], cs[3], cache_shape[0], pages.shape[0], page_size,
+                          kv_cache.data_ptr(), cs[0], cs[1], cs[2], cs[3], cache_shape[0], num_pages, page_size,
                           num_seq, ind.data_ptr(), pages.data_ptr(), ptr.data_ptr(), last.data_ptr())
         self._launch(_lib.lib().aspire_rotary_append, args, what)
         return q_out

@@ -76,7 +76,7 @@ def test_entry_points_refuse_on_the_host():
         return ctypes.byref(a)
 
     both = [dict(dtype=3), dict(dtype=-1), dict(head_dim=257), dict(rotary_dim=31), dict(rotary_dim=66), dict(rotary_dim=0),
-            dict(total_tokens=-1), dict(num_qo_heads=-1), dict(num_kv_heads=1025), dict(turns=None), dict(q=None), dict(q_out=None),
+            dict(total_tokens=-1), dict(total_tokens=1 << 26), dict(num_qo_heads=-1), dict(num_kv_heads=1025), dict(turns=None), dict(q=None), dict(q_out=None),
             dict(k=None)]
     for kw in both:
         for entry in (L.aspire_rotary, L.aspire_rotary_append):
