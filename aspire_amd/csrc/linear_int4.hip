@@ -112,7 +112,7 @@ __device__ __forceinline__ void store4(const Int4Params& p, int64_t m, int col, 
 constexpr int kWaves = 8;
 constexpr int kAhead = 4;     // blocks of 1 KiB a wave has in flight
 
-// Up to 16 rows: bound by the weights' stream. A workgroup walks over output tiles of 16 columns (with swiglu over pairs of a
+// Few rows (16 to a blockIdx.z): bound by the weights' stream. A workgroup walks over output tiles of 16 columns (with swiglu over pairs of a
 // gate and an up tile), for all of k or the split blockIdx.y of at most kAhead * kWaves blocks; its waves take the blocks of
 // 128 k in turn, keep their x in registers, and add up through LDS, in a fixed order. A block is asked for as soon as
 // the one before it in its registers is multiplied, across the ends of tiles, so the stream never pauses.
@@ -167,7 +167,8 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(G =
   int tile = blockIdx.x, half = 0;  // half 1: the up tile
   Block ring[kAhead];
   u32x4 x[kAhead][4];
-  const uint16_t* xrow = p.x + min(r, p.rows - 1) * p.x_st + 8 * grp;
+  const int64_t m = int64_t(blockIdx.z) * 16 + r;
+  const uint16_t* xrow = p.x + min(m, int64_t(p.rows) - 1) * p.x_st + 8 * grp;
 #pragma unroll
   for (int i = 0; i < kAhead; ++i) {
     fetch(ring[i], tile, i);
@@ -198,14 +199,14 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(G =
       }
       if (!last) {
         gate = v;
-      } else if (r < p.rows) {
+      } else if (m < p.rows) {
         if (p.swiglu) v = make_float4(silu(gate.x) * v.x, silu(gate.y) * v.y, silu(gate.z) * v.z, silu(gate.w) * v.w);
         const float o[4] = {v.x, v.y, v.z, v.w};
         const int col = tile * 16 + 4 * grp;
         if (p.splits > 1)
-          *reinterpret_cast<float4*>(p.partials + (int64_t(blockIdx.y) * p.rows + r) * p.n_pad + col) = v;
+          *reinterpret_cast<float4*>(p.partials + (int64_t(blockIdx.y) * p.rows + m) * p.n_pad + col) = v;
         else
-          store4<T>(p, r, col, o);
+          store4<T>(p, m, col, o);
       }
     }
     tile = next, half = next_half;
@@ -546,7 +547,7 @@ template <class T, class S, int G>
 void launch_stream(const Int4Params& p, hipStream_t s) {
   const int tiles = p.swiglu ? p.n / 16 : p.splits > 1 ? p.n_pad / 16 : (p.n + 15) / 16;
   // two workgroups a CU at most; the second ones take what is over of an uneven number of tiles
-  hipLaunchKernelGGL((int4_stream_kernel<T, S, G>), dim3(std::min(tiles, std::max(1, 512 / p.splits)), p.splits), dim3(64 * kWaves), 0, s, p);
+  hipLaunchKernelGGL((int4_stream_kernel<T, S, G>), dim3(std::min(tiles, std::max(1, 512 / p.splits)), p.splits, (p.rows + 15) / 16), dim3(64 * kWaves), 0, s, p);
 }
 
 template <class T, class S, int G, int WM, int TM, int TN>
@@ -561,14 +562,16 @@ struct Shape {
   int rows, cols, splits;
 };
 
-// The stream kernel up to 16 rows, its splits as many blocks as its waves hold. Above, the shortest of the tiles and splits
+// The stream kernel up to 16 rows, its splits as many blocks as its waves hold, and for more rows while every 16 x 16 tile has
+// a CU of its own (64 x 1,024 x 4,096: 8.2 us, 11.8 in tiles; 32 x 4,096 x 4,096, past it, 12.9 and 12.1). Else the shortest of the tiles and splits
 // by what the kernel's parts measured: 2 us to fill the ring and store, the steps, and the slabs' join, in whole
 // rounds of one workgroup a CU. Steps of a 128-wide group in us (groups of 32: a third more):
 //   32 x 128 0.75, 32 x 256 1.05, 64 x 128 1.0, 64 x 256 1.35, 128 x 128 1.4, 128 x 256 2.05.
 // us it chooses between: 33 x 4,096 x 12,288 (128 columns in 1 / 2 / 4 / 8 splits) 91 / 51 / 30 / 22, in 256 118 / 64 / 37 / 26;
 // 208 x 24,576 x 4,096 91 / 90 / 110 / 150, 71 / 84 / 90 / 127; 2,048 x 6,144 x 4,096 147 and 139.
 Shape choose(int rows, int n_pad, int blocks, int group, bool swiglu) {
-  if (rows <= 16) return Shape{0, 0, (blocks + kAhead * kWaves - 1) / (kAhead * kWaves)};
+  const int mine = (blocks + kAhead * kWaves - 1) / (kAhead * kWaves);
+  if (rows <= 16 || (mine == 1 && int64_t(n_pad / 16) * ((rows + 15) / 16) <= 256)) return Shape{0, 0, mine};
   const int bm = rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
   const double mblocks = (rows + bm - 1) / bm;
   Shape best{bm, 128, 1};

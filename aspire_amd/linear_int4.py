@@ -125,7 +125,8 @@ _ARGS = struct.Struct("PqPPPPq7iPq")
 def linear_int4(x: torch.Tensor, w: Int4Weight, out: torch.Tensor, *, swiglu: bool = False) -> torch.Tensor:
     """``out = x @ w.T`` (``[rows, N]``), or with ``swiglu`` ``silu(x @ w[:N/2].T) * (x @ w[N/2:].T)`` (``[rows, N/2]``, N a
     multiple of 32), for bf16 or fp16 ``x`` with 16-byte aligned rows; ``out`` of ``x``'s type with contiguous rows, apart
-    from x. A row of x with an infinity or NaN gives no finite outputs; the other rows are not touched by it."""
+    from x. Not differentiable. A row of x with an infinity or NaN (or bf16 values of 2^112 and more, whose sums may overflow on the way) gives
+    no finite outputs; the other rows are not touched by it."""
     what = "linear_int4"
     if not (x.is_cuda and out.is_cuda and w.codes.is_cuda):
         _lib.require_cuda(x, out, w.codes, what=what)
