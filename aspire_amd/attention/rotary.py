@@ -133,9 +133,8 @@ class RotaryEmbedding:
         self.config = config
         self.turns = _turns(config.frequencies()).to(device)
         self.device = self.turns.device
-        self._index = self.turns.get_device()
+        self._index = self.turns.get_device() if self.turns.is_cuda else -2  # (-2: no tensor's)
         self._dims = (config.head_dim, config.rotated, int(config.layout == "interleaved"))
-        self._tail = (self.turns.data_ptr(), config.scale)
 
     # ------------------------------------------------------------------ checks
     def _heads(self, t: torch.Tensor, dtype: torch.dtype, what: str, name: str):
@@ -200,7 +199,7 @@ class RotaryEmbedding:
                 k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
                 ko = (k_out.data_ptr(), hkv * shape[2], shape[2])
         positions = self._positions(positions, tokens, what)
-        args = _HEAD.pack(*qa, *qo, *ka, *ko, *_NONE, hq, hkv, tokens, *self._dims, code, inverse, *self._tail,
+        args = _HEAD.pack(*qa, *qo, *ka, *ko, *_NONE, hq, hkv, tokens, *self._dims, code, inverse, self.turns.data_ptr(), self.config.scale,
                           positions.dtype is torch.int64, positions.data_ptr()) + _NO_CACHE
         self._launch(_lib.lib().aspire_rotary, args, what)
         return q_out, k_out
@@ -226,9 +225,9 @@ class RotaryEmbedding:
                q_out: torch.Tensor | None = None) -> torch.Tensor:
         """Turn q (in place, or into ``q_out``, which it returns) and append the turned k and v to ``kv_cache``
         ``[P, 2, page, H_kv, D]`` where ``mylib::update_kv_padded`` would put them, in one launch. A token's position is
-        its place in its row's sequence unless ``positions`` ``[T]`` gives another. Tokens of no row are
-        padding: their q passes unchanged, and nothing is written to the cache; nor is it for a token whose
-        page id or list entry lies outside the pool or the list."""
+        its place in its row's sequence unless ``positions`` ``[T]`` gives another (negative: not turned). Tokens of no
+        row are padding: their q passes unchanged, and nothing is written to the cache; nor is it for a token whose
+        page id or list entry lies outside the pool or the list. No two tokens may share a slot."""
         what = "RotaryEmbedding.append"
         code, dtype = self._dtype(q, what), q.dtype
         if code == 2:
@@ -263,8 +262,8 @@ class RotaryEmbedding:
         if positions is not None:
             positions = self._positions(positions, tokens, what)
             at, wide = positions.data_ptr(), positions.dtype is torch.int64
-        args = _ARGS.pack(*qa, *qo, *ka, *_NONE, *va, shape[1], hkv, tokens, *self._dims, code, 0, *self._tail, wide, at,
-                          kv_cache.data_ptr(), cs[0], cs[1], cs[2], cs[3], cache_shape[0], num_pages, page_size,
+        args = _ARGS.pack(*qa, *qo, *ka, *_NONE, *va, shape[1], hkv, tokens, *self._dims, code, 0, self.turns.data_ptr(),
+                          self.config.scale, wide, at, kv_cache.data_ptr(), cs[0], cs[1], cs[2], cs[3], cache_shape[0], num_pages, page_size,
                           num_seq, ind.data_ptr(), pages.data_ptr(), ptr.data_ptr(), last.data_ptr())
         self._launch(_lib.lib().aspire_rotary_append, args, what)
         return q_out

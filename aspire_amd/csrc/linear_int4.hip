@@ -634,8 +634,7 @@ extern "C" int aspire_linear_int4(const aspire_int4_args* a, void* stream) {
   ASPIRE_CHECK_ARG(!a->swiglu || a->n % 32 == 0, "swiglu needs whole 16-row tiles of gate and up rows");
   if (a->rows == 0 || a->n == 0) return ASPIRE_OK;
   ASPIRE_CHECK_ARG(a->x && a->weights && a->scales && a->out, "null pointer");
-  ASPIRE_CHECK_ARG(aligned(a->x, 16) && a->x_stride % 8 == 0 && a->x_stride >= a->k && a->x_stride < (1 << 22),
-                   "x rows must be 16-byte aligned, of less than 2^22 elements");
+  ASPIRE_CHECK_ARG(aligned(a->x, 16) && a->x_stride % 8 == 0 && a->x_stride >= a->k, "x rows must be 16-byte aligned");
   ASPIRE_CHECK_ARG(aligned(a->weights, 16) && aligned(a->scales, 16) && aligned(a->zeros, 16),
                    "weights, scales and zeros must be 16-byte aligned");
   const int outs = a->swiglu ? a->n / 2 : a->n;
@@ -657,6 +656,7 @@ extern "C" int aspire_linear_int4(const aspire_int4_args* a, void* stream) {
   p.wide_out = aligned(a->out, 8) && a->out_stride % 4 == 0;
   hipStream_t s = static_cast<hipStream_t>(stream);
   const Shape f = choose(p.rows, p.n_pad, p.blocks, a->group, a->swiglu != 0);
+  ASPIRE_CHECK_ARG(f.rows == 0 || a->x_stride < (1 << 22), "row strides of 2^22 elements or more past 16 rows");
   p.splits = f.splits;
   p.partials = static_cast<float*>(a->workspace);
   ASPIRE_CHECK_ARG(f.splits == 1 || (a->workspace && aligned(a->workspace, 16) && a->workspace_floats >= partial_floats(f, p.rows, p.n_pad)),

@@ -27,8 +27,6 @@ class Int4Weight:
     def __init__(self, shape, group, codes, scales, zeros):
         self.shape, self.group = tuple(shape), group
         self.codes, self.scales, self.zeros = codes, scales, zeros  # see aspire_hip.h for the layouts
-        self._addresses = (codes.data_ptr(), scales.data_ptr(), 0 if zeros is None else zeros.data_ptr())
-        self._scales_fp16 = scales.dtype is torch.float16
 
     @classmethod
     def from_packed(cls, packed: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None = None, *,
@@ -56,21 +54,20 @@ class Int4Weight:
             return out
 
         # bytes of a lane's word: [tile, row, block, word, lane / 16, byte] -> [tile, block, lane / 16, row, word, byte]
-        b = fill(packed, tiles * 16, blocks * 64).view(tiles, 16, blocks, 4, 4, 4).permute(0, 2, 4, 1, 3, 5)
-        even, odd = torch.empty_like(b, memory_format=torch.contiguous_format), None
-        even.copy_(b)
+        b = fill(packed, tiles * 16, blocks * 64).reshape(tiles, 16, blocks, 4, 4, 4).permute(0, 2, 4, 1, 3, 5)
+        b = b.contiguous()
         # nibble e of 8 goes to place e / 2 + 4 (e % 2): bytes (e1 e0)(e3 e2)(e5 e4)(e7 e6) -> (e2 e0)(e6 e4)(e3 e1)(e7 e5)
-        lo, hi = even & 15, even >> 4
-        codes = torch.empty_like(even)
+        lo, hi = b & 15, b >> 4
+        codes = torch.empty_like(b)
         codes[..., 0] = lo[..., 0] | (lo[..., 1] << 4)
         codes[..., 1] = lo[..., 2] | (lo[..., 3] << 4)
         codes[..., 2] = hi[..., 0] | (hi[..., 1] << 4)
         codes[..., 3] = hi[..., 2] | (hi[..., 3] << 4)
         parts = 128 // group
         # [tile, row, block, group of it] -> [tile, block, row / 4, group, row % 4] and [tile, block, row, group]
-        scales = fill(scales, tiles * 16, blocks * parts).view(tiles, 4, 4, blocks, parts).permute(0, 3, 1, 4, 2).contiguous()
+        scales = fill(scales, tiles * 16, blocks * parts).reshape(tiles, 4, 4, blocks, parts).permute(0, 3, 1, 4, 2).contiguous()
         if zeros is not None:
-            zeros = fill(zeros, tiles * 16, blocks * parts).view(tiles, 16, blocks, parts).transpose(1, 2).contiguous()
+            zeros = fill(zeros, tiles * 16, blocks * parts).reshape(tiles, 16, blocks, parts).transpose(1, 2).contiguous()
         return cls((n, k), group, codes.view(tiles, blocks, 64, 16), scales, zeros)
 
     @classmethod
@@ -79,8 +76,10 @@ class Int4Weight:
         its largest magnitude in 7."""
         if w.dim() != 2 or group not in GROUPS or w.shape[1] % group:
             raise ValueError(f"Int4Weight: w must be [N, K], group one of {GROUPS} and K a multiple of it")
+        if not bool(torch.isfinite(w).all()):
+            raise ValueError("Int4Weight: w must be finite")
         dtype = w.dtype if w.dtype in (torch.bfloat16, torch.float16) else torch.bfloat16
-        v = w.float().view(w.shape[0], -1, group)
+        v = w.float().reshape(w.shape[0], -1, group)
         if symmetric:
             scale, zero = v.abs().amax(-1) / 7, None
         else:
@@ -132,7 +131,7 @@ def linear_int4(x: torch.Tensor, w: Int4Weight, out: torch.Tensor, *, swiglu: bo
         _lib.require_cuda(x, out, w.codes, what=what)
     n, k = w.shape
     shape, st, dtype, at = x.shape, x.stride(), x.dtype, x.data_ptr()
-    if len(shape) != 2 or dtype not in _TYPES or shape[1] != k or st[1] != 1 or st[0] % 8 or at % 16:
+    if len(shape) != 2 or dtype not in _TYPES or shape[1] != k or st[1] != 1 or (st[0] % 8 and shape[0] > 1) or at % 16:
         raise ValueError(f"{what}: x must be bf16 or fp16 [rows, {k}] with 16-byte aligned rows")
     if swiglu and n % 32:
         raise ValueError(f"{what}: swiglu needs N a multiple of 32")
@@ -149,8 +148,10 @@ def linear_int4(x: torch.Tensor, w: Int4Weight, out: torch.Tensor, *, swiglu: bo
     if floats:
         workspace = torch.empty(floats, dtype=torch.float32, device=x.device)
         ws = workspace.data_ptr()
-    args = _ARGS.pack(at, st[0], *w._addresses, out.data_ptr(), to[0], rows, n, k, w.group, swiglu,
-                      dtype is torch.float16, w._scales_fp16, ws, floats)
+    zeros = w.zeros
+    args = _ARGS.pack(at, st[0] if rows > 1 else k, w.codes.data_ptr(), w.scales.data_ptr(),
+                      0 if zeros is None else zeros.data_ptr(), out.data_ptr(), to[0] if rows > 1 else cols, rows, n, k, w.group,
+                      swiglu, dtype is torch.float16, w.scales.dtype is torch.float16, ws, floats)
     stream = torch._C._cuda_getCurrentRawStream(index)
     if torch._C._cuda_getDevice() == index:
         rc = L.aspire_linear_int4(args, stream)

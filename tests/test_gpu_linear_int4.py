@@ -114,6 +114,35 @@ def test_scales_of_the_other_type(gpu):
         close(out, x.double() @ w.t(), product_bound(x, scales, 64, 512))
 
 
+def test_rows_far_apart(gpu):
+    """A last token of each of a few long sequences: row strides past 2^22 values, which tiles past 16 rows refuse."""
+    say("int4 far rows")
+    packed, scales, z, w = weights(8208, 256, 64, True, BF, gpu)
+    pack = Int4Weight.from_packed(packed, scales, z, group=64)
+    hidden = torch.zeros(17, 20000, 256, dtype=BF, device=gpu)   # 5,120,000 values a row
+    x = hidden[:, -1]
+    x.copy_(torch.randn(17, 256, device=gpu))
+    for rows in (1, 5, 16):
+        out = linear_int4(x[:rows], pack, torch.empty(rows, 8208, dtype=BF, device=gpu))
+        assert torch.equal(out, linear_int4(x[:rows].contiguous(), pack, torch.empty_like(out)))
+    with pytest.raises(ValueError):
+        linear_int4(x, pack, torch.empty(17, 8208, dtype=BF, device=gpu))
+
+
+def test_fewer_blocks_than_splits(gpu):
+    """One block of k where the gate and up tiles pair in the join of two splits: an empty split."""
+    say("int4 empty split")
+    for dtype in (BF, HF):
+        packed, scales, z, w = weights(8224, 64, 32, True, dtype, gpu)
+        pack = Int4Weight.from_packed(packed, scales, z, group=32)
+        x = torch.randn(33, 64, device=gpu).to(dtype)
+        out = linear_int4(x, pack, torch.empty(33, 4112, dtype=dtype, device=gpu), swiglu=True)
+        gate, up = (x.double() @ w.t()).chunk(2, dim=1)
+        bg, bu = product_bound(x, scales, 32, 64).chunk(2, dim=1)
+        silu = gate * torch.sigmoid(gate)
+        close(out, silu * up, 1.1 * bg * (up.abs() + bu) + silu.abs() * bu + 8 * 2.0 ** -24 * (silu * up).abs())
+
+
 def test_rows_do_not_mix(gpu):
     """A row with an infinity or NaN is not finite; the other rows are what they were."""
     say("int4 special values")

@@ -5,7 +5,7 @@ import ctypes
 import pytest
 import torch
 
-from aspire_amd import _lib
+from aspire_amd import _lib, linear_int4
 from aspire_amd.linear_int4 import Int4Weight
 
 
@@ -55,8 +55,30 @@ def test_refused_weights(change):
         Int4Weight.from_packed(**{**kw, **change})
 
 
+def test_views_give_the_same_weights():
+    """Packed codes, scales and zeros that are slices of larger or transposed tensors."""
+    g = torch.Generator().manual_seed(5)
+    packed = torch.randint(0, 256, (40, 2 * 96), dtype=torch.uint8, generator=g)[:, ::2][:, :64]
+    scales = torch.rand(2, 40, generator=g).to(torch.bfloat16).t()
+    z = torch.randint(0, 16, (2, 40), dtype=torch.uint8, generator=g).t()
+    a = Int4Weight.from_packed(packed, scales, z, group=64)
+    b = Int4Weight.from_packed(packed.contiguous(), scales.contiguous(), z.contiguous(), group=64)
+    assert torch.equal(a.codes, b.codes) and torch.equal(a.scales, b.scales) and torch.equal(a.zeros, b.zeros)
+    w = torch.randn(128, 32, generator=g).t()
+    assert torch.equal(Int4Weight.quantize(w, group=64).codes, Int4Weight.quantize(w.contiguous(), group=64).codes)
+
+
+def test_packed_arguments_match_the_structure():
+    """The string that the entry point gets in place of the structure: every field at its place."""
+    values = list(range(1, 17))
+    a = _lib.Int4Args.from_buffer_copy(linear_int4._ARGS.pack(*values))
+    assert ctypes.sizeof(_lib.Int4Args) == linear_int4._ARGS.size
+    assert [getattr(a, f[0]) for f in a._fields_] == values
+
+
 def test_refused_matrices():
-    for w, group in ((torch.zeros(4, 100), 64), (torch.zeros(64), 64), (torch.zeros(4, 128), 16)):
+    for w, group in ((torch.zeros(4, 100), 64), (torch.zeros(64), 64), (torch.zeros(4, 128), 16),
+                     (torch.full((4, 64), float("nan")), 64)):
         with pytest.raises(ValueError):
             Int4Weight.quantize(w, group=group)
 
@@ -72,7 +94,7 @@ def test_entry_point_refuses_on_the_host():
             setattr(a, name, value)
         return L.aspire_linear_int4(ctypes.byref(a), None)
 
-    for kw in (dict(rows=-1), dict(rows=1 << 22), dict(n=-1), dict(k=0), dict(k=250), dict(k=1 << 22, x_stride=1 << 22), dict(x_stride=1 << 22), dict(group=16), dict(group=0), dict(x=None),
+    for kw in (dict(rows=-1), dict(rows=1 << 22), dict(n=-1), dict(k=0), dict(k=250), dict(k=1 << 22, x_stride=1 << 22), dict(rows=400, n=1 << 14, out_stride=1 << 14, x_stride=1 << 22), dict(group=16), dict(group=0), dict(x=None),
                dict(weights=None), dict(scales=None), dict(out=None), dict(x=4104), dict(x_stride=260), dict(x_stride=248),
                dict(out_stride=63), dict(n=48, swiglu=1), dict(scales=4100), dict(zeros=4097)):
         assert call(**kw) == _lib.ASPIRE_ERR_INVALID, kw

@@ -8,6 +8,7 @@ import pytest
 import torch
 
 from aspire_amd import _lib
+from aspire_amd.attention import rotary
 from aspire_amd.attention.rope import RopeConfig, rope_frequencies
 from aspire_amd.attention.rotary import RotaryConfig, RotaryEmbedding
 
@@ -91,7 +92,19 @@ def test_entry_points_refuse_on_the_host():
     assert L.aspire_rotary(None, None) == _lib.ASPIRE_ERR_INVALID
 
 
+def test_packed_arguments_match_the_structure():
+    """The string that the entry points get in place of the structure: every field at its place."""
+    values = [float(i) if i == 25 else i for i in range(1, 41)]
+    a = _lib.RotaryArgs.from_buffer_copy(rotary._ARGS.pack(*values))
+    assert ctypes.sizeof(_lib.RotaryArgs) == rotary._ARGS.size
+    assert [getattr(a, f[0]) for f in a._fields_] == values
+
+
 def test_cpu_tensors_are_refused():
     rot = RotaryEmbedding(RotaryConfig(head_dim=64), "cpu")
-    with pytest.raises(RuntimeError):
-        rot.apply(torch.zeros(1, 1, 64), None, torch.zeros(1, dtype=torch.int32))
+    x, pos, i = torch.zeros(1, 1, 64), torch.zeros(1, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    calls = (lambda: rot.apply(x, None, pos), lambda: rot.apply_inplace(x, x.clone(), pos),
+             lambda: rot.append(x.half(), x.half(), x.half(), i, torch.zeros(1, 2, 16, 1, 64).half(), i, i, i[:1], 16))
+    for call in calls:
+        with pytest.raises(RuntimeError, match="GPU"):
+            call()
