@@ -519,10 +519,15 @@ __global__ __launch_bounds__(256) void int4_join_kernel(Int4Params p) {
   const int col = int(i - m * quads) * 4;
   const auto total = [&](int at) {
     const float* from = p.partials + m * p.n_pad + at;
-    float4 v = *reinterpret_cast<const float4*>(from);
-    for (int q = 1; q < p.splits; ++q) {
-      const float4 u = *reinterpret_cast<const float4*>(from + int64_t(q) * p.rows * p.n_pad);
-      v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
+    const int64_t slab = int64_t(p.rows) * p.n_pad;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int q = 0; q < p.splits; q += 8) {  // 8 loads in flight (16 slabs of 33 x 4,016: 4.0 us; one by one 5.7)
+      float4 u[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) u[i] = *reinterpret_cast<const float4*>(from + min(q + i, p.splits - 1) * slab);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (q + i < p.splits) v.x += u[i].x, v.y += u[i].y, v.z += u[i].z, v.w += u[i].w;
     }
     return v;
   };
