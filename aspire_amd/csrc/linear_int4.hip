@@ -257,8 +257,9 @@ __global__ __launch_bounds__(512) void int4_tile_kernel(Int4Params p) {
   constexpr int kParts = 128 / G, kSteps = 4 / kParts;
   constexpr int kDepth = stages(kBM, kTiles, kParts), kStage = stage_bytes(kBM, kTiles, kParts);
   constexpr int kW = kBM * 256, kSc = kW + kTiles * 1024, kZp = kSc + kTiles * 32 * kParts;  // offsets in a stage
-  constexpr int kLoadX = kBM / 32, kLoadW = (kTiles + 7) / 8;   // 1 KiB loads of a wave and stage
-  static_assert(kBM % 32 == 0 && kTiles % 8 == 0, "whole loads a wave");
+  // 1 KiB loads of a wave and stage (of x some twice where they do not come out even: the same bytes to the same place)
+  constexpr int kLoadX = (kBM / 4 + 7) / 8, kLoadW = kTiles / 8;
+  static_assert(kTiles % 8 == 0, "whole loads a wave");
   constexpr int kLater = kDepth - 3;       // stages whose loads may be in flight at a barrier
   __shared__ uint4 ring[kDepth * kStage / 16];
   __shared__ float x_sums[T::kOffset ? 2 * kParts * kBM : 1];
@@ -308,7 +309,7 @@ __global__ __launch_bounds__(512) void int4_tile_kernel(Int4Params p) {
     const uint32_t to = lds_at + uint32_t(s % kDepth) * kStage;
     const bool real = s < steps;
     if (d < kLoadX) {
-      const int left = (p.k - (s0 + s) * 128) * 2, n = wave * kLoadX + d, chunk = x_chunk ^ ((n & 3) * 64);
+      const int left = (p.k - (s0 + s) * 128) * 2, n = min(wave * kLoadX + d, kBM / 4 - 1), chunk = x_chunk ^ ((n & 3) * 64);
       const u32x4 dx = buffer_desc(x_base + int64_t(s) * 256, real ? (rows - 1) * x_row_bytes + left : 0);
       // k past the end: zeros (an offset past the span), whatever lies behind x's rows
       load_lds(dx, chunk >= left ? 0x7ffffff0 : n * 4 * x_row_bytes + x_row + chunk, to + n * 1024);
@@ -568,30 +569,34 @@ struct Shape {
 };
 
 // The stream kernel up to 16 rows, its splits as many blocks as its waves hold, and for more rows while every 16 x 16 tile has
-// a CU of its own (64 x 1,024 x 4,096: 8.2 us, 11.8 in tiles; 32 x 4,096 x 4,096, past it, 12.9 and 12.1). Else the shortest of the tiles and splits
-// by what the kernel's parts measured: 2 us to fill the ring and store, the steps, and the slabs' join, in whole
-// rounds of one workgroup a CU. Steps of a 128-wide group in us (groups of 32: a third more):
-//   32 x 128 0.75, 32 x 256 1.05, 64 x 128 1.0, 64 x 256 1.35, 128 x 128 1.4, 128 x 256 2.05.
-// us it chooses between: 33 x 4,096 x 12,288 (128 columns in 1 / 2 / 4 / 8 splits) 91 / 51 / 30 / 22, in 256 118 / 64 / 37 / 26;
-// 208 x 24,576 x 4,096 91 / 90 / 110 / 150, 71 / 84 / 90 / 127; 2,048 x 6,144 x 4,096 147 and 139.
+// a CU of its own (64 x 1,024 x 4,096: 8.2 us, 11.8 in tiles; 32 x 4,096 x 4,096, past it, 12.9 and 12.1). Else the shortest
+// of the tiles and splits by what the kernel's parts measured: 2.5 us to fill the ring and store, the steps, and the slabs'
+// join, in whole rounds of one workgroup a CU. The steps' us in the table are of groups of 128; groups of 32 take 1.2
+// to 1.4 times as long. us it chooses between: 33 x 4,096 x 12,288 in 128 columns and 1 / 2 / 4 / 8 / 16 splits 89 / 50 / 30 / 20 / 20, in 256
+// 100 / 56 / 34 / 23 / 20; 208 x 24,576 x 4,096 in 1 / 2 / 4 / 8 splits of 128 x 128 84 / 87 / 103 / 141, 112 x 256 59 / 77 / 82 / 117, 128 x 256
+// 64 / 79 / 85 / 120; 2,048 x 6,144 x 4,096 in 112 x 256 123, 128 x 256 125, 128 x 128 147.
 Shape choose(int rows, int n_pad, int blocks, int group, bool swiglu) {
   const int mine = (blocks + kAhead * kWaves - 1) / (kAhead * kWaves);
   if (rows <= 16 || (mine == 1 && int64_t(n_pad / 16) * ((rows + 15) / 16) <= 256)) return Shape{0, 0, mine};
-  const int bm = rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
-  const double mblocks = (rows + bm - 1) / bm;
-  Shape best{bm, 128, 1};
+  static constexpr struct {
+    int rows, cols;
+    double step;
+  } kTile[] = {{32, 128, 0.67}, {32, 256, 0.9},  {48, 128, 0.8},   {48, 256, 1.05},  {64, 128, 0.83},
+               {64, 256, 1.14}, {112, 256, 1.58}, {128, 128, 1.18}, {128, 256, 1.77}};
+  Shape best{};
   double least = 1e30;
-  for (int bn = 128; bn <= 256; bn += 128) {
+  for (const auto& tile : kTile) {
+    if (rows <= 64 ? rows > tile.rows || tile.rows > (rows + 15) / 16 * 16 : tile.rows < 112) continue;
     // 128 columns are one tile a wave up to 64 rows: gate and up tiles do not pair there, but in the join
-    const int from = swiglu && bn == 128 && bm <= 64 ? 2 : 1;
-    const double step = (bm == 32 ? 0.45 : bm == 64 ? 0.65 : 0.75) + (bm == 32 ? 0.3 : bm == 64 ? 0.35 : 0.65) * (bn / 128);
+    const int from = swiglu && tile.cols == 128 && tile.rows <= 64 ? 2 : 1;
+    const double step = tile.step * (group == 32 ? (tile.rows > 64 ? 1.4 : 1.2) : 1.0);
+    const double tiles = std::ceil(double(rows) / tile.rows) * ((n_pad + tile.cols - 1) / tile.cols);
     for (int s = from; s <= std::max(from, std::min(16, blocks / 2)); ++s) {
-      const double rounds = std::ceil(mblocks * ((n_pad + bn - 1) / bn) * s / 256);
-      const double join = s > 1 ? 2.5 + double(s) * rows * n_pad * 8 / 4e6 : 0;
-      const double cost = rounds * (2 + std::ceil(double(blocks) / s) * step * (group == 32 ? 1.33 : 1.0)) + join;
+      const double join = s > 1 ? 3.5 + double(s) * rows * n_pad * 8 / 5e6 : 0;
+      const double cost = std::ceil(tiles * s / 256) * (2.5 + std::ceil(double(blocks) / s) * step) + join;
       if (cost < least) {
         least = cost;
-        best = Shape{bm, bn, s};
+        best = Shape{tile.rows, tile.cols, s};
       }
     }
   }
@@ -603,7 +608,9 @@ void pick(const Int4Params& p, const Shape& f, hipStream_t s) {
   if (f.rows == 0) return launch_stream<T, S, G>(p, s);
   const bool wide = f.cols == 256;
   if (f.rows == 32) return wide ? launch_tile<T, S, G, 1, 2, 2>(p, s) : launch_tile<T, S, G, 1, 2, 1>(p, s);
+  if (f.rows == 48) return wide ? launch_tile<T, S, G, 1, 3, 2>(p, s) : launch_tile<T, S, G, 1, 3, 1>(p, s);
   if (f.rows == 64) return wide ? launch_tile<T, S, G, 1, 4, 2>(p, s) : launch_tile<T, S, G, 1, 4, 1>(p, s);
+  if (f.rows == 112) return launch_tile<T, S, G, 1, 7, 2>(p, s);
   return wide ? launch_tile<T, S, G, 1, 8, 2>(p, s) : launch_tile<T, S, G, 2, 4, 2>(p, s);
 }
 
