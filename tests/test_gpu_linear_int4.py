@@ -54,6 +54,10 @@ SHAPES = [
     (4001, 1024, 32, True, 0, 3),
     (6144, 2176, 64, False, 0, 0),
     (1056, 12288, 128, True, 0, 0),  # a long walk over k
+    (8224, 2944, 128, True, 0, 0),   # 1, 2, 3 and 4 blocks a wave, walked over more tiles than workgroups
+    (8224, 1920, 32, True, 0, 0),
+    (8224, 4000, 32, False, 0, 0),
+    (8224, 4096, 64, True, 0, 0),
     (24608, 640, 128, True, 0, 0),   # many columns
 ]
 
