@@ -586,16 +586,17 @@ struct Shape {
   int rows, cols, splits;
 };
 
-// The stream kernel up to 16 rows, its splits as many blocks as its waves hold, and for more rows while every 16 x 16 tile has
-// a CU of its own (64 x 1,024 x 4,096: 8.2 us, 11.8 in tiles; 32 x 4,096 x 4,096, past it, 12.9 and 12.1). Else the shortest
-// of the tiles and splits by what the kernel's parts measured: 2.5 us to fill the ring and store, the steps, and the slabs'
-// join, in whole rounds of one workgroup a CU. The steps' us in the table are of groups of 128; groups of 32 take 1.2
-// to 1.4 times as long. us it chooses between: 33 x 4,096 x 12,288 in 128 columns and 1 / 2 / 4 / 8 / 16 splits 89 / 50 / 30 / 20 / 20, in 256
+// The stream kernel up to 16 rows, its splits as many blocks as its waves hold. Else the shortest of it (without splits) and
+// the tiles and splits by what the kernels' parts measured: 1 us to start, 2.5 us to fill the ring and store and the steps in
+// whole rounds of one workgroup a CU, and the slabs' join. The steps' us in the table are of groups of 128; groups of 32 take 1.2
+// to 1.4 times as long. The stream kernel takes 2.5 us and in each round 1.25 for a block of each of a workgroup's waves. us it chooses between:
+// 64 x 1,024 x 4,096 in stream 8.2, in tiles 11.8; 64 x 2,048 x 1,024 5.2, 9.1; 128 x 2,048 x 2,048 13.3, 14.9;
+// 128 x 4,096 x 256 12.0, 7.5; 64 x 4,096 x 4,096 22.1, 15.5; 33 x 4,096 x 12,288 in 128 columns and 1 / 2 / 4 / 8 / 16 splits 89 / 50 / 30 / 20 / 20, in 256
 // 100 / 56 / 34 / 23 / 20; 208 x 24,576 x 4,096 in 1 / 2 / 4 / 8 splits of 128 x 128 84 / 87 / 103 / 141, 112 x 256 59 / 77 / 82 / 117, 128 x 256
 // 64 / 79 / 85 / 120; 2,048 x 6,144 x 4,096 in 112 x 256 123, 128 x 256 125, 128 x 128 147.
 Shape choose(int rows, int n_pad, int blocks, int group, bool swiglu) {
   const int mine = (blocks + kMostAhead * kWaves - 1) / (kMostAhead * kWaves);
-  if (rows <= 16 || (mine == 1 && int64_t(n_pad / 16) * ((rows + 15) / 16) <= 256)) return Shape{0, 0, mine};
+  if (rows <= 16) return Shape{0, 0, mine};
   static constexpr struct {
     int rows, cols;
     double step;
@@ -603,6 +604,12 @@ Shape choose(int rows, int n_pad, int blocks, int group, bool swiglu) {
                {64, 256, 1.14}, {112, 256, 1.58}, {128, 128, 1.18}, {128, 256, 1.77}};
   Shape best{};
   double least = 1e30;
+  if (mine == 1) {
+    const int halves = swiglu ? 2 : 1;  // a workgroup takes a gate and its up tile
+    const double tiles = std::ceil(rows / 16.0) * (n_pad / 16 / halves);
+    best = Shape{0, 0, 1};
+    least = 2.5 + std::ceil(tiles / 256) * halves * ((blocks + kWaves - 1) / kWaves) * 1.25;
+  }
   for (const auto& tile : kTile) {
     if (rows <= 64 ? rows > tile.rows || tile.rows > (rows + 15) / 16 * 16 : tile.rows < 112) continue;
     // 128 columns are one tile a wave up to 64 rows: gate and up tiles do not pair there, but in the join
@@ -611,7 +618,7 @@ Shape choose(int rows, int n_pad, int blocks, int group, bool swiglu) {
     const double tiles = std::ceil(double(rows) / tile.rows) * ((n_pad + tile.cols - 1) / tile.cols);
     for (int s = from; s <= std::max(from, std::min(16, blocks / 2)); ++s) {
       const double join = s > 1 ? 3.5 + double(s) * rows * n_pad * 8 / 5e6 : 0;
-      const double cost = std::ceil(tiles * s / 256) * (2.5 + std::ceil(double(blocks) / s) * step) + join;
+      const double cost = 1 + std::ceil(tiles * s / 256) * (2.5 + std::ceil(double(blocks) / s) * step) + join;
       if (cost < least) {
         least = cost;
         best = Shape{tile.rows, tile.cols, s};
