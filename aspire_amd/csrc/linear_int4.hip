@@ -120,16 +120,20 @@ __device__ __forceinline__ void store4(const Int4Params& p, int64_t m, int col, 
 }
 
 constexpr int kWaves = 8;
-constexpr int kMostAhead = 4;  // blocks of 1 KiB a wave has, and has in flight, of a tile: at most
+// Blocks of 1 KiB a wave has, and has in flight, of a tile: at most 6, or 8 where that saves the splits and their join (groups
+// of 32 have no registers for it).
+constexpr int most_ahead(int blocks, int group) { return group > 32 && blocks <= 8 * kWaves ? 8 : 6; }
 
 // Few rows (16 to a blockIdx.z): bound by the weights' stream. A workgroup walks over output tiles of 16 columns (with swiglu over pairs of a
-// gate and an up tile), for all of k or the split blockIdx.y of at most kMostAhead * kWaves blocks; its waves take the blocks of
+// gate and an up tile), for all of k or the split blockIdx.y of at most 6 or 8 blocks a wave; its waves take the blocks of
 // 128 k in turn, keep their x in registers, and add up through LDS, in a fixed order. A block is asked for as soon as
 // the one before it in its registers is multiplied, across the ends of tiles, so the stream never pauses. kAhead is the
 // blocks that a wave has, so that a short k loads none twice: 16 x 24,576 x 1,024 with 1 7.3 us, with 4 14.9; 16 x 24,576 x
-// 2,048 with 2 11.4, with 4 16.6.
+// 2,048 with 2 11.4, with 4 16.6. More than 4 leave a CU one workgroup, and are still faster than splits of at most 4 with
+// their join: 1 x 4,096 x 6,144 with 6 7.5 us, in two splits 9.2; 16 x 24,576 x 8,192 with 8 32.0, in two 34.6; 16 x 4,096 x
+// 12,288 in two splits of 6 17.2, in three of 4 19.0. Two splits of 8 are not: 1 x 4,096 x 16,384 17.2, four of 4 16.2.
 template <class T, class S, int G, int kAhead>
-__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(G == 128 || kAhead < 4 ? 4 : 3))) void int4_stream_kernel(Int4Params p) {
+__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(kAhead > 4 ? 2 : G == 128 || kAhead < 4 ? 4 : 3))) void int4_stream_kernel(Int4Params p) {
   constexpr int kParts = 128 / G;   // groups of a block
   constexpr int kSteps = 4 / kParts;
   __shared__ float4 sums[2][kWaves][64];
@@ -564,13 +568,21 @@ void launch_join(const Int4Params& p, hipStream_t s) {
 template <class T, class S, int G>
 void launch_stream(const Int4Params& p, hipStream_t s) {
   const int tiles = p.swiglu ? p.n / 16 : p.splits > 1 ? p.n_pad / 16 : (p.n + 15) / 16;
-  // two workgroups a CU at most; the second ones take what is over of an uneven number of tiles
-  const dim3 grid(std::min(tiles, std::max(1, 512 / p.splits)), p.splits, (p.rows + 15) / 16), block(64 * kWaves);
-  switch (((p.blocks + p.splits - 1) / p.splits + kWaves - 1) / kWaves) {
+  const int ahead = ((p.blocks + p.splits - 1) / p.splits + kWaves - 1) / kWaves;
+  // two workgroups a CU at most, as the registers allow; the second ones take what is over of an uneven number of tiles
+  const dim3 grid(std::min(tiles, std::max(1, (ahead > 4 ? 256 : 512) / p.splits)), p.splits, (p.rows + 15) / 16), block(64 * kWaves);
+  switch (ahead) {
     case 1: hipLaunchKernelGGL((int4_stream_kernel<T, S, G, 1>), grid, block, 0, s, p); break;
     case 2: hipLaunchKernelGGL((int4_stream_kernel<T, S, G, 2>), grid, block, 0, s, p); break;
     case 3: hipLaunchKernelGGL((int4_stream_kernel<T, S, G, 3>), grid, block, 0, s, p); break;
-    default: hipLaunchKernelGGL((int4_stream_kernel<T, S, G, 4>), grid, block, 0, s, p);
+    case 4: hipLaunchKernelGGL((int4_stream_kernel<T, S, G, 4>), grid, block, 0, s, p); break;
+    case 5: hipLaunchKernelGGL((int4_stream_kernel<T, S, G, 5>), grid, block, 0, s, p); break;
+    case 6: hipLaunchKernelGGL((int4_stream_kernel<T, S, G, 6>), grid, block, 0, s, p); break;
+    default:
+      if constexpr (G > 32) {
+        if (ahead == 7) hipLaunchKernelGGL((int4_stream_kernel<T, S, G, 7>), grid, block, 0, s, p);
+        else hipLaunchKernelGGL((int4_stream_kernel<T, S, G, 8>), grid, block, 0, s, p);
+      }
   }
 }
 
@@ -595,7 +607,7 @@ struct Shape {
 // 100 / 56 / 34 / 23 / 20; 208 x 24,576 x 4,096 in 1 / 2 / 4 / 8 splits of 128 x 128 84 / 87 / 103 / 141, 112 x 256 59 / 77 / 82 / 117, 128 x 256
 // 64 / 79 / 85 / 120; 2,048 x 6,144 x 4,096 in 112 x 256 123, 128 x 256 125, 128 x 128 147.
 Shape choose(int rows, int n_pad, int blocks, int group, bool swiglu) {
-  const int mine = (blocks + kMostAhead * kWaves - 1) / (kMostAhead * kWaves);
+  const int most = most_ahead(blocks, group) * kWaves, mine = (blocks + most - 1) / most;
   if (rows <= 16) return Shape{0, 0, mine};
   static constexpr struct {
     int rows, cols;

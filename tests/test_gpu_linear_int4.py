@@ -54,7 +54,12 @@ SHAPES = [
     (4001, 1024, 32, True, 0, 3),
     (6144, 2176, 64, False, 0, 0),
     (1056, 12288, 128, True, 0, 0),  # a long walk over k
-    (8224, 2944, 128, True, 0, 0),   # 1, 2, 3 and 4 blocks a wave, walked over more tiles than workgroups
+    (4112, 5120, 128, False, 0, 0),  # 5 to 8 blocks a wave, walked over more tiles than workgroups
+    (4112, 6080, 64, True, 0, 0),
+    (4112, 6144, 32, True, 0, 0),
+    (4112, 7168, 128, True, 0, 0),
+    (4112, 8000, 64, False, 0, 0),
+    (8224, 2944, 128, True, 0, 0),   # 2, 3 and 4
     (8224, 1920, 32, True, 0, 0),
     (8224, 4000, 32, False, 0, 0),
     (8224, 4096, 64, True, 0, 0),
@@ -86,7 +91,7 @@ def test_products(gpu, n, k, group, zeros, xpad, opad, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF, HF])
-@pytest.mark.parametrize("n,k,group,zeros", [(32, 128, 128, True), (1056, 2208, 32, True), (2080, 640, 64, False),
+@pytest.mark.parametrize("n,k,group,zeros", [(32, 128, 128, True), (1056, 2208, 32, True), (2080, 640, 64, False), (8256, 8192, 64, True),
                                              (24576, 512, 128, True)])
 def test_swiglu(gpu, n, k, group, zeros, dtype):
     packed, scales, z, w = weights(n, k, group, zeros, dtype, gpu)
