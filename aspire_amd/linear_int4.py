@@ -64,10 +64,13 @@ class Int4Weight:
         codes[..., 2] = hi[..., 0] | (hi[..., 1] << 4)
         codes[..., 3] = hi[..., 2] | (hi[..., 3] << 4)
         parts = 128 // group
-        # [tile, row, block, group of it] -> [tile, block, row / 4, group, row % 4] and [tile, block, row, group]
-        scales = fill(scales, tiles * 16, blocks * parts).reshape(tiles, 4, 4, blocks, parts).permute(0, 3, 1, 4, 2).contiguous()
+        # [tile, row, block, group of it] -> [tile, block, row / 4, group, row % 4] and [tile, block, row, group]; clones, as one
+        # block of 128 k has that order already, and contiguous() would hand the caller's own memory on
+        scales = fill(scales, tiles * 16, blocks * parts).reshape(tiles, 4, 4, blocks, parts).permute(0, 3, 1, 4, 2)
+        scales = scales.clone(memory_format=torch.contiguous_format)
         if zeros is not None:
-            zeros = fill(zeros, tiles * 16, blocks * parts).reshape(tiles, 16, blocks, parts).transpose(1, 2).contiguous()
+            zeros = fill(zeros, tiles * 16, blocks * parts).reshape(tiles, 16, blocks, parts).transpose(1, 2)
+            zeros = zeros.clone(memory_format=torch.contiguous_format)
         return cls((n, k), group, codes.view(tiles, blocks, 64, 16), scales, zeros)
 
     @classmethod

@@ -100,3 +100,21 @@ def test_entry_point_refuses_on_the_host():
         assert call(**kw) == _lib.ASPIRE_ERR_INVALID, kw
     assert call(rows=0) == _lib.ASPIRE_OK and call(n=0) == _lib.ASPIRE_OK
     assert L.aspire_linear_int4(None, None) == _lib.ASPIRE_ERR_INVALID
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("k", [128, 256])
+def test_weights_keep_their_own_copy(k, group):
+    """A loader's buffers, whatever their offset, are free when the weights are made: with one block of k the layout
+    has the order of the checkpoint's own scales and zero points."""
+    n, parts = 32, k // group
+    g = torch.Generator().manual_seed(k + group)
+    packed = torch.randint(0, 256, (n * k // 2 + 1,), dtype=torch.uint8, generator=g)[1:].view(n, k // 2)
+    scales = torch.rand(n * parts + 1, generator=g).to(torch.bfloat16)[1:].view(n, parts)
+    zeros = torch.randint(0, 16, (n * parts + 1,), dtype=torch.uint8, generator=g)[1:].view(n, parts)
+    w = Int4Weight.from_packed(packed, scales, zeros, group=group)
+    before = w.dequantize().clone()
+    for mine, given in ((w.codes, packed), (w.scales, scales), (w.zeros, zeros)):
+        assert mine.untyped_storage().data_ptr() != given.untyped_storage().data_ptr() and mine.data_ptr() % 16 == 0
+        given.zero_()
+    assert torch.equal(w.dequantize(), before)
