@@ -13,6 +13,7 @@ import threading
 from pathlib import Path
 
 import torch
+from torch.autograd import forward_ad
 
 # ASPIRE_HIP_LIB selects another build of the same library (a compile-time kernel variant made
 # with ``build.py --define ... --out ...``), for A/B measurements.
@@ -327,6 +328,13 @@ def require_cuda(*tensors: torch.Tensor, what: str) -> None:
         if t is not None and not t.is_cuda:
             raise RuntimeError(f"{what}: tensors must be on a ROCm GPU (got {t.device}); "
                                "there is no CPU implementation")
+
+
+def has_tangent(*tensors) -> bool:
+    """Whether one of the tensors (None: none) is a dual tensor of forward-mode differentiation, which ``requires_grad``
+    does not show."""
+    return forward_ad._current_level >= 0 and any(
+        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def dense(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:

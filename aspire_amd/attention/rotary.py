@@ -206,9 +206,9 @@ class RotaryEmbedding:
 
     # -------------------------------------------------------------- operators
     def apply(self, q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor):
-        """``(q, k)`` turned at ``positions`` ``[T]``, as new tensors (``k`` may be None); differentiable. Tokens at
-        negative positions are copied."""
-        if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        """``(q, k)`` turned at ``positions`` ``[T]``, as new tensors (``k`` may be None); differentiable, in reverse and in
+        forward mode. Tokens at negative positions are copied."""
+        if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)) or _lib.has_tangent(q, k):
             return _Turn.apply(q, k, positions, self, False)
         return self._turn(q, k, positions, False, False, "RotaryEmbedding.apply")
 
@@ -270,29 +270,43 @@ class RotaryEmbedding:
 
 
 class _Turn(torch.autograd.Function):
-    """The turn by the positions' angles, or back; each is the other's gradient."""
+    """The turn by the positions' angles, or back; each is the other's gradient. It is linear: tangents turn as values do."""
 
     @staticmethod
     def forward(ctx, q, k, positions, rotary, inverse):
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(positions)
+        ctx.save_for_forward(positions)
         ctx.rotary, ctx.inverse = rotary, inverse
+        ctx.shapes = None if q is None else q.shape, None if k is None else k.shape
         return rotary._turn(q, k, positions, inverse, False, "RotaryEmbedding.apply")
 
     @staticmethod
-    def backward(ctx, dq, dk):
+    def _again(ctx, a, b, inverse):
+        """Gradients or tangents of q and k (either may be None) turned, themselves differentiable."""
         (positions,) = ctx.saved_tensors
-        if dq is None and dk is None:
-            return None, None, None, None, None
-        if dq is not None and dq.stride(2) != 1:
-            dq = dq.contiguous()
-        if dk is not None and dk.stride(2) != 1:
-            dk = dk.contiguous()
-        if torch.is_grad_enabled():  # a second derivative is wanted
-            gq, gk = _Turn.apply(dq, dk, positions, ctx.rotary, not ctx.inverse)
-        else:
-            gq, gk = ctx.rotary._turn(dq, dk, positions, not ctx.inverse, False, "RotaryEmbedding.apply")
-        return gq, gk, None, None, None
+        if a is None and b is None:
+            return None, None
+        if a is not None and a.stride(2) != 1:
+            a = a.contiguous()
+        if b is not None and b.stride(2) != 1:
+            b = b.contiguous()
+        if torch.is_grad_enabled() or _lib.has_tangent(a, b):  # a second derivative is wanted
+            return _Turn.apply(a, b, positions, ctx.rotary, inverse)
+        return ctx.rotary._turn(a, b, positions, inverse, False, "RotaryEmbedding.apply")
+
+    @staticmethod
+    def backward(ctx, dq, dk):
+        return *_Turn._again(ctx, dq, dk, not ctx.inverse), None, None, None
+
+    @staticmethod
+    def jvp(ctx, tq, tk, *_):
+        # an output that is not None needs a tangent; one of the two is there
+        if tq is None and ctx.shapes[0] is not None:
+            tq = tk.new_zeros(ctx.shapes[0])
+        if tk is None and ctx.shapes[1] is not None:
+            tk = tq.new_zeros(ctx.shapes[1])
+        return _Turn._again(ctx, tq, tk, ctx.inverse)
 
 
 __all__ = ["RotaryConfig", "RotaryEmbedding"]

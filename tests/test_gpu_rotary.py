@@ -3,6 +3,7 @@
 import numpy as np
 import pytest
 import torch
+import torch.autograd.forward_ad as fwad
 
 from aspire_amd.attention.rotary import RotaryConfig, RotaryEmbedding
 from helpers import bits, say
@@ -389,3 +390,27 @@ def test_refusals(gpu):
     assert empty[0].shape == (0, 4, 64) and empty[1].shape == (0, 2, 64)
     rot.append(q[:0], k[:0], v[:0], dev[0], cache, dev[1], dev[2], dev[3], 16)
     assert not cache.any()
+
+
+@pytest.mark.parametrize("dtype", [BF, SF])
+def test_forward_mode(gpu, dtype):
+    """Tangents of a dual q and k, one alone, and the tangent of a gradient."""
+    say("rotary forward mode", dtype)
+    config = RotaryConfig(head_dim=80, rotary_dim=20, layout="interleaved", **CONFIGS["yarn"])
+    rot = RotaryEmbedding(config, gpu)
+    q, k, _ = (t.contiguous() for t in tensors(9, 4, 2, 80, dtype, gpu))
+    tq, tk, dq = torch.randn_like(q), torch.randn_like(k), torch.randn_like(q)
+    pos = torch.arange(9) * 1001 - 1
+    with fwad.dual_level():
+        a, b = rot.apply(fwad.make_dual(q, tq), fwad.make_dual(k, tk), pos.to(gpu))
+        close(a, turned(q, pos, config), q, config)
+        close(fwad.unpack_dual(a).tangent, turned(tq, pos, config), tq, config)
+        close(fwad.unpack_dual(b).tangent, turned(tk, pos, config), tk, config)
+        a, b = rot.apply(q, fwad.make_dual(k, tk), pos.to(gpu))
+        assert not fwad.unpack_dual(a).tangent.any()
+        close(fwad.unpack_dual(b).tangent, turned(tk, pos, config), tk, config)
+        leaf = q.clone().requires_grad_()
+        a, _ = rot.apply(leaf, None, pos.to(gpu))
+        (grad,) = torch.autograd.grad(a, [leaf], fwad.make_dual(dq, tq))
+        close(grad, turned(dq, pos, config, inverse=True), dq, config)
+        close(fwad.unpack_dual(grad).tangent, turned(tq, pos, config, inverse=True), tq, config)

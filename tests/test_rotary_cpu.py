@@ -6,6 +6,7 @@ import math
 import numpy as np
 import pytest
 import torch
+import torch.autograd.forward_ad as fwad
 
 from aspire_amd import _lib
 from aspire_amd.attention import rotary
@@ -108,3 +109,48 @@ def test_cpu_tensors_are_refused():
     for call in calls:
         with pytest.raises(RuntimeError, match="GPU"):
             call()
+
+
+class PlainTurn(RotaryEmbedding):
+    """The turn in elementary operations, for what autograd does around it (half layout, whole heads)."""
+
+    def _turn(self, q, k, positions, inverse, in_place, what):
+        f = torch.tensor(self.config.frequencies(), dtype=torch.float64)
+        angle = positions.double()[:, None, None] * f * (-1 if inverse else 1)
+        outs = []
+        for x in (q, k):
+            a, b = (None, None) if x is None else x.detach().double().chunk(2, dim=-1)
+            y = None if x is None else torch.cat([a * angle.cos() - b * angle.sin(), b * angle.cos() + a * angle.sin()], -1)
+            outs.append(None if x is None else y.to(x.dtype))
+        return tuple(outs)
+
+
+def test_apply_carries_forward_mode_tangents():
+    """A dual tensor's tangent turns as the values do (with grad mode on and off, of q or k alone, beside a gradient), and a
+    gradient's tangent turns back."""
+    rot = PlainTurn(RotaryConfig(head_dim=8), "cpu")
+    pos = torch.tensor([3, 5, 11])
+    g = torch.Generator().manual_seed(0)
+    q, k, tq, tk = (torch.randn(3, h, 8, generator=g, dtype=torch.float64) for h in (4, 2, 4, 2))
+    wq, wk = rot._turn(tq, tk, pos, False, False, "")
+    back, _ = rot._turn(tq, None, pos, True, False, "")
+    with fwad.dual_level():
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad):
+                a, b = rot.apply(fwad.make_dual(q, tq), fwad.make_dual(k, tk), pos)
+                assert torch.equal(fwad.unpack_dual(a).tangent, wq) and torch.equal(fwad.unpack_dual(b).tangent, wk)
+                a, b = rot.apply(q, fwad.make_dual(k, tk), pos)
+                assert torch.equal(fwad.unpack_dual(b).tangent, wk) and torch.equal(a, rot.apply(q, None, pos)[0])
+                assert not fwad.unpack_dual(a).tangent.any()
+                a, none = rot.apply(fwad.make_dual(q, tq), None, pos)
+                assert torch.equal(fwad.unpack_dual(a).tangent, wq) and none is None
+                a, _ = rot.apply(fwad.make_dual(q, tq.transpose(0, 2).contiguous().transpose(0, 2)), None, pos)
+                assert torch.equal(fwad.unpack_dual(a).tangent, wq)
+        leaf = q.clone().requires_grad_()
+        a, _ = rot.apply(fwad.make_dual(leaf, tq), None, pos)
+        assert torch.equal(fwad.unpack_dual(a).tangent, wq)
+        (grad,) = torch.autograd.grad(a, [leaf], fwad.make_dual(torch.ones_like(q), tq))
+        assert torch.equal(fwad.unpack_dual(grad).tangent, back)
+        a, b = rot.apply(leaf, k.clone().requires_grad_(), pos)
+        (grad,) = torch.autograd.grad([a, b], [leaf], [fwad.make_dual(torch.ones_like(q), tq), torch.ones_like(k)])
+        assert torch.equal(fwad.unpack_dual(grad).tangent, back)
