@@ -215,7 +215,7 @@ class RotaryEmbedding:
     def apply_inplace(self, q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor) -> None:
         """``apply`` on q and k themselves (not differentiable; no two of their rows may share memory)."""
         what = "RotaryEmbedding.apply_inplace"
-        if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)) or _lib.has_tangent(q, k):
             raise ValueError(f"{what}: not differentiable; use apply")
         self._turn(q, k, positions, False, True, what)
 
@@ -229,6 +229,9 @@ class RotaryEmbedding:
         row are padding: their q passes unchanged, and nothing is written to the cache; nor is it for a token whose
         page id or list entry lies outside the pool or the list. No two tokens may share a slot."""
         what = "RotaryEmbedding.append"
+        if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad) \
+                or _lib.has_tangent(q, k, v, q_out, kv_cache):
+            raise ValueError(f"{what}: not differentiable")
         code, dtype = self._dtype(q, what), q.dtype
         if code == 2:
             raise ValueError(f"{what}: the cache holds bf16 or fp16")
@@ -236,8 +239,6 @@ class RotaryEmbedding:
         kv_shape, ka = self._heads(k, dtype, what, "k")
         v_shape, va = self._heads(v, dtype, what, "v")
         tokens, hkv = shape[0], kv_shape[1]
-        if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-            raise ValueError(f"{what}: not differentiable")
         qo = qa
         if q_out is None:
             q_out = q

@@ -130,6 +130,8 @@ def linear_int4(x: torch.Tensor, w: Int4Weight, out: torch.Tensor, *, swiglu: bo
     from x. Not differentiable. A row of x with an infinity or NaN (or bf16 values of 2^112 and more, whose sums may overflow on the way) gives
     no finite outputs; the other rows are not touched by it."""
     what = "linear_int4"
+    if torch.is_grad_enabled() and x.requires_grad or _lib.has_tangent(x, out, w.scales):
+        raise ValueError(f"{what}: not differentiable")
     if not (x.is_cuda and out.is_cuda and w.codes.is_cuda):
         _lib.require_cuda(x, out, w.codes, what=what)
     n, k = w.shape
@@ -144,8 +146,6 @@ def linear_int4(x: torch.Tensor, w: Int4Weight, out: torch.Tensor, *, swiglu: bo
     index = w.codes.get_device()
     if x.get_device() != index or out.get_device() != index:
         raise ValueError(f"{what}: x, out and the weights must be on one device")
-    if torch.is_grad_enabled() and x.requires_grad:
-        raise ValueError(f"{what}: not differentiable")
     L = _lib.lib()
     floats, ws = L.aspire_linear_int4_workspace(rows, n, k, w.group, swiglu), 0
     if floats:

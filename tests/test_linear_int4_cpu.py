@@ -4,6 +4,7 @@ import ctypes
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwad
 
 from aspire_amd import _lib, linear_int4
 from aspire_amd.linear_int4 import Int4Weight
@@ -118,3 +119,15 @@ def test_weights_keep_their_own_copy(k, group):
         assert mine.untyped_storage().data_ptr() != given.untyped_storage().data_ptr() and mine.data_ptr() % 16 == 0
         given.zero_()
     assert torch.equal(w.dequantize(), before)
+
+
+def test_dual_tensors_are_refused():
+    """There is no derivative in forward mode either."""
+    w = Int4Weight.quantize(torch.ones(16, 64), group=64)
+    x, out = torch.zeros(2, 64, dtype=torch.bfloat16), torch.zeros(2, 16, dtype=torch.bfloat16)
+    with fwad.dual_level():
+        dual = lambda t: fwad.make_dual(t, torch.ones_like(t))
+        scaled = Int4Weight(w.shape, w.group, w.codes, dual(w.scales), w.zeros)
+        for args in ((dual(x), w, out), (x, w, dual(out)), (x, scaled, out)):
+            with pytest.raises(ValueError, match="not differentiable"):
+                linear_int4.linear_int4(*args)

@@ -154,3 +154,18 @@ def test_apply_carries_forward_mode_tangents():
         a, b = rot.apply(leaf, k.clone().requires_grad_(), pos)
         (grad,) = torch.autograd.grad([a, b], [leaf], [fwad.make_dual(torch.ones_like(q), tq), torch.ones_like(k)])
         assert torch.equal(fwad.unpack_dual(grad).tangent, back)
+
+
+def test_dual_tensors_are_refused_where_there_is_no_derivative():
+    rot = RotaryEmbedding(RotaryConfig(head_dim=64), "cpu")
+    x, i, pos = torch.zeros(1, 1, 64).half(), torch.zeros(2, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    cache = torch.zeros(1, 2, 16, 1, 64).half()
+    with fwad.dual_level():
+        dual = lambda t: fwad.make_dual(t, torch.ones_like(t))
+        calls = [lambda: rot.apply_inplace(dual(x), None, pos), lambda: rot.apply_inplace(x, dual(x.clone()), pos)]
+        for at in range(5):
+            given = [dual(t) if n == at else t for n, t in enumerate((x, x, x, cache, x.clone()))]
+            calls.append(lambda a=given: rot.append(*a[:3], i, a[3], i, i, i[:1], 16, q_out=a[4]))
+        for call in calls:
+            with pytest.raises(ValueError, match="not differentiable"):
+                call()
