@@ -9,8 +9,9 @@
   (the smoothing of ``RopeConfig``), ``"yarn"`` (between the pairs that turn ``beta_fast`` and ``beta_slow`` times
   over the trained context ``f`` becomes ``f / factor`` linearly; cos and sin times ``0.1 ln(factor) + 1``), or
   divided by given ``pair_factors``;
-* angles ``position * f_i`` are exact at any position (64-bit fixed point), cos and sin and the products fp32, one
-  rounding to the output's type.
+* a frequency is the nearest 64-bit fraction of a turn, made from some 60 digits, and its product with the position drops
+  whole turns only: angles ``position * f_i`` are within ``position * 2^-65`` turns (2^-24 radians at 2^38); cos and sin
+  and the products fp32, one rounding to the output's type.
 
 ``apply`` is differentiable (the gradient turns back by the same angles); ``append`` is
 ``mylib::update_kv_padded`` (aspire/attention/kv_ops.py:63-187) with the turn on the way, one launch.
@@ -21,6 +22,7 @@ from __future__ import annotations
 import math
 import struct
 from dataclasses import dataclass
+from decimal import Context, Decimal, localcontext
 
 import torch
 
@@ -29,6 +31,7 @@ from aspire_amd import _lib
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 SCALINGS = ("none", "linear", "llama3", "yarn")
 MAX_HEAD_DIM = 256
+_PI = Decimal("3.1415926535897932384626433832795028841971693993751058209749445923078164062862089986")
 
 
 @dataclass(frozen=True)
@@ -81,35 +84,46 @@ class RotaryConfig:
             return float(self.amplitude)
         return 0.1 * math.log(self.factor) + 1.0 if self.scaling == "yarn" and self.factor > 1 else 1.0
 
+    def _exact_frequencies(self) -> list[Decimal]:
+        """Radians a position of each pair, to more digits than 64 bits of a turn need (whole turns of a small theta or
+        divisor are dropped later, so their digits come on top)."""
+        r, divisors = self.rotated, (self.factor, *(self.pair_factors or ()))
+        whole = max(0.0, -math.log10(self.theta)) + max(0.0, -math.log10(min(divisors)))
+        with localcontext(Context(prec=60 + math.ceil(whole))):
+            exact = lambda x: Decimal(float(x))
+            ratio, base = (exact(self.theta).ln() * -2 / r).exp(), [Decimal(1)]
+            while len(base) < r // 2:
+                base.append(base[-1] * ratio)
+            if self.pair_factors is not None:
+                return [f / exact(s) for f, s in zip(base, self.pair_factors)]
+            factor = exact(self.factor)
+            if self.scaling == "linear":
+                return [f / factor for f in base]
+            if self.scaling == "llama3":
+                lo, hi, old = exact(self.low_freq_factor), exact(self.high_freq_factor), exact(self.original_max_position)
+                ramp = [(old * f / (2 * _PI) - lo) / (hi - lo) for f in base]
+            elif self.scaling == "yarn":
+                def at(turns):  # the pair that turns so often over the trained context
+                    return r * math.log(self.original_max_position / (2 * math.pi * turns)) / (2 * math.log(self.theta))
+                first, last = max(math.floor(at(self.beta_fast)), 0), min(math.ceil(at(self.beta_slow)), r - 1)
+                width = Decimal(max(last - first, 0.001))
+                ramp = [1 - (i - first) / width for i in range(r // 2)]
+            else:
+                return base
+            keep = [min(max(t, Decimal(0)), Decimal(1)) for t in ramp]
+            return [t * f + (1 - t) * f / factor for t, f in zip(keep, base)]
+
     def frequencies(self) -> list[float]:
-        """Radians a position of each pair (64-bit)."""
-        r = self.rotated
-        base = [self.theta ** (-2.0 * i / r) for i in range(r // 2)]
-        if self.pair_factors is not None:
-            return [f / s for f, s in zip(base, self.pair_factors)]
-        if self.scaling == "linear":
-            return [f / self.factor for f in base]
-        if self.scaling == "llama3":
-            lo, hi, old = self.low_freq_factor, self.high_freq_factor, self.original_max_position
-            keep = [min(max((old * f / (2 * math.pi) - lo) / (hi - lo), 0.0), 1.0) for f in base]
-        elif self.scaling == "yarn":
-            def at(turns):  # the pair that turns so often over the trained context
-                return r * math.log(self.original_max_position / (2 * math.pi * turns)) / (2 * math.log(self.theta))
-            first, last = max(math.floor(at(self.beta_fast)), 0), min(math.ceil(at(self.beta_slow)), r - 1)
-            width = max(last - first, 0.001)
-            keep = [1.0 - min(max((i - first) / width, 0.0), 1.0) for i in range(r // 2)]
-        else:
-            return base
-        return [t * f + (1.0 - t) * f / self.factor for t, f in zip(keep, base)]
+        """Radians a position of each pair, as the nearest doubles."""
+        return [float(f) for f in self._exact_frequencies()]
 
-
-def _turns(frequencies) -> torch.Tensor:
-    """Frequencies as 64-bit fixed-point fractions of a turn a position (int64 holding the bits)."""
-    out = []
-    for f in frequencies:
-        t = int(math.fmod(f / (2 * math.pi), 1.0) * 2.0 ** 64) % (1 << 64)
-        out.append(t - (1 << 64) if t >> 63 else t)
-    return torch.tensor(out, dtype=torch.int64)
+    def _turns(self) -> torch.Tensor:
+        """The frequencies as 64-bit fixed-point fractions of a turn a position, to the nearest (int64 holding the bits)."""
+        frequencies = self._exact_frequencies()
+        with localcontext(Context(prec=60 + max(0, *(f.adjusted() for f in frequencies)))):
+            turn, half = 2 * _PI, Decimal("0.5")
+            turns = [int(f / turn % 1 * 2 ** 64 + half) % (1 << 64) for f in frequencies]
+        return torch.tensor([t - (1 << 64) if t >> 63 else t for t in turns], dtype=torch.int64)
 
 
 def _same_place(a: torch.Tensor, b: torch.Tensor) -> bool:
@@ -131,7 +145,7 @@ class RotaryEmbedding:
 
     def __init__(self, config: RotaryConfig, device="cuda"):
         self.config = config
-        self.turns = _turns(config.frequencies()).to(device)
+        self.turns = config._turns().to(device)
         self.device = self.turns.device
         self._index = self.turns.get_device() if self.turns.is_cuda else -2  # (-2: no tensor's)
         self._dims = (config.head_dim, config.rotated, int(config.layout == "interleaved"))

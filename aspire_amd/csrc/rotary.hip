@@ -5,9 +5,9 @@
 //     y_a = A (a cos - b sin),  y_b = A (b cos + a sin);   dims (i, i + R/2) or (2i, 2i + 1) of the first R.
 // The transpose, which the gradient needs, turns back by the same angle (`inverse`).
 //
-// Angles: f_i comes as a 64-bit fixed-point fraction of a turn, so p f_i modulo one turn is one 64-bit
-// product that drops its overflow, exact for every position; the fp32 product of other rotary codes is
-// off by 2^-24 of the whole angle, 0.06 radians at a million tokens. What is left is reduced to an
+// Angles: f_i comes as the nearest 64-bit fixed-point fraction of a turn, so p f_i modulo one turn is one 64-bit
+// product that drops its overflow and adds no rounding: off by p 2^-65 turns at most, below 2^-24 radians up to position
+// 2^38; the fp32 product of other rotary codes is off by 2^-24 of the whole angle, 0.06 radians at a million tokens. What is left is reduced to an
 // eighth of a turn by its top bits, and the series of sin and cos there end below 2^-26.
 //
 // Bound by HBM at prompt sizes (each value read once and written once: 8,192 tokens of 32 q and 8 kv heads of 128 in
@@ -71,7 +71,7 @@ struct alignas(sizeof(T) * VEC) Vec { T e[VEC]; };
 __device__ __forceinline__ float2 cos_sin_of_turn(uint64_t t) {
   const uint32_t quarter = uint32_t((t + (uint64_t(1) << 61)) >> 62);
   const int64_t r = int64_t(t - (uint64_t(quarter) << 62));  // [-2^61, 2^61): an eighth of a turn either way
-  // both halves as floats keep 24 bits of a small angle, too
+  // r to 24 bits, or (a small r below 0, whose low half is near 2^32) to 2^-56 of a turn
   const float turn = fmaf(float(int32_t(r >> 32)), 4294967296.f, float(uint32_t(r)));
   const float x = turn * 3.4061215800304843e-19f;            // 2 pi / 2^64
   const float x2 = x * x;

@@ -426,8 +426,8 @@ int aspire_rope_frequencies(int32_t head_dim, float rope_theta, float rope_scale
  * Pair i of a token's head turns by position * f_i: y_a = A (a cos - b sin), y_b = A (b cos + a sin), of
  * dims (i, i + rotary_dim / 2), or (2i, 2i + 1) with interleaved; dims from rotary_dim on are copied (in place:
  * left). inverse turns back (times A): the transpose, i.e. the gradient. Tokens at negative positions are
- * copied. f_i comes as turns[i] = f_i / (2 pi) * 2^64 modulo 2^64 (device memory), so angles are exact at any
- * position. Any strides of tokens and heads (elements), head dims contiguous; out equal to in, or apart from it;
+ * copied. f_i comes as turns[i] = f_i / (2 pi) * 2^64 modulo 2^64, to the nearest (device memory), so an angle is
+ * off by position * 2^-65 turns at most. Any strides of tokens and heads (elements), head dims contiguous; out equal to in, or apart from it;
  * head_dim up to 256, fewer than 2^26 tokens.
  *
  * aspire_rotary: q and k to q_out and k_out at positions (32- or 64-bit).

@@ -8,6 +8,7 @@ import torch.autograd.forward_ad as fwad
 from aspire_amd.attention.rotary import RotaryConfig, RotaryEmbedding
 from helpers import bits, say
 from oracle.append import paged_kv_append
+from test_rotary_cpu import PI, true_frequencies
 
 pytestmark = pytest.mark.gpu
 
@@ -414,3 +415,21 @@ def test_forward_mode(gpu, dtype):
         (grad,) = torch.autograd.grad(a, [leaf], fwad.make_dual(dq, tq))
         close(grad, turned(dq, pos, config, inverse=True), dq, config)
         close(fwad.unpack_dual(grad).tangent, turned(tq, pos, config, inverse=True), tq, config)
+
+
+@pytest.mark.parametrize("kw", [dict(head_dim=128, theta=1e6), dict(head_dim=64, **CONFIGS["llama3"])])
+def test_far_positions_against_the_true_frequencies(gpu, kw):
+    """cos and sin themselves, against frequencies to 200 bits. The table's entries are off by half a step of 2^-64 turns,
+    which the position multiplies; the rest is the kernel's own (see close)."""
+    say("rotary far, true", kw)
+    config = RotaryConfig(**kw)
+    rot = RotaryEmbedding(config, gpu)
+    pos = [131071, (1 << 31) - 1, (1 << 33) + 5, 1 << 38]
+    x = torch.zeros(len(pos), 1, config.head_dim, device=gpu)
+    x[..., : config.head_dim // 2] = 1
+    y, _ = rot.apply(x, None, torch.tensor(pos, device=gpu))
+    true = true_frequencies(config)
+    for i, p in enumerate(pos):
+        angle = np.array([float(p * f / (2 * PI) % 1) * 2 * np.pi for f in true])
+        ref = np.concatenate([np.cos(angle), np.sin(angle)])
+        assert np.abs(y[i, 0].cpu().double().numpy() - ref).max() <= 10 * 2.0 ** -24 + p * 2.0 ** -65 * 2 * np.pi

@@ -2,6 +2,7 @@
 
 import ctypes
 import math
+from fractions import Fraction
 
 import numpy as np
 import pytest
@@ -169,3 +170,66 @@ def test_dual_tensors_are_refused_where_there_is_no_derivative():
         for call in calls:
             with pytest.raises(ValueError, match="not differentiable"):
                 call()
+
+
+def arctan_inverse(n, one):
+    """one * arctan(1 / n), its series in whole numbers."""
+    total, power, k = 0, one // n, 1
+    while power:
+        total += power // k if k % 4 == 1 else -(power // k)
+        power, k = power // (n * n), k + 2
+    return total
+
+
+BITS = 260
+PI = Fraction(4 * (4 * arctan_inverse(5, 1 << BITS) - arctan_inverse(239, 1 << BITS)), 1 << BITS)  # Machin
+
+
+def root(x, r):
+    """floor(x ** (1 / r)) by bisection, all whole numbers."""
+    lo, hi = 0, 1 << (x.bit_length() // r + 1)
+    while hi - lo > 1:
+        mid = (lo + hi) // 2
+        lo, hi = (mid, hi) if mid ** r <= x else (lo, mid)
+    return lo
+
+
+def true_frequencies(config):
+    """theta ** (-2 i / R) and what the scalings make of it, to some 200 bits: the R-th root of theta ** (-2 i)."""
+    r, theta = config.rotated, Fraction(config.theta)
+    base = [Fraction(root(int((1 << (220 * r)) / theta ** (2 * i)), r), 1 << 220) for i in range(r // 2)]
+    factor = Fraction(config.factor)
+    if config.pair_factors is not None:
+        return [f / Fraction(s) for f, s in zip(base, config.pair_factors)]
+    if config.scaling == "linear":
+        return [f / factor for f in base]
+    if config.scaling == "llama3":
+        lo, hi = Fraction(config.low_freq_factor), Fraction(config.high_freq_factor)
+        keep = [min(max((config.original_max_position * f / (2 * PI) - lo) / (hi - lo), Fraction(0)), Fraction(1)) for f in base]
+    elif config.scaling == "yarn":
+        # the pairs that turn beta_fast and beta_slow times over the trained context, out to whole numbers
+        ends = [r * math.log(config.original_max_position / (b * 2 * math.pi)) / (2 * math.log(config.theta))
+                for b in (config.beta_fast, config.beta_slow)]
+        first, last = max(math.floor(ends[0]), 0), min(math.ceil(ends[1]), r - 1)
+        keep = [1 - min(max(Fraction(i - first, last - first), Fraction(0)), Fraction(1)) for i in range(r // 2)]
+    else:
+        return base
+    return [t * f + (1 - t) * f / factor for t, f in zip(keep, base)]
+
+
+TABLES = [dict(theta=1e6), dict(theta=1e4, head_dim=80, rotary_dim=20), dict(theta=1e4, scaling="linear", factor=4.0),
+          dict(theta=5e5, scaling="llama3", factor=8.0, original_max_position=8192),
+          dict(theta=1e6, scaling="yarn", factor=4.0, original_max_position=32768, head_dim=64),
+          dict(theta=10000.5, head_dim=2), dict(theta=0.125, head_dim=8, pair_factors=(3.0, 0.001, 1.0, 2.0 ** -40))]
+
+
+@pytest.mark.parametrize("kw", TABLES)
+def test_the_table_of_turns_has_all_its_bits(kw):
+    """Every entry is the nearest 64-bit fraction of a turn (an entry that was made in a double has 53 bits, and a position
+    multiplies what is missing), and frequencies() the nearest doubles."""
+    config = RotaryConfig(**kw)
+    true = true_frequencies(config)
+    for got, f in zip(RotaryEmbedding(config, "cpu").turns.tolist(), true):
+        off = (got - f / (2 * PI) * 2 ** 64) % 2 ** 64
+        assert min(off, 2 ** 64 - off) <= Fraction(1, 2) + Fraction(1, 2 ** 20)
+    assert config.frequencies() == [float(f) for f in true]
