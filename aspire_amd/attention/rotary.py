@@ -141,7 +141,7 @@ _INTS = (torch.int32, torch.int64)
 
 
 class RotaryEmbedding:
-    """A model's rotary positions on one device."""
+    """A model's rotary positions on one device, for up to 1,024 q and 1,024 k heads and 2^26 - 4 tokens a call."""
 
     def __init__(self, config: RotaryConfig, device="cuda"):
         self.config = config

@@ -342,7 +342,8 @@ int rotary(const aspire_rotary_args* a, bool append, const char* what, hipStream
   constexpr int64_t kRotMaxWaves = 1024;
   const int tasks = p.q.heads * p.q.tasks + p.k.heads * p.k.tasks + (append ? p.v.heads * p.v.tasks : 0);
   int wpt_log2 = 0;
-  ROTARY_CHECK(a->total_tokens < (1 << 26), "2^26 tokens or more");  // threads of a launch stay below 2^32
+  // threads of a launch stay below 2^32, those of the last, partly filled workgroup among them
+  ROTARY_CHECK(a->total_tokens <= (1 << 26) - kRotWaves, "more than 2^26 - 4 tokens");
   while (wpt_log2 < 6 && a->total_tokens < (1 << 23) && (64 << wpt_log2) < tasks && (wpt_log2 < 2 || (int64_t(p.total_tokens) << (wpt_log2 + 1)) <= kRotMaxWaves)) ++wpt_log2;
   if (a->dtype == ASPIRE_ROTARY_FP32) {
     dispatch<float, false>(p, vec, wide, a->interleaved != 0, wpt_log2, stream);

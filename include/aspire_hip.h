@@ -428,7 +428,7 @@ int aspire_rope_frequencies(int32_t head_dim, float rope_theta, float rope_scale
  * left). inverse turns back (times A): the transpose, i.e. the gradient. Tokens at negative positions are
  * copied. f_i comes as turns[i] = f_i / (2 pi) * 2^64 modulo 2^64, to the nearest (device memory), so an angle is
  * off by position * 2^-65 turns at most. Any strides of tokens and heads (elements), head dims contiguous; out equal to in, or apart from it;
- * head_dim up to 256, fewer than 2^26 tokens.
+ * head_dim up to 256, up to 1024 heads each, up to 2^26 - 4 tokens.
  *
  * aspire_rotary: q and k to q_out and k_out at positions (32- or 64-bit).
  * aspire_rotary_append (bf16, fp16): q to q_out, the turned k and v to the page pool, where aspire_paged_kv_append

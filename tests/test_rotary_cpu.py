@@ -233,3 +233,14 @@ def test_the_table_of_turns_has_all_its_bits(kw):
         off = (got - f / (2 * PI) * 2 ** 64) % 2 ** 64
         assert min(off, 2 ** 64 - off) <= Fraction(1, 2) + Fraction(1, 2 ** 20)
     assert config.frequencies() == [float(f) for f in true]
+
+
+@pytest.mark.skipif(not _lib.LIB_PATH.exists(), reason="libaspire_hip.so not built")
+@pytest.mark.parametrize("tokens", [(1 << 26) - 3, (1 << 26) - 2, (1 << 26) - 1, (1 << 31) - 1])
+def test_launches_of_2_to_the_32_threads_are_refused(tokens):
+    """Workgroups of 4 tokens and 256 threads: past 2^26 - 4 tokens the last, partly filled one makes 2^32 threads."""
+    L = _lib.lib()
+    a = _lib.RotaryArgs(q=4096, q_out=8192, num_qo_heads=1, total_tokens=tokens, head_dim=64, rotary_dim=64, turns=4096,
+                        amplitude=1.0, positions=4096, kv_cache=4096, num_pages=4, page_size=16)
+    for entry in (L.aspire_rotary, L.aspire_rotary_append):
+        assert entry(ctypes.byref(a), None) == _lib.ASPIRE_ERR_INVALID
