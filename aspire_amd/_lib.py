@@ -63,6 +63,7 @@ EXPORTED = (
     "aspire_add_rms_norm_partials",
     "aspire_linear_int4",
     "aspire_linear_int4_workspace",
+    "aspire_linear_int4_choice",
     "aspire_rotary",
     "aspire_rotary_append",
     "aspire_bandwidth_probe",
@@ -273,6 +274,7 @@ def _declare(lib):
         # the address of the arguments, or the structure's bytes
         "aspire_linear_int4": [vp, vp],
         "aspire_linear_int4_workspace": [i32, i32, i32, i32, i32],
+        "aspire_linear_int4_choice": [i32, i32, i32, i32, i32, vp],
         "aspire_rotary": [vp, vp],
         "aspire_rotary_append": [vp, vp],
         "aspire_bandwidth_probe": [i32, vp, i64, vp, i64, i32, i32, vp],
@@ -282,6 +284,7 @@ def _declare(lib):
         fn.argtypes = argtypes
         fn.restype = ctypes.c_int
     lib.aspire_linear_int4_workspace.restype = i64
+    lib.aspire_linear_int4_choice.restype = None
 
 
 def lib():

@@ -616,7 +616,7 @@ Shape choose(int rows, int n_pad, int blocks, int group, bool swiglu) {
                {64, 256, 1.14}, {112, 256, 1.58}, {128, 128, 1.18}, {128, 256, 1.77}};
   Shape best{};
   double least = 1e30;
-  if (mine == 1) {
+  if (mine == 1 && rows <= 16 * 65535) {  // 16 rows to a workgroup in z
     const int halves = swiglu ? 2 : 1;  // a workgroup takes a gate and its up tile
     const double tiles = std::ceil(rows / 16.0) * (n_pad / 16 / halves);
     best = Shape{0, 0, 1};
@@ -670,6 +670,14 @@ extern "C" int64_t aspire_linear_int4_workspace(int32_t rows, int32_t n, int32_t
   if (rows <= 0 || n <= 0 || k <= 0 || n > (1 << 30)) return 0;
   const int n_pad = (n + 15) / 16 * 16;
   return partial_floats(choose(rows, n_pad, (k + 127) / 128, group, swiglu != 0), rows, n_pad);
+}
+
+extern "C" void aspire_linear_int4_choice(int32_t rows, int32_t n, int32_t k, int32_t group, int32_t swiglu, int32_t choice[3]) {
+  using namespace aspire;
+  choice[0] = choice[1] = choice[2] = 0;
+  if (rows <= 0 || n <= 0 || k <= 0 || n > (1 << 30)) return;
+  const Shape f = choose(rows, (n + 15) / 16 * 16, (k + 127) / 128, group, swiglu != 0);
+  choice[0] = f.rows, choice[1] = f.cols, choice[2] = f.splits;
 }
 
 extern "C" int aspire_linear_int4(const aspire_int4_args* a, void* stream) {

@@ -524,6 +524,10 @@ typedef struct aspire_int4_args {
 /* Floats of workspace that a product needs (0: none): partial sums of k splits, until the call's launches have run. */
 int64_t aspire_linear_int4_workspace(int32_t rows, int32_t n, int32_t k, int32_t group, int32_t swiglu);
 
+/* What a product runs on: the rows and columns of a tile (0, 0: the kernel that streams the weights past 16 rows at a time) and
+ * the splits of k (past 1: slabs in the workspace and a second launch); three zeros for sizes that are refused. */
+void aspire_linear_int4_choice(int32_t rows, int32_t n, int32_t k, int32_t group, int32_t swiglu, int32_t choice[3]);
+
 int aspire_linear_int4(const aspire_int4_args* args, void* stream);
 
 /* aspire_add_rms_norm with delta = bf16(the sum of the slabs partials [splits][rows][dim]). */

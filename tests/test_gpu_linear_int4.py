@@ -247,3 +247,15 @@ def test_refusals(gpu):
     with pytest.raises(RuntimeError):
         linear_int4(x, pack.to("cpu"), out)
     assert linear_int4(x[:0], pack, out[:0]).shape == (0, 48)
+
+
+def test_more_rows_than_the_stream_kernel_takes(gpu):
+    """16 x 65,535 rows and more against a single tile of columns: every copy of the same rows gives the same bits."""
+    rows = 4096 * 257
+    say("int4 rows", rows)
+    packed, scales, z, w = weights(16, 1024, 64, True, BF, gpu)
+    pack = Int4Weight.from_packed(packed, scales, z, group=64)
+    base = torch.randn(4096, 1024, device=gpu).to(BF)
+    out = linear_int4(base.repeat(257, 1), pack, torch.full((rows, 16), float("nan"), dtype=BF, device=gpu)).view(257, 4096, 16)
+    assert (out == out[0]).all()
+    close(out[0], base.double() @ w.t(), product_bound(base, scales, 64, 1024))

@@ -131,3 +131,36 @@ def test_dual_tensors_are_refused():
         for args in ((dual(x), w, out), (x, w, dual(out)), (x, scaled, out)):
             with pytest.raises(ValueError, match="not differentiable"):
                 linear_int4.linear_int4(*args)
+
+
+def choice(rows, n, k, group, swiglu):
+    """Rows and columns of a tile (0, 0: the stream kernel), and the splits of k."""
+    out = (ctypes.c_int32 * 3)()
+    _lib.lib().aspire_linear_int4_choice(rows, n, k, group, swiglu, out)
+    return tuple(out)
+
+
+@pytest.mark.skipif(not _lib.LIB_PATH.exists(), reason="libaspire_hip.so not built")
+@pytest.mark.parametrize("n,ks", [(16, (32, 1024, 2048, 4096)), (32, (64, 1024, 8192)), (96, (4096,)), (4096, (4096, 1 << 21)),
+                                  (151936, (4096,)), ((1 << 23) * 16 - 16, (128,))])
+def test_launches_stay_within_their_limits(n, ks):
+    """65,535 workgroups in y and z, fewer than 2^32 threads in x: the stream kernel has 16 rows in z, the tiles theirs in y."""
+    for rows in (1, 16, 17, 65535 * 16, 65535 * 16 + 1, (1 << 22) - 64):
+        for k in ks:
+            for group in (32, 64, 128):
+                for swiglu in (0, 1):
+                    if k % group or (swiglu and n % 32):
+                        continue
+                    tile, cols, splits = choice(rows, n, k, group, swiglu)
+                    assert splits >= 1
+                    if tile == 0:
+                        assert (rows + 15) // 16 <= 65535 and splits <= 65535
+                    else:
+                        assert (rows + tile - 1) // tile <= 65535
+                        assert 2 * ((n + cols - 1) // cols) * splits * 512 < 1 << 32
+
+
+@pytest.mark.skipif(not _lib.LIB_PATH.exists(), reason="libaspire_hip.so not built")
+def test_choice_of_refused_sizes():
+    for args in ((0, 16, 128, 32, 0), (-1, 16, 128, 32, 0), (1, 0, 128, 32, 0), (1, 16, 0, 32, 0), (1, (1 << 30) + 1, 128, 32, 0)):
+        assert choice(*args) == (0, 0, 0)
