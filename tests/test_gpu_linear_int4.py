@@ -5,6 +5,7 @@ import torch
 
 from aspire_amd.linear_int4 import Int4Weight, linear_int4
 from helpers import say
+from int4_cases import representatives
 
 pytestmark = pytest.mark.gpu
 
@@ -259,3 +260,39 @@ def test_more_rows_than_the_stream_kernel_takes(gpu):
     out = linear_int4(base.repeat(257, 1), pack, torch.full((rows, 16), float("nan"), dtype=BF, device=gpu)).view(257, 4096, 16)
     assert (out == out[0]).all()
     close(out[0], base.double() @ w.t(), product_bound(base, scales, 64, 1024))
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("swiglu", [False, True])
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_every_kernel_that_the_rule_picks(gpu, group, swiglu, dtype):
+    """The least product for each tile, split and number of a stream wave's blocks, and the least that goes round a tile's
+    ring; scales of both types. Sums of whole numbers: (192 + c - z) x and 192 x of a group stay below 399 * 2 * 128 <
+    2^24, and all groups below 15 * 2 * 18,432 * 8 < 2^24 in units of the smallest scale, an eighth of the largest, so fp32 holds every one
+    exactly. With swiglu expf, the sum, the quotient and the product round by at most 8 * 2^-24 of the result; for gates below
+    -88.7 expf(-gate) is infinite, and silu 0 in place of less than 88.8 exp(-88.7) < 2^-121."""
+    for i, (kernel, shapes) in enumerate(representatives(group, int(swiglu)).items()):
+        for rows, n, k in shapes:
+            say("int4 kernel", kernel, rows, n, k, group, swiglu, dtype)
+            for st in (BF, HF):
+                packed, _, z, _ = weights(n, k, group, i % 2 == 0, st, gpu, exact=True)
+                g = torch.Generator(device=gpu).manual_seed(rows + n + k)
+                top = -4 if swiglu else 0  # gates on both sides of silu's bend
+                scales = torch.pow(2.0, torch.randint(top - 3, top + 1, (n, k // group), device=gpu, generator=g).float()).to(st)
+                pack = Int4Weight.from_packed(packed, scales, z, group=group)
+                w = pack.dequantize(torch.float64)
+                x = torch.full((rows, k + 8), float("nan"), dtype=dtype, device=gpu)[:, :k]
+                x.copy_(torch.randint(-2, 3, (rows, k), device=gpu, generator=g))
+                cols = n // 2 if swiglu else n
+                out = torch.full((rows + 1, cols + 3), 7.0, dtype=dtype, device=gpu)
+                linear_int4(x, pack, out[:rows, :cols], swiglu=swiglu)
+                ref = x.double() @ w.t()
+                if swiglu:
+                    gate, up = ref.chunk(2, dim=1)
+                    ref = gate * torch.sigmoid(gate) * up
+                    close(out[:rows, :cols], ref, 8 * 2.0 ** -24 * ref.abs() + 2.0 ** -121 * up.abs())
+                else:
+                    assert torch.equal(out[:rows, :cols], ref.to(dtype))
+                assert (out[rows:] == 7).all() and (out[:, cols:] == 7).all()
+                again = torch.empty(rows, cols, dtype=dtype, device=gpu)
+                assert torch.equal(linear_int4(x, pack, again, swiglu=swiglu), out[:rows, :cols])

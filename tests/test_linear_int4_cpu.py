@@ -8,6 +8,7 @@ import torch.autograd.forward_ad as fwad
 
 from aspire_amd import _lib, linear_int4
 from aspire_amd.linear_int4 import Int4Weight
+from int4_cases import TILES, choice, representatives
 
 
 @pytest.mark.parametrize("n,k,group,zeros", [(16, 128, 128, False), (40, 96, 32, True), (1, 320, 64, True)])
@@ -133,13 +134,6 @@ def test_dual_tensors_are_refused():
                 linear_int4.linear_int4(*args)
 
 
-def choice(rows, n, k, group, swiglu):
-    """Rows and columns of a tile (0, 0: the stream kernel), and the splits of k."""
-    out = (ctypes.c_int32 * 3)()
-    _lib.lib().aspire_linear_int4_choice(rows, n, k, group, swiglu, out)
-    return tuple(out)
-
-
 @pytest.mark.skipif(not _lib.LIB_PATH.exists(), reason="libaspire_hip.so not built")
 @pytest.mark.parametrize("n,ks", [(16, (32, 1024, 2048, 4096)), (32, (64, 1024, 8192)), (96, (4096,)), (4096, (4096, 1 << 21)),
                                   (151936, (4096,)), ((1 << 23) * 16 - 16, (128,))])
@@ -164,3 +158,17 @@ def test_launches_stay_within_their_limits(n, ks):
 def test_choice_of_refused_sizes():
     for args in ((0, 16, 128, 32, 0), (-1, 16, 128, 32, 0), (1, 0, 128, 32, 0), (1, 16, 0, 32, 0), (1, (1 << 30) + 1, 128, 32, 0)):
         assert choice(*args) == (0, 0, 0)
+
+
+@pytest.mark.skipif(not _lib.LIB_PATH.exists(), reason="libaspire_hip.so not built")
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("swiglu", [0, 1])
+def test_every_kernel_has_a_product_that_runs_it(group, swiglu):
+    """The rule picks every tile, with and without splits, and every number of a stream wave's blocks, and no other kernel: what
+    the GPU test of these products runs is all there is. Gate and up tiles of 128 columns and up to 64 rows pair in
+    the join alone; a stream wave has 4 blocks or more where k is split (7 and 8 avoid the split)."""
+    stream = {(0, held, False) for held in range(1, 7 if group == 32 else 9)}
+    stream |= {(0, held, True) for held in range(4 if group == 32 else 5, 7)}
+    tiles = {tile + (split,) for tile in TILES for split in (False, True)
+             if split or not (swiglu and tile[1] == 128 and tile[0] <= 64)}
+    assert set(representatives(group, swiglu)) == stream | tiles
