@@ -335,9 +335,8 @@ def require_cuda(*tensors: torch.Tensor, what: str) -> None:
 
 def has_tangent(*tensors) -> bool:
     """Whether one of the tensors (None: none) is a dual tensor of forward-mode differentiation, which ``requires_grad``
-    does not show."""
-    return forward_ad._current_level >= 0 and any(
-        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+    does not show. (Callers look at ``forward_ad._current_level`` first, which is -1 outside of it: no call in every launch.)"""
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def dense(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:

@@ -25,6 +25,7 @@ from dataclasses import dataclass
 from decimal import Context, Decimal, localcontext
 
 import torch
+from torch.autograd import forward_ad
 
 from aspire_amd import _lib
 
@@ -222,14 +223,16 @@ class RotaryEmbedding:
     def apply(self, q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor):
         """``(q, k)`` turned at ``positions`` ``[T]``, as new tensors (``k`` may be None); differentiable, in reverse and in
         forward mode. Tokens at negative positions are copied."""
-        if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)) or _lib.has_tangent(q, k):
+        if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)) \
+                or forward_ad._current_level >= 0 and _lib.has_tangent(q, k):
             return _Turn.apply(q, k, positions, self, False)
         return self._turn(q, k, positions, False, False, "RotaryEmbedding.apply")
 
     def apply_inplace(self, q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor) -> None:
         """``apply`` on q and k themselves (not differentiable; no two of their rows may share memory)."""
         what = "RotaryEmbedding.apply_inplace"
-        if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)) or _lib.has_tangent(q, k):
+        if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)) \
+                or forward_ad._current_level >= 0 and _lib.has_tangent(q, k):
             raise ValueError(f"{what}: not differentiable; use apply")
         self._turn(q, k, positions, False, True, what)
 
@@ -244,7 +247,7 @@ class RotaryEmbedding:
         page id or list entry lies outside the pool or the list. No two tokens may share a slot."""
         what = "RotaryEmbedding.append"
         if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad) \
-                or _lib.has_tangent(q, k, v, q_out, kv_cache):
+                or forward_ad._current_level >= 0 and _lib.has_tangent(q, k, v, q_out, kv_cache):
             raise ValueError(f"{what}: not differentiable")
         code, dtype = self._dtype(q, what), q.dtype
         if code == 2:
@@ -291,37 +294,37 @@ class _Turn(torch.autograd.Function):
     def forward(ctx, q, k, positions, rotary, inverse):
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(positions)
-        ctx.save_for_forward(positions)
         ctx.rotary, ctx.inverse = rotary, inverse
-        ctx.shapes = None if q is None else q.shape, None if k is None else k.shape
+        if forward_ad._current_level >= 0:  # for jvp, which runs at once
+            ctx.save_for_forward(positions)
+            ctx.shapes = None if q is None else q.shape, None if k is None else k.shape
         return rotary._turn(q, k, positions, inverse, False, "RotaryEmbedding.apply")
 
     @staticmethod
-    def _again(ctx, a, b, inverse):
-        """Gradients or tangents of q and k (either may be None) turned, themselves differentiable."""
-        (positions,) = ctx.saved_tensors
-        if a is None and b is None:
-            return None, None
-        if a is not None and a.stride(2) != 1:
-            a = a.contiguous()
-        if b is not None and b.stride(2) != 1:
-            b = b.contiguous()
-        if torch.is_grad_enabled() or _lib.has_tangent(a, b):  # a second derivative is wanted
-            return _Turn.apply(a, b, positions, ctx.rotary, inverse)
-        return ctx.rotary._turn(a, b, positions, inverse, False, "RotaryEmbedding.apply")
-
-    @staticmethod
     def backward(ctx, dq, dk):
-        return *_Turn._again(ctx, dq, dk, not ctx.inverse), None, None, None
+        (positions,) = ctx.saved_tensors
+        if dq is None and dk is None:
+            return None, None, None, None, None
+        if dq is not None and dq.stride(2) != 1:
+            dq = dq.contiguous()
+        if dk is not None and dk.stride(2) != 1:
+            dk = dk.contiguous()
+        if torch.is_grad_enabled() or forward_ad._current_level >= 0:  # a second derivative is wanted
+            gq, gk = _Turn.apply(dq, dk, positions, ctx.rotary, not ctx.inverse)
+        else:
+            gq, gk = ctx.rotary._turn(dq, dk, positions, not ctx.inverse, False, "RotaryEmbedding.apply")
+        return gq, gk, None, None, None
 
     @staticmethod
     def jvp(ctx, tq, tk, *_):
+        (positions,) = ctx.saved_tensors
         # an output that is not None needs a tangent; one of the two is there
         if tq is None and ctx.shapes[0] is not None:
             tq = tk.new_zeros(ctx.shapes[0])
         if tk is None and ctx.shapes[1] is not None:
             tk = tq.new_zeros(ctx.shapes[1])
-        return _Turn._again(ctx, tq, tk, ctx.inverse)
+        tq, tk = (t if t is None or t.stride(2) == 1 else t.contiguous() for t in (tq, tk))
+        return _Turn.apply(tq, tk, positions, ctx.rotary, ctx.inverse)
 
 
 __all__ = ["RotaryConfig", "RotaryEmbedding"]

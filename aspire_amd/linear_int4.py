@@ -14,6 +14,7 @@ from __future__ import annotations
 import struct
 
 import torch
+from torch.autograd import forward_ad
 
 from aspire_amd import _lib
 
@@ -130,7 +131,7 @@ def linear_int4(x: torch.Tensor, w: Int4Weight, out: torch.Tensor, *, swiglu: bo
     from x. Not differentiable. A row of x with an infinity or NaN (or bf16 values of 2^112 and more, whose sums may overflow on the way) gives
     no finite outputs; the other rows are not touched by it."""
     what = "linear_int4"
-    if torch.is_grad_enabled() and x.requires_grad or _lib.has_tangent(x, out, w.scales):
+    if torch.is_grad_enabled() and x.requires_grad or forward_ad._current_level >= 0 and _lib.has_tangent(x, out, w.scales):
         raise ValueError(f"{what}: not differentiable")
     if not (x.is_cuda and out.is_cuda and w.codes.is_cuda):
         _lib.require_cuda(x, out, w.codes, what=what)
