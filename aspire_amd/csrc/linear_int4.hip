@@ -6,21 +6,24 @@
 // d = c - z from -15 to 15 (one binade, steps of 1), so bytes 0x40 + d, four to an addition, get their upper byte 0x43 from a
 // byte permutation, and the sum over a group starts from -192 sum x, which one MFMA with -192 in the weights' place gives for all of them:
 //     part = sum (192 + d) x - 192 sum x (fp32),  y += s part  for each group.
+// The offset costs the sums of a group up to 5 of fp32's 24 bits, which bf16 outputs have to spare: of 12 x 24,576 x 4,096 with swiglu 0.4% are
+// rounded to another side than plain fp32 sums are, and both are 0.00167 off the exact values (2-norm).
 //
 // Weights are laid out once (aspire_hip.h): 16 rows x 128 k make a block of 1 KiB in which lane l of a
 // wave finds its 32 codes (row l % 16, and for each 32 k the 8 from 8 (l / 16) on) in one 16-byte load; blocks of 16
 // rows follow each other along k. A word's nibbles are ordered so that shifts by 0, 4, 8, 12 leave neighbours in
 // the low and high half.
 //
-// Bound by the weights' stream up to 16 rows (151,936 x 4,096: 4.4 TB/s; smaller ones start up for some 5 us), above by
-// the steps of the tiles, whose products keep the matrix cores 40 to 45% busy. us on MI355X, bf16, groups of 128 with zero
-// points, weights cold / torch.nn.functional.linear with bf16 weights:
-//   rows    4,096 x 4,096   24,576 x 4,096   4,096 x 12,288   151,936 x 4,096
-//      1     6.0 / 12.9       16.8 / 45.5      13.2 / 22.7        75 / 252
-//     16     8.4 / 13.2       20.6 / 45.9      17.8 / 23.2        78 / 261
-//     48    14.0 / 11.9       30.9 / 48.3      20.8 / 33.6       128 / 263
-//    208    26.2 / 18.8       59.6 / 68.1      36.7 / 52.9       321 / 345
-//  2,048    77   / 60        400   / 289      202   / 183
+// Bound by the weights' stream up to 16 rows (151,936 x 4,096: 4.4 TB/s, where a mere read runs at 7.3; smaller ones start up for
+// some 5 us), above by the steps of the tiles, whose matrix cores are busy 36 to 39% of the time and the VALU beside them 34 to 46%, hardly
+// at once. us on MI355X, bf16, groups of 128 with zero points, weights cold / the bf16 products of linear.hip (slabs whose sum
+// is their consumer's; whole for the two wide ones) / torch's (swiglu with silu_mul behind it):
+//   rows     4,096 x 4,096   24,576 x 4,096 + swiglu    4,096 x 12,288      151,936 x 4,096
+//      1     5.8 / 7.9 / 16      17 / 39 / 48           13.8 / 17.6 / 21     78 / 202 / 244
+//     12     7.6 / 8.1 / 16      17 / 37 / 47           15.7 / 17.6 / 22     74 / 200 / 255 (16 rows)
+//     48    14.4 / 10.0 / 14     31 / 43 / 48           20.9 / 20.7 / 32    124 / 214 / 260
+//    208    25.5 / 18.1 / 22     57 / 60 / 68           35.4 / 39.1 / 51    318 / 357 / 330
+//  2,048      67 /  -   / 60    384 /  - / 317           188 /   -  / 177
 #include <algorithm>
 #include <type_traits>
 
@@ -127,7 +130,8 @@ constexpr int most_ahead(int blocks, int group) { return group > 32 && blocks <=
 // Few rows (16 to a blockIdx.z): bound by the weights' stream. A workgroup walks over output tiles of 16 columns (with swiglu over pairs of a
 // gate and an up tile), for all of k or the split blockIdx.y of at most 6 or 8 blocks a wave; its waves take the blocks of
 // 128 k in turn, keep their x in registers, and add up through LDS, in a fixed order. A block is asked for as soon as
-// the one before it in its registers is multiplied, across the ends of tiles, so the stream never pauses. kAhead is the
+// the one before it in its registers is multiplied, across the ends of tiles (once a tile the compiled loop still waits for all
+// of a wave's loads where it has 2 blocks or more: one wait serves the first tile, whose loads go out in another order). kAhead is the
 // blocks that a wave has, so that a short k loads none twice: 16 x 24,576 x 1,024 with 1 7.3 us, with 4 14.9; 16 x 24,576 x
 // 2,048 with 2 11.4, with 4 16.6. More than 4 leave a CU one workgroup, and are still faster than splits of at most 4 with
 // their join: 1 x 4,096 x 6,144 with 6 7.5 us, in two splits 9.2; 16 x 24,576 x 8,192 with 8 32.0, in two 34.6; 16 x 4,096 x

@@ -3,10 +3,11 @@
 The projections of ``aspire_amd.linear`` for checkpoints whose weights are 4-bit codes in groups along K, each with a
 scale and, where the checkpoint has them, a zero point: ``w[n, k] = scales[n, k // group] * (codes[n, k] - zeros[n,
 k // group])``. The weights are read as they are (an eighth of fp32's bytes) and never rounded to 16 bits: codes are
-multiplied exactly, sums are fp32, and the output is rounded once. Any number of token rows, bf16 or fp16.
+multiplied exactly, sums are fp32, and the output is rounded once. Up to 4,194,240 token rows, bf16 or fp16.
 
 ``Int4Weight`` holds a matrix in the kernels' layout, made once from a checkpoint's packed codes
-(``from_packed``) or from a bf16 matrix (``quantize``).
+(``from_packed``) or from a bf16 matrix (``quantize``). A few rows take 0.3 to 0.85 of the time of torch's product with bf16 weights, a prompt's
+2,048 rows 1.05 to 1.4 of it.
 """
 
 from __future__ import annotations
@@ -128,8 +129,9 @@ _ARGS = struct.Struct("PqPPPPq7iPq")
 def linear_int4(x: torch.Tensor, w: Int4Weight, out: torch.Tensor, *, swiglu: bool = False) -> torch.Tensor:
     """``out = x @ w.T`` (``[rows, N]``), or with ``swiglu`` ``silu(x @ w[:N/2].T) * (x @ w[N/2:].T)`` (``[rows, N/2]``, N a
     multiple of 32), for bf16 or fp16 ``x`` with 16-byte aligned rows; ``out`` of ``x``'s type with contiguous rows, apart
-    from x. Not differentiable. A row of x with an infinity or NaN (or bf16 values of 2^112 and more, whose sums may overflow on the way) gives
-    no finite outputs; the other rows are not touched by it."""
+    from x. Past 16 rows, rows of x that lie 2^22 elements or more apart may be refused (ValueError; ``x.contiguous()`` is taken), as
+    the last tokens of long sequences in one tensor do. Not differentiable. A row of x with an infinity or NaN (or bf16 values
+    of 2^112 and more, whose sums may overflow on the way) gives no finite outputs; the other rows are not touched by it."""
     what = "linear_int4"
     if torch.is_grad_enabled() and x.requires_grad or forward_ad._current_level >= 0 and _lib.has_tangent(x, out, w.scales):
         raise ValueError(f"{what}: not differentiable")

@@ -507,7 +507,8 @@ int aspire_linear_partials(const void* x, int64_t x_stride, const void* w, int64
  * l % 16, k 32 c + 8 (l / 16) + e in bits 4 (e / 2) + 16 (e % 2), e = 0 .. 7. For each block, scales (bf16 or fp16) are
  * [4][128 / group][4], row 4 a + b of the tile and group g at [a][g][b], and zeros (bytes of 0 .. 15, NULL: 8) [16][128 / group].
  * Codes and scales of rows past n and columns past k are there and 0. group 32, 64 or 128, k a multiple of it; 16-byte aligned
- * x rows; out rows of any stride, apart from x. */
+ * x rows of any stride up to 16 rows and where the choice below gives no tile, else of strides below 2^22 elements; out rows of any
+ * stride, apart from x; up to 4,194,240 rows, k below 2^22, weights below 2^34 values. */
 typedef struct aspire_int4_args {
   const void* x;
   int64_t x_stride;
