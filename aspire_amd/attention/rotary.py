@@ -9,7 +9,7 @@
   (the smoothing of ``RopeConfig``), ``"yarn"`` (between the pairs that turn ``beta_fast`` and ``beta_slow`` times
   over the trained context ``f`` becomes ``f / factor`` linearly; cos and sin times ``0.1 ln(factor) + 1``), or
   divided by given ``pair_factors``;
-* a frequency is the nearest 64-bit fraction of a turn, made from some 60 digits, and its product with the position drops
+* a frequency is the nearest 64-bit fraction of a turn, made from some 45 digits, and its product with the position drops
   whole turns only: angles ``position * f_i`` are within ``position * 2^-65`` turns (2^-24 radians at 2^38); cos and sin
   and the products fp32, one rounding to the output's type.
 
@@ -90,7 +90,7 @@ class RotaryConfig:
         divisor are dropped later, so their digits come on top)."""
         r, divisors = self.rotated, (self.factor, *(self.pair_factors or ()))
         whole = max(0.0, -math.log10(self.theta)) + max(0.0, -math.log10(min(divisors)))
-        with localcontext(Context(prec=60 + math.ceil(whole))):
+        with localcontext(Context(prec=45 + math.ceil(whole))):
             exact = lambda x: Decimal(float(x))
             ratio, base = (exact(self.theta).ln() * -2 / r).exp(), [Decimal(1)]
             while len(base) < r // 2:
@@ -102,17 +102,17 @@ class RotaryConfig:
                 return [f / factor for f in base]
             if self.scaling == "llama3":
                 lo, hi, old = exact(self.low_freq_factor), exact(self.high_freq_factor), exact(self.original_max_position)
-                ramp = [(old * f / (2 * _PI) - lo) / (hi - lo) for f in base]
+                slope, start = old / (2 * _PI) / (hi - lo), lo / (hi - lo)
+                keep = [f * slope - start for f in base]
             elif self.scaling == "yarn":
                 def at(turns):  # the pair that turns so often over the trained context
                     return r * math.log(self.original_max_position / (2 * math.pi * turns)) / (2 * math.log(self.theta))
                 first, last = max(math.floor(at(self.beta_fast)), 0), min(math.ceil(at(self.beta_slow)), r - 1)
                 width = Decimal(max(last - first, 0.001))
-                ramp = [1 - (i - first) / width for i in range(r // 2)]
+                keep = [1 - (i - first) / width for i in range(r // 2)]
             else:
                 return base
-            keep = [min(max(t, Decimal(0)), Decimal(1)) for t in ramp]
-            return [t * f + (1 - t) * f / factor for t, f in zip(keep, base)]
+            return [f if t >= 1 else f / factor if t <= 0 else t * f + (1 - t) * f / factor for t, f in zip(keep, base)]
 
     def frequencies(self) -> list[float]:
         """Radians a position of each pair, as the nearest doubles."""
@@ -121,9 +121,9 @@ class RotaryConfig:
     def _turns(self) -> torch.Tensor:
         """The frequencies as 64-bit fixed-point fractions of a turn a position, to the nearest (int64 holding the bits)."""
         frequencies = self._exact_frequencies()
-        with localcontext(Context(prec=60 + max(0, *(f.adjusted() for f in frequencies)))):
-            turn, half = 2 * _PI, Decimal("0.5")
-            turns = [int(f / turn % 1 * 2 ** 64 + half) % (1 << 64) for f in frequencies]
+        with localcontext(Context(prec=45 + max(0, *(f.adjusted() for f in frequencies)))):
+            scale, half = 2 ** 63 / _PI, Decimal("0.5")
+            turns = [int(f * scale + half) % (1 << 64) for f in frequencies]
         return torch.tensor([t - (1 << 64) if t >> 63 else t for t in turns], dtype=torch.int64)
 
 
