@@ -678,8 +678,11 @@ extern "C" int64_t aspire_linear_int4_workspace(int32_t rows, int32_t n, int32_t
 
 extern "C" void aspire_linear_int4_choice(int32_t rows, int32_t n, int32_t k, int32_t group, int32_t swiglu, int32_t choice[3]) {
   using namespace aspire;
+  if (choice == nullptr) return;
   choice[0] = choice[1] = choice[2] = 0;
-  if (rows <= 0 || n <= 0 || k <= 0 || n > (1 << 30)) return;
+  if (rows <= 0 || rows > (1 << 22) - 64 || n <= 0 || n > (1 << 30) || k <= 0 || k >= (1 << 22)) return;
+  if ((group != 32 && group != 64 && group != 128) || k % group != 0 || (swiglu && n % 32 != 0)) return;
+  if ((int64_t(n) + 15) / 16 * ((k + 127) / 128) >= (1 << 23)) return;
   const Shape f = choose(rows, (n + 15) / 16 * 16, (k + 127) / 128, group, swiglu != 0);
   choice[0] = f.rows, choice[1] = f.cols, choice[2] = f.splits;
 }

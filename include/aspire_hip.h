@@ -526,7 +526,7 @@ typedef struct aspire_int4_args {
 int64_t aspire_linear_int4_workspace(int32_t rows, int32_t n, int32_t k, int32_t group, int32_t swiglu);
 
 /* What a product runs on: the rows and columns of a tile (0, 0: the kernel that streams the weights past 16 rows at a time) and
- * the splits of k (past 1: slabs in the workspace and a second launch); three zeros for sizes that are refused. */
+ * the splits of k (past 1: slabs in the workspace and a second launch); three zeros for sizes that are refused or empty. */
 void aspire_linear_int4_choice(int32_t rows, int32_t n, int32_t k, int32_t group, int32_t swiglu, int32_t choice[3]);
 
 int aspire_linear_int4(const aspire_int4_args* args, void* stream);

@@ -156,8 +156,11 @@ def test_launches_stay_within_their_limits(n, ks):
 
 @pytest.mark.skipif(not _lib.LIB_PATH.exists(), reason="libaspire_hip.so not built")
 def test_choice_of_refused_sizes():
-    for args in ((0, 16, 128, 32, 0), (-1, 16, 128, 32, 0), (1, 0, 128, 32, 0), (1, 16, 0, 32, 0), (1, (1 << 30) + 1, 128, 32, 0)):
+    for args in ((0, 16, 128, 32, 0), (-1, 16, 128, 32, 0), (1, 0, 128, 32, 0), (1, 16, 0, 32, 0), (1, (1 << 30) + 1, 128, 32, 0),
+                 (1 << 22, 16, 128, 32, 0), (1, 16, 1 << 22, 32, 0), (1, 16, 128, 48, 0), (1, 16, 96, 64, 0), (1, 48, 128, 32, 1),
+                 (1, 1 << 27, 128, 32, 0)):
         assert choice(*args) == (0, 0, 0)
+    _lib.lib().aspire_linear_int4_choice(1, 16, 128, 32, 0, None)
 
 
 @pytest.mark.skipif(not _lib.LIB_PATH.exists(), reason="libaspire_hip.so not built")
