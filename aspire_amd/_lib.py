@@ -66,6 +66,13 @@ EXPORTED = (
     "aspire_linear_int4_choice",
     "aspire_rotary",
     "aspire_rotary_append",
+    "aspire_page_resize",
+    "aspire_step_tables",
+    "aspire_tree_attention",
+    "aspire_tree_attention_workspace",
+    "aspire_verify_tree",
+    "aspire_compact_accepted",
+    "aspire_adjust_logits",
     "aspire_bandwidth_probe",
 )
 
@@ -277,6 +284,13 @@ def _declare(lib):
         "aspire_linear_int4_choice": [i32, i32, i32, i32, i32, vp],
         "aspire_rotary": [vp, vp],
         "aspire_rotary_append": [vp, vp],
+        "aspire_page_resize": [vp, vp],
+        "aspire_step_tables": [vp, vp],
+        "aspire_tree_attention": [vp, vp],
+        "aspire_tree_attention_workspace": [i32, i32, i32, i32, i32],
+        "aspire_verify_tree": [vp, vp, vp, vp, i32, i32, i32, vp, vp, vp, vp],
+        "aspire_compact_accepted": [vp, vp],
+        "aspire_adjust_logits": [vp, vp],
         "aspire_bandwidth_probe": [i32, vp, i64, vp, i64, i32, i32, vp],
     }
     for name, argtypes in sigs.items():
@@ -285,6 +299,7 @@ def _declare(lib):
         fn.restype = ctypes.c_int
     lib.aspire_linear_int4_workspace.restype = i64
     lib.aspire_linear_int4_choice.restype = None
+    lib.aspire_tree_attention_workspace.restype = i64
 
 
 def lib():
@@ -331,6 +346,28 @@ def require_cuda(*tensors: torch.Tensor, what: str) -> None:
         if t is not None and not t.is_cuda:
             raise RuntimeError(f"{what}: tensors must be on a ROCm GPU (got {t.device}); "
                                "there is no CPU implementation")
+
+
+def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the bytes from a tensor's first to its last value meet the other's."""
+    def extent(t):
+        at = t.data_ptr()
+        return at, at + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size() if t.numel() else at
+
+    (a0, a1), (b0, b1) = extent(a), extent(b)
+    return a0 < b1 and b0 < a1
+
+
+def launch(entry, args: bytes, index: int, what: str) -> None:
+    """``entry(args, stream)`` on the current stream of device ``index``, made current for the call."""
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if torch._C._cuda_getDevice() == index:
+        rc = entry(args, stream)
+    else:
+        with torch.cuda.device(index):
+            rc = entry(args, stream)
+    if rc:
+        check(rc, what)
 
 
 def has_tangent(*tensors) -> bool:

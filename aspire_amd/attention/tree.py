@@ -1,0 +1,150 @@
+"""Attention of drafted trees over the paged cache, and the move of what is kept of them (HIP).
+
+The mixed attention kernel verifies chains of drafted tokens (aspire/models/sparse_draft_runner.py:595-612: causal among a
+row's new tokens). A step that drafts a tree for each request appends its tokens in any order that puts parents first,
+turned to the position of their depth (``StepTables.positions`` with ``RotaryEmbedding.append``), and
+
+* ``tree_attention`` lets each of them see the request's cached tokens and its own ancestors;
+* ``aspire_amd.engine.sampling.verify_tree_speculation`` finds the path that the target model agrees with;
+* ``compact_accepted`` moves that path's K and V rows to where a chain of them would stand, in every layer.
+
+All three read lengths on the device and can be captured.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+import struct
+
+import torch
+from torch.autograd import forward_ad
+
+from aspire_amd import _lib
+
+_DTYPES = {torch.bfloat16: 0, torch.float16: 1}
+HEAD_DIMS = (64, 128)
+_ARGS = struct.Struct("PqqPqqqqqqPPPPPqPqqP8ifiPq")  # aspire_tree_attention_args
+_MOVE = struct.Struct("PqqqqqPPPP8i")                # aspire_compact_args
+
+
+def _list(t: torch.Tensor, device, what: str, name: str) -> torch.Tensor:
+    if t.dim() != 1 or t.dtype not in (torch.int32, torch.int64) or t.device != device:
+        raise ValueError(f"{what}: {name} must be 1-D int32 on {device}")
+    return _lib.dense(t, torch.int32)
+
+
+def _rows16(t: torch.Tensor) -> bool:
+    """Whether every row of the last dimension (of a 16-bit type) starts on 16 bytes and is in one piece."""
+    return t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % 8 == 0 or n <= 1 for n, s in zip(t.shape[:-1], t.stride()))
+
+
+def tree_attention(q: torch.Tensor, kv_cache: torch.Tensor, qo_indptr: torch.Tensor, kv_page_indices: torch.Tensor,
+                   kv_page_indptr: torch.Tensor, kv_last_page_len: torch.Tensor, tree_masks: torch.Tensor, page_size: int,
+                   *, sm_scale: float | None = None, out: torch.Tensor | None = None, lse: torch.Tensor | None = None,
+                   return_lse: bool = False):
+    """Attention of the trees' tokens ``q`` ``[T, H_q, D]`` over ``kv_cache`` ``[P, 2, page, H_kv, D]`` (bf16 or fp16, D 64 or
+    128, pages of 16 to 1,024 tokens by powers of two), which holds them already: row ``b`` has tokens ``qo_indptr[b]`` to
+    ``qo_indptr[b + 1]`` and the pages ``kv_page_indices[kv_page_indptr[b] : kv_page_indptr[b + 1]]``, the last one filled to
+    ``kv_last_page_len[b]``; its last keys are its tokens'. ``tree_masks`` int64 ``[T, W]`` has bit ``j % 64`` of word ``j // 64``
+    set where a token sees its row's token ``j`` (itself among them); all cached keys before the tree are seen.
+
+    Returns ``out`` (new, or the tensor given; apart from q and the cache), with ``return_lse`` and the base-2 ``lse`` fp32
+    ``[T, H_q]``. A token that sees no key gets zeros and ``-inf``. Keys that a token does not see do not touch it, whatever they
+    hold. Tokens of no row are left as they were. Sums and softmax are fp32; weights of keys are rounded to q's type for the
+    product with v. Not differentiable."""
+    what = "tree_attention"
+    _lib.require_cuda(q, kv_cache, what=what)
+    if torch.is_grad_enabled() and (q.requires_grad or kv_cache.requires_grad) \
+            or forward_ad._current_level >= 0 and _lib.has_tangent(q, kv_cache, out):
+        raise ValueError(f"{what}: not differentiable")
+    code, device = _DTYPES.get(q.dtype), q.device
+    shape = q.shape
+    if code is None or len(shape) != 3 or shape[2] not in HEAD_DIMS or not _rows16(q):
+        raise ValueError(f"{what}: q must be bf16 or fp16 [T, H_q, 64 or 128] with 16-byte aligned heads")
+    tokens, hq, dim = shape
+    cs = kv_cache.shape
+    if kv_cache.dtype != q.dtype or kv_cache.device != device or len(cs) != 5 or cs[1] != 2 or cs[2] != page_size \
+            or cs[4] != dim or not _rows16(kv_cache):
+        raise ValueError(f"{what}: kv_cache must be {q.dtype} [P, 2, {page_size}, H_kv, {dim}] on {device} with 16-byte aligned heads")
+    if cs[3] < 1 or hq % cs[3]:
+        raise ValueError(f"{what}: q heads must be a multiple of the kv heads")
+    if tree_masks.dtype != torch.int64 or tree_masks.dim() != 2 or tree_masks.shape[0] < tokens or tree_masks.device != device \
+            or (tree_masks.shape[1] > 1 and tree_masks.stride(1) != 1):
+        raise ValueError(f"{what}: tree_masks must be int64 [T, words] on {device} with contiguous rows")
+    qo, ind = _list(qo_indptr, device, what, "qo_indptr"), _list(kv_page_indices, device, what, "kv_page_indices")
+    ptr, last = _list(kv_page_indptr, device, what, "kv_page_indptr"), _list(kv_last_page_len, device, what, "kv_last_page_len")
+    rows = last.shape[0]
+    if qo.shape[0] <= rows or ptr.shape[0] <= rows:
+        raise ValueError(f"{what}: qo_indptr and kv_page_indptr need len(kv_last_page_len) + 1 entries")
+    if out is None:
+        out = torch.empty(shape, dtype=q.dtype, device=device)
+    elif out.shape != shape or out.dtype != q.dtype or out.device != device or not _rows16(out):
+        raise ValueError(f"{what}: out must be {q.dtype} of q's shape on {device} with 16-byte aligned heads")
+    elif _lib.overlap(out, q) or _lib.overlap(out, kv_cache):
+        raise ValueError(f"{what}: out must lie apart from q and the cache")
+    if lse is not None and (lse.dtype != torch.float32 or lse.shape != (tokens, hq) or lse.device != device or not lse.is_contiguous()):
+        raise ValueError(f"{what}: lse must be a contiguous fp32 [T, H_q] tensor on {device}")
+    if lse is None and return_lse:
+        lse = torch.empty(tokens, hq, dtype=torch.float32, device=device)
+    scale = 1.0 / math.sqrt(dim) if sm_scale is None else float(sm_scale)
+    L, ws, at = _lib.lib(), None, 0
+    floats = L.aspire_tree_attention_workspace(tokens, rows, hq, cs[3], dim)
+    if floats:  # the call's own, from torch's pool: calls on several streams or in several graphs share none
+        ws = torch.empty(floats, dtype=torch.float32, device=device)
+        at = ws.data_ptr()
+    qs, c, os = q.stride(), kv_cache.stride(), out.stride()
+    args = _ARGS.pack(q.data_ptr(), qs[0], qs[1], kv_cache.data_ptr(), c[0], c[1], c[2], c[3], cs[0], ind.shape[0], qo.data_ptr(),
+                      ind.data_ptr(), ptr.data_ptr(), last.data_ptr(), tree_masks.data_ptr(), tree_masks.stride(0),
+                      out.data_ptr(), os[0], os[1], _lib.ptr(lse) or 0, tokens, rows, tree_masks.shape[1], hq, cs[3], dim,
+                      page_size, code, scale, 0, at, floats)
+    _lib.launch(L.aspire_tree_attention, args, q.get_device(), what)
+    return (out, lse) if return_lse else out
+
+
+def compact_accepted(kv_caches, path: torch.Tensor, kept: torch.Tensor, qo_indptr: torch.Tensor, slots: torch.Tensor) -> None:
+    """Move each kept token's K and V rows from its slot to that of its place in the path, in place: the row at
+    ``slots[qo_indptr[b] + path[b, j]]`` goes to ``slots[qo_indptr[b] + j]`` for ``j < kept[b]``, in every layer.
+
+    ``kv_caches``: one cache ``[P, 2, page, H, D]``, all layers' as ``[L, P, 2, page, H, D]``, or a list of caches of one layout
+    (any element type; no two of a list the same memory). ``path`` int32 ``[B, M]`` and ``kept`` int32 ``[B]`` are what
+    ``verify_tree_speculation`` returns, ``slots`` int64 ``[T]`` what the step's tables hold. A path rises: entries that are not
+    above their place, or not of the row, are passed over, and so are slots outside the cache."""
+    what = "compact_accepted"
+    if isinstance(kv_caches, torch.Tensor):
+        layers = [kv_caches] if kv_caches.dim() == 5 else list(kv_caches.unbind(0)) if kv_caches.dim() == 6 else None
+    else:
+        layers = list(kv_caches)
+    if layers is None:
+        raise ValueError(f"{what}: kv_caches must be [P, 2, page, H, D], [L, P, 2, page, H, D] or a list of the former")
+    if not layers:
+        return
+    c = layers[0]
+    _lib.require_cuda(*layers, path, kept, qo_indptr, slots, what=what)
+    device, cs, st = c.device, c.shape, c.stride()
+    if c.dim() != 5 or cs[1] != 2 or (cs[4] > 1 and st[4] != 1) or cs[2] < 1 \
+            or any(t.shape != cs or t.stride() != st or t.dtype != c.dtype or t.device != device for t in layers):
+        raise ValueError(f"{what}: the caches must be [P, 2, page, H, D] of one layout and type with contiguous head dims")
+    if any(t.requires_grad for t in layers) and torch.is_grad_enabled() \
+            or forward_ad._current_level >= 0 and _lib.has_tangent(*layers):
+        raise ValueError(f"{what}: not differentiable")
+    starts = [t.data_ptr() for t in layers]
+    if len(set(starts)) != len(starts) and c.numel():
+        raise ValueError(f"{what}: a cache is listed twice")
+    if path.dim() != 2 or path.dtype != torch.int32 or not path.is_contiguous() or path.device != device:
+        raise ValueError(f"{what}: path must be a contiguous int32 [B, M] tensor on {device}")
+    kept, qo = _list(kept, device, what, "kept"), _list(qo_indptr, device, what, "qo_indptr")
+    rows = path.shape[0]
+    if kept.shape[0] != rows or qo.shape[0] <= rows:
+        raise ValueError(f"{what}: kept needs {rows} entries and qo_indptr {rows + 1}")
+    if slots.dim() != 1 or slots.dtype != torch.int64 or slots.device != device:
+        raise ValueError(f"{what}: slots must be int64 [T] on {device}")
+    slots, es = slots.contiguous(), c.element_size()
+    table = (ctypes.c_uint64 * len(starts))(*starts)
+    args = _MOVE.pack(ctypes.addressof(table), st[0] * es, st[1] * es, st[2] * es, st[3] * es, cs[0], path.data_ptr(),
+                      kept.data_ptr(), qo.data_ptr(), slots.data_ptr(), len(starts), cs[3], cs[4] * es, cs[2], rows,
+                      slots.shape[0], path.shape[1], 0)
+    _lib.launch(_lib.lib().aspire_compact_accepted, args, c.get_device(), what)
+
+
+__all__ = ["HEAD_DIMS", "tree_attention", "compact_accepted"]

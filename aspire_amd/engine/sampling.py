@@ -11,6 +11,8 @@
   launch builds each position's local vocabulary (the target's top_k candidates plus one
   entry for any other token) and runs the chain rule over it; ``uniforms`` (optional,
   ``[requests, max_draft + 1]``) fixes the draws.
+* ``verify_tree_speculation`` (not in the reference, which drafts chains): the path of a drafted tree that the target
+  model's tokens follow, one ``aspire_verify_tree`` launch.
 * ``first_eos`` (sampling.py:101-116): torch ops (a handful of elementwise steps).
 """
 
@@ -93,6 +95,39 @@ def verify_topk_speculation(draft_probs: torch.Tensor, draft_ids: torch.Tensor, 
     return output, emitted
 
 
+def verify_tree_speculation(tree_tokens: torch.Tensor, parents: torch.Tensor, target_ids: torch.Tensor,
+                            qo_indptr: torch.Tensor, max_path: int):
+    """``(output [B, max_path], path [B, max_path], kept [B])``, int32: what the target model keeps of each drafted tree.
+
+    Row ``b`` has the tokens ``tree_tokens[qo_indptr[b] : qo_indptr[b + 1]]``, its first one the root, which is certain;
+    ``parents`` holds for each the index in its row of the token that it continues (below its own; -1 for the root), and
+    ``target_ids`` the target model's token after it: its greedy pick, or a draw from its distribution, which makes the kept
+    tokens and the one behind them draws from the target's own distribution. From the root on the path takes the child whose
+    token is the present target (the lowest index of several) and ends where there is none, or after ``max_path`` tokens.
+    ``path`` holds the kept tokens' indices, ``output`` their targets (the kept tokens but the root, then a new one), both -1
+    behind the ``kept`` entries. A row without tokens keeps none."""
+    what = "verify_tree_speculation"
+    _lib.require_cuda(tree_tokens, parents, target_ids, qo_indptr, what=what)
+    ints, device = (torch.int32, torch.int64), tree_tokens.device
+    for name, t in (("tree_tokens", tree_tokens), ("parents", parents), ("target_ids", target_ids), ("qo_indptr", qo_indptr)):
+        if t.dim() != 1 or t.dtype not in ints or t.device != device:
+            raise ValueError(f"{what}: {name} must be 1-D int32 on {device}")
+    tokens, rows = tree_tokens.shape[0], qo_indptr.shape[0] - 1
+    if parents.shape[0] < tokens or target_ids.shape[0] < tokens:
+        raise ValueError(f"{what}: parents and target_ids need {tokens} entries")
+    if rows < 0 or max_path < 1 or rows * max_path >= 1 << 31:
+        raise ValueError(f"{what}: qo_indptr needs an entry more than rows, max_path at least 1, rows * max_path below 2^31")
+    tok, par, tgt, qo = (_lib.dense(t, torch.int32) for t in (tree_tokens, parents, target_ids, qo_indptr))
+    result = torch.empty(rows * (2 * max_path + 1), dtype=torch.int32, device=device)
+    output, path, kept = result.split([rows * max_path, rows * max_path, rows])
+    index, at, size = tok.get_device(), result.data_ptr(), 4 * rows * max_path
+    with torch.cuda.device(index):
+        rc = _lib.lib().aspire_verify_tree(tok.data_ptr(), par.data_ptr(), tgt.data_ptr(), qo.data_ptr(), tokens, rows, max_path,
+                                           at, at + size, at + 2 * size, torch._C._cuda_getCurrentRawStream(index))
+    _lib.check(rc, what)
+    return output.view(rows, max_path), path.view(rows, max_path), kept
+
+
 def first_eos(output: torch.Tensor, committed: torch.Tensor, eos_token_ids: tuple[int, ...]):
     """Cut each row's ``committed`` tokens after its first end-of-sequence token: returns
     ``(committed', found)`` with committed' = index of the first EOS + 1 where one occurs
@@ -109,4 +144,5 @@ def first_eos(output: torch.Tensor, committed: torch.Tensor, eos_token_ids: tupl
     return torch.where(found, first + 1, committed), found
 
 
-__all__ = ["local_topk_candidates", "merge_topk_candidates", "verify_topk_speculation", "first_eos"]
+__all__ = ["local_topk_candidates", "merge_topk_candidates", "verify_topk_speculation", "verify_tree_speculation",
+           "first_eos"]

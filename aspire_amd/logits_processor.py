@@ -6,11 +6,19 @@ one kernel (``aspire_logits_pipe``): fp32 ``softmax(values / temperature)`` and 
 renormalisation per row. ``define_logit_process_op`` registers ``mylib::logit_process``
 around a pipe, as ``_define_logit_op`` does, with the fake (meta) implementation
 torch.compile traces through.
+
+``adjust_logits`` (not in the reference, whose pipes take logits as they are) goes before a pipe, a greedy pick or
+``local_topk_candidates``: penalties for repeated tokens, biases (``LogitBias``) and grammar masks, one launch
+(``aspire_adjust_logits``).
 """
 
 from __future__ import annotations
 
+import math
+import struct
+
 import torch
+from torch.autograd import forward_ad
 
 from aspire_amd import _lib
 
@@ -97,4 +105,125 @@ def build_logits_pipe(temperature: float = 0, top_p: float = 0):
     return LogitsPipe(ops), kwargs
 
 
-__all__ = ["LogitsPipe", "Temperature", "Softmax", "TopP", "define_logit_process_op", "build_logits_pipe"]
+class LogitBias:
+    """Each request's biases (``{token: value}``, or None) on a device, for ``adjust_logits``; made when requests come or go."""
+
+    def __init__(self, biases, device="cuda"):
+        ids, values, ends = [], [], [0]
+        for m in biases:
+            for token, value in sorted((m or {}).items()):
+                if not 0 <= int(token) < 1 << 31 or math.isnan(value):
+                    raise ValueError("LogitBias: tokens must be 0 to 2^31 - 1, values not NaN")
+                ids.append(int(token))
+                values.append(float(value))
+            ends.append(len(ids))
+        self.requests = len(ends) - 1
+        self.ids = torch.tensor(ids, dtype=torch.int32, device=device)
+        self.values = torch.tensor(values, dtype=torch.float32, device=device)
+        self.indptr = torch.tensor(ends, dtype=torch.int32, device=device)
+
+
+_LOGIT_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_ADJUST = struct.Struct("PqPqPPqPPPPPPPqPPPPqPq8i")  # aspire_adjust_logits_args
+
+
+def adjust_logits(logits: torch.Tensor, *, qo_indptr: torch.Tensor | None = None, history: torch.Tensor | None = None,
+                  history_lens: torch.Tensor | None = None, prompt_lens: torch.Tensor | None = None,
+                  repetition: torch.Tensor | None = None, presence: torch.Tensor | None = None,
+                  frequency: torch.Tensor | None = None, tree_tokens: torch.Tensor | None = None,
+                  tree_masks: torch.Tensor | None = None, bias: LogitBias | None = None,
+                  grammar: torch.Tensor | None = None, grammar_rows: torch.Tensor | None = None, vocab_start: int = 0,
+                  out: torch.Tensor | None = None) -> torch.Tensor:
+    """Logits ``[T, V]`` (bf16, fp16 or fp32) with penalties for repeated tokens, biases and masks, as a new tensor or in
+    ``out`` (which may be ``logits`` itself).
+
+    Request ``b`` (of at most 65,535) has the rows ``qo_indptr[b]`` to ``qo_indptr[b + 1]`` (None: row ``b``, as many requests as
+    rows); rows of no request are left as they were in ``out``. In this order, in fp32, rounded once:
+
+    * ``x / repetition`` for ``x > 0``, else ``x * repetition``, for every token of the request's prompt or output; then
+      ``x - frequency * count - presence * (count > 0)``, ``count`` its occurrences in the output (fp32 ``[B]`` each, None: 1, 0
+      and 0). ``history`` int32 ``[B, H]`` holds ``history_lens[b]`` tokens, the first ``prompt_lens[b]`` the prompt's (None: none).
+      With ``tree_tokens`` int32 ``[T]`` and ``tree_masks`` int64 ``[T, W]`` (as ``tree_attention`` takes them) the drafted tokens
+      that a row sees, itself among them, are output too: they are then not in the history. Tokens outside the vocabulary do not count;
+    * ``x + bias`` for the request's ``LogitBias`` entries;
+    * ``-inf`` where the row's mask does not allow a token: bit ``i % 32`` of word ``i // 32`` of ``grammar`` int32 ``[G, ceil(V / 32)]``,
+      row ``grammar_rows[t]`` (int32 ``[T]``; an index outside: no mask) or ``t``.
+
+    ``vocab_start`` is the token of column 0, for a shard of the vocabulary; masks are the shard's. Not differentiable."""
+    what = "adjust_logits"
+    _lib.require_cuda(logits, what=what)
+    if torch.is_grad_enabled() and logits.requires_grad or forward_ad._current_level >= 0 and _lib.has_tangent(logits, out):
+        raise ValueError(f"{what}: not differentiable")
+    code, device = _LOGIT_DTYPES.get(logits.dtype), logits.device
+    if code is None or logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise ValueError(f"{what}: logits must be bf16, fp16 or fp32 [T, V] with contiguous rows")
+    tokens, vocab = logits.shape
+    if out is None:
+        out = torch.empty((tokens, vocab), dtype=logits.dtype, device=device)
+    elif out is not logits:
+        if out.shape != logits.shape or out.dtype != logits.dtype or out.device != device or (vocab > 1 and out.stride(1) != 1):
+            raise ValueError(f"{what}: out must be of logits' shape and type on {device} with contiguous rows")
+        if _lib.overlap(out, logits) and (out.data_ptr() != logits.data_ptr() or out.stride() != logits.stride()):
+            raise ValueError(f"{what}: out must be logits itself or apart from it")
+    if tokens > 1 and out.stride(0) < vocab:
+        raise ValueError(f"{what}: the rows of out share memory")
+
+    def vector(t, name, dtype, length=None, least=None):
+        if t is None:
+            return None
+        good = t.dim() == 1 and t.device == device and (t.dtype == dtype or dtype is torch.int32 and t.dtype == torch.int64)
+        if not good or length is not None and t.shape[0] != length or least is not None and t.shape[0] < least:
+            raise ValueError(f"{what}: {name} must be {dtype} [{length if length is not None else f'at least {least or 0}'}] on {device}")
+        return _lib.dense(t, dtype)
+
+    i32, f32 = torch.int32, torch.float32
+    qo = vector(qo_indptr, "qo_indptr", i32, least=1)
+    requests = tokens if qo is None else qo.shape[0] - 1
+    lens = vector(history_lens, "history_lens", i32, requests)
+    told = vector(prompt_lens, "prompt_lens", i32, requests)
+    rep, pres, freq = (vector(t, n, f32, requests) for t, n in ((repetition, "repetition"), (presence, "presence"),
+                                                                (frequency, "frequency")))
+    history_stride = history_len = mask_stride = words = grammar_stride = grammar_count = 0
+    if history is not None:
+        if history.dim() != 2 or history.dtype != i32 or history.shape[0] != requests or history.device != device \
+                or (history.shape[1] > 1 and history.stride(1) != 1) or lens is None:
+            raise ValueError(f"{what}: history must be int32 [{requests}, H] on {device} with contiguous rows, and history_lens given")
+        history_stride, history_len = history.stride(0), history.shape[1]
+    elif lens is not None or told is not None:
+        raise ValueError(f"{what}: history_lens and prompt_lens go with history")
+    if (tree_tokens is None) != (tree_masks is None) or tree_masks is not None and qo is None:
+        raise ValueError(f"{what}: tree_tokens and tree_masks go together, with qo_indptr")
+    tree = vector(tree_tokens, "tree_tokens", i32, least=tokens)
+    if tree_masks is not None:
+        if tree_masks.dtype != torch.int64 or tree_masks.dim() != 2 or tree_masks.shape[0] < tokens or tree_masks.device != device \
+                or (tree_masks.shape[1] > 1 and tree_masks.stride(1) != 1):
+            raise ValueError(f"{what}: tree_masks must be int64 [T, words] on {device} with contiguous rows")
+        mask_stride, words = tree_masks.stride(0), tree_masks.shape[1]
+    if (history is not None or tree is not None) and rep is None and pres is None and freq is None:
+        raise ValueError(f"{what}: a history or a tree needs repetition, presence or frequency")
+    if history is None and tree is None and (rep is not None or pres is not None or freq is not None):
+        raise ValueError(f"{what}: penalties need a history or a tree")
+    if bias is not None and (bias.requests != requests or bias.indptr.device != device):
+        raise ValueError(f"{what}: bias must hold {requests} requests on {device}")
+    if grammar is not None:
+        if grammar.dtype != i32 or grammar.dim() != 2 or grammar.shape[1] < (vocab + 31) // 32 or grammar.device != device \
+                or (grammar.shape[1] > 1 and grammar.stride(1) != 1) or (grammar_rows is None and grammar.shape[0] < tokens):
+            raise ValueError(f"{what}: grammar must be int32 [rows, {(vocab + 31) // 32}] on {device} with contiguous rows, a row for each "
+                             "row of logits or grammar_rows given")
+        grammar_stride, grammar_count = grammar.stride(0), grammar.shape[0]
+    elif grammar_rows is not None:
+        raise ValueError(f"{what}: grammar_rows go with grammar")
+    which = vector(grammar_rows, "grammar_rows", i32, least=tokens)
+    if not 0 <= vocab_start < 1 << 31:
+        raise ValueError(f"{what}: vocab_start must be 0 to 2^31 - 1")
+    at = lambda t: 0 if t is None else t.data_ptr()
+    b = (None, None, None) if bias is None else (bias.ids, bias.values, bias.indptr)
+    args = _ADJUST.pack(logits.data_ptr(), logits.stride(0), out.data_ptr(), out.stride(0), at(qo), at(history), history_stride,
+                        at(lens), at(told), at(rep), at(pres), at(freq), at(tree), at(tree_masks), mask_stride, at(b[0]), at(b[1]),
+                        at(b[2]), at(grammar), grammar_stride, at(which), vocab_start, tokens, vocab, requests, code, history_len,
+                        words, grammar_count, 0 if bias is None else bias.ids.shape[0])
+    _lib.launch(_lib.lib().aspire_adjust_logits, args, logits.get_device(), what)
+    return out
+
+
+__all__ = ["LogitBias", "adjust_logits", "LogitsPipe", "Temperature", "Softmax", "TopP", "define_logit_process_op", "build_logits_pipe"]

@@ -640,6 +640,114 @@ int aspire_verify_topk_speculation(const float* draft_probs, const int64_t* draf
                                    const float* uniforms, int32_t requests, int32_t max_draft, int32_t top_k,
                                    int64_t* output, int32_t* emitted, void* stream);
 
+/* ------------------------------------------------------ drafted trees
+ * A step that drafts a tree of tokens for each request: its pages and device tables, the attention of its tokens, the
+ * adjustment of their logits, and what is kept of it. Every count that a request brings is read on the device, so none
+ * of these entries waits for the host and all of them can be captured. */
+
+/* A pool of pages as three arrays: block_table [rows, width] (the pages of each row, -1 behind its held[row]), and
+ * free_pages [num_pages], a stack whose first *free_count entries are the pages of no row. The call makes every row hold
+ * the pages of lengths[row] tokens (ceil(length / page_size); a negative length leaves the row as it is): rows give back what
+ * they hold above that, then rows take what they lack, in row order. The k-th page given back comes to free_pages[count +
+ * given - 1 - k], the k-th taken is free_pages[count - 1 - k]. From the first row on that lacks more than is left, or
+ * more pages than the table is wide, no row takes any, and shortage[row] is what it lacks (0 for all others). rows <= 4096. */
+typedef struct {
+  int32_t* block_table; int32_t* held; int32_t* free_pages; int32_t* free_count; int32_t* shortage;
+  const int32_t* lengths;
+  int32_t rows; int32_t width; int32_t num_pages; int32_t page_size;
+} aspire_page_resize_args;
+
+int aspire_page_resize(const aspire_page_resize_args* args, void* stream);
+
+/* One step's tables. Row b has cached[b] tokens in its pages and fresh[b] new ones behind them (none if one is negative or
+ * both make more than 2^31 - 1).
+ * qo_indptr, kv_indptr [max_rows + 1]: running counts of tokens, and of the pages of rows with new tokens (entries from
+ * rows on repeat the last); kv_indices: those pages in order, -1 where the table has none; last_page_len [max_rows] (0
+ * without new tokens). For each token positions = cached + depth (its place when parents is NULL) and slots = page *
+ * page_size + offset of its place in the pages (-1 without a page). parents[t] is the index in its row of the
+ * token that t continues, -1 (or any index that is not below t's own) for none; masks [max_tokens, tree_words] has bit j of a
+ * token's words set for its row's token j among its ancestors and itself (NULL parents: a chain). Tokens behind the last
+ * row have position and slot -1 and mask 0. From the first row on whose tokens pass max_tokens or 64 * tree_words, or
+ * whose pages pass max_entries, no row has tokens or pages; totals = tokens and pages that all rows ask for, and that first
+ * row (rows: none). rows <= max_rows <= 4096, tree_words <= 64. */
+typedef struct {
+  const int32_t* block_table; int64_t table_stride; const int32_t* cached; const int32_t* fresh; const int32_t* parents;
+  int32_t rows; int32_t width; int32_t max_rows; int32_t max_tokens; int32_t max_entries; int32_t page_size;
+  int32_t tree_words; int32_t reserved;
+  int32_t* qo_indptr; int32_t* kv_indptr; int32_t* kv_indices; int32_t* last_page_len; int32_t* positions;
+  int64_t* slots; int64_t* masks; int64_t* totals;
+} aspire_step_tables_args;
+
+int aspire_step_tables(const aspire_step_tables_args* args, void* stream);
+
+/* Attention of trees over a paged cache [P, 2, page, H_kv, D]. Row b has tokens qo_indptr[b] .. qo_indptr[b + 1] - 1 (n of
+ * them) and kv_len = (pages - 1) * page_size + last_page_len keys, whose last n are its tokens'. A token sees the keys before those,
+ * and of those key j where bit j of its words in masks [tokens, mask_words] is set. out = softmax(sm_scale q.k) v over
+ * the keys that it sees, 0 where it sees none; lse (optional, fp32 [tokens, H_q]) base 2, -inf there. Keys on a page id
+ * outside [0, num_pages) or an entry outside [0, num_page_indices) are not seen. Tokens of no row are left as they are.
+ * dtype 0 bf16, 1 fp16; head_dim 64 or 128; page_size a power of two from 16; 16-byte aligned rows.
+ * workspace: aspire_tree_attention_workspace floats. */
+typedef struct {
+  const void* q; int64_t q_stride_t; int64_t q_stride_h;
+  const void* kv_cache; int64_t cache_stride_p; int64_t cache_stride_kv; int64_t cache_stride_t; int64_t cache_stride_h;
+  int64_t num_pages; int64_t num_page_indices;
+  const int32_t* qo_indptr; const int32_t* kv_indices; const int32_t* kv_indptr; const int32_t* kv_last_page_len;
+  const int64_t* masks; int64_t mask_stride;
+  void* out; int64_t out_stride_t; int64_t out_stride_h;
+  float* lse;
+  int32_t tokens; int32_t rows; int32_t mask_words; int32_t num_qo_heads; int32_t num_kv_heads; int32_t head_dim;
+  int32_t page_size; int32_t dtype; float sm_scale; int32_t reserved;
+  float* workspace; int64_t workspace_floats;
+} aspire_tree_attention_args;
+
+int64_t aspire_tree_attention_workspace(int32_t tokens, int32_t rows, int32_t num_qo_heads, int32_t num_kv_heads,
+                                        int32_t head_dim);
+int aspire_tree_attention(const aspire_tree_attention_args* args, void* stream);
+
+/* What is kept of each tree: from a row's first token (its root) on, the lowest child (parents, as above) whose token is
+ * the present one's target. path [rows, max_path]: the kept tokens' indices in their row, output: their targets, both -1
+ * behind the kept[row] kept ones (0 for a row without tokens). At most max_path are kept. */
+int aspire_verify_tree(const int32_t* tree_tokens, const int32_t* parents, const int32_t* targets, const int32_t* qo_indptr,
+                       int32_t tokens, int32_t rows, int32_t max_path, int32_t* output, int32_t* path, int32_t* kept,
+                       void* stream);
+
+/* Moves the kept tokens' K and V rows to where a chain of them would stand: the row at slots[first + path[row, j]] goes to
+ * slots[first + j], first = qo_indptr[row], for j = 1 .. kept[row] - 1, in every layer's cache [P, 2, page, H, D]. A path
+ * rises; entries that do not lie in (j, the row's tokens) and slots outside the pool are passed over. caches: host array of
+ * layers addresses of one layout; strides and sizes in bytes, head_bytes = D * element size. */
+typedef struct {
+  const uint64_t* caches; int64_t stride_p; int64_t stride_kv; int64_t stride_t; int64_t stride_h;
+  int64_t num_pages; const int32_t* path; const int32_t* kept; const int32_t* qo_indptr; const int64_t* slots;
+  int32_t layers; int32_t heads; int32_t head_bytes; int32_t page_size; int32_t rows; int32_t tokens; int32_t max_path;
+  int32_t reserved;
+} aspire_compact_args;
+
+int aspire_compact_accepted(const aspire_compact_args* args, void* stream);
+
+/* Penalties, biases and masks on the logits [tokens, vocab] (dtype 0 bf16, 1 fp16, 2 fp32), fp32 inside, rounded once into
+ * out (which may be logits). Request b has the tokens qo_indptr[b] .. qo_indptr[b + 1] - 1 (qo_indptr NULL: token b). Its
+ * history [requests, history_len] holds history_lens[b] tokens, the first prompt_lens[b] of them its prompt's (NULL: none);
+ * tree_tokens / tree_masks (both or neither) add, to each token's output, the drafted tokens whose bits it has. With count the
+ * occurrences among output tokens: x of a token of the prompt or the output becomes x / repetition (x > 0) or x * repetition; then
+ * x -= frequency * count, and presence where count > 0; then x += bias; then -inf where the token's bit in grammar is not
+ * set (int32 words, 32 tokens each; row grammar_rows[t] of num_grammar_rows, or t; a row outside them: no mask). Column i is token
+ * vocab_start + i of histories, trees and biases, and bit i of a mask. Biases: ids and values of request b at
+ * bias_indptr[b] .. bias_indptr[b + 1] - 1. Pointers of parts that are not wanted are NULL. */
+typedef struct {
+  const void* logits; int64_t stride; void* out; int64_t out_stride;
+  const int32_t* qo_indptr;
+  const int32_t* history; int64_t history_stride; const int32_t* history_lens; const int32_t* prompt_lens;
+  const float* repetition; const float* presence; const float* frequency;
+  const int32_t* tree_tokens; const int64_t* tree_masks; int64_t mask_stride;
+  const int32_t* bias_ids; const float* bias_values; const int32_t* bias_indptr;
+  const int32_t* grammar; int64_t grammar_stride; const int32_t* grammar_rows;
+  int64_t vocab_start;
+  int32_t tokens; int32_t vocab; int32_t requests; int32_t dtype; int32_t history_len; int32_t mask_words;
+  int32_t num_grammar_rows; int32_t bias_entries;
+} aspire_adjust_logits_args;
+
+int aspire_adjust_logits(const aspire_adjust_logits_args* args, void* stream);
+
 /* ----------------------------------------------------------------- (d) -- */
 /* HBM calibration (no reference counterpart: the measurement row asks for the
  * bandwidth achieved on the box, measured with a streaming kernel, beside the
