@@ -1,10 +1,27 @@
 // Attention of drafted trees over a paged cache (gfx950): a request's tokens see its cached keys and, of its own last n keys,
-// those of their ancestors.
+// those that their mask bits name.
 //
-// One workgroup a (token, q head): a wave takes every fourth key, a lane head_dim / 64 of its values; the running maximum and sum
-// stay in registers and the four waves join through LDS.
+// The n tokens of a request are n * G query rows of each kv head (G = q heads per kv head), cut into tiles of kRows. A tile's keys
+// are a stream that every row of it shares, so up to some hundred rows the cache's bytes bound the kernel. A
+// workgroup takes a tile's keys in steps of 32, its four waves every fourth step, each through an LDS ring of its own (no
+// barrier on the way): K and V rows go from HBM straight into LDS (buffer_load ... lds), K two steps ahead from when its
+// fragments are read, V from when its are. Per step and 16 query rows:
+//   * S^T = K . Q^T with v_mfma_f32_16x16x32 (K rows from LDS, Q in registers): lane (r, grp) holds keys 4 grp + i of row r;
+//   * softmax in fp32 with the scale folded into exp2's argument; the running maximum moves only when a key exceeds it by
+//     more than kSlack, so most steps take no maximum across lanes and rescale nothing;
+//   * O^T += V^T . P^T: the lane's 8 keys of P^T are those that S^T left it with, V^T comes by transpose reads.
+// At the end of its keys the waves join through LDS.
+//
+// Which workgroup takes which keys is decided on the device: lengths are read there alone, so a captured launch serves any. The
+// units (request, tile) of one kv head form a line of steps, each unit preceded by kStartCost steps for its start and end;
+// group j of `groups` takes the j-th equal part of the line, for each kv head. A unit that falls to several groups is written as
+// fp32 pieces (each normalised by its own sum, with its base-2 LSE) and joined by a second launch in the order of its
+// keys: results do not depend on timing. The kv head runs fastest over the workgroups, so with 8 kv heads the
+// round-robin spread over the XCDs keeps each head's pages in one L2.
 #include <algorithm>
 #include <cmath>
+#include <initializer_list>
+#include <type_traits>
 
 #include "common.h"
 
@@ -12,84 +29,583 @@ namespace aspire {
 namespace {
 
 constexpr float kNegInfT = -__builtin_huge_valf();
+constexpr float kSlack = 8.f;       // log2 units
+constexpr int kStepKeys = 32;
+constexpr int kTreeWaves = 4;
+constexpr int kTreeThreads = 64 * kTreeWaves;
+constexpr int kStartCost = 4;       // a piece's start and end, in steps
+constexpr int kMinPart = 2;         // the least that a group takes, in steps
+constexpr int kTreeGroups = 256;    // workgroups of a launch: one a CU
+constexpr uint32_t kTreeBuffer = 0x00020000u;  // gfx9 raw buffer dword 3
+
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 
 struct TreeParams {
   aspire_tree_attention_args a;
   float scale_log2;
+  int32_t group;       // q heads per kv head
+  int32_t groups;      // workgroups per kv head
+  int32_t page_shift;  // log2(page_size / 16)
+  uint32_t num_entries, num_pages;  // of the list and the pool, below 2^31
+  // of workgroup w: pieces[w] = (tile's first row among n * G, row count | kv head << 16, first token, number of pieces of the
+  // unit that starts in it and ends in a later one, or 0); its partial rows: slot 2 w of a unit that began
+  // before it, 2 w + 1 of one that goes on after it
+  int4* pieces;
+  float* part_lse;     // [2 * workgroups][rows of a tile]
+  float* part_o;       // [2 * workgroups][rows of a tile][head_dim]
 };
 
-template <bool kFp16>
-__device__ __forceinline__ float widen(uint16_t x) {
-  return kFp16 ? float(__builtin_bit_cast(_Float16, x)) : __uint_as_float(uint32_t(x) << 16);
+template <bool kF16>
+__device__ __forceinline__ f32x4 mfma32(uint4 a, uint4 b, f32x4 c) {
+  if (kF16) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  return mfma_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c);
 }
-template <bool kFp16>
-__device__ __forceinline__ uint16_t narrow(float x) {
-  return kFp16 ? __builtin_bit_cast(uint16_t, static_cast<_Float16>(x)) : __builtin_bit_cast(uint16_t, static_cast<__bf16>(x));
+typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
+template <bool kF16>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {  // to nearest even
+  if (kF16) {
+    const f16x2 v = {static_cast<_Float16>(lo), static_cast<_Float16>(hi)};
+    return __builtin_bit_cast(uint32_t, v);
+  }
+  return pack_bf16x2_rne(lo, hi);
+}
+template <bool kF16>
+__device__ __forceinline__ float widen(uint32_t x) {  // of the low half
+  return kF16 ? float(__builtin_bit_cast(_Float16, uint16_t(x))) : __uint_as_float(x << 16);
+}
+// Ones in every half whose value is infinite or NaN.
+template <bool kF16>
+__device__ __forceinline__ uint32_t special(uint32_t x) {
+  constexpr uint32_t e = kF16 ? 0x7c00u : 0x7f80u;
+  return ((x & e) == e ? 0xffffu : 0u) | ((x & (e << 16)) == (e << 16) ? 0xffff0000u : 0u);
 }
 
-template <bool kFp16, int kDim>
-__global__ __launch_bounds__(256) void tree_attention_kernel(TreeParams p) {
-  constexpr int kPer = kDim / 64;
-  __shared__ float top[4], sum[4], part[4][kDim];
+template <typename T>
+__device__ __forceinline__ T* tree_uniform(T* ptr) {
+  const uint64_t v = reinterpret_cast<uint64_t>(ptr);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane(uint32_t(v)), hi = __builtin_amdgcn_readfirstlane(uint32_t(v >> 32));
+  return reinterpret_cast<T*>((uint64_t(hi) << 32) | lo);
+}
+
+__device__ __forceinline__ int64_t wave_uniform64(int64_t v) {
+  return int64_t((uint64_t(uint32_t(__builtin_amdgcn_readfirstlane(int(v >> 32)))) << 32) | uint32_t(__builtin_amdgcn_readfirstlane(int(v))));
+}
+
+// 16 bytes a lane from its offset into the buffer to the lane's place behind dst.
+__device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t rs, uint4* dst, int offset) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)dst, 16, offset, 0, 0, 0);
+}
+
+// A request as the arrays have it, its tokens cut to those that there are.
+struct Request {
+  int q0, n, first, pages, len;
+};
+__device__ __forceinline__ Request request(const TreeParams& p, int b) {
+  const aspire_tree_attention_args& a = p.a;
+  Request r;
+  const int q0 = a.qo_indptr[b], q1 = a.qo_indptr[b + 1], first = a.kv_indptr[b], end = a.kv_indptr[b + 1];
+  const int last = a.kv_last_page_len[b];
+  r.q0 = max(q0, 0);
+  r.n = max(min(q1, a.tokens) - r.q0, 0);
+  r.first = first;
+  r.pages = int(min(max(int64_t(end) - first, int64_t(0)), int64_t(0x7fffffff)));
+  const int64_t len = r.pages > 0 ? int64_t(r.pages - 1) * a.page_size + min(max(last, 0), a.page_size) : 0;
+  r.len = int(min(len, int64_t(0x7fff0000)));
+  return r;
+}
+
+__device__ __forceinline__ int64_t wave_sum_i64(int64_t v) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d, 64);
+  return v;
+}
+
+// Tiles and steps of request b, and its length on the line of steps.
+template <int kRows>
+__device__ __forceinline__ int64_t cost(const TreeParams& p, int b, int& tiles, int& steps) {
+  const Request r = request(p, b);
+  tiles = (r.n * p.group + kRows - 1) / kRows;
+  steps = (r.len + kStepKeys - 1) / kStepKeys;
+  return int64_t(tiles) * (steps + kStartCost);
+}
+
+// kD: head_dim; kT: 16-row tiles of queries a wave holds (every wave all of the workgroup's).
+template <bool kF16, int kD, int kT>
+__global__ __launch_bounds__(kTreeThreads) void tree_stream_kernel(TreeParams p) {
+  constexpr int kRows = 16 * kT, kChunks = kD / 8, kC = kD / 32, kJ = kD / 16;
+  constexpr int kHalf = 16 * kChunks;           // 16-byte chunks of 16 keys
+  constexpr int kLoads = 2 * kHalf / 64;        // loads of a step's K, or its V
+  constexpr int kPerLoad = 64 / kChunks;        // rows of one load
+  constexpr float kBias = kF16 ? 7.f : 0.f;     // weights are 2^7 larger in fp16, whose smallest normal number is 2^-14
+  constexpr float kSumLimit = float(1 << (8 + (kF16 ? 7 : 0)));  // 2^(kSlack + kBias)
+  __shared__ uint4 k0[kTreeWaves * 2 * kHalf], v0[kTreeWaves * 2 * kHalf], k1[kTreeWaves * 2 * kHalf], v1[kTreeWaves * 2 * kHalf];
+  __shared__ float stat_m[kTreeWaves][kRows], stat_l[kTreeWaves][kRows];
   const aspire_tree_attention_args& a = p.a;
   const int lane = threadIdx.x & 63, wave = wave_uniform(threadIdx.x >> 6);
-  const int t = blockIdx.x, head = blockIdx.y, kv_head = head / (a.num_qo_heads / a.num_kv_heads);
-  const int b = wave_last_le(a.qo_indptr, a.rows, t);
-  if (b < 0 || t >= a.qo_indptr[b + 1]) return;
-  const int q0 = a.qo_indptr[b], n = a.qo_indptr[b + 1] - q0;
-  const int first = a.kv_indptr[b], pages = a.kv_indptr[b + 1] - first;
-  const int len = pages > 0 ? (pages - 1) * a.page_size + a.kv_last_page_len[b] : 0;
-  const uint16_t* const q = static_cast<const uint16_t*>(a.q) + t * a.q_stride_t + head * a.q_stride_h;
-  float qv[kPer], o[kPer], m = kNegInfT, l = 0.f;
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) qv[i] = widen<kFp16>(q[lane * kPer + i]), o[i] = 0.f;
-  for (int key = wave; key < len; key += 4) {
-    const int j = key - (len - n);
-    if (j >= 0 && !(j < 64 * a.mask_words && ((a.masks[t * a.mask_stride + (j >> 6)] >> (j & 63)) & 1))) continue;
-    const int64_t entry = int64_t(first) + key / a.page_size;
-    if (entry < 0 || entry >= a.num_page_indices) continue;
-    const int page = a.kv_indices[entry];
-    if (page < 0 || page >= a.num_pages) continue;
-    const uint16_t* const k = static_cast<const uint16_t*>(a.kv_cache) + page * a.cache_stride_p +
-                              (key % a.page_size) * a.cache_stride_t + kv_head * a.cache_stride_h + lane * kPer;
-    float x = 0.f;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) x += qv[i] * widen<kFp16>(k[i]);
-    x = wave_sum_f(x) * p.scale_log2;
-    const float up = fmaxf(m, x), use = up == kNegInfT ? 0.f : up;
-    const float keep = __builtin_amdgcn_exp2f(m - use), w = __builtin_amdgcn_exp2f(x - use);
-    m = up;
-    l = l * keep + w;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) o[i] = o[i] * keep + (w != 0.f ? w * widen<kFp16>(k[a.cache_stride_kv + i]) : 0.f);
+  const int r = lane & 15, grp = lane >> 4, G = p.group, hkv = a.num_kv_heads;
+  const int g = wave_uniform(int(blockIdx.x) % hkv), j = wave_uniform(int(blockIdx.x) / hkv);
+
+  // this group's part [line0, line1) of the line, and the row that holds its first step
+  int64_t all = 0;
+  for (int b = lane; b < a.rows; b += 64) {
+    int tiles, steps;
+    all += cost<kRows>(p, b, tiles, steps);
   }
-  if (lane == 0) top[wave] = m, sum[wave] = l;
+  all = wave_uniform64(wave_sum_i64(all));
+  const int groups = int(min(max(all / kMinPart, int64_t(1)), int64_t(p.groups)));  // each has kMinPart steps at least
+  const int64_t line0 = all * j / groups, line1 = all * (j + 1) / groups;
+  if (threadIdx.x == 0) p.pieces[blockIdx.x].w = 0;
+  if (j >= groups || all == 0) return;
+  int64_t at = 0;  // where row b begins
+  int b = 0;
+  for (int b0 = 0; b0 < a.rows; b0 += 64) {
+    int tiles, steps;
+    const int64_t c = b0 + lane < a.rows ? cost<kRows>(p, b0 + lane, tiles, steps) : 0;
+    int64_t end = c;
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) part[wave][lane * kPer + i] = o[i];
-  __syncthreads();
-  if (wave != 0) return;
-  m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-  const float use = m == kNegInfT ? 0.f : m;
-  l = 0.f;
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) o[i] = 0.f;
-  for (int w = 0; w < 4; ++w) {
-    const float keep = __builtin_amdgcn_exp2f(top[w] - use);
-    l += keep * sum[w];
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) o[i] += keep * part[w][lane * kPer + i];
+    for (int d = 1; d < 64; d <<= 1) {
+      const int64_t up = __shfl_up(end, d, 64);
+      if (lane >= d) end += up;
+    }
+    const uint64_t past = __ballot(at + end > line0);
+    if (past) {
+      const int l = __builtin_ctzll(past);
+      b = b0 + l;
+      at += __shfl(end - c, l, 64);
+      break;
+    }
+    at += __shfl(end, 63, 64);
   }
-  uint16_t* const out = static_cast<uint16_t*>(a.out) + t * a.out_stride_t + head * a.out_stride_h;
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  b = wave_uniform(b);
+  at = wave_uniform64(at);
+
+  const int row_bytes = int(a.cache_stride_t) * 2;
+  const uint32_t num_entries = p.num_entries, num_pages = p.num_pages;
+  const char* const cache = static_cast<const char*>(a.kv_cache) + int64_t(g) * a.cache_stride_h * 2;
+  int voff_k[kLoads / 2], voff_v[kLoads / 2];  // this lane's chunks of 16 keys: the one that belongs at its place in LDS
+  const auto swizzle_k = [](int row) { return kD == 128 ? row : row >> 1; };
+  const auto swizzle_v = [](int row) { return kD == 128 ? ((row & 3) << 2) | (row >> 2) : ((row >> 1) & 1) << 2; };
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) out[lane * kPer + i] = narrow<kFp16>(o[i] * inv);
-  if (a.lse != nullptr && lane == 0) a.lse[int64_t(t) * a.num_qo_heads + head] = l == 0.f ? kNegInfT : use + __builtin_log2f(l);
+  for (int i = 0; i < kLoads / 2; ++i) {
+    const int row = kPerLoad * i + lane / kChunks, c = lane % kChunks;
+    voff_k[i] = row * row_bytes + (c ^ swizzle_k(row)) * 16;
+    voff_v[i] = row * row_bytes + (c ^ swizzle_v(row)) * 16;
+  }
+  int kidx[kC], vidx[(kJ + 1) / 2];
+  const int vt_row = 4 * grp + (r >> 2);
+#pragma unroll
+  for (int c = 0; c < kC; ++c) kidx[c] = r * kChunks + ((4 * c + grp) ^ swizzle_k(r));
+#pragma unroll
+  for (int c = 0; c < (kJ + 1) / 2; ++c) vidx[c] = vt_row * kChunks + ((4 * c + (r & 3)) ^ swizzle_v(vt_row));
+  uint4* const mk[2] = {k0 + wave * 2 * kHalf, k1 + wave * 2 * kHalf};
+  uint4* const mv[2] = {v0 + wave * 2 * kHalf, v1 + wave * 2 * kHalf};
+
+  for (; b < a.rows; ++b) {
+    const Request rq = request(p, b);
+    const int q0 = wave_uniform(rq.q0), n = wave_uniform(rq.n), len = wave_uniform(rq.len);
+    const int list = wave_uniform(rq.first), pages = wave_uniform(rq.pages);
+    const int total_rows = n * G, tiles = (total_rows + kRows - 1) / kRows, steps = (len + kStepKeys - 1) / kStepKeys;
+    if (at >= line1) break;
+    const int unit = steps + kStartCost;
+    // the first tile that reaches into this group's part
+    int m = wave_uniform(at >= line0 ? 0 : int((line0 - at) / unit));
+    typedef const __attribute__((address_space(4))) int32_t* const_ids_t;
+    const const_ids_t ids = (const_ids_t)a.kv_indices;
+    const int tree_start = len - n;
+    for (; m < tiles; ++m) {
+      const int64_t unit0 = at + int64_t(m) * unit;
+      if (unit0 >= line1) break;
+      const int begin = wave_uniform(int(min(max(line0 - unit0 - kStartCost, int64_t(0)), int64_t(steps))));
+      const int end = wave_uniform(int(min(max(line1 - unit0 - kStartCost, int64_t(0)), int64_t(steps))));
+      const bool starts = line0 <= unit0;  // a unit without keys is written where it starts
+      if (begin >= end && !(steps == 0 && starts)) continue;
+      const bool whole = begin == 0 && end == steps;
+      const int row0 = m * kRows, rows = min(kRows, total_rows - row0);
+
+      uint4 qf[kT][kC];
+      const int64_t* words[kT];
+#pragma unroll
+      for (int t = 0; t < kT; ++t) {
+        const int row = min(t * 16 + r, rows - 1) + row0, node = row / G, head = g * G + row - node * G;
+        const uint16_t* const src = static_cast<const uint16_t*>(a.q) + int64_t(q0 + node) * a.q_stride_t + int64_t(head) * a.q_stride_h;
+#pragma unroll
+        for (int c = 0; c < kC; ++c) qf[t][c] = *reinterpret_cast<const uint4*>(src + 32 * c + 8 * grp);
+        words[t] = a.masks + int64_t(q0 + node) * a.mask_stride;
+      }
+      float mx[kT], use[kT], l[kT];
+      f32x4 acc[kT][kJ];
+#pragma unroll
+      for (int t = 0; t < kT; ++t) {
+        mx[t] = kNegInfT, use[t] = 0.f, l[t] = 0.f;
+#pragma unroll
+        for (int i = 0; i < kJ; ++i) acc[t][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+      }
+
+      // Loads of one half (16 keys) of a step's K or V; half-steps on a page that the pool does not have, or past the end, load
+      // nothing: out-of-range loads write zeros into LDS, and every step issues the same loads.
+      const auto page_of = [&](int step, int h) -> int {
+        const int e = (2 * step + h) >> p.page_shift;
+        const uint32_t entry = uint32_t(list) + uint32_t(e);  // 32-bit compares: there are no scalar 64-bit ones
+        const bool there = step < end && e < pages && entry < num_entries;
+        const int id = ids[there ? entry : 0u];
+        return there && uint32_t(id) < num_pages ? id : -1;
+      };
+      const auto issue = [&](uint4* buf, int step, int id0, int id1, bool v) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int id = h ? id1 : id0, sub = (2 * step + h) & ((1 << p.page_shift) - 1);
+          const int valid = id < 0 ? 0 : min(max(len - (2 * step + h) * 16, 0), 16);
+          const int span = wave_uniform(valid > 0 ? (valid - 1) * row_bytes + 2 * kD : 0);
+          const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+              const_cast<char*>(tree_uniform(cache + (int64_t(max(id, 0)) * a.cache_stride_p + (v ? a.cache_stride_kv : 0)) * 2 +
+                                             int64_t(sub) * 16 * row_bytes)), (short)0, span, kTreeBuffer);
+#pragma unroll
+          for (int i = 0; i < kLoads / 2; ++i)
+            load_to_lds(rs, buf + h * kHalf + i * 64, v ? voff_v[i] : voff_k[i]);
+        }
+      };
+      uint4 pf[kT];
+      uint32_t vis[kT];
+      const auto scores = [&](const uint4* kb, f32x4 (&s)[kT][2]) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint4 kr[kC];
+#pragma unroll
+          for (int c = 0; c < kC; ++c) kr[c] = kb[h * kHalf + kidx[c]];
+#pragma unroll
+          for (int t = 0; t < kT; ++t) {
+            s[t][h] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < kC; ++c) s[t][h] = mfma32<kF16>(kr[c], qf[t][c], s[t][h]);
+          }
+        }
+      };
+      // bits of the step's 32 keys that each row sees
+      const auto see = [&](int step, int id0, int id1) {
+        const int off = step * kStepKeys - tree_start;  // of the step's first key among the row's tokens
+        const int there = len - step * kStepKeys;
+        uint32_t limit = there >= 32 ? ~0u : (1u << max(there, 0)) - 1;
+        if (id0 < 0) limit &= 0xffff0000u;
+        if (id1 < 0) limit &= 0xffffu;
+#pragma unroll
+        for (int t = 0; t < kT; ++t) {
+          uint32_t bits = ~0u;
+          if (off > -32) {
+            const int w = max(off, 0) >> 6, sh = max(off, 0) & 63;
+            uint64_t x = w < a.mask_words ? uint64_t(words[t][w]) >> sh : 0;
+            if (sh > 32 && w + 1 < a.mask_words) x |= uint64_t(words[t][w + 1]) << (64 - sh);
+            bits = off < 0 ? (uint32_t(x) << -off) | ((1u << -off) - 1) : uint32_t(x);
+          }
+          vis[t] = bits & limit;
+        }
+      };
+      const auto softmax = [&](f32x4 (&s)[kT][2], bool masked, bool first) {
+        float x[kT][8], pv[kT][8], ps[kT];
+#pragma unroll
+        for (int t = 0; t < kT; ++t) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[t][i] = s[t][0][i], x[t][4 + i] = s[t][1][i];
+          if (masked) {
+            const uint32_t bits = vis[t] >> (4 * grp);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              x[t][i] = (bits >> i) & 1 ? x[t][i] : kNegInfT;
+              x[t][4 + i] = (bits >> (16 + i)) & 1 ? x[t][4 + i] : kNegInfT;
+            }
+          }
+        }
+        const auto exponentials = [&]() {
+#pragma unroll
+          for (int t = 0; t < kT; ++t) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) pv[t][i] = __builtin_amdgcn_exp2f(fmaf(x[t][i], p.scale_log2, -use[t]));
+            ps[t] = ((pv[t][0] + pv[t][1]) + (pv[t][2] + pv[t][3])) + ((pv[t][4] + pv[t][5]) + (pv[t][6] + pv[t][7]));
+          }
+        };
+        exponentials();
+        // a row that has seen no key yet has no offset to go by: a masked step may be its first
+        bool over = first || masked;
+#pragma unroll
+        for (int t = 0; t < kT; ++t) over |= ps[t] > kSumLimit || mx[t] == kNegInfT;
+        if (__builtin_amdgcn_ballot_w64(over) != 0) {
+#pragma unroll
+          for (int t = 0; t < kT; ++t) {
+            float top = fmaxf(fmaxf(fmaxf(x[t][0], x[t][1]), fmaxf(x[t][2], x[t][3])),
+                              fmaxf(fmaxf(x[t][4], x[t][5]), fmaxf(x[t][6], x[t][7])));
+            top = max_xor32(max_xor16(top)) * p.scale_log2;
+            const float m_new = top > mx[t] + kSlack ? top : mx[t];
+            // a row without a key before has zero sums: they stay zero
+            const float alpha = __builtin_amdgcn_exp2f(mx[t] - (m_new == kNegInfT ? 0.f : m_new));
+            mx[t] = m_new;
+            use[t] = m_new == kNegInfT ? 0.f : m_new - kBias;
+#pragma unroll
+            for (int i = 0; i < kJ; ++i) acc[t][i] *= alpha;
+            l[t] *= alpha;
+          }
+          exponentials();
+        }
+#pragma unroll
+        for (int t = 0; t < kT; ++t) {
+          pf[t] = make_uint4(pack2<kF16>(pv[t][0], pv[t][1]), pack2<kF16>(pv[t][2], pv[t][3]), pack2<kF16>(pv[t][4], pv[t][5]),
+                             pack2<kF16>(pv[t][6], pv[t][7]));
+          l[t] += ps[t];
+        }
+      };
+      const auto values = [&](const uint4* vb, bool masked) {
+        // A key that some rows see and others do not may hold infinities or NaN, which a product with weight 0 would carry over:
+        // they are taken out of the product and added for the rows that see them.
+        bool bad = false;
+        if (masked) {
+#pragma unroll
+          for (int i = 0; i < 2 * kHalf / 64; ++i) {
+            const uint4 x = vb[i * 64 + lane];
+            bad |= (special<kF16>(x.x) | special<kF16>(x.y) | special<kF16>(x.z) | special<kF16>(x.w)) != 0;
+          }
+          bad = __builtin_amdgcn_ballot_w64(bad) != 0;
+        }
+        const char* const va = reinterpret_cast<const char*>(vb);
+        const auto product = [&](auto clean) {
+#pragma unroll
+          for (int i = 0; i < kJ; ++i) {
+            const int off = vidx[i >> 1] * 16 + 8 * (i & 1);
+            uint2 wa = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(va + off)));
+            uint2 wb = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                                     (__attribute__((address_space(3))) i16x4*)(va + kHalf * 16 + off)));
+            if (decltype(clean)::value) {
+              wa.x &= ~special<kF16>(wa.x), wa.y &= ~special<kF16>(wa.y);
+              wb.x &= ~special<kF16>(wb.x), wb.y &= ~special<kF16>(wb.y);
+            }
+#pragma unroll
+            for (int t = 0; t < kT; ++t) acc[t][i] = mfma32<kF16>(make_uint4(wa.x, wa.y, wb.x, wb.y), pf[t], acc[t][i]);
+          }
+        };
+        if (!bad) {
+          product(std::false_type{});
+        } else {
+          product(std::true_type{});
+          for (int key = 0; key < kStepKeys; ++key) {
+            const int row = key & 15, e = (key & 3) + 4 * (key >> 4), from = r + 16 * (row >> 2);
+            float w[kT];
+#pragma unroll
+            for (int t = 0; t < kT; ++t) {
+              const uint32_t p0 = pf[t].x, p1 = pf[t].y, p2 = pf[t].z, p3 = pf[t].w;
+              uint32_t two = p0;
+              two = (e >> 1) == 1 ? p1 : two;
+              two = (e >> 1) == 2 ? p2 : two;
+              two = (e >> 1) == 3 ? p3 : two;
+              w[t] = __shfl(widen<kF16>((two >> (16 * (e & 1))) & 0xffffu), from, 64);
+            }
+#pragma unroll
+            for (int i = 0; i < kJ; ++i) {
+              const int c = (key >> 4) * kHalf + row * kChunks + ((4 * (i >> 1) + grp) ^ swizzle_v(row));
+              const uint2 x = *reinterpret_cast<const uint2*>(va + c * 16 + 8 * (i & 1));
+              const uint32_t sx = special<kF16>(x.x), sy = special<kF16>(x.y);
+#pragma unroll
+              for (int t = 0; t < kT; ++t) {
+                if (!((vis[t] >> key) & 1)) continue;
+                if (sx & 0xffffu) acc[t][i][0] += w[t] * widen<kF16>(x.x & 0xffffu);
+                if (sx >> 16) acc[t][i][1] += w[t] * widen<kF16>(x.x >> 16);
+                if (sy & 0xffffu) acc[t][i][2] += w[t] * widen<kF16>(x.y & 0xffffu);
+                if (sy >> 16) acc[t][i][3] += w[t] * widen<kF16>(x.y >> 16);
+              }
+            }
+          }
+        }
+      };
+
+      // this wave's steps: begin + wave, and every fourth from there; step s + 8 goes into the ring's place of step s
+      const int first = begin + wave;
+      if (first < end) {
+        int id[2][2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int s = first + u * kTreeWaves;
+          id[u][0] = page_of(s, 0), id[u][1] = page_of(s, 1);
+          issue(mk[u], s, id[u][0], id[u][1], false);
+          issue(mv[u], s, id[u][0], id[u][1], true);
+        }
+        int next0 = page_of(first + 2 * kTreeWaves, 0), next1 = page_of(first + 2 * kTreeWaves, 1);
+        const auto body = [&](int s, uint4* kb, uint4* vb, int& id0, int& id1) {
+          const bool masked = (s + 1) * kStepKeys > tree_start || (id0 | id1) < 0;
+          if (masked) see(s, id0, id1);
+          f32x4 sc[kT][2];
+          __builtin_amdgcn_s_waitcnt(0xf70 | ((3 * kLoads) & 15) | (((3 * kLoads) >> 4) << 14));  // vmcnt: this step's K
+          asm volatile("" ::: "memory");
+          scores(kb, sc);
+          const int far = s + 2 * kTreeWaves, n0 = next0, n1 = next1;
+          next0 = page_of(far + kTreeWaves, 0), next1 = page_of(far + kTreeWaves, 1);
+          issue(kb, far, n0, n1, false);
+          softmax(sc, masked, s == first);
+          __builtin_amdgcn_s_waitcnt(0xf70 | ((3 * kLoads) & 15) | (((3 * kLoads) >> 4) << 14));  // vmcnt: its V
+          asm volatile("" ::: "memory");
+          values(vb, masked);
+          issue(vb, far, n0, n1, true);
+          id0 = n0, id1 = n1;
+        };
+        for (int s = first;;) {  // no way back to the top but past both bodies: waits are counted by the order of the loads
+          body(s, mk[0], mv[0], id[0][0], id[0][1]);
+          if ((s += kTreeWaves) >= end) break;
+          body(s, mk[1], mv[1], id[1][0], id[1][1]);
+          if ((s += kTreeWaves) >= end) break;
+        }
+      }
+
+      // the waves join: each takes its share of the head's values from all
+#pragma unroll
+      for (int t = 0; t < kT; ++t) {
+        l[t] = add_xor32(add_xor16(l[t]));
+        if (grp == 0) stat_m[wave][t * 16 + r] = mx[t], stat_l[wave][t * 16 + r] = l[t];
+      }
+      __builtin_amdgcn_s_waitcnt(0xf70);  // vmcnt(0): the loads past the end have written their zeros
+      __syncthreads();
+      constexpr int kShare = kJ / kTreeWaves;  // 16-value tiles a wave writes
+      uint4* const places[4] = {k0, v0, k1, v1};
+      float inv[kT], lse[kT];
+#pragma unroll
+      for (int t = 0; t < kT; ++t) {
+        float top = kNegInfT, sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < kTreeWaves; ++w) top = fmaxf(top, stat_m[w][t * 16 + r]);
+        const float zero = top == kNegInfT ? 0.f : top;
+#pragma unroll
+        for (int w = 0; w < kTreeWaves; ++w) sum += stat_l[w][t * 16 + r] * __builtin_amdgcn_exp2f(stat_m[w][t * 16 + r] - zero);
+        const float scale = __builtin_amdgcn_exp2f(mx[t] - zero);
+        inv[t] = sum == 0.f ? 0.f : 1.f / sum;
+        lse[t] = sum == 0.f ? kNegInfT : zero - kBias + __builtin_log2f(sum);
+#pragma unroll
+        for (int i = 0; i < kJ; ++i) {
+          const f32x4 x = acc[t][i] * scale;
+          places[i / kShare][((wave * kT + t) * kShare + i % kShare) * 64 + lane] = __builtin_bit_cast(uint4, x);
+        }
+      }
+      __syncthreads();
+      const uint4* const mine = wave == 0 ? k0 : wave == 1 ? v0 : wave == 2 ? k1 : v1;
+      const int slot = 2 * blockIdx.x + (begin == 0 ? 1 : 0);
+#pragma unroll
+      for (int t = 0; t < kT; ++t) {
+        const int row = t * 16 + r;
+        f32x4 o[kShare];
+#pragma unroll
+        for (int i = 0; i < kShare; ++i) {
+          o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int w = 0; w < kTreeWaves; ++w) o[i] += __builtin_bit_cast(f32x4, mine[((w * kT + t) * kShare + i) * 64 + lane]);
+          o[i] *= inv[t];
+        }
+        if (row >= rows) continue;
+        // value of o[i][e]: 16-value tile wave * kShare + i holds 32 (tile / 2) + 8 grp + 4 (tile % 2) + e
+        const int d = kShare == 2 ? 32 * wave + 8 * grp : 32 * (wave >> 1) + 8 * grp + 4 * (wave & 1);
+        if (whole) {
+          const int node = (row0 + row) / G, head = g * G + row0 + row - node * G;
+          uint16_t* const dst = static_cast<uint16_t*>(a.out) + int64_t(q0 + node) * a.out_stride_t + int64_t(head) * a.out_stride_h + d;
+          uint32_t packed[2 * kShare];
+#pragma unroll
+          for (int i = 0; i < kShare; ++i) packed[2 * i] = pack2<kF16>(o[i][0], o[i][1]), packed[2 * i + 1] = pack2<kF16>(o[i][2], o[i][3]);
+          if (kShare == 2) *reinterpret_cast<uint4*>(dst) = make_uint4(packed[0], packed[1], packed[2 * kShare - 2], packed[2 * kShare - 1]);
+          else *reinterpret_cast<uint2*>(dst) = make_uint2(packed[0], packed[1]);
+          if (a.lse != nullptr && wave == 0 && grp == 0) a.lse[int64_t(q0 + node) * a.num_qo_heads + head] = lse[t];
+        } else {
+          float* const dst = p.part_o + (int64_t(slot) * kRows + row) * kD + d;
+#pragma unroll
+          for (int i = 0; i < kShare; ++i) *reinterpret_cast<f32x4*>(dst + 4 * i) = o[i];
+          if (wave == 0 && grp == 0) p.part_lse[int64_t(slot) * kRows + row] = lse[t];
+        }
+      }
+      if (begin == 0 && end < steps && threadIdx.x == 0) {
+        // the groups that hold the unit's other steps: the last one's part holds its last step
+        const int64_t last = unit0 + unit - 1;
+        int jl = int(last * groups / all);
+        while (all * (jl + 1) / groups <= last) ++jl;
+        while (all * jl / groups > last) --jl;
+        p.pieces[blockIdx.x] = make_int4(row0, rows | (g << 16), q0, jl - j + 1);
+      }
+      __syncthreads();  // the ring is free again
+    }
+    at += int64_t(tiles) * unit;
+  }
 }
+
+// Units cut into pieces: out = sum_i 2^(lse_i - m) o_i / sum_i 2^(lse_i - m), rounded once, pieces in the order of their keys. A
+// workgroup takes 256 / (kD / 8) rows of the unit that starts in workgroup blockIdx.x of the launch before.
+template <bool kF16, int kD>
+__global__ __launch_bounds__(256) void tree_join_kernel(TreeParams p, int tile_rows) {
+  constexpr int kLanes = kD / 8, kRound = 4;
+  const aspire_tree_attention_args& a = p.a;
+  const int4 u = p.pieces[blockIdx.x];
+  const int row = blockIdx.y * (256 / kLanes) + threadIdx.x / kLanes, d = (threadIdx.x % kLanes) * 8;
+  if (u.w == 0 || row >= (u.y & 0xffff)) return;
+  const int w = blockIdx.x, hkv = a.num_kv_heads;
+  const auto slot = [&](int i) { return (int64_t(2) * (w + i * hkv) + (i == 0 ? 1 : 0)) * tile_rows + row; };
+  float top = kNegInfT, sum = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  for (int k = 0; k < u.w; k += kRound) {
+    float lse[kRound];
+    float4 x[kRound], y[kRound];
+#pragma unroll
+    for (int i = 0; i < kRound; ++i) {
+      const int64_t s = slot(min(k + i, u.w - 1));
+      lse[i] = k + i < u.w ? p.part_lse[s] : kNegInfT;
+      x[i] = *reinterpret_cast<const float4*>(p.part_o + s * kD + d);
+      y[i] = *reinterpret_cast<const float4*>(p.part_o + s * kD + d + 4);
+    }
+    float next = top;
+#pragma unroll
+    for (int i = 0; i < kRound; ++i) next = fmaxf(next, lse[i]);
+    const float zero = next == kNegInfT ? 0.f : next, keep = __builtin_amdgcn_exp2f(top - zero);
+    sum *= keep;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] *= keep;
+#pragma unroll
+    for (int i = 0; i < kRound; ++i) {
+      if (k + i >= u.w) break;
+      const float f = __builtin_amdgcn_exp2f(lse[i] - zero);
+      sum += f;
+      o[0] += f * x[i].x, o[1] += f * x[i].y, o[2] += f * x[i].z, o[3] += f * x[i].w;
+      o[4] += f * y[i].x, o[5] += f * y[i].y, o[6] += f * y[i].z, o[7] += f * y[i].w;
+    }
+    top = next;
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const int at = u.x + row, node = at / p.group, token = u.z + node, head = (u.y >> 16) * p.group + at - node * p.group;
+  *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + int64_t(token) * a.out_stride_t + int64_t(head) * a.out_stride_h + d) =
+      make_uint4(pack2<kF16>(o[0] * inv, o[1] * inv), pack2<kF16>(o[2] * inv, o[3] * inv), pack2<kF16>(o[4] * inv, o[5] * inv),
+                 pack2<kF16>(o[6] * inv, o[7] * inv));
+  if (a.lse != nullptr && d == 0) a.lse[int64_t(token) * a.num_qo_heads + head] = sum == 0.f ? kNegInfT : top + __builtin_log2f(sum);
+}
+
+// What a launch is made of: 16-row tiles a wave, groups a kv head.
+struct TreeChoice {
+  int tiles, groups;
+};
+TreeChoice choose(int tokens, int rows, int hq, int hkv) {
+  // the smallest tile that holds a mean request's query rows
+  const int64_t mean = (int64_t(tokens) + rows - 1) / rows * (hq / hkv);
+  const int tiles = mean <= 16 ? 1 : mean <= 32 ? 2 : 4;
+  return {tiles, std::max(1, kTreeGroups / hkv)};
+}
+template <bool kF16, int kD>
+void launch(const TreeParams& p, TreeChoice c, hipStream_t s) {
+  const int wgs = c.groups * p.a.num_kv_heads, tile_rows = 16 * c.tiles;
+  if (c.tiles == 1) tree_stream_kernel<kF16, kD, 1><<<wgs, kTreeThreads, 0, s>>>(p);
+  else if (c.tiles == 2) tree_stream_kernel<kF16, kD, 2><<<wgs, kTreeThreads, 0, s>>>(p);
+  else tree_stream_kernel<kF16, kD, 4><<<wgs, kTreeThreads, 0, s>>>(p);
+  constexpr int kJoinRows = 256 / (kD / 8);
+  tree_join_kernel<kF16, kD><<<dim3(wgs, (tile_rows + kJoinRows - 1) / kJoinRows), 256, 0, s>>>(p, tile_rows);
+}
+int64_t piece_bytes(int64_t workgroups) { return (workgroups * int64_t(sizeof(int4)) + 255) / 256 * 256; }
 
 }  // namespace
 }  // namespace aspire
 
-extern "C" int64_t aspire_tree_attention_workspace(int32_t, int32_t, int32_t, int32_t, int32_t) { return 0; }
+extern "C" int64_t aspire_tree_attention_workspace(int32_t tokens, int32_t rows, int32_t num_qo_heads, int32_t num_kv_heads,
+                                                   int32_t head_dim) {
+  using namespace aspire;
+  if (tokens <= 0 || rows <= 0 || num_kv_heads <= 0 || num_qo_heads <= 0 || num_qo_heads % num_kv_heads != 0 || head_dim <= 0 ||
+      num_qo_heads > 1024)
+    return 0;
+  const TreeChoice c = choose(tokens, rows, num_qo_heads, num_kv_heads);
+  const int64_t wgs = int64_t(c.groups) * num_kv_heads;
+  return piece_bytes(wgs) / 4 + 2 * wgs * 16 * c.tiles * (head_dim + 1);
+}
 
 extern "C" int aspire_tree_attention(const aspire_tree_attention_args* a, void* stream) {
   using namespace aspire;
@@ -101,19 +617,42 @@ extern "C" int aspire_tree_attention(const aspire_tree_attention_args* a, void* 
   ASPIRE_CHECK_ARG(a->page_size >= 16 && a->page_size <= 1024 && (a->page_size & (a->page_size - 1)) == 0, "page_size must be a power of two from 16 to 1,024");
   ASPIRE_CHECK_ARG(a->dtype == 0 || a->dtype == 1, "dtype must be 0 or 1");
   ASPIRE_CHECK_ARG(std::isfinite(a->sm_scale) && a->sm_scale > 0.f && a->sm_scale <= 1e30f, "sm_scale must be positive and finite");
+  ASPIRE_CHECK_ARG(a->tokens <= (1 << 20) && a->rows <= (1 << 20), "more than 2^20 tokens or rows");
   if (a->tokens == 0 || a->rows == 0) return ASPIRE_OK;
-  ASPIRE_CHECK_ARG(a->q && a->out && a->qo_indptr && a->kv_indptr && a->kv_last_page_len &&
-                       (a->masks || a->mask_words == 0) && (a->kv_cache || a->num_pages == 0) &&
-                       (a->kv_indices || a->num_page_indices == 0), "null array");
-  TreeParams p{*a, a->sm_scale * 1.4426950408889634f};
-  const dim3 grid(a->tokens, a->num_qo_heads);
+  ASPIRE_CHECK_ARG(a->q && a->out && a->qo_indptr && a->kv_indptr && a->kv_last_page_len && (a->masks || a->mask_words == 0), "null array");
+  ASPIRE_CHECK_ARG(a->num_pages > 0 && a->num_page_indices > 0 && a->kv_cache && a->kv_indices, "no pages");
+  ASPIRE_CHECK_ARG(a->cache_stride_t >= a->head_dim && a->cache_stride_t < (int64_t(1) << 26), "tokens of a page must lie head_dim to 2^26 - 1 values apart");
+  const auto aligned = [](const void* ptr, std::initializer_list<int64_t> strides) {
+    int64_t bits = static_cast<int64_t>(reinterpret_cast<uintptr_t>(ptr)) / 2 % 8;
+    for (int64_t s : strides) bits |= s;
+    return (bits & 7) == 0;
+  };
+  ASPIRE_CHECK_ARG(aligned(a->q, {a->q_stride_t, a->q_stride_h}) && aligned(a->out, {a->out_stride_t, a->out_stride_h}) &&
+                       aligned(a->kv_cache, {a->cache_stride_p, a->cache_stride_kv, a->cache_stride_t, a->cache_stride_h}),
+                   "heads must start on 16 bytes");
+  const TreeChoice c = choose(a->tokens, a->rows, a->num_qo_heads, a->num_kv_heads);
+  const int wgs = c.groups * a->num_kv_heads, tile_rows = 16 * c.tiles;
+  ASPIRE_CHECK_ARG(a->workspace && a->workspace_floats >= aspire_tree_attention_workspace(a->tokens, a->rows, a->num_qo_heads, a->num_kv_heads, a->head_dim),
+                   "workspace too small");
+  ASPIRE_CHECK_ARG((reinterpret_cast<uintptr_t>(a->workspace) & 15) == 0, "workspace must start on 16 bytes");
+  TreeParams p{};
+  p.a = *a;
+  p.scale_log2 = a->sm_scale * 1.4426950408889634f;
+  p.group = a->num_qo_heads / a->num_kv_heads;
+  p.groups = c.groups;
+  p.num_entries = static_cast<uint32_t>(std::min<int64_t>(a->num_page_indices, 0x7fffffff));
+  p.num_pages = static_cast<uint32_t>(std::min<int64_t>(a->num_pages, 0x7fffffff));
+  while ((16 << p.page_shift) < a->page_size) ++p.page_shift;
+  p.pieces = reinterpret_cast<int4*>(a->workspace);
+  p.part_o = a->workspace + piece_bytes(wgs) / 4;
+  p.part_lse = p.part_o + int64_t(2) * wgs * tile_rows * a->head_dim;
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (a->dtype == 1) {
-    if (a->head_dim == 128) tree_attention_kernel<true, 128><<<grid, 256, 0, s>>>(p);
-    else tree_attention_kernel<true, 64><<<grid, 256, 0, s>>>(p);
+    if (a->head_dim == 128) launch<true, 128>(p, c, s);
+    else launch<true, 64>(p, c, s);
   } else {
-    if (a->head_dim == 128) tree_attention_kernel<false, 128><<<grid, 256, 0, s>>>(p);
-    else tree_attention_kernel<false, 64><<<grid, 256, 0, s>>>(p);
+    if (a->head_dim == 128) launch<false, 128>(p, c, s);
+    else launch<false, 64>(p, c, s);
   }
   ASPIRE_CHECK_LAUNCH();
   return ASPIRE_OK;
