@@ -120,47 +120,251 @@ __device__ __forceinline__ int64_t wave_sum_i64(int64_t v) {
   return v;
 }
 
-// Tiles and steps of request b, and its length on the line of steps.
+// Request b's length on the line of steps.
 template <int kRows>
-__device__ __forceinline__ int64_t cost(const TreeParams& p, int b, int& tiles, int& steps) {
+__device__ __forceinline__ int64_t cost(const TreeParams& p, int b) {
   const Request r = request(p, b);
-  tiles = (r.n * p.group + kRows - 1) / kRows;
-  steps = (r.len + kStepKeys - 1) / kStepKeys;
-  return int64_t(tiles) * (steps + kStartCost);
+  return int64_t((r.n * p.group + kRows - 1) / kRows) * ((r.len + kStepKeys - 1) / kStepKeys + kStartCost);
 }
 
-// kD: head_dim; kT: 16-row tiles of queries a wave holds (every wave all of the workgroup's).
+// One wave's query rows and what it does with a step of 32 keys: K rows in kb, V rows in vb, 16 keys after 16.
 template <bool kF16, int kD, int kT>
-__global__ __launch_bounds__(kTreeThreads) void tree_stream_kernel(TreeParams p) {
-  constexpr int kRows = 16 * kT, kChunks = kD / 8, kC = kD / 32, kJ = kD / 16;
-  constexpr int kHalf = 16 * kChunks;           // 16-byte chunks of 16 keys
-  constexpr int kLoads = 2 * kHalf / 64;        // loads of a step's K, or its V
-  constexpr int kPerLoad = 64 / kChunks;        // rows of one load
-  constexpr float kBias = kF16 ? 7.f : 0.f;     // weights are 2^7 larger in fp16, whose smallest normal number is 2^-14
-  constexpr float kSumLimit = float(1 << (8 + (kF16 ? 7 : 0)));  // 2^(kSlack + kBias)
-  __shared__ uint4 k0[kTreeWaves * 2 * kHalf], v0[kTreeWaves * 2 * kHalf], k1[kTreeWaves * 2 * kHalf], v1[kTreeWaves * 2 * kHalf];
-  __shared__ float stat_m[kTreeWaves][kRows], stat_l[kTreeWaves][kRows];
+struct TreeWave {
+  static constexpr int kChunks = kD / 8, kC = kD / 32, kJ = kD / 16;
+  static constexpr int kHalf = 16 * kChunks;           // 16-byte chunks of 16 keys
+  static constexpr int kLoads = kHalf / 64;            // 1 KiB loads of them
+  static constexpr int kPerLoad = 64 / kChunks;        // rows of one load
+  static constexpr float kBias = kF16 ? 7.f : 0.f;     // weights are 2^7 larger in fp16, whose smallest normal number is 2^-14
+  static constexpr float kSumLimit = float(1 << (8 + (kF16 ? 7 : 0)));  // 2^(kSlack + kBias)
+
+  int r, grp;
+  int kidx[kC], vidx[(kJ + 1) / 2];
+  float scale_log2;
+  uint4 qf[kT][kC];
+  const int64_t* words[kT];
+  float mx[kT], use[kT], l[kT];
+  f32x4 acc[kT][kJ];
+  f32x4 sc[kT][2];
+  uint4 pf[kT];
+  uint32_t vis[kT];
+
+  // LDS places: chunk c of a K row r is at c ^ swizzle_k(r), so that 16 rows' chunks c lie in different banks, and a V row's
+  // where transpose reads of 4 rows do
+  static __device__ __forceinline__ int swizzle_k(int row) { return kD == 128 ? row : row >> 1; }
+  static __device__ __forceinline__ int swizzle_v(int row) { return kD == 128 ? ((row & 3) << 2) | (row >> 2) : ((row >> 1) & 1) << 2; }
+
+  __device__ __forceinline__ void init(int lane, float scale) {
+    r = lane & 15, grp = lane >> 4, scale_log2 = scale;
+    const int vt_row = 4 * grp + (r >> 2);
+#pragma unroll
+    for (int c = 0; c < kC; ++c) kidx[c] = r * kChunks + ((4 * c + grp) ^ swizzle_k(r));
+#pragma unroll
+    for (int c = 0; c < (kJ + 1) / 2; ++c) vidx[c] = vt_row * kChunks + ((4 * c + (r & 3)) ^ swizzle_v(vt_row));
+  }
+  // rows row0 .. of a request's (past its last one the last again: they are computed and not written)
+  __device__ __forceinline__ void start(const TreeParams& p, int q0, int row0, int last, int g) {
+    const aspire_tree_attention_args& a = p.a;
+#pragma unroll
+    for (int t = 0; t < kT; ++t) {
+      const int row = min(row0 + t * 16 + r, last), node = row / p.group, head = g * p.group + row - node * p.group;
+      const uint16_t* const src = static_cast<const uint16_t*>(a.q) + int64_t(q0 + node) * a.q_stride_t + int64_t(head) * a.q_stride_h;
+#pragma unroll
+      for (int c = 0; c < kC; ++c) qf[t][c] = *reinterpret_cast<const uint4*>(src + 32 * c + 8 * grp);
+      words[t] = a.masks + int64_t(q0 + node) * a.mask_stride;
+      mx[t] = kNegInfT, use[t] = 0.f, l[t] = 0.f;
+#pragma unroll
+      for (int i = 0; i < kJ; ++i) acc[t][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+  }
+  // Bits of the 32 keys from key0 on that each row sees, of `there` that are left; off: key0's place among the tree's tokens.
+  __device__ __forceinline__ void see(int off, int there, bool page0, bool page1, int mask_words) {
+    uint32_t limit = there >= 32 ? ~0u : (1u << max(there, 0)) - 1;
+    if (!page0) limit &= 0xffff0000u;
+    if (!page1) limit &= 0xffffu;
+#pragma unroll
+    for (int t = 0; t < kT; ++t) {
+      uint32_t bits = ~0u;
+      if (off > -32) {
+        const int w = max(off, 0) >> 6, sh = max(off, 0) & 63;
+        uint64_t x = w < mask_words ? uint64_t(words[t][w]) >> sh : 0;
+        if (sh > 32 && w + 1 < mask_words) x |= uint64_t(words[t][w + 1]) << (64 - sh);
+        bits = off < 0 ? (uint32_t(x) << -off) | ((1u << -off) - 1) : uint32_t(x);
+      }
+      vis[t] = bits & limit;
+    }
+  }
+  __device__ __forceinline__ void scores(const uint4* kb) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint4 kr[kC];
+#pragma unroll
+      for (int c = 0; c < kC; ++c) kr[c] = kb[h * kHalf + kidx[c]];
+#pragma unroll
+      for (int t = 0; t < kT; ++t) {
+        sc[t][h] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < kC; ++c) sc[t][h] = mfma32<kF16>(kr[c], qf[t][c], sc[t][h]);
+      }
+    }
+  }
+  __device__ __forceinline__ void softmax(bool masked) {
+    float x[kT][8], pv[kT][8], ps[kT];
+#pragma unroll
+    for (int t = 0; t < kT; ++t) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[t][i] = sc[t][0][i], x[t][4 + i] = sc[t][1][i];
+    }
+    if (masked) {
+#pragma unroll
+      for (int t = 0; t < kT; ++t) {
+        const uint32_t bits = vis[t] >> (4 * grp);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          x[t][i] = (bits >> i) & 1 ? x[t][i] : kNegInfT;
+          x[t][4 + i] = (bits >> (16 + i)) & 1 ? x[t][4 + i] : kNegInfT;
+        }
+      }
+    }
+    const auto exponentials = [&]() {
+#pragma unroll
+      for (int t = 0; t < kT; ++t) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) pv[t][i] = __builtin_amdgcn_exp2f(fmaf(x[t][i], scale_log2, -use[t]));
+        ps[t] = ((pv[t][0] + pv[t][1]) + (pv[t][2] + pv[t][3])) + ((pv[t][4] + pv[t][5]) + (pv[t][6] + pv[t][7]));
+      }
+    };
+    exponentials();
+    // a row that has seen no key yet (on its first step; later if that one was masked) has no offset to go by
+    bool over = masked;
+#pragma unroll
+    for (int t = 0; t < kT; ++t) over |= ps[t] > kSumLimit || mx[t] == kNegInfT;
+    if (__builtin_amdgcn_ballot_w64(over) != 0) {
+#pragma unroll
+      for (int t = 0; t < kT; ++t) {
+        float top = fmaxf(fmaxf(fmaxf(x[t][0], x[t][1]), fmaxf(x[t][2], x[t][3])),
+                          fmaxf(fmaxf(x[t][4], x[t][5]), fmaxf(x[t][6], x[t][7])));
+        top = max_xor32(max_xor16(top)) * scale_log2;
+        const float m_new = top > mx[t] + kSlack ? top : mx[t];
+        // a row without a key before has zero sums: they stay zero
+        const float alpha = __builtin_amdgcn_exp2f(mx[t] - (m_new == kNegInfT ? 0.f : m_new));
+        mx[t] = m_new;
+        use[t] = m_new == kNegInfT ? 0.f : m_new - kBias;
+#pragma unroll
+        for (int i = 0; i < kJ; ++i) acc[t][i] *= alpha;
+        l[t] *= alpha;
+      }
+      exponentials();
+    }
+#pragma unroll
+    for (int t = 0; t < kT; ++t) {
+      pf[t] = make_uint4(pack2<kF16>(pv[t][0], pv[t][1]), pack2<kF16>(pv[t][2], pv[t][3]), pack2<kF16>(pv[t][4], pv[t][5]),
+                         pack2<kF16>(pv[t][6], pv[t][7]));
+      l[t] += ps[t];
+    }
+  }
+  template <bool kClean>
+  __device__ __forceinline__ void product(const uint4* vb) {
+    const char* const va = reinterpret_cast<const char*>(vb);
+#pragma unroll
+    for (int i = 0; i < kJ; ++i) {
+      const int off = vidx[i >> 1] * 16 + 8 * (i & 1);
+      uint2 wa = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(va + off)));
+      uint2 wb = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                               (__attribute__((address_space(3))) i16x4*)(va + kHalf * 16 + off)));
+      if (kClean) {
+        wa.x &= ~special<kF16>(wa.x), wa.y &= ~special<kF16>(wa.y);
+        wb.x &= ~special<kF16>(wb.x), wb.y &= ~special<kF16>(wb.y);
+      }
+#pragma unroll
+      for (int t = 0; t < kT; ++t) acc[t][i] = mfma32<kF16>(make_uint4(wa.x, wa.y, wb.x, wb.y), pf[t], acc[t][i]);
+    }
+  }
+  // A key that some rows see and others do not may hold infinities or NaN, which a product with weight 0 would carry over: then
+  // they are taken out of the product and added for the rows that see them.
+  __device__ __forceinline__ void values(const uint4* vb, bool masked) {
+    bool bad = false;
+    if (masked) {
+#pragma unroll
+      for (int i = 0; i < 2 * kLoads; ++i) {
+        const uint4 x = vb[i * 64 + 16 * grp + r];
+        bad |= (special<kF16>(x.x) | special<kF16>(x.y) | special<kF16>(x.z) | special<kF16>(x.w)) != 0;
+      }
+      bad = __builtin_amdgcn_ballot_w64(bad) != 0;
+    }
+    if (!bad) {
+      product<false>(vb);
+      return;
+    }
+    product<true>(vb);
+    const char* const va = reinterpret_cast<const char*>(vb);
+    for (int key = 0; key < kStepKeys; ++key) {
+      const int row = key & 15, e = (key & 3) + 4 * (key >> 4), from = r + 16 * (row >> 2);
+      float w[kT];
+#pragma unroll
+      for (int t = 0; t < kT; ++t) {
+        const uint32_t p0 = pf[t].x, p1 = pf[t].y, p2 = pf[t].z, p3 = pf[t].w;
+        uint32_t two = p0;
+        two = (e >> 1) == 1 ? p1 : two;
+        two = (e >> 1) == 2 ? p2 : two;
+        two = (e >> 1) == 3 ? p3 : two;
+        w[t] = __shfl(widen<kF16>((two >> (16 * (e & 1))) & 0xffffu), from, 64);
+      }
+#pragma unroll
+      for (int i = 0; i < kJ; ++i) {
+        const int c = (key >> 4) * kHalf + row * kChunks + ((4 * (i >> 1) + grp) ^ swizzle_v(row));
+        const uint2 x = *reinterpret_cast<const uint2*>(va + c * 16 + 8 * (i & 1));
+        const uint32_t sx = special<kF16>(x.x), sy = special<kF16>(x.y);
+#pragma unroll
+        for (int t = 0; t < kT; ++t) {
+          if (!((vis[t] >> key) & 1)) continue;
+          if (sx & 0xffffu) acc[t][i][0] += w[t] * widen<kF16>(x.x & 0xffffu);
+          if (sx >> 16) acc[t][i][1] += w[t] * widen<kF16>(x.x >> 16);
+          if (sy & 0xffffu) acc[t][i][2] += w[t] * widen<kF16>(x.y & 0xffffu);
+          if (sy >> 16) acc[t][i][3] += w[t] * widen<kF16>(x.y >> 16);
+        }
+      }
+    }
+  }
+};
+
+// A workgroup's four waves are kRW row groups (16 kT query rows each) times kKW = 4 / kRW key groups: a stage is 32 keys for each
+// key group.
+//   kRW = 1: every wave has all rows and every fourth step in an LDS ring of two of its own. No barrier on the way: K is
+//     refilled, two steps ahead, once its fragments have been read, V once its have.
+//   kRW = 2, 4: the waves of a key group share its keys; kStages stages in LDS, one barrier a stage, loads kStages - 1 stages
+//     ahead.
+template <bool kF16, int kD, int kT, int kRW>
+__global__ __launch_bounds__(kTreeThreads) __attribute__((amdgpu_waves_per_eu(kRW == 1 ? 1 : 2))) void tree_attention_kernel(
+    TreeParams p) {
+  typedef TreeWave<kF16, kD, kT> Wave;
+  constexpr int kKW = kTreeWaves / kRW, kGroupRows = 16 * kT, kRows = kGroupRows * kRW;
+  constexpr int kHalf = Wave::kHalf, kLoads = Wave::kLoads, kJ = Wave::kJ;
+  constexpr int kStages = kRW == 4 ? 4 : 2;
+  constexpr int kStage = kKW * 4 * kHalf;  // chunks: for each key group K of 32 keys, then V
+  // separate objects, so that the compiler can tell a load into one from a read of another
+  __shared__ uint4 st0[kRW == 1 ? 8 * kHalf : kStage];   // kRW = 1: K of the rings' first places
+  __shared__ uint4 st1[kRW == 1 ? 8 * kHalf : kStage];   // their V
+  __shared__ uint4 st2[kRW == 1 ? 8 * kHalf : kStages > 2 ? kStage : 1];
+  __shared__ uint4 st3[kRW == 1 ? 8 * kHalf : kStages > 3 ? kStage : 1];
+  __shared__ float stat_m[kTreeWaves][kGroupRows], stat_l[kTreeWaves][kGroupRows];
   const aspire_tree_attention_args& a = p.a;
   const int lane = threadIdx.x & 63, wave = wave_uniform(threadIdx.x >> 6);
-  const int r = lane & 15, grp = lane >> 4, G = p.group, hkv = a.num_kv_heads;
+  const int rw = wave % kRW, kw = wave / kRW;
+  const int G = p.group, hkv = a.num_kv_heads;
   const int g = wave_uniform(int(blockIdx.x) % hkv), j = wave_uniform(int(blockIdx.x) / hkv);
 
   // this group's part [line0, line1) of the line, and the row that holds its first step
   int64_t all = 0;
-  for (int b = lane; b < a.rows; b += 64) {
-    int tiles, steps;
-    all += cost<kRows>(p, b, tiles, steps);
-  }
+  for (int b = lane; b < a.rows; b += 64) all += cost<kRows>(p, b);
   all = wave_uniform64(wave_sum_i64(all));
-  const int groups = int(min(max(all / kMinPart, int64_t(1)), int64_t(p.groups)));  // each has kMinPart steps at least
+  const int groups = wave_uniform(int(min(max(all / kMinPart, int64_t(1)), int64_t(p.groups))));  // each has kMinPart steps at least
   const int64_t line0 = all * j / groups, line1 = all * (j + 1) / groups;
   if (threadIdx.x == 0) p.pieces[blockIdx.x].w = 0;
   if (j >= groups || all == 0) return;
   int64_t at = 0;  // where row b begins
   int b = 0;
   for (int b0 = 0; b0 < a.rows; b0 += 64) {
-    int tiles, steps;
-    const int64_t c = b0 + lane < a.rows ? cost<kRows>(p, b0 + lane, tiles, steps) : 0;
+    const int64_t c = b0 + lane < a.rows ? cost<kRows>(p, b0 + lane) : 0;
     int64_t end = c;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
@@ -180,38 +384,28 @@ __global__ __launch_bounds__(kTreeThreads) void tree_stream_kernel(TreeParams p)
   at = wave_uniform64(at);
 
   const int row_bytes = int(a.cache_stride_t) * 2;
-  const uint32_t num_entries = p.num_entries, num_pages = p.num_pages;
   const char* const cache = static_cast<const char*>(a.kv_cache) + int64_t(g) * a.cache_stride_h * 2;
-  int voff_k[kLoads / 2], voff_v[kLoads / 2];  // this lane's chunks of 16 keys: the one that belongs at its place in LDS
-  const auto swizzle_k = [](int row) { return kD == 128 ? row : row >> 1; };
-  const auto swizzle_v = [](int row) { return kD == 128 ? ((row & 3) << 2) | (row >> 2) : ((row >> 1) & 1) << 2; };
+  const uint32_t num_entries = p.num_entries, num_pages = p.num_pages;
+  int voff_k[kLoads], voff_v[kLoads];  // this lane's chunks of 16 keys: the one that belongs at its place in LDS
 #pragma unroll
-  for (int i = 0; i < kLoads / 2; ++i) {
-    const int row = kPerLoad * i + lane / kChunks, c = lane % kChunks;
-    voff_k[i] = row * row_bytes + (c ^ swizzle_k(row)) * 16;
-    voff_v[i] = row * row_bytes + (c ^ swizzle_v(row)) * 16;
+  for (int i = 0; i < kLoads; ++i) {
+    const int row = Wave::kPerLoad * i + lane / Wave::kChunks, c = lane % Wave::kChunks;
+    voff_k[i] = row * row_bytes + (c ^ Wave::swizzle_k(row)) * 16;
+    voff_v[i] = row * row_bytes + (c ^ Wave::swizzle_v(row)) * 16;
   }
-  int kidx[kC], vidx[(kJ + 1) / 2];
-  const int vt_row = 4 * grp + (r >> 2);
-#pragma unroll
-  for (int c = 0; c < kC; ++c) kidx[c] = r * kChunks + ((4 * c + grp) ^ swizzle_k(r));
-#pragma unroll
-  for (int c = 0; c < (kJ + 1) / 2; ++c) vidx[c] = vt_row * kChunks + ((4 * c + (r & 3)) ^ swizzle_v(vt_row));
-  uint4* const mk[2] = {k0 + wave * 2 * kHalf, k1 + wave * 2 * kHalf};
-  uint4* const mv[2] = {v0 + wave * 2 * kHalf, v1 + wave * 2 * kHalf};
+  Wave w;
+  w.init(lane, p.scale_log2);
 
-  for (; b < a.rows; ++b) {
+  for (; b < a.rows && at < line1; ++b) {
     const Request rq = request(p, b);
     const int q0 = wave_uniform(rq.q0), n = wave_uniform(rq.n), len = wave_uniform(rq.len);
     const int list = wave_uniform(rq.first), pages = wave_uniform(rq.pages);
     const int total_rows = n * G, tiles = (total_rows + kRows - 1) / kRows, steps = (len + kStepKeys - 1) / kStepKeys;
-    if (at >= line1) break;
-    const int unit = steps + kStartCost;
+    const int unit = steps + kStartCost, tree_start = len - n;
     // the first tile that reaches into this group's part
     int m = wave_uniform(at >= line0 ? 0 : int((line0 - at) / unit));
     typedef const __attribute__((address_space(4))) int32_t* const_ids_t;
     const const_ids_t ids = (const_ids_t)a.kv_indices;
-    const int tree_start = len - n;
     for (; m < tiles; ++m) {
       const int64_t unit0 = at + int64_t(m) * unit;
       if (unit0 >= line1) break;
@@ -220,29 +414,11 @@ __global__ __launch_bounds__(kTreeThreads) void tree_stream_kernel(TreeParams p)
       const bool starts = line0 <= unit0;  // a unit without keys is written where it starts
       if (begin >= end && !(steps == 0 && starts)) continue;
       const bool whole = begin == 0 && end == steps;
-      const int row0 = m * kRows, rows = min(kRows, total_rows - row0);
+      const int row0 = m * kRows + rw * kGroupRows, last = total_rows - 1;  // this wave's rows
+      w.start(p, q0, row0, last, g);
 
-      uint4 qf[kT][kC];
-      const int64_t* words[kT];
-#pragma unroll
-      for (int t = 0; t < kT; ++t) {
-        const int row = min(t * 16 + r, rows - 1) + row0, node = row / G, head = g * G + row - node * G;
-        const uint16_t* const src = static_cast<const uint16_t*>(a.q) + int64_t(q0 + node) * a.q_stride_t + int64_t(head) * a.q_stride_h;
-#pragma unroll
-        for (int c = 0; c < kC; ++c) qf[t][c] = *reinterpret_cast<const uint4*>(src + 32 * c + 8 * grp);
-        words[t] = a.masks + int64_t(q0 + node) * a.mask_stride;
-      }
-      float mx[kT], use[kT], l[kT];
-      f32x4 acc[kT][kJ];
-#pragma unroll
-      for (int t = 0; t < kT; ++t) {
-        mx[t] = kNegInfT, use[t] = 0.f, l[t] = 0.f;
-#pragma unroll
-        for (int i = 0; i < kJ; ++i) acc[t][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-      }
-
-      // Loads of one half (16 keys) of a step's K or V; half-steps on a page that the pool does not have, or past the end, load
-      // nothing: out-of-range loads write zeros into LDS, and every step issues the same loads.
+      // The page of 16 keys: half h of a step. Halves on a page that the pool does not have, or past the end, load nothing:
+      // out-of-range loads write zeros into LDS, and every step issues the same loads.
       const auto page_of = [&](int step, int h) -> int {
         const int e = (2 * step + h) >> p.page_shift;
         const uint32_t entry = uint32_t(list) + uint32_t(e);  // 32-bit compares: there are no scalar 64-bit ones
@@ -250,276 +426,203 @@ __global__ __launch_bounds__(kTreeThreads) void tree_stream_kernel(TreeParams p)
         const int id = ids[there ? entry : 0u];
         return there && uint32_t(id) < num_pages ? id : -1;
       };
-      const auto issue = [&](uint4* buf, int step, int id0, int id1, bool v) {
+      const auto issue = [&](uint4* dst, int step, int h, int id, bool v) {
+        const int sub = (2 * step + h) & ((1 << p.page_shift) - 1);
+        const int valid = id < 0 ? 0 : min(max(len - (2 * step + h) * 16, 0), 16);
+        const int span = wave_uniform(valid > 0 ? (valid - 1) * row_bytes + 2 * kD : 0);
+        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<char*>(tree_uniform(cache + (int64_t(max(id, 0)) * a.cache_stride_p + (v ? a.cache_stride_kv : 0)) * 2 +
+                                           int64_t(sub) * 16 * row_bytes)), (short)0, span, kTreeBuffer);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int id = h ? id1 : id0, sub = (2 * step + h) & ((1 << p.page_shift) - 1);
-          const int valid = id < 0 ? 0 : min(max(len - (2 * step + h) * 16, 0), 16);
-          const int span = wave_uniform(valid > 0 ? (valid - 1) * row_bytes + 2 * kD : 0);
-          const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
-              const_cast<char*>(tree_uniform(cache + (int64_t(max(id, 0)) * a.cache_stride_p + (v ? a.cache_stride_kv : 0)) * 2 +
-                                             int64_t(sub) * 16 * row_bytes)), (short)0, span, kTreeBuffer);
-#pragma unroll
-          for (int i = 0; i < kLoads / 2; ++i)
-            load_to_lds(rs, buf + h * kHalf + i * 64, v ? voff_v[i] : voff_k[i]);
-        }
+        for (int i = 0; i < kLoads; ++i) load_to_lds(rs, dst + i * 64, v ? voff_v[i] : voff_k[i]);
       };
-      uint4 pf[kT];
-      uint32_t vis[kT];
-      const auto scores = [&](const uint4* kb, f32x4 (&s)[kT][2]) {
+      const auto masked_step = [&](int step, int id0, int id1) {
+        const bool masked = (step + 1) * kStepKeys > tree_start || (id0 | id1) < 0;
+        if (masked) w.see(step * kStepKeys - tree_start, len - step * kStepKeys, id0 >= 0, id1 >= 0, a.mask_words);
+        return masked;
+      };
+
+      if constexpr (kRW == 1) {
+        // this wave's steps: begin + wave, and every fourth from there; step s + 8 goes into the ring's place of step s
+        const int first = begin + wave;
+        if (first < end) {
+          uint4* const mk[2] = {st0 + wave * 2 * kHalf, st2 + wave * 2 * kHalf};
+          uint4* const mv[2] = {st1 + wave * 2 * kHalf, st3 + wave * 2 * kHalf};
+          int id[2][2];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint4 kr[kC];
+          for (int u = 0; u < 2; ++u) {
+            const int s = first + u * kTreeWaves;
 #pragma unroll
-          for (int c = 0; c < kC; ++c) kr[c] = kb[h * kHalf + kidx[c]];
+            for (int h = 0; h < 2; ++h) issue(mk[u] + h * kHalf, s, h, id[u][h] = page_of(s, h), false);
 #pragma unroll
-          for (int t = 0; t < kT; ++t) {
-            s[t][h] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int c = 0; c < kC; ++c) s[t][h] = mfma32<kF16>(kr[c], qf[t][c], s[t][h]);
+            for (int h = 0; h < 2; ++h) issue(mv[u] + h * kHalf, s, h, id[u][h], true);
           }
-        }
-      };
-      // bits of the step's 32 keys that each row sees
-      const auto see = [&](int step, int id0, int id1) {
-        const int off = step * kStepKeys - tree_start;  // of the step's first key among the row's tokens
-        const int there = len - step * kStepKeys;
-        uint32_t limit = there >= 32 ? ~0u : (1u << max(there, 0)) - 1;
-        if (id0 < 0) limit &= 0xffff0000u;
-        if (id1 < 0) limit &= 0xffffu;
-#pragma unroll
-        for (int t = 0; t < kT; ++t) {
-          uint32_t bits = ~0u;
-          if (off > -32) {
-            const int w = max(off, 0) >> 6, sh = max(off, 0) & 63;
-            uint64_t x = w < a.mask_words ? uint64_t(words[t][w]) >> sh : 0;
-            if (sh > 32 && w + 1 < a.mask_words) x |= uint64_t(words[t][w + 1]) << (64 - sh);
-            bits = off < 0 ? (uint32_t(x) << -off) | ((1u << -off) - 1) : uint32_t(x);
-          }
-          vis[t] = bits & limit;
-        }
-      };
-      const auto softmax = [&](f32x4 (&s)[kT][2], bool masked, bool first) {
-        float x[kT][8], pv[kT][8], ps[kT];
-#pragma unroll
-        for (int t = 0; t < kT; ++t) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) x[t][i] = s[t][0][i], x[t][4 + i] = s[t][1][i];
-          if (masked) {
-            const uint32_t bits = vis[t] >> (4 * grp);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              x[t][i] = (bits >> i) & 1 ? x[t][i] : kNegInfT;
-              x[t][4 + i] = (bits >> (16 + i)) & 1 ? x[t][4 + i] : kNegInfT;
+          int next0 = page_of(first + 2 * kTreeWaves, 0), next1 = page_of(first + 2 * kTreeWaves, 1);
+          constexpr int kAhead = 6 * kLoads;  // loads behind this step's K, and again behind its V
+          constexpr int kWait = 0xf70 | (kAhead & 15) | ((kAhead >> 4) << 14);
+          const auto body = [&](int s, uint4* kb, uint4* vb, int& id0, int& id1) {
+            bool masked = false;
+            __builtin_amdgcn_s_waitcnt(kWait);  // vmcnt: K has landed
+            asm volatile("" ::: "memory");
+            if (s < end) {
+              masked = masked_step(s, id0, id1);
+              w.scores(kb);
             }
+            const int far = s + 2 * kTreeWaves, n0 = next0, n1 = next1;
+            next0 = page_of(far + kTreeWaves, 0), next1 = page_of(far + kTreeWaves, 1);
+            issue(kb, far, 0, n0, false), issue(kb + kHalf, far, 1, n1, false);
+            if (s < end) w.softmax(masked);
+            __builtin_amdgcn_s_waitcnt(kWait);  // vmcnt: V has landed
+            asm volatile("" ::: "memory");
+            if (s < end) w.values(vb, masked);
+            issue(vb, far, 0, n0, true), issue(vb + kHalf, far, 1, n1, true);
+            id0 = n0, id1 = n1;
+          };
+          for (int s = first; s < end; s += 2 * kTreeWaves) {
+            body(s, mk[0], mv[0], id[0][0], id[0][1]);
+            body(s + kTreeWaves, mk[1], mv[1], id[1][0], id[1][1]);
           }
         }
-        const auto exponentials = [&]() {
-#pragma unroll
-          for (int t = 0; t < kT; ++t) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) pv[t][i] = __builtin_amdgcn_exp2f(fmaf(x[t][i], p.scale_log2, -use[t]));
-            ps[t] = ((pv[t][0] + pv[t][1]) + (pv[t][2] + pv[t][3])) + ((pv[t][4] + pv[t][5]) + (pv[t][6] + pv[t][7]));
+      } else {
+        // Stage t holds the steps begin + kKW t + (0 .. kKW - 1). A wave loads one kind: K or V of a key group (kKW = 2), or
+        // half of it (kKW = 1); it computes on its key group's.
+        const int lkw = kKW == 2 ? wave >> 1 : 0, lh = wave >> 1, kind = wave & 1;
+        constexpr int kMine = (kKW == 2 ? 2 : 1) * kLoads;  // its loads of a stage
+        constexpr int kAhead = (kStages - 2) * kMine;       // loads behind the next stage's
+        constexpr int kWait = 0x70 | (kAhead & 15) | ((kAhead >> 4) << 14);  // vmcnt, and lgkmcnt(0): its reads of the last stage
+        const int stages = (end - begin + kKW - 1) / kKW;
+        uint4* const buf[4] = {st0, st1, st2, st3};
+        const auto load = [&](uint4* stage, int t, int i0, int i1) {
+          const int s = begin + t * kKW + lkw;
+          uint4* const dst = stage + lkw * 4 * kHalf + kind * 2 * kHalf;
+          if (kKW == 2) {
+            issue(dst, s, 0, i0, kind), issue(dst + kHalf, s, 1, i1, kind);
+          } else {
+            issue(dst + lh * kHalf, s, lh, lh ? i1 : i0, kind);
           }
         };
-        exponentials();
-        // a row that has seen no key yet has no offset to go by: a masked step may be its first
-        bool over = first || masked;
+        const auto id_of = [&](int t, int key_group, int h) { return page_of(begin + t * kKW + key_group, h); };
 #pragma unroll
-        for (int t = 0; t < kT; ++t) over |= ps[t] > kSumLimit || mx[t] == kNegInfT;
-        if (__builtin_amdgcn_ballot_w64(over) != 0) {
-#pragma unroll
-          for (int t = 0; t < kT; ++t) {
-            float top = fmaxf(fmaxf(fmaxf(x[t][0], x[t][1]), fmaxf(x[t][2], x[t][3])),
-                              fmaxf(fmaxf(x[t][4], x[t][5]), fmaxf(x[t][6], x[t][7])));
-            top = max_xor32(max_xor16(top)) * p.scale_log2;
-            const float m_new = top > mx[t] + kSlack ? top : mx[t];
-            // a row without a key before has zero sums: they stay zero
-            const float alpha = __builtin_amdgcn_exp2f(mx[t] - (m_new == kNegInfT ? 0.f : m_new));
-            mx[t] = m_new;
-            use[t] = m_new == kNegInfT ? 0.f : m_new - kBias;
-#pragma unroll
-            for (int i = 0; i < kJ; ++i) acc[t][i] *= alpha;
-            l[t] *= alpha;
+        for (int t = 0; t < kStages - 1; ++t) load(buf[t], t, id_of(t, lkw, 0), id_of(t, lkw, 1));
+        int load0 = id_of(kStages - 1, lkw, 0), load1 = id_of(kStages - 1, lkw, 1);
+        int mine0 = id_of(0, kw, 0), mine1 = id_of(0, kw, 1);
+        const bool has_rows = row0 <= last;
+        const auto body = [&](int t, uint4* cur, uint4* fill) {
+          __builtin_amdgcn_s_waitcnt(kWait);
+          asm volatile("" ::: "memory");
+          __builtin_amdgcn_s_barrier();
+          asm volatile("" ::: "memory");
+          load(fill, t + kStages - 1, load0, load1);
+          const int s = begin + t * kKW + kw, id0 = mine0, id1 = mine1;
+          load0 = id_of(t + kStages, lkw, 0), load1 = id_of(t + kStages, lkw, 1);
+          mine0 = id_of(t + 1, kw, 0), mine1 = id_of(t + 1, kw, 1);
+          if (s < end && has_rows) {
+            const uint4* const kb = cur + kw * 4 * kHalf;
+            const bool masked = masked_step(s, id0, id1);
+            w.scores(kb);
+            w.softmax(masked);
+            w.values(kb + 2 * kHalf, masked);
           }
-          exponentials();
+        };
+        for (int t = 0; t < stages; t += kStages) {
+#pragma unroll
+          for (int u = 0; u < kStages; ++u) body(t + u, buf[u], buf[(u + kStages - 1) % kStages]);
         }
+      }
+
+      // the key groups join: each takes its share of the head's values from all
+#pragma unroll
+      for (int t = 0; t < kT; ++t) {
+        w.l[t] = add_xor32(add_xor16(w.l[t]));
+        if (kKW > 1 && w.grp == 0) stat_m[wave][t * 16 + w.r] = w.mx[t], stat_l[wave][t * 16 + w.r] = w.l[t];
+      }
+      constexpr int kShare = kJ / kKW;  // 16-value tiles a wave writes
+      f32x4 o[kT][kShare];
+      float lse[kT];
+      if constexpr (kKW > 1) {
+        __builtin_amdgcn_s_waitcnt(0xf70);  // vmcnt(0): the loads past the end have written their zeros
+        __syncthreads();
+        uint4* const places[4] = {st0, st1, st2, st3};
 #pragma unroll
         for (int t = 0; t < kT; ++t) {
-          pf[t] = make_uint4(pack2<kF16>(pv[t][0], pv[t][1]), pack2<kF16>(pv[t][2], pv[t][3]), pack2<kF16>(pv[t][4], pv[t][5]),
-                             pack2<kF16>(pv[t][6], pv[t][7]));
-          l[t] += ps[t];
-        }
-      };
-      const auto values = [&](const uint4* vb, bool masked) {
-        // A key that some rows see and others do not may hold infinities or NaN, which a product with weight 0 would carry over:
-        // they are taken out of the product and added for the rows that see them.
-        bool bad = false;
-        if (masked) {
+          float top = kNegInfT, sum = 0.f;
 #pragma unroll
-          for (int i = 0; i < 2 * kHalf / 64; ++i) {
-            const uint4 x = vb[i * 64 + lane];
-            bad |= (special<kF16>(x.x) | special<kF16>(x.y) | special<kF16>(x.z) | special<kF16>(x.w)) != 0;
-          }
-          bad = __builtin_amdgcn_ballot_w64(bad) != 0;
-        }
-        const char* const va = reinterpret_cast<const char*>(vb);
-        const auto product = [&](auto clean) {
+          for (int k = 0; k < kKW; ++k) top = fmaxf(top, stat_m[k * kRW + rw][t * 16 + w.r]);
+          const float zero = top == kNegInfT ? 0.f : top;
+#pragma unroll
+          for (int k = 0; k < kKW; ++k)
+            sum += stat_l[k * kRW + rw][t * 16 + w.r] * __builtin_amdgcn_exp2f(stat_m[k * kRW + rw][t * 16 + w.r] - zero);
+          const float scale = __builtin_amdgcn_exp2f(w.mx[t] - zero);
+          w.l[t] = sum;
+          w.use[t] = zero - Wave::kBias;
 #pragma unroll
           for (int i = 0; i < kJ; ++i) {
-            const int off = vidx[i >> 1] * 16 + 8 * (i & 1);
-            uint2 wa = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(va + off)));
-            uint2 wb = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                                     (__attribute__((address_space(3))) i16x4*)(va + kHalf * 16 + off)));
-            if (decltype(clean)::value) {
-              wa.x &= ~special<kF16>(wa.x), wa.y &= ~special<kF16>(wa.y);
-              wb.x &= ~special<kF16>(wb.x), wb.y &= ~special<kF16>(wb.y);
-            }
-#pragma unroll
-            for (int t = 0; t < kT; ++t) acc[t][i] = mfma32<kF16>(make_uint4(wa.x, wa.y, wb.x, wb.y), pf[t], acc[t][i]);
-          }
-        };
-        if (!bad) {
-          product(std::false_type{});
-        } else {
-          product(std::true_type{});
-          for (int key = 0; key < kStepKeys; ++key) {
-            const int row = key & 15, e = (key & 3) + 4 * (key >> 4), from = r + 16 * (row >> 2);
-            float w[kT];
-#pragma unroll
-            for (int t = 0; t < kT; ++t) {
-              const uint32_t p0 = pf[t].x, p1 = pf[t].y, p2 = pf[t].z, p3 = pf[t].w;
-              uint32_t two = p0;
-              two = (e >> 1) == 1 ? p1 : two;
-              two = (e >> 1) == 2 ? p2 : two;
-              two = (e >> 1) == 3 ? p3 : two;
-              w[t] = __shfl(widen<kF16>((two >> (16 * (e & 1))) & 0xffffu), from, 64);
-            }
-#pragma unroll
-            for (int i = 0; i < kJ; ++i) {
-              const int c = (key >> 4) * kHalf + row * kChunks + ((4 * (i >> 1) + grp) ^ swizzle_v(row));
-              const uint2 x = *reinterpret_cast<const uint2*>(va + c * 16 + 8 * (i & 1));
-              const uint32_t sx = special<kF16>(x.x), sy = special<kF16>(x.y);
-#pragma unroll
-              for (int t = 0; t < kT; ++t) {
-                if (!((vis[t] >> key) & 1)) continue;
-                if (sx & 0xffffu) acc[t][i][0] += w[t] * widen<kF16>(x.x & 0xffffu);
-                if (sx >> 16) acc[t][i][1] += w[t] * widen<kF16>(x.x >> 16);
-                if (sy & 0xffffu) acc[t][i][2] += w[t] * widen<kF16>(x.y & 0xffffu);
-                if (sy >> 16) acc[t][i][3] += w[t] * widen<kF16>(x.y >> 16);
-              }
-            }
+            const f32x4 x = w.acc[t][i] * scale;
+            places[i / kShare][((wave * kT + t) * kShare + i % kShare) * 64 + lane] = __builtin_bit_cast(uint4, x);
           }
         }
-      };
-
-      // this wave's steps: begin + wave, and every fourth from there; step s + 8 goes into the ring's place of step s
-      const int first = begin + wave;
-      if (first < end) {
-        int id[2][2];
+        __syncthreads();
+        const uint4* const mine = kw == 0 ? st0 : kw == 1 ? st1 : kw == 2 ? st2 : st3;
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int s = first + u * kTreeWaves;
-          id[u][0] = page_of(s, 0), id[u][1] = page_of(s, 1);
-          issue(mk[u], s, id[u][0], id[u][1], false);
-          issue(mv[u], s, id[u][0], id[u][1], true);
+        for (int t = 0; t < kT; ++t) {
+#pragma unroll
+          for (int i = 0; i < kShare; ++i) {
+            o[t][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int k = 0; k < kKW; ++k)
+              o[t][i] += __builtin_bit_cast(f32x4, mine[(((k * kRW + rw) * kT + t) * kShare + i) * 64 + lane]);
+          }
         }
-        int next0 = page_of(first + 2 * kTreeWaves, 0), next1 = page_of(first + 2 * kTreeWaves, 1);
-        const auto body = [&](int s, uint4* kb, uint4* vb, int& id0, int& id1) {
-          const bool masked = (s + 1) * kStepKeys > tree_start || (id0 | id1) < 0;
-          if (masked) see(s, id0, id1);
-          f32x4 sc[kT][2];
-          __builtin_amdgcn_s_waitcnt(0xf70 | ((3 * kLoads) & 15) | (((3 * kLoads) >> 4) << 14));  // vmcnt: this step's K
-          asm volatile("" ::: "memory");
-          scores(kb, sc);
-          const int far = s + 2 * kTreeWaves, n0 = next0, n1 = next1;
-          next0 = page_of(far + kTreeWaves, 0), next1 = page_of(far + kTreeWaves, 1);
-          issue(kb, far, n0, n1, false);
-          softmax(sc, masked, s == first);
-          __builtin_amdgcn_s_waitcnt(0xf70 | ((3 * kLoads) & 15) | (((3 * kLoads) >> 4) << 14));  // vmcnt: its V
-          asm volatile("" ::: "memory");
-          values(vb, masked);
-          issue(vb, far, n0, n1, true);
-          id0 = n0, id1 = n1;
-        };
-        for (int s = first;;) {  // no way back to the top but past both bodies: waits are counted by the order of the loads
-          body(s, mk[0], mv[0], id[0][0], id[0][1]);
-          if ((s += kTreeWaves) >= end) break;
-          body(s, mk[1], mv[1], id[1][0], id[1][1]);
-          if ((s += kTreeWaves) >= end) break;
-        }
+      } else {
+#pragma unroll
+        for (int t = 0; t < kT; ++t)
+#pragma unroll
+          for (int i = 0; i < kShare; ++i) o[t][i] = w.acc[t][i];
       }
-
-      // the waves join: each takes its share of the head's values from all
-#pragma unroll
-      for (int t = 0; t < kT; ++t) {
-        l[t] = add_xor32(add_xor16(l[t]));
-        if (grp == 0) stat_m[wave][t * 16 + r] = mx[t], stat_l[wave][t * 16 + r] = l[t];
-      }
-      __builtin_amdgcn_s_waitcnt(0xf70);  // vmcnt(0): the loads past the end have written their zeros
-      __syncthreads();
-      constexpr int kShare = kJ / kTreeWaves;  // 16-value tiles a wave writes
-      uint4* const places[4] = {k0, v0, k1, v1};
-      float inv[kT], lse[kT];
-#pragma unroll
-      for (int t = 0; t < kT; ++t) {
-        float top = kNegInfT, sum = 0.f;
-#pragma unroll
-        for (int w = 0; w < kTreeWaves; ++w) top = fmaxf(top, stat_m[w][t * 16 + r]);
-        const float zero = top == kNegInfT ? 0.f : top;
-#pragma unroll
-        for (int w = 0; w < kTreeWaves; ++w) sum += stat_l[w][t * 16 + r] * __builtin_amdgcn_exp2f(stat_m[w][t * 16 + r] - zero);
-        const float scale = __builtin_amdgcn_exp2f(mx[t] - zero);
-        inv[t] = sum == 0.f ? 0.f : 1.f / sum;
-        lse[t] = sum == 0.f ? kNegInfT : zero - kBias + __builtin_log2f(sum);
-#pragma unroll
-        for (int i = 0; i < kJ; ++i) {
-          const f32x4 x = acc[t][i] * scale;
-          places[i / kShare][((wave * kT + t) * kShare + i % kShare) * 64 + lane] = __builtin_bit_cast(uint4, x);
-        }
-      }
-      __syncthreads();
-      const uint4* const mine = wave == 0 ? k0 : wave == 1 ? v0 : wave == 2 ? k1 : v1;
       const int slot = 2 * blockIdx.x + (begin == 0 ? 1 : 0);
 #pragma unroll
       for (int t = 0; t < kT; ++t) {
-        const int row = t * 16 + r;
-        f32x4 o[kShare];
+        const float inv = w.l[t] == 0.f ? 0.f : 1.f / w.l[t];
+        lse[t] = w.l[t] == 0.f ? kNegInfT : w.use[t] + __builtin_log2f(w.l[t]);
 #pragma unroll
-        for (int i = 0; i < kShare; ++i) {
-          o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int w = 0; w < kTreeWaves; ++w) o[i] += __builtin_bit_cast(f32x4, mine[((w * kT + t) * kShare + i) * 64 + lane]);
-          o[i] *= inv[t];
-        }
-        if (row >= rows) continue;
-        // value of o[i][e]: 16-value tile wave * kShare + i holds 32 (tile / 2) + 8 grp + 4 (tile % 2) + e
-        const int d = kShare == 2 ? 32 * wave + 8 * grp : 32 * (wave >> 1) + 8 * grp + 4 * (wave & 1);
+        for (int i = 0; i < kShare; ++i) o[t][i] *= inv;
+        const int row = row0 + t * 16 + w.r;
+        if (row > last) continue;
+        // value e of 16-value tile i: 32 (i / 2) + 8 grp + 4 (i % 2) + e
+        const int tile0 = kw * kShare;
         if (whole) {
-          const int node = (row0 + row) / G, head = g * G + row0 + row - node * G;
-          uint16_t* const dst = static_cast<uint16_t*>(a.out) + int64_t(q0 + node) * a.out_stride_t + int64_t(head) * a.out_stride_h + d;
-          uint32_t packed[2 * kShare];
+          const int node = row / G, head = g * G + row - node * G;
+          uint16_t* const dst = static_cast<uint16_t*>(a.out) + int64_t(q0 + node) * a.out_stride_t + int64_t(head) * a.out_stride_h;
+          if constexpr (kShare > 1) {
 #pragma unroll
-          for (int i = 0; i < kShare; ++i) packed[2 * i] = pack2<kF16>(o[i][0], o[i][1]), packed[2 * i + 1] = pack2<kF16>(o[i][2], o[i][3]);
-          if (kShare == 2) *reinterpret_cast<uint4*>(dst) = make_uint4(packed[0], packed[1], packed[2 * kShare - 2], packed[2 * kShare - 1]);
-          else *reinterpret_cast<uint2*>(dst) = make_uint2(packed[0], packed[1]);
-          if (a.lse != nullptr && wave == 0 && grp == 0) a.lse[int64_t(q0 + node) * a.num_qo_heads + head] = lse[t];
+            for (int i = 0; i < kShare; i += 2)
+              *reinterpret_cast<uint4*>(dst + 16 * (tile0 + i) + 8 * w.grp) =
+                  make_uint4(pack2<kF16>(o[t][i][0], o[t][i][1]), pack2<kF16>(o[t][i][2], o[t][i][3]),
+                             pack2<kF16>(o[t][i + 1][0], o[t][i + 1][1]), pack2<kF16>(o[t][i + 1][2], o[t][i + 1][3]));
+          } else {
+            *reinterpret_cast<uint2*>(dst + 32 * (tile0 >> 1) + 8 * w.grp + 4 * (tile0 & 1)) =
+                make_uint2(pack2<kF16>(o[t][0][0], o[t][0][1]), pack2<kF16>(o[t][0][2], o[t][0][3]));
+          }
+          if (a.lse != nullptr && kw == 0 && w.grp == 0) a.lse[int64_t(q0 + node) * a.num_qo_heads + head] = lse[t];
         } else {
-          float* const dst = p.part_o + (int64_t(slot) * kRows + row) * kD + d;
+          const int64_t at_row = int64_t(slot) * kRows + row - m * kRows;
+          float* const dst = p.part_o + at_row * kD;
 #pragma unroll
-          for (int i = 0; i < kShare; ++i) *reinterpret_cast<f32x4*>(dst + 4 * i) = o[i];
-          if (wave == 0 && grp == 0) p.part_lse[int64_t(slot) * kRows + row] = lse[t];
+          for (int i = 0; i < kShare; ++i)
+            *reinterpret_cast<f32x4*>(dst + 32 * ((tile0 + i) >> 1) + 8 * w.grp + 4 * ((tile0 + i) & 1)) = o[t][i];
+          if (kw == 0 && w.grp == 0) p.part_lse[at_row] = lse[t];
         }
       }
       if (begin == 0 && end < steps && threadIdx.x == 0) {
         // the groups that hold the unit's other steps: the last one's part holds its last step
-        const int64_t last = unit0 + unit - 1;
-        int jl = int(last * groups / all);
-        while (all * (jl + 1) / groups <= last) ++jl;
-        while (all * jl / groups > last) --jl;
-        p.pieces[blockIdx.x] = make_int4(row0, rows | (g << 16), q0, jl - j + 1);
+        const int64_t last_step = unit0 + unit - 1;
+        int jl = int(last_step * groups / all);
+        while (all * (jl + 1) / groups <= last_step) ++jl;
+        while (all * jl / groups > last_step) --jl;
+        p.pieces[blockIdx.x] = make_int4(m * kRows, min(kRows, total_rows - m * kRows) | (g << 16), q0, jl - j + 1);
       }
-      __syncthreads();  // the ring is free again
+      if (kKW == 1) __builtin_amdgcn_s_waitcnt(0xf70);  // vmcnt(0): no load past the end meets the next unit's
+      __syncthreads();  // the stages are free again
     }
     at += int64_t(tiles) * unit;
   }
@@ -572,24 +675,27 @@ __global__ __launch_bounds__(256) void tree_join_kernel(TreeParams p, int tile_r
   if (a.lse != nullptr && d == 0) a.lse[int64_t(token) * a.num_qo_heads + head] = sum == 0.f ? kNegInfT : top + __builtin_log2f(sum);
 }
 
-// What a launch is made of: 16-row tiles a wave, groups a kv head.
+// What a launch is made of: 16-row tiles a wave, row groups of a workgroup, workgroups a kv head.
 struct TreeChoice {
-  int tiles, groups;
+  int tiles, row_groups, groups;
+  int rows() const { return 16 * tiles * row_groups; }
 };
 TreeChoice choose(int tokens, int rows, int hq, int hkv) {
   // the smallest tile that holds a mean request's query rows
   const int64_t mean = (int64_t(tokens) + rows - 1) / rows * (hq / hkv);
-  const int tiles = mean <= 16 ? 1 : mean <= 32 ? 2 : 4;
-  return {tiles, std::max(1, kTreeGroups / hkv)};
+  TreeChoice c{mean <= 16 ? 1 : 2, mean <= 32 ? 1 : mean <= 64 ? 2 : 4, 0};
+  c.groups = std::max(1, (c.row_groups == 1 ? 1 : 2) * kTreeGroups / hkv);
+  return c;
 }
 template <bool kF16, int kD>
 void launch(const TreeParams& p, TreeChoice c, hipStream_t s) {
-  const int wgs = c.groups * p.a.num_kv_heads, tile_rows = 16 * c.tiles;
-  if (c.tiles == 1) tree_stream_kernel<kF16, kD, 1><<<wgs, kTreeThreads, 0, s>>>(p);
-  else if (c.tiles == 2) tree_stream_kernel<kF16, kD, 2><<<wgs, kTreeThreads, 0, s>>>(p);
-  else tree_stream_kernel<kF16, kD, 4><<<wgs, kTreeThreads, 0, s>>>(p);
+  const int wgs = c.groups * p.a.num_kv_heads;
+  if (c.tiles == 1) tree_attention_kernel<kF16, kD, 1, 1><<<wgs, kTreeThreads, 0, s>>>(p);
+  else if (c.row_groups == 1) tree_attention_kernel<kF16, kD, 2, 1><<<wgs, kTreeThreads, 0, s>>>(p);
+  else if (c.row_groups == 2) tree_attention_kernel<kF16, kD, 2, 2><<<wgs, kTreeThreads, 0, s>>>(p);
+  else tree_attention_kernel<kF16, kD, 2, 4><<<wgs, kTreeThreads, 0, s>>>(p);
   constexpr int kJoinRows = 256 / (kD / 8);
-  tree_join_kernel<kF16, kD><<<dim3(wgs, (tile_rows + kJoinRows - 1) / kJoinRows), 256, 0, s>>>(p, tile_rows);
+  tree_join_kernel<kF16, kD><<<dim3(wgs, (c.rows() + kJoinRows - 1) / kJoinRows), 256, 0, s>>>(p, c.rows());
 }
 int64_t piece_bytes(int64_t workgroups) { return (workgroups * int64_t(sizeof(int4)) + 255) / 256 * 256; }
 
@@ -604,7 +710,7 @@ extern "C" int64_t aspire_tree_attention_workspace(int32_t tokens, int32_t rows,
     return 0;
   const TreeChoice c = choose(tokens, rows, num_qo_heads, num_kv_heads);
   const int64_t wgs = int64_t(c.groups) * num_kv_heads;
-  return piece_bytes(wgs) / 4 + 2 * wgs * 16 * c.tiles * (head_dim + 1);
+  return piece_bytes(wgs) / 4 + 2 * wgs * c.rows() * (head_dim + 1);
 }
 
 extern "C" int aspire_tree_attention(const aspire_tree_attention_args* a, void* stream) {
@@ -631,7 +737,7 @@ extern "C" int aspire_tree_attention(const aspire_tree_attention_args* a, void* 
                        aligned(a->kv_cache, {a->cache_stride_p, a->cache_stride_kv, a->cache_stride_t, a->cache_stride_h}),
                    "heads must start on 16 bytes");
   const TreeChoice c = choose(a->tokens, a->rows, a->num_qo_heads, a->num_kv_heads);
-  const int wgs = c.groups * a->num_kv_heads, tile_rows = 16 * c.tiles;
+  const int wgs = c.groups * a->num_kv_heads, tile_rows = c.rows();
   ASPIRE_CHECK_ARG(a->workspace && a->workspace_floats >= aspire_tree_attention_workspace(a->tokens, a->rows, a->num_qo_heads, a->num_kv_heads, a->head_dim),
                    "workspace too small");
   ASPIRE_CHECK_ARG((reinterpret_cast<uintptr_t>(a->workspace) & 15) == 0, "workspace must start on 16 bytes");
