@@ -31,10 +31,8 @@ namespace {
 constexpr float kNegInfT = -__builtin_huge_valf();
 constexpr float kSlack = 8.f;       // log2 units
 constexpr int kStepKeys = 32;
-constexpr int kTreeWaves = 4;
-constexpr int kTreeThreads = 64 * kTreeWaves;
 constexpr int kStartCost = 4;       // a piece's start and end, in steps
-constexpr int kMinPart = 2;         // the least that a group takes, in steps
+constexpr int kMinPart = 4;         // the least that a group takes, in steps
 constexpr int kTreeGroups = 256;    // workgroups of a launch: one a CU
 constexpr uint32_t kTreeBuffer = 0x00020000u;  // gfx9 raw buffer dword 3
 
@@ -47,7 +45,7 @@ struct TreeParams {
   int32_t groups;      // workgroups per kv head
   int32_t page_shift;  // log2(page_size / 16)
   uint32_t num_entries, num_pages;  // of the list and the pool, below 2^31
-  // of workgroup w: pieces[w] = (tile's first row among n * G, row count | kv head << 16, first token, number of pieces of the
+  // of workgroup w: pieces[w] = (tile's first row among n * G, row count, first token, number of pieces of the
   // unit that starts in it and ends in a later one, or 0); its partial rows: slot 2 w of a unit that began
   // before it, 2 w + 1 of one that goes on after it
   int4* pieces;
@@ -91,8 +89,16 @@ __device__ __forceinline__ int64_t wave_uniform64(int64_t v) {
   return int64_t((uint64_t(uint32_t(__builtin_amdgcn_readfirstlane(int(v >> 32)))) << 32) | uint32_t(__builtin_amdgcn_readfirstlane(int(v))));
 }
 
-// 16 bytes a lane from its offset into the buffer to the lane's place behind dst.
-__device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t rs, uint4* dst, int offset) {
+// 16 bytes a lane from its offset into the buffer to the lane's place behind dst; once: keys that no other workgroup reads
+// (non-temporal: 32 x 32,768 tokens 735 -> 658 us, but 164 -> 222 where seven tiles share them).
+template <bool kOnce>
+__device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t rs, uint4* dst, int offset);
+template <>
+__device__ __forceinline__ void load_to_lds<true>(__amdgpu_buffer_rsrc_t rs, uint4* dst, int offset) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)dst, 16, offset, 0, 0, 2);
+}
+template <>
+__device__ __forceinline__ void load_to_lds<false>(__amdgpu_buffer_rsrc_t rs, uint4* dst, int offset) {
   __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)dst, 16, offset, 0, 0, 0);
 }
 
@@ -327,26 +333,28 @@ struct TreeWave {
   }
 };
 
-// A workgroup's four waves are kRW row groups (16 kT query rows each) times kKW = 4 / kRW key groups: a stage is 32 keys for each
-// key group.
+// A workgroup's four waves (eight for kRW = 8) are kRW row groups (16 kT query rows each) times kKW key groups: a stage is 32 keys for
+// each key group.
 //   kRW = 1: every wave has all rows and every fourth step in an LDS ring of two of its own. No barrier on the way: K is
 //     refilled, two steps ahead, once its fragments have been read, V once its have.
-//   kRW = 2, 4: the waves of a key group share its keys; kStages stages in LDS, one barrier a stage, loads kStages - 1 stages
+//   kRW = 2, 4, 8: the waves of a key group share its keys; kStages stages in LDS, one barrier a stage, loads kStages - 1 stages
 //     ahead.
-template <bool kF16, int kD, int kT, int kRW>
-__global__ __launch_bounds__(kTreeThreads) __attribute__((amdgpu_waves_per_eu(kRW == 1 ? 1 : 2))) void tree_attention_kernel(
+constexpr int tree_waves(int row_groups) { return row_groups == 8 ? 8 : 4; }
+
+template <bool kF16, int kD, int kT, int kRW, bool kOnce>
+__global__ __launch_bounds__(64 * tree_waves(kRW)) __attribute__((amdgpu_waves_per_eu(kRW == 1 ? 1 : 2))) void tree_attention_kernel(
     TreeParams p) {
   typedef TreeWave<kF16, kD, kT> Wave;
-  constexpr int kKW = kTreeWaves / kRW, kGroupRows = 16 * kT, kRows = kGroupRows * kRW;
+  constexpr int kWaves = tree_waves(kRW), kKW = kWaves / kRW, kGroupRows = 16 * kT, kRows = kGroupRows * kRW;
   constexpr int kHalf = Wave::kHalf, kLoads = Wave::kLoads, kJ = Wave::kJ;
-  constexpr int kStages = kRW == 4 ? 4 : 2;
+  constexpr int kStages = kKW == 1 ? 4 : 2;
   constexpr int kStage = kKW * 4 * kHalf;  // chunks: for each key group K of 32 keys, then V
   // separate objects, so that the compiler can tell a load into one from a read of another
   __shared__ uint4 st0[kRW == 1 ? 8 * kHalf : kStage];   // kRW = 1: K of the rings' first places
   __shared__ uint4 st1[kRW == 1 ? 8 * kHalf : kStage];   // their V
   __shared__ uint4 st2[kRW == 1 ? 8 * kHalf : kStages > 2 ? kStage : 1];
   __shared__ uint4 st3[kRW == 1 ? 8 * kHalf : kStages > 3 ? kStage : 1];
-  __shared__ float stat_m[kTreeWaves][kGroupRows], stat_l[kTreeWaves][kGroupRows];
+  __shared__ float stat_m[kKW == 1 ? 1 : kWaves][kGroupRows], stat_l[kKW == 1 ? 1 : kWaves][kGroupRows];
   const aspire_tree_attention_args& a = p.a;
   const int lane = threadIdx.x & 63, wave = wave_uniform(threadIdx.x >> 6);
   const int rw = wave % kRW, kw = wave / kRW;
@@ -386,10 +394,13 @@ __global__ __launch_bounds__(kTreeThreads) __attribute__((amdgpu_waves_per_eu(kR
   const int row_bytes = int(a.cache_stride_t) * 2;
   const char* const cache = static_cast<const char*>(a.kv_cache) + int64_t(g) * a.cache_stride_h * 2;
   const uint32_t num_entries = p.num_entries, num_pages = p.num_pages;
-  int voff_k[kLoads], voff_v[kLoads];  // this lane's chunks of 16 keys: the one that belongs at its place in LDS
+  // This lane's chunks of 16 keys: the ones that belong at its places in LDS. Of eight waves each loads half of them.
+  constexpr int kPart = kWaves == 8 ? kLoads / 2 : kLoads;
+  const int part0 = kWaves == 8 ? (wave >> 2) * kPart : 0;
+  int voff_k[kPart], voff_v[kPart];
 #pragma unroll
-  for (int i = 0; i < kLoads; ++i) {
-    const int row = Wave::kPerLoad * i + lane / Wave::kChunks, c = lane % Wave::kChunks;
+  for (int i = 0; i < kPart; ++i) {
+    const int row = Wave::kPerLoad * (part0 + i) + lane / Wave::kChunks, c = lane % Wave::kChunks;
     voff_k[i] = row * row_bytes + (c ^ Wave::swizzle_k(row)) * 16;
     voff_v[i] = row * row_bytes + (c ^ Wave::swizzle_v(row)) * 16;
   }
@@ -417,14 +428,17 @@ __global__ __launch_bounds__(kTreeThreads) __attribute__((amdgpu_waves_per_eu(kR
       const int row0 = m * kRows + rw * kGroupRows, last = total_rows - 1;  // this wave's rows
       w.start(p, q0, row0, last, g);
 
-      // The page of 16 keys: half h of a step. Halves on a page that the pool does not have, or past the end, load nothing:
-      // out-of-range loads write zeros into LDS, and every step issues the same loads.
-      const auto page_of = [&](int step, int h) -> int {
-        const int e = (2 * step + h) >> p.page_shift;
-        const uint32_t entry = uint32_t(list) + uint32_t(e);  // 32-bit compares: there are no scalar 64-bit ones
-        const bool there = step < end && e < pages && entry < num_entries;
-        const int id = ids[there ? entry : 0u];
-        return there && uint32_t(id) < num_pages ? id : -1;
+      // The page of 16 keys: half h of a step. raw() only loads it (a scalar load, used a step later: to wait for four of them where
+      // they are issued took a third of a step), page() is -1 on a page that the pool does not have, or past the end: such
+      // halves load nothing. Out-of-range loads write zeros into LDS, and every step issues the same loads.
+      const auto raw = [&](int step, int h) -> int {
+        const uint32_t entry = uint32_t(list) + uint32_t((2 * step + h) >> p.page_shift);
+        return ids[min(entry, num_entries - 1)];
+      };
+      const auto page = [&](int step, int h, int id) -> int {
+        const uint32_t e = uint32_t(2 * step + h) >> p.page_shift;  // 32-bit compares: there are no scalar 64-bit ones
+        const bool there = step < end && e < uint32_t(pages) && uint32_t(list) + e < num_entries && uint32_t(id) < num_pages;
+        return there ? id : -1;
       };
       const auto issue = [&](uint4* dst, int step, int h, int id, bool v) {
         const int sub = (2 * step + h) & ((1 << p.page_shift) - 1);
@@ -434,11 +448,11 @@ __global__ __launch_bounds__(kTreeThreads) __attribute__((amdgpu_waves_per_eu(kR
             const_cast<char*>(tree_uniform(cache + (int64_t(max(id, 0)) * a.cache_stride_p + (v ? a.cache_stride_kv : 0)) * 2 +
                                            int64_t(sub) * 16 * row_bytes)), (short)0, span, kTreeBuffer);
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) load_to_lds(rs, dst + i * 64, v ? voff_v[i] : voff_k[i]);
+        for (int i = 0; i < kPart; ++i) load_to_lds<kOnce>(rs, dst + (part0 + i) * 64, v ? voff_v[i] : voff_k[i]);
       };
-      const auto masked_step = [&](int step, int id0, int id1) {
-        const bool masked = (step + 1) * kStepKeys > tree_start || (id0 | id1) < 0;
-        if (masked) w.see(step * kStepKeys - tree_start, len - step * kStepKeys, id0 >= 0, id1 >= 0, a.mask_words);
+      const auto masked_step = [&](int step, bool page0, bool page1) {
+        const bool masked = (step + 1) * kStepKeys > tree_start || !page0 || !page1;
+        if (masked) w.see(step * kStepKeys - tree_start, len - step * kStepKeys, page0, page1, a.mask_words);
         return masked;
       };
 
@@ -451,13 +465,13 @@ __global__ __launch_bounds__(kTreeThreads) __attribute__((amdgpu_waves_per_eu(kR
           int id[2][2];
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
-            const int s = first + u * kTreeWaves;
+            const int s = first + u * kWaves;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) issue(mk[u] + h * kHalf, s, h, id[u][h] = page_of(s, h), false);
+            for (int h = 0; h < 2; ++h) issue(mk[u] + h * kHalf, s, h, id[u][h] = page(s, h, raw(s, h)), false);
 #pragma unroll
             for (int h = 0; h < 2; ++h) issue(mv[u] + h * kHalf, s, h, id[u][h], true);
           }
-          int next0 = page_of(first + 2 * kTreeWaves, 0), next1 = page_of(first + 2 * kTreeWaves, 1);
+          int next0 = raw(first + 2 * kWaves, 0), next1 = raw(first + 2 * kWaves, 1);
           constexpr int kAhead = 6 * kLoads;  // loads behind this step's K, and again behind its V
           constexpr int kWait = 0xf70 | (kAhead & 15) | ((kAhead >> 4) << 14);
           const auto body = [&](int s, uint4* kb, uint4* vb, int& id0, int& id1) {
@@ -465,11 +479,11 @@ __global__ __launch_bounds__(kTreeThreads) __attribute__((amdgpu_waves_per_eu(kR
             __builtin_amdgcn_s_waitcnt(kWait);  // vmcnt: K has landed
             asm volatile("" ::: "memory");
             if (s < end) {
-              masked = masked_step(s, id0, id1);
+              masked = masked_step(s, id0 >= 0, id1 >= 0);
               w.scores(kb);
             }
-            const int far = s + 2 * kTreeWaves, n0 = next0, n1 = next1;
-            next0 = page_of(far + kTreeWaves, 0), next1 = page_of(far + kTreeWaves, 1);
+            const int far = s + 2 * kWaves, n0 = page(far, 0, next0), n1 = page(far, 1, next1);
+            next0 = raw(far + kWaves, 0), next1 = raw(far + kWaves, 1);
             issue(kb, far, 0, n0, false), issue(kb + kHalf, far, 1, n1, false);
             if (s < end) w.softmax(masked);
             __builtin_amdgcn_s_waitcnt(kWait);  // vmcnt: V has landed
@@ -478,47 +492,48 @@ __global__ __launch_bounds__(kTreeThreads) __attribute__((amdgpu_waves_per_eu(kR
             issue(vb, far, 0, n0, true), issue(vb + kHalf, far, 1, n1, true);
             id0 = n0, id1 = n1;
           };
-          for (int s = first; s < end; s += 2 * kTreeWaves) {
+          for (int s = first; s < end; s += 2 * kWaves) {
             body(s, mk[0], mv[0], id[0][0], id[0][1]);
-            body(s + kTreeWaves, mk[1], mv[1], id[1][0], id[1][1]);
+            body(s + kWaves, mk[1], mv[1], id[1][0], id[1][1]);
           }
         }
       } else {
-        // Stage t holds the steps begin + kKW t + (0 .. kKW - 1). A wave loads one kind: K or V of a key group (kKW = 2), or
-        // half of it (kKW = 1); it computes on its key group's.
-        const int lkw = kKW == 2 ? wave >> 1 : 0, lh = wave >> 1, kind = wave & 1;
-        constexpr int kMine = (kKW == 2 ? 2 : 1) * kLoads;  // its loads of a stage
+        // Stage t holds the steps begin + kKW t + (0 .. kKW - 1). A wave loads one kind of its key group's: K or V (kKW = 2), or a
+        // half or a quarter of them (kKW = 1).
+        const int lh = (wave >> 1) & 1, kind = wave & 1;
+        constexpr int kMine = kKW == 2 ? 2 * kLoads : 4 * kLoads / kWaves;  // its loads of a stage
         constexpr int kAhead = (kStages - 2) * kMine;       // loads behind the next stage's
         constexpr int kWait = 0x70 | (kAhead & 15) | ((kAhead >> 4) << 14);  // vmcnt, and lgkmcnt(0): its reads of the last stage
         const int stages = (end - begin + kKW - 1) / kKW;
         uint4* const buf[4] = {st0, st1, st2, st3};
-        const auto load = [&](uint4* stage, int t, int i0, int i1) {
-          const int s = begin + t * kKW + lkw;
-          uint4* const dst = stage + lkw * 4 * kHalf + kind * 2 * kHalf;
+        const auto step_of = [&](int t) { return begin + t * kKW + kw; };
+        uint32_t there = 0;  // two bits a stage: whether its halves have pages, the last one that was loaded lowest
+        const auto load = [&](uint4* stage, int t, int raw0, int raw1) {
+          const int s = step_of(t), id0 = page(s, 0, raw0), id1 = page(s, 1, raw1);
+          there = (there << 2) | (id0 >= 0 ? 1u : 0u) | (id1 >= 0 ? 2u : 0u);
+          uint4* const dst = stage + kw * 4 * kHalf + kind * 2 * kHalf;
           if (kKW == 2) {
-            issue(dst, s, 0, i0, kind), issue(dst + kHalf, s, 1, i1, kind);
+            issue(dst, s, 0, id0, kind), issue(dst + kHalf, s, 1, id1, kind);
           } else {
-            issue(dst + lh * kHalf, s, lh, lh ? i1 : i0, kind);
+            issue(dst + lh * kHalf, s, lh, lh ? id1 : id0, kind);
           }
         };
-        const auto id_of = [&](int t, int key_group, int h) { return page_of(begin + t * kKW + key_group, h); };
 #pragma unroll
-        for (int t = 0; t < kStages - 1; ++t) load(buf[t], t, id_of(t, lkw, 0), id_of(t, lkw, 1));
-        int load0 = id_of(kStages - 1, lkw, 0), load1 = id_of(kStages - 1, lkw, 1);
-        int mine0 = id_of(0, kw, 0), mine1 = id_of(0, kw, 1);
+        for (int t = 0; t < kStages - 1; ++t) load(buf[t], t, raw(step_of(t), 0), raw(step_of(t), 1));
+        int next0 = raw(step_of(kStages - 1), 0), next1 = raw(step_of(kStages - 1), 1);
         const bool has_rows = row0 <= last;
         const auto body = [&](int t, uint4* cur, uint4* fill) {
           __builtin_amdgcn_s_waitcnt(kWait);
           asm volatile("" ::: "memory");
           __builtin_amdgcn_s_barrier();
           asm volatile("" ::: "memory");
-          load(fill, t + kStages - 1, load0, load1);
-          const int s = begin + t * kKW + kw, id0 = mine0, id1 = mine1;
-          load0 = id_of(t + kStages, lkw, 0), load1 = id_of(t + kStages, lkw, 1);
-          mine0 = id_of(t + 1, kw, 0), mine1 = id_of(t + 1, kw, 1);
+          load(fill, t + kStages - 1, next0, next1);
+          next0 = raw(step_of(t + kStages), 0), next1 = raw(step_of(t + kStages), 1);
+          const int s = step_of(t);
           if (s < end && has_rows) {
             const uint4* const kb = cur + kw * 4 * kHalf;
-            const bool masked = masked_step(s, id0, id1);
+            const uint32_t mine = there >> (2 * (kStages - 1));
+            const bool masked = masked_step(s, mine & 1, mine & 2);
             w.scores(kb);
             w.softmax(masked);
             w.values(kb + 2 * kHalf, masked);
@@ -619,7 +634,7 @@ __global__ __launch_bounds__(kTreeThreads) __attribute__((amdgpu_waves_per_eu(kR
         int jl = int(last_step * groups / all);
         while (all * (jl + 1) / groups <= last_step) ++jl;
         while (all * jl / groups > last_step) --jl;
-        p.pieces[blockIdx.x] = make_int4(m * kRows, min(kRows, total_rows - m * kRows) | (g << 16), q0, jl - j + 1);
+        p.pieces[blockIdx.x] = make_int4(m * kRows, min(kRows, total_rows - m * kRows), q0, jl - j + 1);
       }
       if (kKW == 1) __builtin_amdgcn_s_waitcnt(0xf70);  // vmcnt(0): no load past the end meets the next unit's
       __syncthreads();  // the stages are free again
@@ -628,74 +643,107 @@ __global__ __launch_bounds__(kTreeThreads) __attribute__((amdgpu_waves_per_eu(kR
   }
 }
 
-// Units cut into pieces: out = sum_i 2^(lse_i - m) o_i / sum_i 2^(lse_i - m), rounded once, pieces in the order of their keys. A
-// workgroup takes 256 / (kD / 8) rows of the unit that starts in workgroup blockIdx.x of the launch before.
-template <bool kF16, int kD>
+// Units cut into pieces: out = sum_i 2^(lse_i - m) o_i / sum_i 2^(lse_i - m), rounded once, in the order of the keys. Workgroup
+// (w, y) has rows of the unit that starts in workgroup w of the launch before and ends in another; a wave takes kTake rows, one after another in flight together; 64 / (kD / 8) pieces of a row at a time, kRound times.
+template <bool kF16, int kD, int kTake>
 __global__ __launch_bounds__(256) void tree_join_kernel(TreeParams p, int tile_rows) {
-  constexpr int kLanes = kD / 8, kRound = 4;
+  constexpr int kLanes = kD / 8, kAtOnce = 64 / kLanes, kRound = 2;
   const aspire_tree_attention_args& a = p.a;
+  const int hkv = a.num_kv_heads, g = blockIdx.x % hkv;
+  const int lane = threadIdx.x & 63, d = (lane % kLanes) * 8, part = lane / kLanes;
+  const int row0 = (blockIdx.y * 4 + wave_uniform(threadIdx.x >> 6)) * kTake;
   const int4 u = p.pieces[blockIdx.x];
-  const int row = blockIdx.y * (256 / kLanes) + threadIdx.x / kLanes, d = (threadIdx.x % kLanes) * 8;
-  if (u.w == 0 || row >= (u.y & 0xffff)) return;
-  const int w = blockIdx.x, hkv = a.num_kv_heads;
-  const auto slot = [&](int i) { return (int64_t(2) * (w + i * hkv) + (i == 0 ? 1 : 0)) * tile_rows + row; };
-  float top = kNegInfT, sum = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  for (int k = 0; k < u.w; k += kRound) {
-    float lse[kRound];
-    float4 x[kRound], y[kRound];
+  const int rows = wave_uniform(u.y), splits = wave_uniform(u.w);
+  if (splits == 0 || row0 >= rows) return;
+  float top[kTake], sum[kTake], o[kTake][8];
 #pragma unroll
-    for (int i = 0; i < kRound; ++i) {
-      const int64_t s = slot(min(k + i, u.w - 1));
-      lse[i] = k + i < u.w ? p.part_lse[s] : kNegInfT;
-      x[i] = *reinterpret_cast<const float4*>(p.part_o + s * kD + d);
-      y[i] = *reinterpret_cast<const float4*>(p.part_o + s * kD + d + 4);
-    }
-    float next = top;
+  for (int t = 0; t < kTake; ++t) {
+    top[t] = kNegInfT, sum[t] = 0.f;
 #pragma unroll
-    for (int i = 0; i < kRound; ++i) next = fmaxf(next, lse[i]);
-    const float zero = next == kNegInfT ? 0.f : next, keep = __builtin_amdgcn_exp2f(top - zero);
-    sum *= keep;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) o[e] *= keep;
-#pragma unroll
-    for (int i = 0; i < kRound; ++i) {
-      if (k + i >= u.w) break;
-      const float f = __builtin_amdgcn_exp2f(lse[i] - zero);
-      sum += f;
-      o[0] += f * x[i].x, o[1] += f * x[i].y, o[2] += f * x[i].z, o[3] += f * x[i].w;
-      o[4] += f * y[i].x, o[5] += f * y[i].y, o[6] += f * y[i].z, o[7] += f * y[i].w;
-    }
-    top = next;
+    for (int e = 0; e < 8; ++e) o[t][e] = 0.f;
   }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  const int at = u.x + row, node = at / p.group, token = u.z + node, head = (u.y >> 16) * p.group + at - node * p.group;
-  *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + int64_t(token) * a.out_stride_t + int64_t(head) * a.out_stride_h + d) =
-      make_uint4(pack2<kF16>(o[0] * inv, o[1] * inv), pack2<kF16>(o[2] * inv, o[3] * inv), pack2<kF16>(o[4] * inv, o[5] * inv),
-                 pack2<kF16>(o[6] * inv, o[7] * inv));
-  if (a.lse != nullptr && d == 0) a.lse[int64_t(token) * a.num_qo_heads + head] = sum == 0.f ? kNegInfT : top + __builtin_log2f(sum);
+  for (int k = 0; k < splits; k += kAtOnce * kRound) {
+    float lse[kTake][kRound];
+    float4 x[kTake][kRound], y[kTake][kRound];
+#pragma unroll
+    for (int t = 0; t < kTake; ++t) {
+#pragma unroll
+      for (int i = 0; i < kRound; ++i) {
+        const int s = k + i * kAtOnce + part;
+        const int64_t slot = 2 * (int64_t(blockIdx.x) + int64_t(min(s, splits - 1)) * hkv) + (min(s, splits - 1) == 0 ? 1 : 0);
+        const int64_t at = slot * tile_rows + min(row0 + t, rows - 1);
+        lse[t][i] = s < splits ? p.part_lse[at] : kNegInfT;
+        x[t][i] = *reinterpret_cast<const float4*>(p.part_o + at * kD + d);
+        y[t][i] = *reinterpret_cast<const float4*>(p.part_o + at * kD + d + 4);
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < kTake; ++t) {
+      float next = top[t];
+#pragma unroll
+      for (int i = 0; i < kRound; ++i) next = fmaxf(next, lse[t][i]);
+      const float zero = next == kNegInfT ? 0.f : next, keep = __builtin_amdgcn_exp2f(top[t] - zero);
+      sum[t] *= keep;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[t][e] *= keep;
+#pragma unroll
+      for (int i = 0; i < kRound; ++i) {
+        if (k + i * kAtOnce + part >= splits) continue;
+        const float f = __builtin_amdgcn_exp2f(lse[t][i] - zero);
+        sum[t] += f;
+        o[t][0] += f * x[t][i].x, o[t][1] += f * x[t][i].y, o[t][2] += f * x[t][i].z, o[t][3] += f * x[t][i].w;
+        o[t][4] += f * y[t][i].x, o[t][5] += f * y[t][i].y, o[t][6] += f * y[t][i].z, o[t][7] += f * y[t][i].w;
+      }
+      top[t] = next;
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < kTake; ++t) {
+    // the pieces' lanes, in a fixed order
+#pragma unroll
+    for (int step = kLanes; step < 64; step <<= 1) {
+      const float other = __shfl_xor(top[t], step, 64), next = fmaxf(top[t], other), zero = next == kNegInfT ? 0.f : next;
+      const float f = __builtin_amdgcn_exp2f(top[t] - zero), h = __builtin_amdgcn_exp2f(other - zero);
+      sum[t] = f * sum[t] + h * __shfl_xor(sum[t], step, 64);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[t][e] = f * o[t][e] + h * __shfl_xor(o[t][e], step, 64);
+      top[t] = next;
+    }
+    if (row0 + t >= rows || part != 0) continue;
+    const float inv = sum[t] == 0.f ? 0.f : 1.f / sum[t];
+    const int at = u.x + row0 + t, node = at / p.group, token = u.z + node, head = g * p.group + at - node * p.group;
+    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + int64_t(token) * a.out_stride_t + int64_t(head) * a.out_stride_h + d) =
+        make_uint4(pack2<kF16>(o[t][0] * inv, o[t][1] * inv), pack2<kF16>(o[t][2] * inv, o[t][3] * inv),
+                   pack2<kF16>(o[t][4] * inv, o[t][5] * inv), pack2<kF16>(o[t][6] * inv, o[t][7] * inv));
+    if (a.lse != nullptr && d == 0)
+      a.lse[int64_t(token) * a.num_qo_heads + head] = sum[t] == 0.f ? kNegInfT : top[t] + __builtin_log2f(sum[t]);
+  }
 }
 
-// What a launch is made of: 16-row tiles a wave, row groups of a workgroup, workgroups a kv head.
+// What a launch is made of: 16-row tiles a wave, row groups of a workgroup, workgroups a kv head, and whether keys are mostly read by
+// one tile alone.
 struct TreeChoice {
   int tiles, row_groups, groups;
+  bool once;
   int rows() const { return 16 * tiles * row_groups; }
 };
 TreeChoice choose(int tokens, int rows, int hq, int hkv) {
   // the smallest tile that holds a mean request's query rows
   const int64_t mean = (int64_t(tokens) + rows - 1) / rows * (hq / hkv);
-  TreeChoice c{mean <= 16 ? 1 : 2, mean <= 32 ? 1 : mean <= 64 ? 2 : 4, 0};
-  c.groups = std::max(1, (c.row_groups == 1 ? 1 : 2) * kTreeGroups / hkv);
+  TreeChoice c{mean <= 16 ? 1 : 2, mean <= 32 ? 1 : mean <= 64 ? 2 : mean <= 128 ? 4 : 8, 0, mean <= 128};
+  c.groups = std::max(1, (c.row_groups == 1 || c.row_groups == 8 ? 1 : 2) * kTreeGroups / hkv);
   return c;
 }
 template <bool kF16, int kD>
 void launch(const TreeParams& p, TreeChoice c, hipStream_t s) {
   const int wgs = c.groups * p.a.num_kv_heads;
-  if (c.tiles == 1) tree_attention_kernel<kF16, kD, 1, 1><<<wgs, kTreeThreads, 0, s>>>(p);
-  else if (c.row_groups == 1) tree_attention_kernel<kF16, kD, 2, 1><<<wgs, kTreeThreads, 0, s>>>(p);
-  else if (c.row_groups == 2) tree_attention_kernel<kF16, kD, 2, 2><<<wgs, kTreeThreads, 0, s>>>(p);
-  else tree_attention_kernel<kF16, kD, 2, 4><<<wgs, kTreeThreads, 0, s>>>(p);
-  constexpr int kJoinRows = 256 / (kD / 8);
-  tree_join_kernel<kF16, kD><<<dim3(wgs, (c.rows() + kJoinRows - 1) / kJoinRows), 256, 0, s>>>(p, c.rows());
+  if (c.tiles == 1) tree_attention_kernel<kF16, kD, 1, 1, true><<<wgs, 256, 0, s>>>(p);
+  else if (c.row_groups == 1) tree_attention_kernel<kF16, kD, 2, 1, true><<<wgs, 256, 0, s>>>(p);
+  else if (c.row_groups == 2) tree_attention_kernel<kF16, kD, 2, 2, true><<<wgs, 256, 0, s>>>(p);
+  else if (c.row_groups == 4) tree_attention_kernel<kF16, kD, 2, 4, true><<<wgs, 256, 0, s>>>(p);
+  else tree_attention_kernel<kF16, kD, 2, 8, false><<<wgs, 512, 0, s>>>(p);
+  if (c.rows() <= 32) tree_join_kernel<kF16, kD, 1><<<dim3(wgs, c.rows() / 4), 256, 0, s>>>(p, c.rows());
+  else tree_join_kernel<kF16, kD, 4><<<dim3(wgs, c.rows() / 16), 256, 0, s>>>(p, c.rows());
 }
 int64_t piece_bytes(int64_t workgroups) { return (workgroups * int64_t(sizeof(int4)) + 255) / 256 * 256; }
 
