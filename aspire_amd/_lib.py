@@ -351,8 +351,12 @@ def require_cuda(*tensors: torch.Tensor, what: str) -> None:
 def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Whether the bytes from a tensor's first to its last value meet the other's."""
     def extent(t):
-        at = t.data_ptr()
-        return at, at + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size() if t.numel() else at
+        at, last = t.data_ptr(), 1
+        for n, s in zip(t.shape, t.stride()):
+            if n == 0:
+                return at, at
+            last += (n - 1) * s
+        return at, at + last * t.element_size()
 
     (a0, a1), (b0, b1) = extent(a), extent(b)
     return a0 < b1 and b0 < a1

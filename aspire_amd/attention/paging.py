@@ -27,10 +27,14 @@ _RESIZE = struct.Struct("6P4i")          # aspire_page_resize_args
 _TABLES = struct.Struct("PqPPP8i8P")     # aspire_step_tables_args
 
 
-def _counts(t: torch.Tensor, length: int | None, device, what: str, name: str) -> torch.Tensor:
-    """An int32 vector on ``device``, in one piece."""
-    if t.dim() != 1 or t.dtype not in (torch.int32, torch.int64) or t.device != device or (length is not None and t.shape[0] != length):
-        raise ValueError(f"{what}: {name} must be int32 [{'requests' if length is None else length}] on {device}")
+def _counts(t: torch.Tensor, length: int | None, index: int, what: str, name: str) -> torch.Tensor:
+    """An int32 vector on device ``index``, in one piece."""
+    if t.dtype is torch.int32 and t.get_device() == index and t.dim() == 1 and t.is_contiguous() \
+            and (length is None or t.shape[0] == length):
+        return t
+    _lib.require_cuda(t, what=what)
+    if t.dim() != 1 or t.dtype not in (torch.int32, torch.int64) or t.get_device() != index or (length is not None and t.shape[0] != length):
+        raise ValueError(f"{what}: {name} must be int32 [{'requests' if length is None else length}] on cuda:{index}")
     return _lib.dense(t, torch.int32)
 
 
@@ -53,7 +57,7 @@ class PagePool:
         self.free = torch.arange(num_pages - 1, -1, -1, **i32)  # page 0 is taken first
         self.free_count = torch.full((1,), num_pages, **i32)
         self.shortage = torch.zeros(max_requests, **i32)
-        self.device = self.held.device
+        self.device, self._index = self.held.device, self.held.get_device()
 
     def resize(self, lengths: torch.Tensor) -> torch.Tensor:
         """Give request ``b`` the pages of ``lengths[b]`` tokens, ``lengths`` int32 ``[max_requests]``: 0 gives all of its pages
@@ -61,12 +65,13 @@ class PagePool:
         take what they lack in row order. From the first one on that lacks more pages than are left, or more than
         ``max_pages``, none takes any: ``shortage`` (returned) has what each of them lacks, 0 for the others."""
         what = "PagePool.resize"
-        _lib.require_cuda(self.held, lengths, what=what)
-        lengths = _counts(lengths, self.max_requests, self.device, what, "lengths")
+        if self._index < 0:
+            _lib.require_cuda(self.held, what=what)
+        lengths = _counts(lengths, self.max_requests, self._index, what, "lengths")
         args = _RESIZE.pack(self.block_table.data_ptr(), self.held.data_ptr(), self.free.data_ptr(), self.free_count.data_ptr(),
                             self.shortage.data_ptr(), lengths.data_ptr(), self.max_requests, self.max_pages, self.num_pages,
                             self.page_size)
-        _lib.launch(_lib.lib().aspire_page_resize, args, self.held.get_device(), what)
+        _lib.launch(_lib.lib().aspire_page_resize, args, self._index, what)
         return self.shortage
 
 
@@ -92,7 +97,7 @@ class StepTables:
         self.positions, self.slots = torch.full((max_tokens,), -1, **i32), torch.full((max_tokens,), -1, **i64)
         self.masks = torch.zeros(max_tokens, tree_words, **i64) if tree_words else None
         self.totals = torch.zeros(3, **i64)
-        self.device = self.totals.device
+        self.device, self._index = self.totals.device, self.totals.get_device()
         self._outputs = tuple(_lib.ptr(t) or 0 for t in (self.qo_indptr, self.kv_indptr, self.kv_indices, self.last_page_len,
                                                          self.positions, self.slots, self.masks, self.totals))
 
@@ -105,25 +110,28 @@ class StepTables:
         is -1. Rows without new tokens list no pages. From the first row on that does not fit (``max_tokens``,
         ``max_entries``, or more than ``64 * tree_words`` tokens) no row has tokens or pages."""
         what = "StepTables.build"
-        _lib.require_cuda(self.totals, block_table, cached, new_tokens, parents, what=what)
-        cached = _counts(cached, None, self.device, what, "cached")
+        index = self._index
+        if index < 0:
+            _lib.require_cuda(self.totals, what=what)
+        cached = _counts(cached, None, index, what, "cached")
         rows = cached.shape[0]
-        new_tokens = _counts(new_tokens, rows, self.device, what, "new_tokens")
+        new_tokens = _counts(new_tokens, rows, index, what, "new_tokens")
         if rows > self.max_rows:
             raise ValueError(f"{what}: {rows} rows, but the tables hold {self.max_rows}")
         shape, strides = block_table.shape, block_table.stride()
-        if len(shape) != 2 or block_table.dtype != torch.int32 or shape[0] < rows or block_table.device != self.device \
+        if len(shape) != 2 or block_table.dtype is not torch.int32 or shape[0] < rows or block_table.get_device() != index \
                 or (shape[1] > 1 and strides[1] != 1):
+            _lib.require_cuda(block_table, what=what)
             raise ValueError(f"{what}: block_table must be int32 [at least {rows}, pages] on {self.device} with contiguous rows")
         at = 0
         if parents is not None:
-            parents = _counts(parents, None, self.device, what, "parents")
+            parents = _counts(parents, None, index, what, "parents")
             if parents.shape[0] < self.max_tokens:
                 raise ValueError(f"{what}: parents needs {self.max_tokens} entries")
             at = parents.data_ptr()
         args = _TABLES.pack(block_table.data_ptr(), strides[0], cached.data_ptr(), new_tokens.data_ptr(), at, rows, shape[1],
                             self.max_rows, self.max_tokens, self.max_entries, self.page_size, self.tree_words, 0, *self._outputs)
-        _lib.launch(_lib.lib().aspire_step_tables, args, self.totals.get_device(), what)
+        _lib.launch(_lib.lib().aspire_step_tables, args, index, what)
         return self
 
 

@@ -14,7 +14,6 @@ All three read lengths on the device and can be captured.
 from __future__ import annotations
 
 import ctypes
-import math
 import struct
 
 import torch
@@ -25,18 +24,42 @@ from aspire_amd import _lib
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1}
 HEAD_DIMS = (64, 128)
 _ARGS = struct.Struct("PqqPqqqqqqPPPPPqPqqP8ifiPq")  # aspire_tree_attention_args
-_MOVE = struct.Struct("PqqqqqPPPP8i")                # aspire_compact_args
+_MOVE = struct.Struct("PPqqqqqqPPPP8i")              # aspire_compact_args
 
 
-def _list(t: torch.Tensor, device, what: str, name: str) -> torch.Tensor:
-    if t.dim() != 1 or t.dtype not in (torch.int32, torch.int64) or t.device != device:
-        raise ValueError(f"{what}: {name} must be 1-D int32 on {device}")
+def _list(t: torch.Tensor, index: int, what: str, name: str) -> torch.Tensor:
+    """An index array as int32 in one piece."""
+    if t.dtype is torch.int32 and t.get_device() == index and t.dim() == 1 and t.is_contiguous():
+        return t
+    if t.dim() != 1 or t.dtype not in (torch.int32, torch.int64) or t.get_device() != index:
+        raise ValueError(f"{what}: {name} must be 1-D int32 on cuda:{index}")
     return _lib.dense(t, torch.int32)
 
 
-def _rows16(t: torch.Tensor) -> bool:
-    """Whether every row of the last dimension (of a 16-bit type) starts on 16 bytes and is in one piece."""
-    return t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % 8 == 0 or n <= 1 for n, s in zip(t.shape[:-1], t.stride()))
+def _rows16(t: torch.Tensor):
+    """The strides of a 16-bit tensor if every row of its last dimension is in one piece that starts on 16 bytes (0 for
+    dimensions of one), else None."""
+    st = t.stride()
+    if st[-1] == 1 and t.data_ptr() % 16 == 0:
+        for s in st[:-1]:
+            if s % 8:
+                break
+        else:
+            return st
+    if (st[-1] != 1 and t.shape[-1] > 1) or t.data_ptr() % 16:
+        return None
+    st = tuple(0 if n <= 1 else s for n, s in zip(t.shape, st))
+    return None if any(s % 8 for s in st[:-1]) else st
+
+
+def _bytes(t: torch.Tensor, st) -> tuple[int, int]:
+    """First byte of a tensor of these strides and the one behind its last."""
+    at, last = t.data_ptr(), 1
+    for n, s in zip(t.shape, st):
+        if n == 0:
+            return at, at
+        last += (n - 1) * s
+    return at, at + last * t.element_size()
 
 
 def tree_attention(q: torch.Tensor, kv_cache: torch.Tensor, qo_indptr: torch.Tensor, kv_page_indices: torch.Tensor,
@@ -54,51 +77,56 @@ def tree_attention(q: torch.Tensor, kv_cache: torch.Tensor, qo_indptr: torch.Ten
     hold. Tokens of no row are left as they were. Sums and softmax are fp32; weights of keys are rounded to q's type for the
     product with v. Not differentiable."""
     what = "tree_attention"
-    _lib.require_cuda(q, kv_cache, what=what)
+    index, dtype, shape, cs = q.get_device(), q.dtype, q.shape, kv_cache.shape
+    if index < 0:
+        _lib.require_cuda(q, what=what)
     if torch.is_grad_enabled() and (q.requires_grad or kv_cache.requires_grad) \
             or forward_ad._current_level >= 0 and _lib.has_tangent(q, kv_cache, out):
         raise ValueError(f"{what}: not differentiable")
-    code, device = _DTYPES.get(q.dtype), q.device
-    shape = q.shape
-    if code is None or len(shape) != 3 or shape[2] not in HEAD_DIMS or not _rows16(q):
+    code = _DTYPES.get(dtype)
+    if code is None or len(shape) != 3 or shape[2] not in HEAD_DIMS or (qs := _rows16(q)) is None:
         raise ValueError(f"{what}: q must be bf16 or fp16 [T, H_q, 64 or 128] with 16-byte aligned heads")
     tokens, hq, dim = shape
-    cs = kv_cache.shape
-    if kv_cache.dtype != q.dtype or kv_cache.device != device or len(cs) != 5 or cs[1] != 2 or cs[2] != page_size \
-            or cs[4] != dim or not _rows16(kv_cache):
-        raise ValueError(f"{what}: kv_cache must be {q.dtype} [P, 2, {page_size}, H_kv, {dim}] on {device} with 16-byte aligned heads")
+    if kv_cache.dtype is not dtype or kv_cache.get_device() != index or len(cs) != 5 or cs[1] != 2 or cs[2] != page_size \
+            or cs[4] != dim or (c := _rows16(kv_cache)) is None:
+        raise ValueError(f"{what}: kv_cache must be {dtype} [P, 2, {page_size}, H_kv, {dim}] on {q.device} with 16-byte aligned heads")
     if cs[3] < 1 or hq % cs[3]:
         raise ValueError(f"{what}: q heads must be a multiple of the kv heads")
-    if tree_masks.dtype != torch.int64 or tree_masks.dim() != 2 or tree_masks.shape[0] < tokens or tree_masks.device != device \
-            or (tree_masks.shape[1] > 1 and tree_masks.stride(1) != 1):
-        raise ValueError(f"{what}: tree_masks must be int64 [T, words] on {device} with contiguous rows")
-    qo, ind = _list(qo_indptr, device, what, "qo_indptr"), _list(kv_page_indices, device, what, "kv_page_indices")
-    ptr, last = _list(kv_page_indptr, device, what, "kv_page_indptr"), _list(kv_last_page_len, device, what, "kv_last_page_len")
+    ms, mst = tree_masks.shape, tree_masks.stride()
+    if tree_masks.dtype is not torch.int64 or len(ms) != 2 or ms[0] < tokens or tree_masks.get_device() != index \
+            or (ms[1] > 1 and mst[1] != 1):
+        raise ValueError(f"{what}: tree_masks must be int64 [T, words] on {q.device} with contiguous rows")
+    qo, ind = _list(qo_indptr, index, what, "qo_indptr"), _list(kv_page_indices, index, what, "kv_page_indices")
+    ptr, last = _list(kv_page_indptr, index, what, "kv_page_indptr"), _list(kv_last_page_len, index, what, "kv_last_page_len")
     rows = last.shape[0]
     if qo.shape[0] <= rows or ptr.shape[0] <= rows:
         raise ValueError(f"{what}: qo_indptr and kv_page_indptr need len(kv_last_page_len) + 1 entries")
     if out is None:
-        out = torch.empty(shape, dtype=q.dtype, device=device)
-    elif out.shape != shape or out.dtype != q.dtype or out.device != device or not _rows16(out):
-        raise ValueError(f"{what}: out must be {q.dtype} of q's shape on {device} with 16-byte aligned heads")
-    elif _lib.overlap(out, q) or _lib.overlap(out, kv_cache):
-        raise ValueError(f"{what}: out must lie apart from q and the cache")
-    if lse is not None and (lse.dtype != torch.float32 or lse.shape != (tokens, hq) or lse.device != device or not lse.is_contiguous()):
-        raise ValueError(f"{what}: lse must be a contiguous fp32 [T, H_q] tensor on {device}")
-    if lse is None and return_lse:
-        lse = torch.empty(tokens, hq, dtype=torch.float32, device=device)
-    scale = 1.0 / math.sqrt(dim) if sm_scale is None else float(sm_scale)
+        out = torch.empty(shape, dtype=dtype, device=q.device)
+        os = out.stride()
+    elif out.shape != shape or out.dtype is not dtype or out.get_device() != index or (os := _rows16(out)) is None:
+        raise ValueError(f"{what}: out must be {dtype} of q's shape on {q.device} with 16-byte aligned heads")
+    else:
+        o0, o1 = _bytes(out, os)
+        for t, st in ((q, qs), (kv_cache, c)):
+            t0, t1 = _bytes(t, st)
+            if o0 < t1 and t0 < o1:
+                raise ValueError(f"{what}: out must lie apart from q and the cache")
+    if lse is not None:
+        if lse.dtype is not torch.float32 or lse.shape != (tokens, hq) or lse.get_device() != index or not lse.is_contiguous():
+            raise ValueError(f"{what}: lse must be a contiguous fp32 [T, H_q] tensor on {q.device}")
+    elif return_lse:
+        lse = torch.empty(tokens, hq, dtype=torch.float32, device=q.device)
     L, ws, at = _lib.lib(), None, 0
     floats = L.aspire_tree_attention_workspace(tokens, rows, hq, cs[3], dim)
     if floats:  # the call's own, from torch's pool: calls on several streams or in several graphs share none
-        ws = torch.empty(floats, dtype=torch.float32, device=device)
+        ws = torch.empty(floats, dtype=torch.float32, device=q.device)
         at = ws.data_ptr()
-    qs, c, os = q.stride(), kv_cache.stride(), out.stride()
     args = _ARGS.pack(q.data_ptr(), qs[0], qs[1], kv_cache.data_ptr(), c[0], c[1], c[2], c[3], cs[0], ind.shape[0], qo.data_ptr(),
-                      ind.data_ptr(), ptr.data_ptr(), last.data_ptr(), tree_masks.data_ptr(), tree_masks.stride(0),
-                      out.data_ptr(), os[0], os[1], _lib.ptr(lse) or 0, tokens, rows, tree_masks.shape[1], hq, cs[3], dim,
-                      page_size, code, scale, 0, at, floats)
-    _lib.launch(L.aspire_tree_attention, args, q.get_device(), what)
+                      ind.data_ptr(), ptr.data_ptr(), last.data_ptr(), tree_masks.data_ptr(), mst[0], out.data_ptr(), os[0], os[1],
+                      0 if lse is None else lse.data_ptr(), tokens, rows, ms[1], hq, cs[3], dim, page_size, code,
+                      dim ** -0.5 if sm_scale is None else float(sm_scale), 0, at, floats)
+    _lib.launch(L.aspire_tree_attention, args, index, what)
     return (out, lse) if return_lse else out
 
 
@@ -111,40 +139,60 @@ def compact_accepted(kv_caches, path: torch.Tensor, kept: torch.Tensor, qo_indpt
     ``verify_tree_speculation`` returns, ``slots`` int64 ``[T]`` what the step's tables hold. A path rises: entries that are not
     above their place, or not of the row, are passed over, and so are slots outside the cache."""
     what = "compact_accepted"
-    if isinstance(kv_caches, torch.Tensor):
-        layers = [kv_caches] if kv_caches.dim() == 5 else list(kv_caches.unbind(0)) if kv_caches.dim() == 6 else None
-    else:
-        layers = list(kv_caches)
-    if layers is None:
-        raise ValueError(f"{what}: kv_caches must be [P, 2, page, H, D], [L, P, 2, page, H, D] or a list of the former")
+    index = path.get_device()
+    if index < 0:
+        _lib.require_cuda(path, what=what)
+    stacked = isinstance(kv_caches, torch.Tensor)
+    layers = [kv_caches] if stacked else list(kv_caches)
     if not layers:
         return
     c = layers[0]
-    _lib.require_cuda(*layers, path, kept, qo_indptr, slots, what=what)
-    device, cs, st = c.device, c.shape, c.stride()
-    if c.dim() != 5 or cs[1] != 2 or (cs[4] > 1 and st[4] != 1) or cs[2] < 1 \
-            or any(t.shape != cs or t.stride() != st or t.dtype != c.dtype or t.device != device for t in layers):
-        raise ValueError(f"{what}: the caches must be [P, 2, page, H, D] of one layout and type with contiguous head dims")
-    if any(t.requires_grad for t in layers) and torch.is_grad_enabled() \
-            or forward_ad._current_level >= 0 and _lib.has_tangent(*layers):
-        raise ValueError(f"{what}: not differentiable")
-    starts = [t.data_ptr() for t in layers]
-    if len(set(starts)) != len(starts) and c.numel():
-        raise ValueError(f"{what}: a cache is listed twice")
-    if path.dim() != 2 or path.dtype != torch.int32 or not path.is_contiguous() or path.device != device:
-        raise ValueError(f"{what}: path must be a contiguous int32 [B, M] tensor on {device}")
-    kept, qo = _list(kept, device, what, "kept"), _list(qo_indptr, device, what, "qo_indptr")
-    rows = path.shape[0]
+    cs, st, es, dtype = c.shape, c.stride(), c.element_size(), c.dtype
+    if len(cs) == 6 and stacked:
+        count, step, cs, st = cs[0], st[0] * es, cs[1:], st[1:]
+        if count > 1 and step < cs[0] * st[0] * es and not _apart(c):
+            raise ValueError(f"{what}: the layers share memory")
+    else:
+        count, step = len(layers), 0
+    if len(cs) != 5 or cs[1] != 2 or (cs[4] > 1 and st[4] != 1) or cs[2] < 1:
+        raise ValueError(f"{what}: the caches must be [P, 2, page, H, D], or stacked as [L, P, 2, page, H, D], with contiguous head dims")
+    table = None
+    for t in layers:
+        if t.get_device() != index:
+            _lib.require_cuda(t, what=what)
+            raise ValueError(f"{what}: a cache is on {t.device}, path on {path.device}")
+        if t.requires_grad and torch.is_grad_enabled() or forward_ad._current_level >= 0 and _lib.has_tangent(t):
+            raise ValueError(f"{what}: not differentiable")
+    if not stacked:
+        if any(t.shape != cs or t.stride() != st or t.dtype is not dtype for t in layers):
+            raise ValueError(f"{what}: the caches must be of one layout and type")
+        starts = [t.data_ptr() for t in layers]
+        if len(set(starts)) != len(starts) and c.numel():
+            raise ValueError(f"{what}: a cache is listed twice")
+        table = (ctypes.c_uint64 * count)(*starts)
+    if path.dim() != 2 or path.dtype is not torch.int32 or not path.is_contiguous():
+        raise ValueError(f"{what}: path must be a contiguous int32 [B, M] tensor")
+    kept, qo = _list(kept, index, what, "kept"), _list(qo_indptr, index, what, "qo_indptr")
+    rows, most = path.shape
     if kept.shape[0] != rows or qo.shape[0] <= rows:
         raise ValueError(f"{what}: kept needs {rows} entries and qo_indptr {rows + 1}")
-    if slots.dim() != 1 or slots.dtype != torch.int64 or slots.device != device:
-        raise ValueError(f"{what}: slots must be int64 [T] on {device}")
-    slots, es = slots.contiguous(), c.element_size()
-    table = (ctypes.c_uint64 * len(starts))(*starts)
-    args = _MOVE.pack(ctypes.addressof(table), st[0] * es, st[1] * es, st[2] * es, st[3] * es, cs[0], path.data_ptr(),
-                      kept.data_ptr(), qo.data_ptr(), slots.data_ptr(), len(starts), cs[3], cs[4] * es, cs[2], rows,
-                      slots.shape[0], path.shape[1], 0)
-    _lib.launch(_lib.lib().aspire_compact_accepted, args, c.get_device(), what)
+    if slots.dim() != 1 or slots.dtype is not torch.int64 or slots.get_device() != index:
+        raise ValueError(f"{what}: slots must be int64 [T] on {path.device}")
+    slots = slots.contiguous()
+    args = _MOVE.pack(0 if table is None else ctypes.addressof(table), c.data_ptr(), step, st[0] * es, st[1] * es, st[2] * es, st[3] * es,
+                      cs[0], path.data_ptr(), kept.data_ptr(), qo.data_ptr(), slots.data_ptr(), count, cs[3], cs[4] * es, cs[2], rows,
+                      slots.shape[0], most, 0)
+    _lib.launch(_lib.lib().aspire_compact_accepted, args, index, what)
+
+
+def _apart(t: torch.Tensor) -> bool:
+    """Whether no two elements of a tensor share memory, by its dimensions in the order of their strides."""
+    reach = 0
+    for s, n in sorted((s, n) for n, s in zip(t.shape, t.stride()) if n > 1):
+        if s <= reach:
+            return False
+        reach += (n - 1) * s
+    return True
 
 
 __all__ = ["HEAD_DIMS", "tree_attention", "compact_accepted"]

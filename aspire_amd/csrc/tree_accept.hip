@@ -146,13 +146,16 @@ extern "C" int aspire_compact_accepted(const aspire_compact_args* a, void* strea
   if (a->layers == 0 || a->heads == 0 || a->head_bytes == 0 || a->rows == 0 || a->max_path < 2 || a->tokens == 0 || a->num_pages == 0)
     return ASPIRE_OK;
   ASPIRE_CHECK_ARG(int64_t(a->heads) * a->head_bytes <= (1 << 28), "more than 2^28 bytes a token");
-  ASPIRE_CHECK_ARG(a->caches && a->path && a->kept && a->qo_indptr && a->slots, "null array");
+  ASPIRE_CHECK_ARG((a->caches || a->first_cache) && a->path && a->kept && a->qo_indptr && a->slots, "null array");
   // the widest vectors that every row starts and ends on
   uint64_t bits = static_cast<uint64_t>(a->head_bytes);
   for (int64_t s : {a->stride_p, a->stride_kv, a->stride_t, a->stride_h}) bits |= static_cast<uint64_t>(s);
+  const auto address = [&](int l) {
+    return a->caches ? a->caches[l] : reinterpret_cast<uintptr_t>(a->first_cache) + uint64_t(l) * static_cast<uint64_t>(a->stride_l);
+  };
   for (int l = 0; l < a->layers; ++l) {
-    ASPIRE_CHECK_ARG(a->caches[l] != 0, "null cache");
-    bits |= a->caches[l];
+    ASPIRE_CHECK_ARG(address(l) != 0, "null cache");
+    bits |= address(l);
   }
   int vec = 16;
   while (bits & static_cast<uint64_t>(vec - 1)) vec /= 2;
@@ -164,7 +167,7 @@ extern "C" int aspire_compact_accepted(const aspire_compact_args* a, void* strea
   hipStream_t s = static_cast<hipStream_t>(stream);
   for (int l0 = 0; l0 < a->layers; l0 += kMoveLayers) {
     const int layers = std::min(a->layers - l0, kMoveLayers);
-    for (int l = 0; l < layers; ++l) p.caches[l] = reinterpret_cast<char*>(a->caches[l0 + l]);
+    for (int l = 0; l < layers; ++l) p.caches[l] = reinterpret_cast<char*>(address(l0 + l));
     const dim3 grid(a->rows, layers);
     if (vec == 16) compact_kernel<uint4><<<grid, kMoveThreads, 0, s>>>(p);
     else if (vec == 8) compact_kernel<uint2><<<grid, kMoveThreads, 0, s>>>(p);

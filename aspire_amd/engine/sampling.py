@@ -107,25 +107,38 @@ def verify_tree_speculation(tree_tokens: torch.Tensor, parents: torch.Tensor, ta
     ``path`` holds the kept tokens' indices, ``output`` their targets (the kept tokens but the root, then a new one), both -1
     behind the ``kept`` entries. A row without tokens keeps none."""
     what = "verify_tree_speculation"
-    _lib.require_cuda(tree_tokens, parents, target_ids, qo_indptr, what=what)
-    ints, device = (torch.int32, torch.int64), tree_tokens.device
-    for name, t in (("tree_tokens", tree_tokens), ("parents", parents), ("target_ids", target_ids), ("qo_indptr", qo_indptr)):
-        if t.dim() != 1 or t.dtype not in ints or t.device != device:
-            raise ValueError(f"{what}: {name} must be 1-D int32 on {device}")
-    tokens, rows = tree_tokens.shape[0], qo_indptr.shape[0] - 1
-    if parents.shape[0] < tokens or target_ids.shape[0] < tokens:
+    index = tree_tokens.get_device()
+    if index < 0:
+        _lib.require_cuda(tree_tokens, what=what)
+    lists = [tree_tokens, parents, target_ids, qo_indptr]
+    for i, t in enumerate(lists):
+        if t.dtype is not torch.int32 or t.get_device() != index or t.dim() != 1 or not t.is_contiguous():
+            if t.dim() != 1 or t.dtype not in (torch.int32, torch.int64) or t.get_device() != index:
+                _lib.require_cuda(t, what=what)
+                raise ValueError(f"{what}: {('tree_tokens', 'parents', 'target_ids', 'qo_indptr')[i]} must be 1-D int32 on "
+                                 f"{tree_tokens.device}")
+            lists[i] = _lib.dense(t, torch.int32)
+    tok, par, tgt, qo = lists
+    tokens, rows = tok.shape[0], qo.shape[0] - 1
+    if par.shape[0] < tokens or tgt.shape[0] < tokens:
         raise ValueError(f"{what}: parents and target_ids need {tokens} entries")
     if rows < 0 or max_path < 1 or rows * max_path >= 1 << 31:
         raise ValueError(f"{what}: qo_indptr needs an entry more than rows, max_path at least 1, rows * max_path below 2^31")
-    tok, par, tgt, qo = (_lib.dense(t, torch.int32) for t in (tree_tokens, parents, target_ids, qo_indptr))
-    result = torch.empty(rows * (2 * max_path + 1), dtype=torch.int32, device=device)
-    output, path, kept = result.split([rows * max_path, rows * max_path, rows])
-    index, at, size = tok.get_device(), result.data_ptr(), 4 * rows * max_path
-    with torch.cuda.device(index):
-        rc = _lib.lib().aspire_verify_tree(tok.data_ptr(), par.data_ptr(), tgt.data_ptr(), qo.data_ptr(), tokens, rows, max_path,
-                                           at, at + size, at + 2 * size, torch._C._cuda_getCurrentRawStream(index))
-    _lib.check(rc, what)
-    return output.view(rows, max_path), path.view(rows, max_path), kept
+    device = tok.device
+    output = torch.empty((rows, max_path), dtype=torch.int32, device=device)
+    path = torch.empty((rows, max_path), dtype=torch.int32, device=device)
+    kept = torch.empty(rows, dtype=torch.int32, device=device)
+    args = (tok.data_ptr(), par.data_ptr(), tgt.data_ptr(), qo.data_ptr(), tokens, rows, max_path, output.data_ptr(),
+            path.data_ptr(), kept.data_ptr())
+    stream, entry = torch._C._cuda_getCurrentRawStream(index), _lib.lib().aspire_verify_tree
+    if torch._C._cuda_getDevice() == index:
+        rc = entry(*args, stream)
+    else:
+        with torch.cuda.device(index):
+            rc = entry(*args, stream)
+    if rc:
+        _lib.check(rc, what)
+    return output, path, kept
 
 
 def first_eos(output: torch.Tensor, committed: torch.Tensor, eos_token_ids: tuple[int, ...]):

@@ -151,27 +151,36 @@ def adjust_logits(logits: torch.Tensor, *, qo_indptr: torch.Tensor | None = None
 
     ``vocab_start`` is the token of column 0, for a shard of the vocabulary; masks are the shard's. Not differentiable."""
     what = "adjust_logits"
-    _lib.require_cuda(logits, what=what)
+    index, shape, st, dtype = logits.get_device(), logits.shape, logits.stride(), logits.dtype
+    if index < 0:
+        _lib.require_cuda(logits, what=what)
     if torch.is_grad_enabled() and logits.requires_grad or forward_ad._current_level >= 0 and _lib.has_tangent(logits, out):
         raise ValueError(f"{what}: not differentiable")
-    code, device = _LOGIT_DTYPES.get(logits.dtype), logits.device
-    if code is None or logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+    code = _LOGIT_DTYPES.get(dtype)
+    if code is None or len(shape) != 2 or (shape[1] > 1 and st[1] != 1):
         raise ValueError(f"{what}: logits must be bf16, fp16 or fp32 [T, V] with contiguous rows")
-    tokens, vocab = logits.shape
+    tokens, vocab = shape
+    device = logits.device
     if out is None:
-        out = torch.empty((tokens, vocab), dtype=logits.dtype, device=device)
-    elif out is not logits:
-        if out.shape != logits.shape or out.dtype != logits.dtype or out.device != device or (vocab > 1 and out.stride(1) != 1):
+        out, os = torch.empty((tokens, vocab), dtype=dtype, device=device), (vocab, 1)
+    elif out is logits:
+        os = st
+    else:
+        os = out.stride()
+        if out.shape != shape or out.dtype is not dtype or out.get_device() != index or (vocab > 1 and os[1] != 1):
             raise ValueError(f"{what}: out must be of logits' shape and type on {device} with contiguous rows")
-        if _lib.overlap(out, logits) and (out.data_ptr() != logits.data_ptr() or out.stride() != logits.stride()):
+        if _lib.overlap(out, logits) and (out.data_ptr() != logits.data_ptr() or os != st):
             raise ValueError(f"{what}: out must be logits itself or apart from it")
-    if tokens > 1 and out.stride(0) < vocab:
+    if tokens > 1 and os[0] < vocab:
         raise ValueError(f"{what}: the rows of out share memory")
 
     def vector(t, name, dtype, length=None, least=None):
         if t is None:
             return None
-        good = t.dim() == 1 and t.device == device and (t.dtype == dtype or dtype is torch.int32 and t.dtype == torch.int64)
+        if t.dtype is dtype and t.get_device() == index and t.dim() == 1 and t.is_contiguous() \
+                and (length is None or t.shape[0] == length) and (least is None or t.shape[0] >= least):
+            return t
+        good = t.dim() == 1 and t.get_device() == index and (t.dtype == dtype or dtype is torch.int32 and t.dtype == torch.int64)
         if not good or length is not None and t.shape[0] != length or least is not None and t.shape[0] < least:
             raise ValueError(f"{what}: {name} must be {dtype} [{length if length is not None else f'at least {least or 0}'}] on {device}")
         return _lib.dense(t, dtype)
@@ -181,11 +190,12 @@ def adjust_logits(logits: torch.Tensor, *, qo_indptr: torch.Tensor | None = None
     requests = tokens if qo is None else qo.shape[0] - 1
     lens = vector(history_lens, "history_lens", i32, requests)
     told = vector(prompt_lens, "prompt_lens", i32, requests)
-    rep, pres, freq = (vector(t, n, f32, requests) for t, n in ((repetition, "repetition"), (presence, "presence"),
-                                                                (frequency, "frequency")))
+    rep = vector(repetition, "repetition", f32, requests)
+    pres = vector(presence, "presence", f32, requests)
+    freq = vector(frequency, "frequency", f32, requests)
     history_stride = history_len = mask_stride = words = grammar_stride = grammar_count = 0
     if history is not None:
-        if history.dim() != 2 or history.dtype != i32 or history.shape[0] != requests or history.device != device \
+        if history.dim() != 2 or history.dtype is not i32 or history.shape[0] != requests or history.get_device() != index \
                 or (history.shape[1] > 1 and history.stride(1) != 1) or lens is None:
             raise ValueError(f"{what}: history must be int32 [{requests}, H] on {device} with contiguous rows, and history_lens given")
         history_stride, history_len = history.stride(0), history.shape[1]
@@ -195,7 +205,7 @@ def adjust_logits(logits: torch.Tensor, *, qo_indptr: torch.Tensor | None = None
         raise ValueError(f"{what}: tree_tokens and tree_masks go together, with qo_indptr")
     tree = vector(tree_tokens, "tree_tokens", i32, least=tokens)
     if tree_masks is not None:
-        if tree_masks.dtype != torch.int64 or tree_masks.dim() != 2 or tree_masks.shape[0] < tokens or tree_masks.device != device \
+        if tree_masks.dtype != torch.int64 or tree_masks.dim() != 2 or tree_masks.shape[0] < tokens or tree_masks.get_device() != index \
                 or (tree_masks.shape[1] > 1 and tree_masks.stride(1) != 1):
             raise ValueError(f"{what}: tree_masks must be int64 [T, words] on {device} with contiguous rows")
         mask_stride, words = tree_masks.stride(0), tree_masks.shape[1]
@@ -203,10 +213,10 @@ def adjust_logits(logits: torch.Tensor, *, qo_indptr: torch.Tensor | None = None
         raise ValueError(f"{what}: a history or a tree needs repetition, presence or frequency")
     if history is None and tree is None and (rep is not None or pres is not None or freq is not None):
         raise ValueError(f"{what}: penalties need a history or a tree")
-    if bias is not None and (bias.requests != requests or bias.indptr.device != device):
+    if bias is not None and (bias.requests != requests or bias.indptr.get_device() != index):
         raise ValueError(f"{what}: bias must hold {requests} requests on {device}")
     if grammar is not None:
-        if grammar.dtype != i32 or grammar.dim() != 2 or grammar.shape[1] < (vocab + 31) // 32 or grammar.device != device \
+        if grammar.dtype != i32 or grammar.dim() != 2 or grammar.shape[1] < (vocab + 31) // 32 or grammar.get_device() != index \
                 or (grammar.shape[1] > 1 and grammar.stride(1) != 1) or (grammar_rows is None and grammar.shape[0] < tokens):
             raise ValueError(f"{what}: grammar must be int32 [rows, {(vocab + 31) // 32}] on {device} with contiguous rows, a row for each "
                              "row of logits or grammar_rows given")
@@ -218,11 +228,11 @@ def adjust_logits(logits: torch.Tensor, *, qo_indptr: torch.Tensor | None = None
         raise ValueError(f"{what}: vocab_start must be 0 to 2^31 - 1")
     at = lambda t: 0 if t is None else t.data_ptr()
     b = (None, None, None) if bias is None else (bias.ids, bias.values, bias.indptr)
-    args = _ADJUST.pack(logits.data_ptr(), logits.stride(0), out.data_ptr(), out.stride(0), at(qo), at(history), history_stride,
+    args = _ADJUST.pack(logits.data_ptr(), st[0], out.data_ptr(), os[0], at(qo), at(history), history_stride,
                         at(lens), at(told), at(rep), at(pres), at(freq), at(tree), at(tree_masks), mask_stride, at(b[0]), at(b[1]),
                         at(b[2]), at(grammar), grammar_stride, at(which), vocab_start, tokens, vocab, requests, code, history_len,
                         words, grammar_count, 0 if bias is None else bias.ids.shape[0])
-    _lib.launch(_lib.lib().aspire_adjust_logits, args, logits.get_device(), what)
+    _lib.launch(_lib.lib().aspire_adjust_logits, args, index, what)
     return out
 
 

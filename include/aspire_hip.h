@@ -714,9 +714,10 @@ int aspire_verify_tree(const int32_t* tree_tokens, const int32_t* parents, const
 /* Moves the kept tokens' K and V rows to where a chain of them would stand: the row at slots[first + path[row, j]] goes to
  * slots[first + j], first = qo_indptr[row], for j = 1 .. kept[row] - 1, in every layer's cache [P, 2, page, H, D]. A path
  * rises; entries that do not lie in (j, the row's tokens) and slots outside the pool are passed over. caches: host array of
- * layers addresses of one layout; strides and sizes in bytes, head_bytes = D * element size. */
+ * layers addresses of one layout, or NULL: layer l at first_cache + l * stride_l. Strides and sizes in bytes, head_bytes = D *
+ * element size. */
 typedef struct {
-  const uint64_t* caches; int64_t stride_p; int64_t stride_kv; int64_t stride_t; int64_t stride_h;
+  const uint64_t* caches; void* first_cache; int64_t stride_l; int64_t stride_p; int64_t stride_kv; int64_t stride_t; int64_t stride_h;
   int64_t num_pages; const int32_t* path; const int32_t* kept; const int32_t* qo_indptr; const int64_t* slots;
   int32_t layers; int32_t heads; int32_t head_bytes; int32_t page_size; int32_t rows; int32_t tokens; int32_t max_path;
   int32_t reserved;
