@@ -12,26 +12,30 @@ namespace {
 
 constexpr int kMaxPageRows = 4096;  // running counts of all rows fit in LDS
 
-// Inclusive prefix sum over the workgroup (kThreads a multiple of 64); total is everyone's. sums holds kThreads / 64 values.
+// Inclusive prefix sums of two values over the workgroup (kThreads a multiple of 64); the totals are everyone's. sums holds
+// kThreads / 64 pairs, not in use elsewhere.
+struct Pair {
+  int64_t a, b;
+};
 template <int kThreads>
-__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* sums, int64_t& total) {
+__device__ __forceinline__ Pair block_scan(Pair v, Pair* sums, Pair& total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
-    const int64_t up = __shfl_up(v, d, 64);
-    if (lane >= d) v += up;
+    const int64_t up_a = __shfl_up(v.a, d, 64), up_b = __shfl_up(v.b, d, 64);
+    if (lane >= d) v.a += up_a, v.b += up_b;
   }
-  __syncthreads();  // the sums of an earlier scan have been read
   if (lane == 63) sums[wave] = v;
   __syncthreads();
-  int64_t before = 0;
-  total = 0;
+  Pair before{0, 0};
+  total = Pair{0, 0};
 #pragma unroll
   for (int w = 0; w < kThreads / 64; ++w) {
-    if (w < wave) before += sums[w];
-    total += sums[w];
+    const Pair s = sums[w];
+    if (w < wave) before.a += s.a, before.b += s.b;
+    total.a += s.a, total.b += s.b;
   }
-  return v + before;
+  return {v.a + before.a, v.b + before.b};
 }
 
 // The row of item i: the last one in [0, rows) whose first item offsets[row] is at most i.
@@ -48,97 +52,73 @@ __device__ __forceinline__ int row_of(const int32_t* offsets, int rows, int i) {
 // ------------------------------------------------------------------------------------------- the pool
 // One workgroup: the stack is one object, and what a step moves is a page a row. Thread t owns rows t * per .. t * per
 // + per - 1. First all pages that are given back go onto the stack, then, behind a barrier, pages are taken from it.
-constexpr int kResizeThreads = 1024;
+constexpr int kResizeThreads = 512;
 
 __global__ __launch_bounds__(kResizeThreads) void page_resize_kernel(aspire_page_resize_args a) {
   extern __shared__ int32_t resize_lds[];
-  __shared__ int64_t sums[kResizeThreads / 64];
-  __shared__ int32_t first_short;
-  int32_t* const offsets = resize_lds;       // first moved page of each row, among the moved ones
-  int32_t* const start = resize_lds + a.rows;  // the row's first moved entry of the table
+  __shared__ Pair sums[kResizeThreads / 64];
+  __shared__ int32_t first_short, took;
+  int32_t* const given_at = resize_lds;                // the row's first page among those given back
+  int32_t* const taken_at = resize_lds + a.rows;       // and among those taken
+  int32_t* const start = resize_lds + 2 * a.rows;      // the row's first entry that is moved
   const int per = (a.rows + kResizeThreads - 1) / kResizeThreads;
-  const int row0 = threadIdx.x * per, row1 = min(row0 + per, a.rows);
+  const int row0 = min(int(threadIdx.x) * per, a.rows), row1 = min(row0 + per, a.rows);
   const auto held_of = [&](int b) { return min(max(a.held[b], 0), a.width); };
   const auto want_of = [&](int b, int held) {
     const int len = a.lengths[b];
     return len < 0 ? held : int((int64_t(len) + a.page_size - 1) / a.page_size);
   };
   const int count = min(max(*a.free_count, 0), a.num_pages);
+  if (threadIdx.x == 0) first_short = a.rows;
 
-  // pages given back
-  int64_t back = 0;
+  Pair sum{0, 0}, total;
   for (int b = row0; b < row1; ++b) {
     const int held = held_of(b), want = want_of(b, held);
-    back += max(held - want, 0);
+    sum.a += max(held - want, 0);
+    sum.b += max(want - held, 0);
   }
-  int64_t total;
-  int64_t at = block_scan<kResizeThreads>(back, sums, total) - back;
-  const int given = int(total);  // below rows * width, which the host holds under 2^31
+  Pair at = block_scan<kResizeThreads>(sum, sums, total);
+  at.a -= sum.a, at.b -= sum.b;
+  const int given = int(total.a);  // at most rows * width, which the host holds under 2^31
+  const int64_t free_now = min(int64_t(count) + given, int64_t(a.num_pages));
+  if (threadIdx.x == 0) took = int(min(total.b, int64_t(0x7fffffff)));
+  // rows that cannot be served: from the first one on
+  int64_t after = at.b;
+  for (int b = row0; b < row1; ++b) {
+    const int held = held_of(b), want = want_of(b, held);
+    given_at[b] = int(at.a);
+    at.a += max(held - want, 0);
+    taken_at[b] = int(min(after, int64_t(0x7fffffff)));  // (where it is cut no row is served)
+    after += max(want - held, 0);
+    start[b] = min(held, want);
+    if (want > held && (want > a.width || after > free_now)) atomicMin(&first_short, b);
+  }
+  __syncthreads();
+  const int served = first_short;
+  for (int b = row0; b < row1; ++b) {
+    const int held = held_of(b), want = want_of(b, held);
+    if (b == served) took = taken_at[b];
+    a.shortage[b] = b < served ? 0 : max(want - held, 0);
+    if (want < held || b < served) a.held[b] = want;
+  }
   if (given > 0) {
-    for (int b = row0; b < row1; ++b) {
-      const int held = held_of(b), want = want_of(b, held);
-      offsets[b] = int(at);
-      start[b] = want;
-      if (held > want) {
-        at += held - want;
-        a.held[b] = want;
-      }
-    }
-    __syncthreads();
     for (int k = threadIdx.x; k < given; k += kResizeThreads) {
-      const int b = row_of(offsets, a.rows, k);
-      int32_t* const entry = a.block_table + int64_t(b) * a.width + start[b] + (k - offsets[b]);
+      const int b = row_of(given_at, a.rows, k);
+      int32_t* const entry = a.block_table + int64_t(b) * a.width + start[b] + (k - given_at[b]);
       const int64_t place = int64_t(count) + given - 1 - k;
       if (place < a.num_pages) a.free_pages[place] = *entry;
       *entry = -1;
     }
   }
-  const int64_t free_now = min(int64_t(count) + given, int64_t(a.num_pages));
-
-  // pages taken: the rows before the first that cannot be served
-  if (threadIdx.x == 0) first_short = a.rows;
   __syncthreads();
-  int64_t lack = 0;
-  for (int b = row0; b < row1; ++b) {
-    const int held = held_of(b), want = want_of(b, held);
-    lack += max(want - held, 0);
-  }
-  at = block_scan<kResizeThreads>(lack, sums, total) - lack;
-  int64_t after = at;
-  for (int b = row0; b < row1; ++b) {
-    const int held = held_of(b), want = want_of(b, held);
-    if (want <= held) continue;
-    after += want - held;
-    if (want > a.width || after > free_now) {
-      atomicMin(&first_short, b);
-      break;
-    }
-  }
-  __syncthreads();
-  const int served = first_short;
-  int64_t taken = 0;
-  for (int b = row0; b < row1; ++b) {
-    const int held = held_of(b), want = want_of(b, held), n = max(want - held, 0);
-    if (b < served) {
-      offsets[b] = int(at);
-      start[b] = held;
-      at += n;
-      taken += n;
-      if (n > 0) a.held[b] = want;
-    } else {
-      offsets[b] = 0x7fffffff;
-    }
-    a.shortage[b] = b < served ? 0 : n;
-  }
-  block_scan<kResizeThreads>(taken, sums, total);  // its barriers also show every row's offset
-  const int took = int(total);
-  for (int k = threadIdx.x; k < took; k += kResizeThreads) {
-    const int b = row_of(offsets, a.rows, k);
+  const int taken = took;
+  for (int k = threadIdx.x; k < taken; k += kResizeThreads) {
+    const int b = row_of(taken_at, served, k);
     const int64_t place = free_now - 1 - k;
-    a.block_table[int64_t(b) * a.width + start[b] + (k - offsets[b])] = a.free_pages[place];
+    a.block_table[int64_t(b) * a.width + start[b] + (k - taken_at[b])] = a.free_pages[place];
     a.free_pages[place] = -1;
   }
-  if (threadIdx.x == 0) *a.free_count = int(free_now) - took;
+  if (threadIdx.x == 0) *a.free_count = int(free_now) - taken;
 }
 
 // -------------------------------------------------------------------------------------------- the tables
@@ -149,7 +129,7 @@ constexpr int kParentWindow = 1024;  // parents before a workgroup's own tokens 
 
 __global__ __launch_bounds__(kTableThreads) void step_tables_kernel(aspire_step_tables_args a) {
   extern __shared__ int32_t tables_lds[];
-  __shared__ int64_t sums[kTableThreads / 64];
+  __shared__ Pair sums[kTableThreads / 64];
   __shared__ int32_t first_out;
   __shared__ int32_t window[kParentWindow + kTableThreads];
   int32_t* const tok = tables_lds;               // rows + 1
@@ -163,15 +143,15 @@ __global__ __launch_bounds__(kTableThreads) void step_tables_kernel(aspire_step_
   const auto pages_of = [&](int b, int fresh) {
     return fresh == 0 ? int64_t(0) : (int64_t(a.cached[b]) + fresh + a.page_size - 1) / a.page_size;
   };
-  int64_t tokens = 0, pages = 0, all_tokens, all_pages;
+  Pair sum{0, 0}, all;  // tokens and pages
   for (int b = row0; b < row1; ++b) {
     const int fresh = fresh_of(b);
-    tokens += fresh;
-    pages += pages_of(b, fresh);
+    sum.a += fresh;
+    sum.b += pages_of(b, fresh);
   }
   if (threadIdx.x == 0) first_out = a.rows;
-  int64_t t = block_scan<kTableThreads>(tokens, sums, all_tokens) - tokens;
-  int64_t e = block_scan<kTableThreads>(pages, sums, all_pages) - pages;
+  const Pair upto = block_scan<kTableThreads>(sum, sums, all);
+  int64_t t = upto.a - sum.a, e = upto.b - sum.b;
   for (int b = row0; b < row1; ++b) {
     const int fresh = fresh_of(b);
     // counts behind a row that is left out are never used: what they are cut to does not matter
@@ -186,8 +166,8 @@ __global__ __launch_bounds__(kTableThreads) void step_tables_kernel(aspire_step_
     }
   }
   if (threadIdx.x == kTableThreads - 1) {
-    tok[a.rows] = int(min(all_tokens, int64_t(0x7fffffff)));
-    pag[a.rows] = int(min(all_pages, int64_t(0x7fffffff)));
+    tok[a.rows] = int(min(all.a, int64_t(0x7fffffff)));
+    pag[a.rows] = int(min(all.b, int64_t(0x7fffffff)));
   }
   __syncthreads();
   const int served = first_out;
@@ -202,8 +182,8 @@ __global__ __launch_bounds__(kTableThreads) void step_tables_kernel(aspire_step_
       a.last_page_len[b] = n > 0 ? int(int64_t(a.cached[b]) + a.fresh[b] - int64_t(n - 1) * a.page_size) : 0;
     }
     if (threadIdx.x == 0) {
-      a.totals[0] = all_tokens;
-      a.totals[1] = all_pages;
+      a.totals[0] = all.a;
+      a.totals[1] = all.b;
       a.totals[2] = served;
     }
   }
@@ -275,7 +255,7 @@ extern "C" int aspire_page_resize(const aspire_page_resize_args* a, void* stream
   if (a->rows == 0) return ASPIRE_OK;
   ASPIRE_CHECK_ARG(a->held && a->free_count && a->shortage && a->lengths && (a->block_table || a->width == 0) &&
                        (a->free_pages || a->num_pages == 0), "null array");
-  page_resize_kernel<<<1, kResizeThreads, 8 * a->rows, static_cast<hipStream_t>(stream)>>>(*a);
+  page_resize_kernel<<<1, kResizeThreads, 12 * a->rows, static_cast<hipStream_t>(stream)>>>(*a);
   ASPIRE_CHECK_LAUNCH();
   return ASPIRE_OK;
 }

@@ -67,7 +67,7 @@ __global__ __launch_bounds__(64) void verify_tree_kernel(const int32_t* tree_tok
 // source).
 constexpr int kMoveThreads = 256;
 constexpr int kMoveLayers = 64;  // addresses in a launch's arguments
-constexpr int kMoveRound = 4;
+constexpr int kMoveRound = 8;
 
 struct CompactParams {
   char* caches[kMoveLayers];
@@ -78,6 +78,9 @@ struct CompactParams {
   const int64_t* slots;
   int32_t heads, per_head, page_size, tokens, max_path;  // per_head: vectors of a head
 };
+
+typedef __attribute__((ext_vector_type(4))) uint32_t u32x4m;
+typedef __attribute__((ext_vector_type(2))) uint32_t u32x2m;
 
 template <typename V>
 __global__ __launch_bounds__(kMoveThreads) void compact_kernel(CompactParams p) {
@@ -109,12 +112,17 @@ __global__ __launch_bounds__(kMoveThreads) void compact_kernel(CompactParams p) 
       char* const base = cache + kv * p.s_kv + h * p.s_h + (w - h * p.per_head) * int64_t(sizeof(V));
       for (int k = 0; k < part; k += kMoveRound) {
         V x[kMoveRound];
+        int64_t src[kMoveRound], dst[kMoveRound];
+#pragma unroll
+        for (int i = 0; i < kMoveRound; ++i) {
+          src[i] = k + i < part ? from[k + i] : -1;
+          dst[i] = to[min(k + i, part - 1)];
+          x[i] = V(0);
+          if (src[i] >= 0) x[i] = *reinterpret_cast<const V*>(base + src[i]);
+        }
 #pragma unroll
         for (int i = 0; i < kMoveRound; ++i)
-          if (k + i < part && from[k + i] >= 0) x[i] = *reinterpret_cast<const V*>(base + from[k + i]);
-#pragma unroll
-        for (int i = 0; i < kMoveRound; ++i)
-          if (k + i < part && from[k + i] >= 0) *reinterpret_cast<V*>(base + to[k + i]) = x[i];
+          if (src[i] >= 0) *reinterpret_cast<V*>(base + dst[i]) = x[i];
       }
     }
   }
@@ -169,8 +177,8 @@ extern "C" int aspire_compact_accepted(const aspire_compact_args* a, void* strea
     const int layers = std::min(a->layers - l0, kMoveLayers);
     for (int l = 0; l < layers; ++l) p.caches[l] = reinterpret_cast<char*>(address(l0 + l));
     const dim3 grid(a->rows, layers);
-    if (vec == 16) compact_kernel<uint4><<<grid, kMoveThreads, 0, s>>>(p);
-    else if (vec == 8) compact_kernel<uint2><<<grid, kMoveThreads, 0, s>>>(p);
+    if (vec == 16) compact_kernel<u32x4m><<<grid, kMoveThreads, 0, s>>>(p);
+    else if (vec == 8) compact_kernel<u32x2m><<<grid, kMoveThreads, 0, s>>>(p);
     else if (vec == 4) compact_kernel<uint32_t><<<grid, kMoveThreads, 0, s>>>(p);
     else if (vec == 2) compact_kernel<uint16_t><<<grid, kMoveThreads, 0, s>>>(p);
     else compact_kernel<uint8_t><<<grid, kMoveThreads, 0, s>>>(p);
