@@ -3,11 +3,13 @@
 // A workgroup takes one chunk of the vocabulary for one request (or some of its rows). It counts the request's history tokens of
 // the chunk in LDS (a 32-bit word a token: occurrences in the output, one bit for the prompt's, one for tokens that the request's
 // tree drafts) and lays the chunk's biases beside them, while its first logits are on their way; then the chunk of every row
-// streams through: 16 or 32 bytes of logits a thread, their words from LDS, a byte of the mask, one rounding, two vectors a thread
-// in flight. Rows only read the words: a token that the tree drafts is counted on a row's own path where it is met.
+// streams through: vectors of 8 logits, their words from LDS, a byte of the mask, one rounding, the next row's in flight
+// meanwhile. (Counts and biases kept in registers over the rows take 121 VGPRs, half the waves, and as long.) A token that the
+// tree drafts is counted on a row's own path where it is met. Chunks of low tokens, which histories and trees meet most, start first.
 // HBM bounds it at batch sizes (logits once in, once out, and an eighth of a byte of mask a token); history is
 // read once a chunk, from L2.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.h"
 
@@ -16,13 +18,13 @@ namespace {
 
 struct LogitsParams {
   aspire_adjust_logits_args a;
-  int32_t chunk_log2;  // tokens a workgroup takes, 1,024 to 8,192
-  int32_t row_parts;   // workgroups that share a request's rows of a chunk
+  int32_t row_parts;  // workgroups that share a request's rows of a chunk
 };
 
 constexpr int kLogitThreads = 512;
+constexpr int kVec = 8;          // logits of a vector: a byte of mask
 constexpr uint32_t kPrompt = 0x80000000u, kDrafted = 0x40000000u;  // the rest of a word counts
-constexpr int kTreeList = 512;  // drafted tokens of a request, and words of rows' masks, that are held in LDS
+constexpr int kTreeList = 512;   // drafted tokens of a request, and words of rows' masks, that are held in LDS
 
 template <typename T> struct Pack;
 struct Bf16 {};
@@ -46,76 +48,67 @@ template <> struct Pack<float> {
 // n values at any 2- or 4-byte aligned place, in one access
 template <typename R, int n> struct __attribute__((packed, aligned(sizeof(R)))) Vec { R v[n]; };
 
-template <typename T, bool kCounts, bool kBias, bool kMask>
-__global__ __launch_bounds__(kLogitThreads) void adjust_logits_kernel(LogitsParams p) {
+// A workgroup's chunk is kJ vectors a thread.
+template <typename T, int kJ, bool kCounts, bool kBias, bool kMask>
+__global__ __launch_bounds__(kLogitThreads, kJ == 1 || std::is_same<T, Bf16>::value ? 8 : 6) void adjust_logits_kernel(LogitsParams p) {
   typedef typename Pack<T>::raw R;
-  constexpr int kVec = 8, kAhead = 2;  // a byte of mask a vector; vectors in flight
-  extern __shared__ uint32_t logits_lds[];
-  __shared__ int32_t drafted[kCounts ? kTreeList : 1];
-  __shared__ uint64_t paths[kCounts ? kTreeList : 1];
+  constexpr int kChunk = kJ * kVec * kLogitThreads;
+  extern __shared__ uint4 logits_lds[];
+  uint32_t* const counts = reinterpret_cast<uint32_t*>(logits_lds);
+  float* const bias = reinterpret_cast<float*>(counts + (kCounts ? kChunk : 0));
+  uint64_t* const paths = reinterpret_cast<uint64_t*>(bias + (kBias ? kChunk : 0));  // there only for trees
+  int32_t* const drafted = reinterpret_cast<int32_t*>(paths + kTreeList);
   const aspire_adjust_logits_args& a = p.a;
-  const int chunk = 1 << p.chunk_log2;
-  uint32_t* const counts = logits_lds;
-  float* const bias = reinterpret_cast<float*>(logits_lds + (kCounts ? chunk : 0));
-  const int b = blockIdx.y, v0 = blockIdx.x << p.chunk_log2, width = min(chunk, a.vocab - v0);
+  const int nth = wave_uniform(int(blockIdx.x / uint32_t(a.requests))), b = int(blockIdx.x) - nth * a.requests, v0 = nth * kChunk, width = min(kChunk, a.vocab - v0);
   const uint32_t token0 = uint32_t(a.vocab_start) + v0;  // the chunk's first token; its last one is below 2^31
   int first = b, end = b + 1;
   if (a.qo_indptr != nullptr) {
     first = max(a.qo_indptr[b], 0);
     end = min(a.qo_indptr[b + 1], a.tokens);
   }
-  const int n = end - first;
+  const int n = max(end - first, 0);
   // this workgroup's rows
-  const int row0 = first + int(int64_t(max(n, 0)) * blockIdx.z / p.row_parts);
-  const int row1 = first + int(int64_t(max(n, 0)) * (blockIdx.z + 1) / p.row_parts);
+  const int row0 = first + int(int64_t(n) * blockIdx.y / p.row_parts), row1 = first + int(int64_t(n) * (blockIdx.y + 1) / p.row_parts);
   if (row0 >= row1) return;
 
-  // Item i: vector i % per of row row0 + i / per. The last vector of the vocabulary may be short.
-  const int per_log2 = p.chunk_log2 - 3, per = 1 << per_log2;
-  const int64_t items = int64_t(row1 - row0) << per_log2;
-  Vec<R, kVec> x[kAhead];
-  uint32_t allowed[kAhead];
-  const auto fetch = [&](int64_t i, int u) {
-    const int row = row0 + int(i >> per_log2), at = int(i & (per - 1)) * kVec;
-    allowed[u] = 255u;
-    if (i >= items || at >= width) return;
-    const R* const in = static_cast<const R*>(a.logits) + row * a.stride + v0 + at;
-    if (at + kVec <= width) {
-      x[u] = *reinterpret_cast<const Vec<R, kVec>*>(in);
-    } else {
+  const int whole = width / kVec;  // whole vectors; the vocabulary's last logits come one by one, to the first threads
+  const int tail = whole * kVec + int(threadIdx.x);
+  Vec<R, kVec> x[kJ];
+  uint32_t allowed[kJ];
+  const auto mask_of = [&](int row) -> const uint8_t* {
+    const int g = !kMask ? -1 : a.grammar_rows != nullptr ? a.grammar_rows[row] : row;
+    return g >= 0 && g < a.num_grammar_rows ? reinterpret_cast<const uint8_t*>(a.grammar + g * a.grammar_stride) + (v0 >> 3) : nullptr;
+  };
+  const auto fetch = [&](int row) {
+    const R* const in = static_cast<const R*>(a.logits) + row * a.stride + v0;
+    const uint8_t* const mask = mask_of(row);
 #pragma unroll
-      for (int e = 0; e < kVec; ++e)
-        if (e < width - at) x[u].v[e] = in[e];
-    }
-    if (kMask) {
-      const int g = a.grammar_rows != nullptr ? a.grammar_rows[row] : row;
-      if (g >= 0 && g < a.num_grammar_rows)
-        allowed[u] = reinterpret_cast<const uint8_t*>(a.grammar + g * a.grammar_stride)[(v0 + at) >> 3];
+    for (int j = 0; j < kJ; ++j) {
+      const int k = j * kLogitThreads + threadIdx.x;
+      if (k >= whole) break;
+      x[j] = *reinterpret_cast<const Vec<R, kVec>*>(in + k * kVec);
+      allowed[j] = kMask && mask != nullptr ? mask[k] : 255u;
     }
   };
-#pragma unroll
-  for (int u = 0; u < kAhead; ++u) fetch(threadIdx.x + u * kLogitThreads, u);
+  fetch(row0);
 
-  float repetition = 1.f, inverse = 1.f, presence = 0.f, frequency = 0.f;
   if (kCounts || kBias) {
-    for (int i = threadIdx.x * 4; i < chunk; i += kLogitThreads * 4) {
-      if (kCounts) *reinterpret_cast<uint4*>(counts + i) = make_uint4(0, 0, 0, 0);
-      if (kBias) *reinterpret_cast<float4*>(bias + i) = make_float4(0.f, 0.f, 0.f, 0.f);
-    }
+    for (int i = threadIdx.x; i < (kChunk / 4) * ((kCounts ? 1 : 0) + (kBias ? 1 : 0)); i += kLogitThreads) logits_lds[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
   }
   const bool tree = kCounts && a.tree_masks != nullptr;
   const int words = min(a.mask_words, (n + 63) / 64);  // of a row's mask that hold its request's tokens
   const bool listed = int64_t(row1 - row0) * words <= kTreeList;
+  float repetition = 1.f, inverse = 1.f, presence = 0.f, frequency = 0.f;
   if (kCounts) {
     if (a.repetition != nullptr) repetition = a.repetition[b];
     if (a.presence != nullptr) presence = a.presence[b];
     if (a.frequency != nullptr) frequency = a.frequency[b];
-    inverse = 1.f / repetition;
+    inverse = 1.f / repetition;  // (a product by it is off by one rounding more than the quotient)
     if (a.history != nullptr) {
       const int32_t* const history = a.history + b * a.history_stride;
       const int len = min(a.history_lens[b], a.history_len), told = a.prompt_lens != nullptr ? a.prompt_lens[b] : 0;
-      constexpr int kRound = 4;  // 16-byte loads of a thread in flight: one trip to L2 for 4,096 tokens
+      constexpr int kRound = 4;  // 16-byte loads of a thread in flight: one trip to L2 for 8,192 tokens
       const auto count = [&](int32_t token, int i) {
         const uint32_t at = uint32_t(token) - token0;  // negative tokens wrap to beyond the chunk, too
         if (at >= uint32_t(width)) return;
@@ -138,13 +131,10 @@ __global__ __launch_bounds__(kLogitThreads) void adjust_logits_kernel(LogitsPara
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
           const int i = i0 + u * kLogitThreads + threadIdx.x;
-          h[u] = i < len ? history[i] : -1;
+          h[u] = i < len ? history[i] : -1;  // of no column
         }
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          const int i = i0 + u * kLogitThreads + threadIdx.x;
-          if (i < len) count(h[u], i);
-        }
+        for (int u = 0; u < 8; ++u) count(h[u], i0 + u * kLogitThreads + threadIdx.x);
       }
     }
     if (tree) {
@@ -168,16 +158,20 @@ __global__ __launch_bounds__(kLogitThreads) void adjust_logits_kernel(LogitsPara
   }
   if (kCounts || kBias) __syncthreads();
 
+  // the bits of word w of a row's path, and the drafted token of a node
+  const auto path_word = [&](int row, int w) {
+    const uint64_t bits = listed ? paths[(row - row0) * words + w] : uint64_t(a.tree_masks[row * a.mask_stride + w]);
+    return n - 64 * w < 64 ? bits & ((uint64_t(1) << (n - 64 * w)) - 1) : bits;
+  };
+  const auto node_token = [&](int i) { return i < kTreeList ? drafted[i] : a.tree_tokens[first + i]; };
   // Adds to the words c of this lane's 8 tokens how often the row's path has them: the wave walks the path together, node tokens in
   // lanes, and passes over those outside its 512 tokens from token base on.
   const auto add_path = [&](int row, uint32_t base, uint32_t (&c)[kVec]) {
     const int lane = threadIdx.x & 63;
     for (int w = 0; w < words; ++w) {
-      const int i = 64 * w + lane;
-      const int32_t token = i >= n ? -1 : i < kTreeList ? drafted[i] : a.tree_tokens[first + i];
-      uint64_t bits = listed ? paths[(row - row0) * words + w] : uint64_t(a.tree_masks[row * a.mask_stride + w]);
+      const int32_t token = 64 * w + lane < n ? node_token(64 * w + lane) : -1;
+      uint64_t bits = path_word(row, w);
       bits = (uint64_t(uint32_t(wave_uniform(int(bits >> 32)))) << 32) | uint32_t(wave_uniform(int(uint32_t(bits))));
-      if (n - 64 * w < 64) bits &= (uint64_t(1) << (n - 64 * w)) - 1;
       for (; bits != 0; bits &= bits - 1) {
         const uint32_t at = uint32_t(__builtin_amdgcn_readlane(token, __builtin_ctzll(bits))) - base;
         if (at >= 64 * kVec) continue;
@@ -186,43 +180,41 @@ __global__ __launch_bounds__(kLogitThreads) void adjust_logits_kernel(LogitsPara
       }
     }
   };
-  for (int64_t i0 = threadIdx.x; i0 < items; i0 += kAhead * kLogitThreads) {
-    Vec<R, kVec> y[kAhead];
-    uint32_t now[kAhead];
+  const auto penalty = [&](float f, uint32_t c) {
+    const uint32_t written = c & ~kPrompt;
+    const float seen = f * (f > 0.f ? inverse : repetition);
+    f = c != 0 ? seen : f;
+    return written != 0 ? (f - frequency * float(written)) - presence : f;
+  };
+  for (int row = row0; row < row1; ++row) {
+    R* const out = static_cast<R*>(a.out) + row * a.out_stride + v0;
+    Vec<R, kVec> y[kJ];
+    uint32_t now[kJ];
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) y[u] = x[u], now[u] = allowed[u];
+    for (int j = 0; j < kJ; ++j) y[j] = x[j], now[j] = allowed[j];
+    if (row + 1 < row1) fetch(row + 1);
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) fetch(i0 + (kAhead + u) * kLogitThreads, u);
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      const int64_t i = i0 + u * kLogitThreads;
-      const int row = row0 + int(i >> per_log2), at = int(i & (per - 1)) * kVec;
-      const bool live = i < items && at < width;
+    for (int j = 0; j < kJ; ++j) {
+      const int k = j * kLogitThreads + threadIdx.x;
+      if (k - int(threadIdx.x & 63) >= whole) break;  // of the whole wave
       float f[kVec];
 #pragma unroll
-      for (int e = 0; e < kVec; ++e) f[e] = Pack<T>::up(y[u].v[e]);
+      for (int e = 0; e < kVec; ++e) f[e] = Pack<T>::up(y[j].v[e]);
+      const int at = k * kVec;
       if (kCounts) {
-        uint4 c0 = make_uint4(0, 0, 0, 0), c1 = c0;
-        if (live) c0 = *reinterpret_cast<const uint4*>(counts + at), c1 = *reinterpret_cast<const uint4*>(counts + at + 4);
+        const uint4 c0 = *reinterpret_cast<const uint4*>(counts + at), c1 = *reinterpret_cast<const uint4*>(counts + at + 4);
         uint32_t c[kVec] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
         const uint32_t some = c0.x | c0.y | c0.z | c0.w | c1.x | c1.y | c1.z | c1.w;
-        if (tree && __ballot(some & kDrafted)) {  // a wave's vectors are one row's
+        if (tree && __ballot((some & kDrafted) != 0)) {
 #pragma unroll
           for (int e = 0; e < kVec; ++e) c[e] &= ~kDrafted;
-          add_path(wave_uniform(row), token0 + wave_uniform(at), c);
+          add_path(row, token0 + wave_uniform(at), c);
         }
         if (some != 0) {
 #pragma unroll
-          for (int e = 0; e < kVec; ++e) {
-            const uint32_t written = c[e] & ~kPrompt;
-            // (a product by the rounded inverse is off by one rounding more than the quotient)
-            const float seen = f[e] * (f[e] > 0.f ? inverse : repetition);
-            f[e] = c[e] != 0 ? seen : f[e];
-            f[e] = written != 0 ? (f[e] - frequency * float(written)) - presence : f[e];
-          }
+          for (int e = 0; e < kVec; ++e) f[e] = penalty(f[e], c[e]);
         }
       }
-      if (!live) continue;
       if (kBias) {
         const float4 b0 = *reinterpret_cast<const float4*>(bias + at), b1 = *reinterpret_cast<const float4*>(bias + at + 4);
         f[0] += b0.x, f[1] += b0.y, f[2] += b0.z, f[3] += b0.w;
@@ -230,32 +222,54 @@ __global__ __launch_bounds__(kLogitThreads) void adjust_logits_kernel(LogitsPara
       }
 #pragma unroll
       for (int e = 0; e < kVec; ++e) {
-        if (kMask) f[e] = (now[u] >> e) & 1 ? f[e] : -__builtin_huge_valf();
-        y[u].v[e] = Pack<T>::down(f[e]);
+        if (kMask) f[e] = (now[j] >> e) & 1 ? f[e] : -__builtin_huge_valf();
+        y[j].v[e] = Pack<T>::down(f[e]);
       }
-      R* const out = static_cast<R*>(a.out) + row * a.out_stride + v0 + at;
-      if (at + kVec <= width) {
-        *reinterpret_cast<Vec<R, kVec>*>(out) = y[u];
-      } else {
-#pragma unroll
-        for (int e = 0; e < kVec; ++e)
-          if (e < width - at) out[e] = y[u].v[e];
+      if (k < whole) *reinterpret_cast<Vec<R, kVec>*>(out + at) = y[j];
+    }
+    if (tail < width) {  // up to 7 threads
+      float f = Pack<T>::up((static_cast<const R*>(a.logits) + row * a.stride + v0)[tail]);
+      if (kCounts) {
+        uint32_t c = counts[tail];
+        if (c & kDrafted) {
+          c &= ~kDrafted;
+          for (int w = 0; w < words; ++w)
+            for (uint64_t bits = path_word(row, w); bits != 0; bits &= bits - 1)
+              c += uint32_t(node_token(64 * w + __builtin_ctzll(bits))) == token0 + tail ? 1u : 0u;
+        }
+        f = penalty(f, c);
       }
+      if (kBias) f += bias[tail];
+      const uint8_t* const mask = mask_of(row);
+      if (kMask && mask != nullptr && !((mask[tail >> 3] >> (tail & 7)) & 1)) f = -__builtin_huge_valf();
+      out[tail] = Pack<T>::down(f);
     }
   }
 }
 
-template <typename T, bool kCounts, bool kBias>
-void launch_mask(const LogitsParams& p, dim3 grid, int lds, hipStream_t s) {
-  if (p.a.grammar != nullptr) adjust_logits_kernel<T, kCounts, kBias, true><<<grid, kLogitThreads, lds, s>>>(p);
-  else adjust_logits_kernel<T, kCounts, kBias, false><<<grid, kLogitThreads, lds, s>>>(p);
+struct LogitsLaunch {
+  int vectors;  // of a thread
+  bool counts, bias;
+  dim3 grid;
+  int lds;
+  hipStream_t stream;
+};
+template <typename T, int kJ, bool kCounts, bool kBias>
+void launch_mask(const LogitsParams& p, const LogitsLaunch& l) {
+  if (p.a.grammar != nullptr) adjust_logits_kernel<T, kJ, kCounts, kBias, true><<<l.grid, kLogitThreads, l.lds, l.stream>>>(p);
+  else adjust_logits_kernel<T, kJ, kCounts, kBias, false><<<l.grid, kLogitThreads, l.lds, l.stream>>>(p);
+}
+template <typename T, int kJ>
+void launch_parts(const LogitsParams& p, const LogitsLaunch& l) {
+  if (l.counts && l.bias) launch_mask<T, kJ, true, true>(p, l);
+  else if (l.counts) launch_mask<T, kJ, true, false>(p, l);
+  else if (l.bias) launch_mask<T, kJ, false, true>(p, l);
+  else launch_mask<T, kJ, false, false>(p, l);
 }
 template <typename T>
-void launch_logits(const LogitsParams& p, bool counts, bool bias, dim3 grid, int lds, hipStream_t s) {
-  if (counts && bias) launch_mask<T, true, true>(p, grid, lds, s);
-  else if (counts) launch_mask<T, true, false>(p, grid, lds, s);
-  else if (bias) launch_mask<T, false, true>(p, grid, lds, s);
-  else launch_mask<T, false, false>(p, grid, lds, s);
+void launch_logits(const LogitsParams& p, const LogitsLaunch& l) {
+  if (l.vectors == 2) launch_parts<T, 2>(p, l);
+  else launch_parts<T, 1>(p, l);
 }
 
 }  // namespace
@@ -278,21 +292,21 @@ extern "C" int aspire_adjust_logits(const aspire_adjust_logits_args* a, void* st
   ASPIRE_CHECK_ARG(!a->bias_indptr || a->bias_entries == 0 || (a->bias_ids && a->bias_values), "null biases");
   const bool counts = (a->history || a->tree_masks) && (a->repetition || a->presence || a->frequency);
   const bool bias = a->bias_indptr != nullptr && a->bias_entries > 0;
-  // Chunks of 8,192 tokens, shorter while that leaves fewer than two workgroups a CU; then a request's rows are shared by several, four
-  // rows or more each, up to eight workgroups a CU. (A history is counted once a workgroup; without enough of them too few loads are
-  // in flight: 16 trees of 1 to 24 tokens over 128,257 took 68 us on 256 workgroups.)
-  LogitsParams p{*a, 13, 1};
-  const auto chunks = [&] { return (int64_t(a->vocab) + (1 << p.chunk_log2) - 1) >> p.chunk_log2; };
-  while (p.chunk_log2 > 10 && chunks() * a->requests < 512) --p.chunk_log2;
+  // Chunks of 8,192 tokens, or 4,096 with two tables in LDS (four workgroups a CU either way) or while longer ones leave fewer than two
+  // workgroups a CU; then a request's rows are shared by several, eight rows or more each, up to eight workgroups a CU (a history is
+  // counted once a workgroup: 16 trees of 1 to 24 tokens, 128,257 logits, take 54 us without sharing, 59 with a third of the rows each).
+  LogitsLaunch l{counts && bias ? 1 : 2, counts, bias, dim3(), 0, static_cast<hipStream_t>(stream)};
+  const auto chunk = [&] { return l.vectors * kVec * kLogitThreads; };
+  const auto chunks = [&] { return (int64_t(a->vocab) + chunk() - 1) / chunk(); };
+  if (chunks() * a->requests < 512) l.vectors = 1;
   const int64_t wgs = chunks() * a->requests, mean = a->qo_indptr ? a->tokens / a->requests : 1;
-  p.row_parts = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({mean / 4, 2048 / wgs, 65535})));
-  ASPIRE_CHECK_ARG(chunks() <= (1 << 24) / a->requests, "vocabulary times requests too large");
-  const dim3 grid(static_cast<uint32_t>(chunks()), a->requests, p.row_parts);
-  const int lds = (4 << p.chunk_log2) * ((counts ? 1 : 0) + (bias ? 1 : 0));
-  hipStream_t s = static_cast<hipStream_t>(stream);
-  if (a->dtype == 0) launch_logits<Bf16>(p, counts, bias, grid, lds, s);
-  else if (a->dtype == 1) launch_logits<Fp16>(p, counts, bias, grid, lds, s);
-  else launch_logits<float>(p, counts, bias, grid, lds, s);
+  LogitsParams p{*a, static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({mean / 8, 2048 / wgs, 65535})))};
+  ASPIRE_CHECK_ARG(wgs <= (1 << 23), "vocabulary times requests too large");
+  l.grid = dim3(static_cast<uint32_t>(wgs), p.row_parts);
+  l.lds = chunk() * 4 * ((counts ? 1 : 0) + (bias ? 1 : 0)) + (counts && a->tree_masks ? kTreeList * 12 : 0);
+  if (a->dtype == 0) launch_logits<Bf16>(p, l);
+  else if (a->dtype == 1) launch_logits<Fp16>(p, l);
+  else launch_logits<float>(p, l);
   ASPIRE_CHECK_LAUNCH();
   return ASPIRE_OK;
 }
