@@ -9,7 +9,6 @@
 // HBM bounds it at batch sizes (logits once in, once out, and an eighth of a byte of mask a token); history is
 // read once a chunk, from L2.
 #include <algorithm>
-#include <type_traits>
 
 #include "common.h"
 
@@ -31,16 +30,19 @@ struct Bf16 {};
 struct Fp16 {};
 template <> struct Pack<Bf16> {
   typedef uint16_t raw;
+  static constexpr bool kLean = true;  // fits in 64 registers with two vectors a thread
   static __device__ __forceinline__ float up(raw x) { return __uint_as_float(uint32_t(x) << 16); }
   static __device__ __forceinline__ raw down(float x) { return __builtin_bit_cast(uint16_t, static_cast<__bf16>(x)); }
 };
 template <> struct Pack<Fp16> {
   typedef uint16_t raw;
+  static constexpr bool kLean = false;
   static __device__ __forceinline__ float up(raw x) { return float(__builtin_bit_cast(_Float16, x)); }
   static __device__ __forceinline__ raw down(float x) { return __builtin_bit_cast(uint16_t, static_cast<_Float16>(x)); }
 };
 template <> struct Pack<float> {
   typedef float raw;
+  static constexpr bool kLean = false;
   static __device__ __forceinline__ float up(raw x) { return x; }
   static __device__ __forceinline__ raw down(float x) { return x; }
 };
@@ -50,7 +52,7 @@ template <typename R, int n> struct __attribute__((packed, aligned(sizeof(R)))) 
 
 // A workgroup's chunk is kJ vectors a thread.
 template <typename T, int kJ, bool kCounts, bool kBias, bool kMask>
-__global__ __launch_bounds__(kLogitThreads, kJ == 1 || std::is_same<T, Bf16>::value ? 8 : 6) void adjust_logits_kernel(LogitsParams p) {
+__global__ __launch_bounds__(kLogitThreads, kJ == 1 || Pack<T>::kLean ? 8 : 6) void adjust_logits_kernel(LogitsParams p) {
   typedef typename Pack<T>::raw R;
   constexpr int kChunk = kJ * kVec * kLogitThreads;
   extern __shared__ uint4 logits_lds[];
