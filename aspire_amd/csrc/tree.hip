@@ -31,6 +31,7 @@ namespace {
 constexpr float kNegInfT = -__builtin_huge_valf();
 constexpr float kSlack = 8.f;       // log2 units
 constexpr int kStepKeys = 32;
+constexpr int kWaves = 4;           // of a workgroup
 constexpr int kStartCost = 4;       // a piece's start and end, in steps
 constexpr int kMinPart = 4;         // the least that a group takes, in steps
 constexpr int kTreeGroups = 256;    // workgroups of a launch: one a CU
@@ -147,7 +148,6 @@ struct TreeWave {
   int kidx[kC], vidx[(kJ + 1) / 2];
   float scale_log2;
   uint4 qf[kT][kC];
-  const int64_t* words[kT];
   float mx[kT], use[kT], l[kT];
   f32x4 acc[kT][kJ];
   f32x4 sc[kT][2];
@@ -176,14 +176,13 @@ struct TreeWave {
       const uint16_t* const src = static_cast<const uint16_t*>(a.q) + int64_t(q0 + node) * a.q_stride_t + int64_t(head) * a.q_stride_h;
 #pragma unroll
       for (int c = 0; c < kC; ++c) qf[t][c] = *reinterpret_cast<const uint4*>(src + 32 * c + 8 * grp);
-      words[t] = a.masks + int64_t(q0 + node) * a.mask_stride;
       mx[t] = kNegInfT, use[t] = 0.f, l[t] = 0.f;
 #pragma unroll
       for (int i = 0; i < kJ; ++i) acc[t][i] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
   }
   // Bits of the 32 keys from key0 on that each row sees, of `there` that are left; off: key0's place among the tree's tokens.
-  __device__ __forceinline__ void see(int off, int there, bool page0, bool page1, int mask_words) {
+  __device__ __forceinline__ void see(const TreeParams& p, int q0, int row0, int last, int off, int there, bool page0, bool page1) {
     uint32_t limit = there >= 32 ? ~0u : (1u << max(there, 0)) - 1;
     if (!page0) limit &= 0xffff0000u;
     if (!page1) limit &= 0xffffu;
@@ -191,9 +190,10 @@ struct TreeWave {
     for (int t = 0; t < kT; ++t) {
       uint32_t bits = ~0u;
       if (off > -32) {
+        const int64_t* const words = p.a.masks + int64_t(q0 + min(row0 + t * 16 + r, last) / p.group) * p.a.mask_stride;
         const int w = max(off, 0) >> 6, sh = max(off, 0) & 63;
-        uint64_t x = w < mask_words ? uint64_t(words[t][w]) >> sh : 0;
-        if (sh > 32 && w + 1 < mask_words) x |= uint64_t(words[t][w + 1]) << (64 - sh);
+        uint64_t x = w < p.a.mask_words ? uint64_t(words[w]) >> sh : 0;
+        if (sh > 32 && w + 1 < p.a.mask_words) x |= uint64_t(words[w + 1]) << (64 - sh);
         bits = off < 0 ? (uint32_t(x) << -off) | ((1u << -off) - 1) : uint32_t(x);
       }
       vis[t] = bits & limit;
@@ -268,40 +268,30 @@ struct TreeWave {
       l[t] += ps[t];
     }
   }
-  template <bool kClean>
   __device__ __forceinline__ void product(const uint4* vb) {
     const char* const va = reinterpret_cast<const char*>(vb);
 #pragma unroll
     for (int i = 0; i < kJ; ++i) {
       const int off = vidx[i >> 1] * 16 + 8 * (i & 1);
-      uint2 wa = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(va + off)));
-      uint2 wb = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                               (__attribute__((address_space(3))) i16x4*)(va + kHalf * 16 + off)));
-      if (kClean) {
-        wa.x &= ~special<kF16>(wa.x), wa.y &= ~special<kF16>(wa.y);
-        wb.x &= ~special<kF16>(wb.x), wb.y &= ~special<kF16>(wb.y);
-      }
+      const uint2 wa = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(va + off)));
+      const uint2 wb = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                                     (__attribute__((address_space(3))) i16x4*)(va + kHalf * 16 + off)));
 #pragma unroll
       for (int t = 0; t < kT; ++t) acc[t][i] = mfma32<kF16>(make_uint4(wa.x, wa.y, wb.x, wb.y), pf[t], acc[t][i]);
     }
   }
-  // A key that some rows see and others do not may hold infinities or NaN, which a product with weight 0 would carry over: then
-  // they are taken out of the product and added for the rows that see them.
-  __device__ __forceinline__ void values(const uint4* vb, bool masked) {
+  // A key that some rows see and others do not may hold infinities or NaN in V, which a product with weight 0 would carry over. Such
+  // values are added for the rows that see them and put to 0 in LDS before the product.
+  __device__ __forceinline__ bool has_special(const uint4* vb) const {
     bool bad = false;
-    if (masked) {
 #pragma unroll
-      for (int i = 0; i < 2 * kLoads; ++i) {
-        const uint4 x = vb[i * 64 + 16 * grp + r];
-        bad |= (special<kF16>(x.x) | special<kF16>(x.y) | special<kF16>(x.z) | special<kF16>(x.w)) != 0;
-      }
-      bad = __builtin_amdgcn_ballot_w64(bad) != 0;
+    for (int i = 0; i < 2 * kLoads; ++i) {
+      const uint4 x = vb[i * 64 + 16 * grp + r];
+      bad |= (special<kF16>(x.x) | special<kF16>(x.y) | special<kF16>(x.z) | special<kF16>(x.w)) != 0;
     }
-    if (!bad) {
-      product<false>(vb);
-      return;
-    }
-    product<true>(vb);
+    return bad;
+  }
+  __device__ __forceinline__ void add_special(const uint4* vb) {
     const char* const va = reinterpret_cast<const char*>(vb);
     for (int key = 0; key < kStepKeys; ++key) {
       const int row = key & 15, e = (key & 3) + 4 * (key >> 4), from = r + 16 * (row >> 2);
@@ -331,23 +321,31 @@ struct TreeWave {
       }
     }
   }
+  __device__ __forceinline__ void clear_special(uint4* vb) const {
+#pragma unroll
+    for (int i = 0; i < 2 * kLoads; ++i) {
+      uint4 x = vb[i * 64 + 16 * grp + r];
+      x.x &= ~special<kF16>(x.x), x.y &= ~special<kF16>(x.y), x.z &= ~special<kF16>(x.z), x.w &= ~special<kF16>(x.w);
+      vb[i * 64 + 16 * grp + r] = x;
+    }
+  }
 };
 
-// A workgroup's four waves (eight for kRW = 8) are kRW row groups (16 kT query rows each) times kKW key groups: a stage is 32 keys for
-// each key group.
+// A workgroup's four waves are kRW row groups (16 kT query rows each) times kKW = 4 / kRW key groups: a stage is 32 keys for each
+// key group.
 //   kRW = 1: every wave has all rows and every fourth step in an LDS ring of two of its own. No barrier on the way: K is
 //     refilled, two steps ahead, once its fragments have been read, V once its have.
-//   kRW = 2, 4, 8: the waves of a key group share its keys; kStages stages in LDS, one barrier a stage, loads kStages - 1 stages
-//     ahead.
-constexpr int tree_waves(int row_groups) { return row_groups == 8 ? 8 : 4; }
-
+//   kRW = 2, 4: the waves of a key group share its keys; kStages stages in LDS, one barrier a stage, loads kStages - 1 stages
+//     ahead, two workgroups a CU. (Tiles of 256 rows on eight waves halve the reads of shared keys but take 165 us where four
+//     waves take 146, trees of up to 190 nodes, 40 / 8 heads; half of the eight meeting the barrier half a stage later, 169;
+//     three workgroups of three stages at 168 registers 185.)
 template <bool kF16, int kD, int kT, int kRW, bool kOnce>
-__global__ __launch_bounds__(64 * tree_waves(kRW)) __attribute__((amdgpu_waves_per_eu(kRW == 1 ? 1 : 2))) void tree_attention_kernel(
+__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(kRW == 1 ? 1 : 2))) void tree_attention_kernel(
     TreeParams p) {
   typedef TreeWave<kF16, kD, kT> Wave;
-  constexpr int kWaves = tree_waves(kRW), kKW = kWaves / kRW, kGroupRows = 16 * kT, kRows = kGroupRows * kRW;
+  constexpr int kKW = kWaves / kRW, kGroupRows = 16 * kT, kRows = kGroupRows * kRW;
   constexpr int kHalf = Wave::kHalf, kLoads = Wave::kLoads, kJ = Wave::kJ;
-  constexpr int kStages = kKW == 1 ? 4 : 2;
+  constexpr int kStages = kRW == 4 ? 4 : 2;
   constexpr int kStage = kKW * 4 * kHalf;  // chunks: for each key group K of 32 keys, then V
   // separate objects, so that the compiler can tell a load into one from a read of another
   __shared__ uint4 st0[kRW == 1 ? 8 * kHalf : kStage];   // kRW = 1: K of the rings' first places
@@ -392,17 +390,19 @@ __global__ __launch_bounds__(64 * tree_waves(kRW)) __attribute__((amdgpu_waves_p
   at = wave_uniform64(at);
 
   const int row_bytes = int(a.cache_stride_t) * 2;
-  const char* const cache = static_cast<const char*>(a.kv_cache) + int64_t(g) * a.cache_stride_h * 2;
+  const char* const k_base = static_cast<const char*>(a.kv_cache) + int64_t(g) * a.cache_stride_h * 2;
+  const char* const v_base = k_base + a.cache_stride_kv * 2;
+  const uint32_t page_bytes = uint32_t(a.cache_stride_p) * 2u, sub_bytes = uint32_t(row_bytes) * 16u;  // below 2^32 (checked on the host)
+  const int sub_mask = (1 << p.page_shift) - 1;
   const uint32_t num_entries = p.num_entries, num_pages = p.num_pages;
-  // This lane's chunks of 16 keys: the ones that belong at its places in LDS. Of eight waves each loads half of them.
-  constexpr int kPart = kWaves == 8 ? kLoads / 2 : kLoads;
-  const int part0 = kWaves == 8 ? (wave >> 2) * kPart : 0;
-  int voff_k[kPart], voff_v[kPart];
+  // This lane's chunks of 16 keys: the ones that belong at its places in LDS. With kRW > 1 a wave loads K or V alone.
+  const bool loads_v = kRW > 1 && (wave & 1);
+  int voff_k[kLoads], voff_v[kRW == 1 ? kLoads : 1];
 #pragma unroll
-  for (int i = 0; i < kPart; ++i) {
-    const int row = Wave::kPerLoad * (part0 + i) + lane / Wave::kChunks, c = lane % Wave::kChunks;
-    voff_k[i] = row * row_bytes + (c ^ Wave::swizzle_k(row)) * 16;
-    voff_v[i] = row * row_bytes + (c ^ Wave::swizzle_v(row)) * 16;
+  for (int i = 0; i < kLoads; ++i) {
+    const int row = Wave::kPerLoad * i + lane / Wave::kChunks, c = lane % Wave::kChunks;
+    voff_k[i] = row * row_bytes + (c ^ (loads_v ? Wave::swizzle_v(row) : Wave::swizzle_k(row))) * 16;
+    if (kRW == 1) voff_v[i] = row * row_bytes + (c ^ Wave::swizzle_v(row)) * 16;
   }
   Wave w;
   w.init(lane, p.scale_log2);
@@ -441,18 +441,16 @@ __global__ __launch_bounds__(64 * tree_waves(kRW)) __attribute__((amdgpu_waves_p
         return there ? id : -1;
       };
       const auto issue = [&](uint4* dst, int step, int h, int id, bool v) {
-        const int sub = (2 * step + h) & ((1 << p.page_shift) - 1);
-        const int valid = id < 0 ? 0 : min(max(len - (2 * step + h) * 16, 0), 16);
-        const int span = wave_uniform(valid > 0 ? (valid - 1) * row_bytes + 2 * kD : 0);
-        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
-            const_cast<char*>(tree_uniform(cache + (int64_t(max(id, 0)) * a.cache_stride_p + (v ? a.cache_stride_kv : 0)) * 2 +
-                                           int64_t(sub) * 16 * row_bytes)), (short)0, span, kTreeBuffer);
+        const int half = 2 * step + h, left = len - half * 16;
+        const int span = wave_uniform(id < 0 ? 0 : left >= 16 ? 15 * row_bytes + 2 * kD : left > 0 ? (left - 1) * row_bytes + 2 * kD : 0);
+        const char* const at = (v ? v_base : k_base) + uint64_t(uint32_t(max(id, 0))) * page_bytes + uint32_t(half & sub_mask) * sub_bytes;
+        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(tree_uniform(at)), (short)0, span, kTreeBuffer);
 #pragma unroll
-        for (int i = 0; i < kPart; ++i) load_to_lds<kOnce>(rs, dst + (part0 + i) * 64, v ? voff_v[i] : voff_k[i]);
+        for (int i = 0; i < kLoads; ++i) load_to_lds<kOnce>(rs, dst + i * 64, kRW == 1 && v ? voff_v[kRW == 1 ? i : 0] : voff_k[i]);
       };
       const auto masked_step = [&](int step, bool page0, bool page1) {
         const bool masked = (step + 1) * kStepKeys > tree_start || !page0 || !page1;
-        if (masked) w.see(step * kStepKeys - tree_start, len - step * kStepKeys, page0, page1, a.mask_words);
+        if (masked) w.see(p, q0, row0, last, step * kStepKeys - tree_start, len - step * kStepKeys, page0, page1);
         return masked;
       };
 
@@ -488,7 +486,14 @@ __global__ __launch_bounds__(64 * tree_waves(kRW)) __attribute__((amdgpu_waves_p
             if (s < end) w.softmax(masked);
             __builtin_amdgcn_s_waitcnt(kWait);  // vmcnt: V has landed
             asm volatile("" ::: "memory");
-            if (s < end) w.values(vb, masked);
+            if (s < end) {
+              // (a step in front of the tree has no key that rows see differently)
+              if ((s + 1) * kStepKeys > tree_start && __builtin_amdgcn_ballot_w64(w.has_special(vb)) != 0) {
+                w.add_special(vb);
+                w.clear_special(vb);
+              }
+              w.product(vb);
+            }
             issue(vb, far, 0, n0, true), issue(vb + kHalf, far, 1, n1, true);
             id0 = n0, id1 = n1;
           };
@@ -498,14 +503,13 @@ __global__ __launch_bounds__(64 * tree_waves(kRW)) __attribute__((amdgpu_waves_p
           }
         }
       } else {
-        // Stage t holds the steps begin + kKW t + (0 .. kKW - 1). A wave loads one kind of its key group's: K or V (kKW = 2), or a
-        // half or a quarter of them (kKW = 1).
+        // Stage t holds the steps begin + kKW t + (0 .. kKW - 1). A wave loads one kind of its key group's: K or V (kKW = 2), or
+        // half of them (kKW = 1).
         const int lh = (wave >> 1) & 1, kind = wave & 1;
-        constexpr int kMine = kKW == 2 ? 2 * kLoads : 4 * kLoads / kWaves;  // its loads of a stage
-        constexpr int kAhead = (kStages - 2) * kMine;       // loads behind the next stage's
+        constexpr int kMine = kKW == 2 ? 2 * kLoads : kLoads;  // its loads of a stage
+        constexpr int kAhead = (kStages - 2) * kMine;          // loads behind the next stage's
         constexpr int kWait = 0x70 | (kAhead & 15) | ((kAhead >> 4) << 14);  // vmcnt, and lgkmcnt(0): its reads of the last stage
         const int stages = (end - begin + kKW - 1) / kKW;
-        uint4* const buf[4] = {st0, st1, st2, st3};
         const auto step_of = [&](int t) { return begin + t * kKW + kw; };
         uint32_t there = 0;  // two bits a stage: whether its halves have pages, the last one that was loaded lowest
         const auto load = [&](uint4* stage, int t, int raw0, int raw1) {
@@ -518,8 +522,9 @@ __global__ __launch_bounds__(64 * tree_waves(kRW)) __attribute__((amdgpu_waves_p
             issue(dst + lh * kHalf, s, lh, lh ? id1 : id0, kind);
           }
         };
-#pragma unroll
-        for (int t = 0; t < kStages - 1; ++t) load(buf[t], t, raw(step_of(t), 0), raw(step_of(t), 1));
+        const auto begin_stage = [&](uint4* stage, int t) { load(stage, t, raw(step_of(t), 0), raw(step_of(t), 1)); };
+        begin_stage(st0, 0);
+        if constexpr (kStages > 2) begin_stage(st1, 1), begin_stage(st2, 2);
         int next0 = raw(step_of(kStages - 1), 0), next1 = raw(step_of(kStages - 1), 1);
         const bool has_rows = row0 <= last;
         const auto body = [&](int t, uint4* cur, uint4* fill) {
@@ -530,18 +535,38 @@ __global__ __launch_bounds__(64 * tree_waves(kRW)) __attribute__((amdgpu_waves_p
           load(fill, t + kStages - 1, next0, next1);
           next0 = raw(step_of(t + kStages), 0), next1 = raw(step_of(t + kStages), 1);
           const int s = step_of(t);
-          if (s < end && has_rows) {
-            const uint4* const kb = cur + kw * 4 * kHalf;
+          uint4* const kb = cur + kw * 4 * kHalf;
+          const bool computes = s < end && has_rows;
+          bool bad = false;
+          if ((begin + (t + 1) * kKW) * kStepKeys > tree_start)  // every wave's: the stage reaches into the tree
+            bad = __syncthreads_or(w.has_special(kb + 2 * kHalf)) != 0;
+          if (computes) {
             const uint32_t mine = there >> (2 * (kStages - 1));
             const bool masked = masked_step(s, mine & 1, mine & 2);
             w.scores(kb);
             w.softmax(masked);
-            w.values(kb + 2 * kHalf, masked);
           }
+          if (bad) {
+            if (computes) w.add_special(kb + 2 * kHalf);
+            __syncthreads();
+            w.clear_special(kb + 2 * kHalf);  // (waves of a key group write the same)
+            __syncthreads();
+          }
+          if (computes) w.product(kb + 2 * kHalf);
         };
-        for (int t = 0; t < stages; t += kStages) {
-#pragma unroll
-          for (int u = 0; u < kStages; ++u) body(t + u, buf[u], buf[(u + kStages - 1) % kStages]);
+        // Stage by stage, and back to the top only from the last place: waits are counted by the order of the loads. (The places
+        // are named, not indexed.)
+        int t = 0;
+        const auto next = [&](uint4* cur, uint4* fill) {
+          body(t, cur, fill);
+          return ++t < stages;
+        };
+        if (stages > 0) {
+          if constexpr (kStages == 2) {
+            while (next(st0, st1) && next(st1, st0)) {}
+          } else {
+            while (next(st0, st3) && next(st1, st0) && next(st2, st1) && next(st3, st2)) {}
+          }
         }
       }
 
@@ -730,8 +755,8 @@ struct TreeChoice {
 TreeChoice choose(int tokens, int rows, int hq, int hkv) {
   // the smallest tile that holds a mean request's query rows
   const int64_t mean = (int64_t(tokens) + rows - 1) / rows * (hq / hkv);
-  TreeChoice c{mean <= 16 ? 1 : 2, mean <= 32 ? 1 : mean <= 64 ? 2 : mean <= 128 ? 4 : 8, 0, mean <= 128};
-  c.groups = std::max(1, (c.row_groups == 1 || c.row_groups == 8 ? 1 : 2) * kTreeGroups / hkv);
+  TreeChoice c{mean <= 16 ? 1 : 2, mean <= 32 ? 1 : mean <= 64 ? 2 : 4, 0, mean <= 128};
+  c.groups = std::max(1, (c.row_groups == 1 ? 1 : 2) * kTreeGroups / hkv);
   return c;
 }
 template <bool kF16, int kD>
@@ -740,8 +765,8 @@ void launch(const TreeParams& p, TreeChoice c, hipStream_t s) {
   if (c.tiles == 1) tree_attention_kernel<kF16, kD, 1, 1, true><<<wgs, 256, 0, s>>>(p);
   else if (c.row_groups == 1) tree_attention_kernel<kF16, kD, 2, 1, true><<<wgs, 256, 0, s>>>(p);
   else if (c.row_groups == 2) tree_attention_kernel<kF16, kD, 2, 2, true><<<wgs, 256, 0, s>>>(p);
-  else if (c.row_groups == 4) tree_attention_kernel<kF16, kD, 2, 4, true><<<wgs, 256, 0, s>>>(p);
-  else tree_attention_kernel<kF16, kD, 2, 8, false><<<wgs, 512, 0, s>>>(p);
+  else if (c.once) tree_attention_kernel<kF16, kD, 2, 4, true><<<wgs, 256, 0, s>>>(p);
+  else tree_attention_kernel<kF16, kD, 2, 4, false><<<wgs, 256, 0, s>>>(p);
   if (c.rows() <= 32) tree_join_kernel<kF16, kD, 1><<<dim3(wgs, c.rows() / 4), 256, 0, s>>>(p, c.rows());
   else tree_join_kernel<kF16, kD, 4><<<dim3(wgs, c.rows() / 16), 256, 0, s>>>(p, c.rows());
 }
@@ -775,7 +800,8 @@ extern "C" int aspire_tree_attention(const aspire_tree_attention_args* a, void* 
   if (a->tokens == 0 || a->rows == 0) return ASPIRE_OK;
   ASPIRE_CHECK_ARG(a->q && a->out && a->qo_indptr && a->kv_indptr && a->kv_last_page_len && (a->masks || a->mask_words == 0), "null array");
   ASPIRE_CHECK_ARG(a->num_pages > 0 && a->num_page_indices > 0 && a->kv_cache && a->kv_indices, "no pages");
-  ASPIRE_CHECK_ARG(a->cache_stride_t >= a->head_dim && a->cache_stride_t < (int64_t(1) << 26), "tokens of a page must lie head_dim to 2^26 - 1 values apart");
+  ASPIRE_CHECK_ARG(a->cache_stride_t >= a->head_dim && a->cache_stride_t < (1 << 20), "tokens of a page must lie head_dim to 2^20 - 1 values apart");
+  ASPIRE_CHECK_ARG(a->cache_stride_p >= 0 && a->cache_stride_p < (int64_t(1) << 31), "pages must lie less than 2^31 values apart");
   const auto aligned = [](const void* ptr, std::initializer_list<int64_t> strides) {
     int64_t bits = static_cast<int64_t>(reinterpret_cast<uintptr_t>(ptr)) / 2 % 8;
     for (int64_t s : strides) bits |= s;
