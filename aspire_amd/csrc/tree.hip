@@ -21,7 +21,6 @@
 #include <algorithm>
 #include <cmath>
 #include <initializer_list>
-#include <type_traits>
 
 #include "common.h"
 
@@ -91,7 +90,8 @@ __device__ __forceinline__ int64_t wave_uniform64(int64_t v) {
 }
 
 // 16 bytes a lane from its offset into the buffer to the lane's place behind dst; once: keys that no other workgroup reads
-// (non-temporal: 32 x 32,768 tokens 735 -> 658 us, but 164 -> 222 where seven tiles share them).
+// (non-temporal: 32 requests of 32,768 keys 737 -> 665 us; the loads alone of tiles that share keys, seven to a request, 164 ->
+// 222).
 template <bool kOnce>
 __device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t rs, uint4* dst, int offset);
 template <>
@@ -414,7 +414,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(kRW
     const int total_rows = n * G, tiles = (total_rows + kRows - 1) / kRows, steps = (len + kStepKeys - 1) / kStepKeys;
     const int unit = steps + kStartCost, tree_start = len - n;
     // the first tile that reaches into this group's part
-    int m = wave_uniform(at >= line0 ? 0 : int((line0 - at) / unit));
+    int m = wave_uniform(at >= line0 ? 0 : int(min((line0 - at) / unit, int64_t(tiles))));
     typedef const __attribute__((address_space(4))) int32_t* const_ids_t;
     const const_ids_t ids = (const_ids_t)a.kv_indices;
     for (; m < tiles; ++m) {
@@ -428,9 +428,8 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(kRW
       const int row0 = m * kRows + rw * kGroupRows, last = total_rows - 1;  // this wave's rows
       w.start(p, q0, row0, last, g);
 
-      // The page of 16 keys: half h of a step. raw() only loads it (a scalar load, used a step later: to wait for four of them where
-      // they are issued took a third of a step), page() is -1 on a page that the pool does not have, or past the end: such
-      // halves load nothing. Out-of-range loads write zeros into LDS, and every step issues the same loads.
+      // The page of 16 keys: half h of a step. raw() only loads it (a scalar load, used a step later), page() is -1 on a page that
+      // the pool does not have, or past the end: such halves load nothing. Out-of-range loads write zeros into LDS, and every step issues the same loads.
       const auto raw = [&](int step, int h) -> int {
         const uint32_t entry = uint32_t(list) + uint32_t((2 * step + h) >> p.page_shift);
         return ids[min(entry, num_entries - 1)];
@@ -657,8 +656,9 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(kRW
         // the groups that hold the unit's other steps: the last one's part holds its last step
         const int64_t last_step = unit0 + unit - 1;
         int jl = int(last_step * groups / all);
-        while (all * (jl + 1) / groups <= last_step) ++jl;
-        while (all * jl / groups > last_step) --jl;
+        jl = min(max(jl, j), groups - 1);
+        while (jl < groups - 1 && all * (jl + 1) / groups <= last_step) ++jl;
+        while (jl > j && all * jl / groups > last_step) --jl;
         p.pieces[blockIdx.x] = make_int4(m * kRows, min(kRows, total_rows - m * kRows), q0, jl - j + 1);
       }
       if (kKW == 1) __builtin_amdgcn_s_waitcnt(0xf70);  // vmcnt(0): no load past the end meets the next unit's
@@ -768,7 +768,7 @@ void launch(const TreeParams& p, TreeChoice c, hipStream_t s) {
   else if (c.once) tree_attention_kernel<kF16, kD, 2, 4, true><<<wgs, 256, 0, s>>>(p);
   else tree_attention_kernel<kF16, kD, 2, 4, false><<<wgs, 256, 0, s>>>(p);
   if (c.rows() <= 32) tree_join_kernel<kF16, kD, 1><<<dim3(wgs, c.rows() / 4), 256, 0, s>>>(p, c.rows());
-  else tree_join_kernel<kF16, kD, 4><<<dim3(wgs, c.rows() / 16), 256, 0, s>>>(p, c.rows());
+  else tree_join_kernel<kF16, kD, 2><<<dim3(wgs, c.rows() / 8), 256, 0, s>>>(p, c.rows());
 }
 int64_t piece_bytes(int64_t workgroups) { return (workgroups * int64_t(sizeof(int4)) + 255) / 256 * 256; }
 
@@ -799,7 +799,8 @@ extern "C" int aspire_tree_attention(const aspire_tree_attention_args* a, void* 
   ASPIRE_CHECK_ARG(a->tokens <= (1 << 20) && a->rows <= (1 << 20), "more than 2^20 tokens or rows");
   if (a->tokens == 0 || a->rows == 0) return ASPIRE_OK;
   ASPIRE_CHECK_ARG(a->q && a->out && a->qo_indptr && a->kv_indptr && a->kv_last_page_len && (a->masks || a->mask_words == 0), "null array");
-  ASPIRE_CHECK_ARG(a->num_pages > 0 && a->num_page_indices > 0 && a->kv_cache && a->kv_indices, "no pages");
+  const bool none = a->num_pages == 0 || a->num_page_indices == 0;  // no page is there: no key is seen
+  ASPIRE_CHECK_ARG(none || (a->kv_cache && a->kv_indices), "null cache or list");
   ASPIRE_CHECK_ARG(a->cache_stride_t >= a->head_dim && a->cache_stride_t < (1 << 20), "tokens of a page must lie head_dim to 2^20 - 1 values apart");
   ASPIRE_CHECK_ARG(a->cache_stride_p >= 0 && a->cache_stride_p < (int64_t(1) << 31), "pages must lie less than 2^31 values apart");
   const auto aligned = [](const void* ptr, std::initializer_list<int64_t> strides) {
@@ -820,8 +821,9 @@ extern "C" int aspire_tree_attention(const aspire_tree_attention_args* a, void* 
   p.scale_log2 = a->sm_scale * 1.4426950408889634f;
   p.group = a->num_qo_heads / a->num_kv_heads;
   p.groups = c.groups;
-  p.num_entries = static_cast<uint32_t>(std::min<int64_t>(a->num_page_indices, 0x7fffffff));
-  p.num_pages = static_cast<uint32_t>(std::min<int64_t>(a->num_pages, 0x7fffffff));
+  if (none) p.a.kv_indices = a->qo_indptr;  // an entry to load; its value is no page's id
+  p.num_entries = none ? 1u : static_cast<uint32_t>(std::min<int64_t>(a->num_page_indices, 0x7fffffff));
+  p.num_pages = none ? 0u : static_cast<uint32_t>(std::min<int64_t>(a->num_pages, 0x7fffffff));
   while ((16 << p.page_shift) < a->page_size) ++p.page_shift;
   p.pieces = reinterpret_cast<int4*>(a->workspace);
   p.part_o = a->workspace + piece_bytes(wgs) / 4;

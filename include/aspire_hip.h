@@ -685,7 +685,8 @@ int aspire_step_tables(const aspire_step_tables_args* args, void* stream);
  * and of those key j where bit j of its words in masks [tokens, mask_words] is set. out = softmax(sm_scale q.k) v over
  * the keys that it sees, 0 where it sees none; lse (optional, fp32 [tokens, H_q]) base 2, -inf there. Keys on a page id
  * outside [0, num_pages) or an entry outside [0, num_page_indices) are not seen. Tokens of no row are left as they are.
- * dtype 0 bf16, 1 fp16; head_dim 64 or 128; page_size a power of two from 16; 16-byte aligned rows.
+ * dtype 0 bf16, 1 fp16; head_dim 64 or 128; page_size a power of two from 16 to 1,024; rows that start on 16 bytes; tokens and
+ * rows up to 2^20; a page's tokens less than 2^20 values apart, pages less than 2^31.
  * workspace: aspire_tree_attention_workspace floats. */
 typedef struct {
   const void* q; int64_t q_stride_t; int64_t q_stride_h;

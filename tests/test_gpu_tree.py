@@ -319,3 +319,28 @@ def test_refusals(gpu):
     empty = call(q=c.q[:0], tree_masks=c.masks[:0], qo_indptr=c.dev([0]), kv_page_indptr=c.dev([0]), kv_last_page_len=c.dev([]),
                  kv_page_indices=c.dev([]))
     assert empty.shape == (0, 8, 128)
+
+
+def test_no_pages_at_all(gpu):
+    say("tree attention no pages")
+    c = Case(gpu, [20], [4], 8, 2, 128)
+    for cache, ids in ((c.cache[:0], c.dev(c.ids)), (c.cache, c.dev([]))):
+        out, lse = tree_attention(c.q, cache, c.dev(c.qo), ids, c.dev(c.kvp), c.dev(c.last), c.masks, 16, return_lse=True)
+        assert (out == 0).all() and torch.isneginf(lse).all()
+
+
+def test_many_rows(gpu):
+    """More rows than a wave reads at once, most of them empty, and more than the chip has workgroups."""
+    say("tree attention many rows")
+    r = np.random.default_rng(0)
+    nodes = [int(n) for n in r.integers(0, 3, size=700)]
+    c = Case(gpu, [int(x) if n else 0 for x, n in zip(r.integers(0, 60, size=700), nodes)], nodes, 4, 1, 64)
+    c.check(*c.run())
+
+
+def test_out_whose_rows_share_memory(gpu):
+    say("tree attention out shared")
+    c = Case(gpu, [20], [4], 8, 2, 128)
+    for bad in (torch.zeros(1, 8, 128, dtype=BF, device=gpu).expand(4, -1, -1), torch.zeros(4, 1, 128, dtype=BF, device=gpu).expand(-1, 8, -1)):
+        with pytest.raises(ValueError, match="share memory"):
+            c.run(out=bad)
