@@ -67,9 +67,9 @@ def tree_attention(q: torch.Tensor, kv_cache: torch.Tensor, qo_indptr: torch.Ten
                    *, sm_scale: float | None = None, out: torch.Tensor | None = None, lse: torch.Tensor | None = None,
                    return_lse: bool = False):
     """Attention of the trees' tokens ``q`` ``[T, H_q, D]`` over ``kv_cache`` ``[P, 2, page, H_kv, D]`` (bf16 or fp16, D 64 or
-    128, pages of 16 to 1,024 tokens by powers of two), which holds them already: row ``b`` has tokens ``qo_indptr[b]`` to
-    ``qo_indptr[b + 1]`` and the pages ``kv_page_indices[kv_page_indptr[b] : kv_page_indptr[b + 1]]``, the last one filled to
-    ``kv_last_page_len[b]``; its last keys are its tokens'. ``tree_masks`` int64 ``[T, W]`` has bit ``j % 64`` of word ``j // 64``
+    128, pages of 16 to 1,024 tokens by powers of two; up to 2^20 tokens and rows), which holds them already: row ``b`` has
+    tokens ``qo_indptr[b]`` to ``qo_indptr[b + 1]`` and the pages ``kv_page_indices[kv_page_indptr[b] : kv_page_indptr[b + 1]]``,
+    the last one filled to ``kv_last_page_len[b]``; its last keys are its tokens'. ``tree_masks`` int64 ``[T, W]`` has bit ``j % 64`` of word ``j // 64``
     set where a token sees its row's token ``j`` (itself among them); all cached keys before the tree are seen.
 
     Returns ``out`` (new, or the tensor given; apart from q and the cache), with ``return_lse`` and the base-2 ``lse`` fp32
@@ -107,6 +107,8 @@ def tree_attention(q: torch.Tensor, kv_cache: torch.Tensor, qo_indptr: torch.Ten
     elif out.shape != shape or out.dtype is not dtype or out.get_device() != index or (os := _rows16(out)) is None:
         raise ValueError(f"{what}: out must be {dtype} of q's shape on {q.device} with 16-byte aligned heads")
     else:
+        if tokens > 1 and os[0] == 0 or hq > 1 and os[1] == 0 or not (out.is_contiguous() or _apart(shape, os)):
+            raise ValueError(f"{what}: the rows of out share memory")
         o0, o1 = _bytes(out, os)
         for t, st in ((q, qs), (kv_cache, c)):
             t0, t1 = _bytes(t, st)
@@ -135,7 +137,7 @@ def compact_accepted(kv_caches, path: torch.Tensor, kept: torch.Tensor, qo_indpt
     ``slots[qo_indptr[b] + path[b, j]]`` goes to ``slots[qo_indptr[b] + j]`` for ``j < kept[b]``, in every layer.
 
     ``kv_caches``: one cache ``[P, 2, page, H, D]``, all layers' as ``[L, P, 2, page, H, D]``, or a list of caches of one layout
-    (any element type; no two of a list the same memory). ``path`` int32 ``[B, M]`` and ``kept`` int32 ``[B]`` are what
+    (any element type; no two may share memory). ``path`` int32 ``[B, M]`` and ``kept`` int32 ``[B]`` are what
     ``verify_tree_speculation`` returns, ``slots`` int64 ``[T]`` what the step's tables hold. A path rises: entries that are not
     above their place, or not of the row, are passed over, and so are slots outside the cache."""
     what = "compact_accepted"
@@ -150,8 +152,6 @@ def compact_accepted(kv_caches, path: torch.Tensor, kept: torch.Tensor, qo_indpt
     cs, st, es, dtype = c.shape, c.stride(), c.element_size(), c.dtype
     if len(cs) == 6 and stacked:
         count, step, cs, st = cs[0], st[0] * es, cs[1:], st[1:]
-        if count > 1 and step < cs[0] * st[0] * es and not _apart(c):
-            raise ValueError(f"{what}: the layers share memory")
     else:
         count, step = len(layers), 0
     if len(cs) != 5 or cs[1] != 2 or (cs[4] > 1 and st[4] != 1) or cs[2] < 1:
@@ -167,9 +167,11 @@ def compact_accepted(kv_caches, path: torch.Tensor, kept: torch.Tensor, qo_indpt
         if any(t.shape != cs or t.stride() != st or t.dtype is not dtype for t in layers):
             raise ValueError(f"{what}: the caches must be of one layout and type")
         starts = [t.data_ptr() for t in layers]
-        if len(set(starts)) != len(starts) and c.numel():
-            raise ValueError(f"{what}: a cache is listed twice")
         table = (ctypes.c_uint64 * count)(*starts)
+        if count > 1 and c.numel() and not _starts_apart(starts, cs, st, es):
+            raise ValueError(f"{what}: the caches share memory")
+    if not (c.is_contiguous() or _apart(c.shape, c.stride())):
+        raise ValueError(f"{what}: parts of a cache share memory")
     if path.dim() != 2 or path.dtype is not torch.int32 or not path.is_contiguous():
         raise ValueError(f"{what}: path must be a contiguous int32 [B, M] tensor")
     kept, qo = _list(kept, index, what, "kept"), _list(qo_indptr, index, what, "qo_indptr")
@@ -185,14 +187,25 @@ def compact_accepted(kv_caches, path: torch.Tensor, kept: torch.Tensor, qo_indpt
     _lib.launch(_lib.lib().aspire_compact_accepted, args, index, what)
 
 
-def _apart(t: torch.Tensor) -> bool:
-    """Whether no two elements of a tensor share memory, by its dimensions in the order of their strides."""
+def _apart(shape, strides) -> bool:
+    """Whether no two elements share memory, by the dimensions in the order of their strides."""
     reach = 0
-    for s, n in sorted((s, n) for n, s in zip(t.shape, t.stride()) if n > 1):
+    for s, n in sorted((s, n) for n, s in zip(shape, strides) if n > 1):
         if s <= reach:
             return False
         reach += (n - 1) * s
     return True
+
+
+def _starts_apart(starts, shape, strides, es: int) -> bool:
+    """Whether tensors of one layout at these addresses share no memory: they lie behind each other, or interleaved at equal
+    distances (layers inside of pages)."""
+    starts = sorted(starts)
+    gaps = [b - a for a, b in zip(starts, starts[1:])]
+    least = min(gaps)
+    if least >= (1 + sum((n - 1) * s for n, s in zip(shape, strides))) * es:
+        return True
+    return max(gaps) == least and least > 0 and least % es == 0 and _apart((len(starts), *shape), (least // es, *strides))
 
 
 __all__ = ["HEAD_DIMS", "tree_attention", "compact_accepted"]

@@ -135,7 +135,7 @@ extern "C" int aspire_verify_tree(const int32_t* tree_tokens, const int32_t* par
                                   const int32_t* qo_indptr, int32_t tokens, int32_t rows, int32_t max_path, int32_t* output,
                                   int32_t* path, int32_t* kept, void* stream) {
   using namespace aspire;
-  ASPIRE_CHECK_ARG(tokens >= 0 && rows >= 0 && max_path >= 1, "bad sizes");
+  ASPIRE_CHECK_ARG(tokens >= 0 && rows >= 0 && max_path >= 1 && max_path <= (1 << 30), "bad sizes");
   ASPIRE_CHECK_ARG(rows <= (1 << 24), "more than 2^24 rows");
   if (rows == 0) return ASPIRE_OK;
   ASPIRE_CHECK_ARG(qo_indptr && output && path && kept && (tokens == 0 || (tree_tokens && parents && targets)), "null array");
@@ -149,7 +149,7 @@ extern "C" int aspire_compact_accepted(const aspire_compact_args* a, void* strea
   using namespace aspire;
   ASPIRE_CHECK_ARG(a != nullptr, "null arguments");
   ASPIRE_CHECK_ARG(a->layers >= 0 && a->heads >= 0 && a->head_bytes >= 0 && a->page_size > 0 && a->rows >= 0 &&
-                       a->tokens >= 0 && a->max_path >= 0 && a->num_pages >= 0, "bad sizes");
+                       a->tokens >= 0 && a->max_path >= 0 && a->max_path <= (1 << 30) && a->num_pages >= 0, "bad sizes");
   ASPIRE_CHECK_ARG(a->rows <= (1 << 22), "more than 2^22 rows");
   if (a->layers == 0 || a->heads == 0 || a->head_bytes == 0 || a->rows == 0 || a->max_path < 2 || a->tokens == 0 || a->num_pages == 0)
     return ASPIRE_OK;

@@ -122,8 +122,8 @@ def verify_tree_speculation(tree_tokens: torch.Tensor, parents: torch.Tensor, ta
     tokens, rows = tok.shape[0], qo.shape[0] - 1
     if par.shape[0] < tokens or tgt.shape[0] < tokens:
         raise ValueError(f"{what}: parents and target_ids need {tokens} entries")
-    if rows < 0 or max_path < 1 or rows * max_path >= 1 << 31:
-        raise ValueError(f"{what}: qo_indptr needs an entry more than rows, max_path at least 1, rows * max_path below 2^31")
+    if rows < 0 or not 1 <= max_path <= 1 << 30 or rows * max_path >= 1 << 31:
+        raise ValueError(f"{what}: qo_indptr needs an entry more than rows, max_path 1 to 2^30, rows * max_path below 2^31")
     device = tok.device
     output = torch.empty((rows, max_path), dtype=torch.int32, device=device)
     path = torch.empty((rows, max_path), dtype=torch.int32, device=device)

@@ -200,3 +200,15 @@ def test_refusals(gpu):
                  (c.clone().requires_grad_(), path, i(2), i(3), slots), (c.transpose(3, 4), path, i(2), i(3), slots)):
         with pytest.raises(ValueError):
             compact_accepted(*args)
+
+
+def test_shared_memory_is_refused(gpu):
+    say("compact shared memory")
+    path, kept = torch.zeros(1, 2, dtype=torch.int32, device=gpu), torch.zeros(1, dtype=torch.int32, device=gpu)
+    qo, slots = torch.zeros(2, dtype=torch.int32, device=gpu), torch.zeros(4, dtype=torch.int64, device=gpu)
+    c = torch.zeros(2, 4, 2, 16, 2, 8, device=gpu)
+    for caches in ([c[0, :3], c[0, 1:]], [c[0], c[0]], c[:1].expand(2, -1, -1, -1, -1, -1), c[0, :, :, :, :1].expand(-1, -1, -1, 2, -1)):
+        with pytest.raises(ValueError, match="share memory"):
+            compact_accepted(caches, path, kept, qo, slots)
+    compact_accepted([c[0], c[1]], path, kept, qo, slots)
+    compact_accepted(list(torch.zeros(4, 2, 2, 16, 2, 8, device=gpu).unbind(1)), path, kept, qo, slots)
