@@ -7,7 +7,9 @@
 // meanwhile. (Counts and biases kept in registers over the rows take 121 VGPRs, half the waves, and as long.) A token that the
 // tree drafts is counted on a row's own path where it is met. Chunks of low tokens, which histories and trees meet most, start first.
 // HBM bounds it at batch sizes (logits once in, once out, and an eighth of a byte of mask a token); history is
-// read once a chunk, from L2.
+// read once a chunk, from L2. Measured: 64 x 151,936 bf16 logits with histories and masks 14 us = 2.9 TB/s, the history's chain (lengths,
+// tokens, LDS) before the first store; 16 trees of up to 24 tokens over 128,257 with 20,000 tokens of history and 100 biases 46 us = 3.1
+// TB/s, of which counting takes its part and rows whose trees draft tokens of the chunk theirs; one row of 32,000 4.3 us, latency.
 #include <algorithm>
 
 #include "common.h"
@@ -296,7 +298,8 @@ extern "C" int aspire_adjust_logits(const aspire_adjust_logits_args* a, void* st
   const bool bias = a->bias_indptr != nullptr && a->bias_entries > 0;
   // Chunks of 8,192 tokens, or 4,096 with two tables in LDS (four workgroups a CU either way) or while longer ones leave fewer than two
   // workgroups a CU; then a request's rows are shared by several, eight rows or more each, up to eight workgroups a CU (a history is
-  // counted once a workgroup: 16 trees of 1 to 24 tokens, 128,257 logits, take 54 us without sharing, 59 with a third of the rows each).
+  // counted once a workgroup: 16 trees of 1 to 24 tokens, 128,257 logits, took 54 us
+  // unshared and 59 shared by three when that was measured).
   LogitsLaunch l{counts && bias ? 1 : 2, counts, bias, dim3(), 0, static_cast<hipStream_t>(stream)};
   const auto chunk = [&] { return l.vectors * kVec * kLogitThreads; };
   const auto chunks = [&] { return (int64_t(a->vocab) + chunk() - 1) / chunk(); };

@@ -17,7 +17,14 @@
 // group j of `groups` takes the j-th equal part of the line, for each kv head. A unit that falls to several groups is written as
 // fp32 pieces (each normalised by its own sum, with its base-2 LSE) and joined by a second launch in the order of its
 // keys: results do not depend on timing. The kv head runs fastest over the workgroups, so with 8 kv heads the
-// round-robin spread over the XCDs keeps each head's pages in one L2.
+// round-robin spread over the XCDs keeps each head's pages in one L2. (Equal pieces of one key range side by side, a piece a
+// workgroup, took 176 us instead of 145 for 5 requests of up to 190 tokens over 12,001, and 134 instead of 106 for 16 of up to 40
+// over 8,192; each head's pages on one XCD by hand, 782 instead of 735.)
+//
+// Measured, both launches: 32 requests of 16 tokens over 32,768 keys (32 / 8 heads of 128, 4.3 GB) 665 us = 6.5 TB/s, and the loads
+// alone 733 of 737 when that was the time: the stream into LDS bounds it, whatever the order of pages. 16 uneven trees of up to 40 over
+// 8,192 106 us; 5 of up to 190 over 12,001, 40 / 8 heads, 141 us = 480 TFLOP/s: tiles that share keys read them again from L2, and
+// softmax and products take turns. One tree of 8 over 2,048: 11 + 4 us, a chain of a few trips to memory in each launch.
 #include <algorithm>
 #include <cmath>
 #include <initializer_list>
@@ -669,7 +676,8 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(kRW
 }
 
 // Units cut into pieces: out = sum_i 2^(lse_i - m) o_i / sum_i 2^(lse_i - m), rounded once, in the order of the keys. Workgroup
-// (w, y) has rows of the unit that starts in workgroup w of the launch before and ends in another; a wave takes kTake rows, one after another in flight together; 64 / (kD / 8) pieces of a row at a time, kRound times.
+// (w, y) has rows of the unit that starts in workgroup w of the launch before and ends in another; a wave takes kTake rows at
+// once, 64 / (kD / 8) pieces of each at a time, kRound times. Latency bounds it, 3.5 to 11 us: the pieces' list, then their rows.
 template <bool kF16, int kD, int kTake>
 __global__ __launch_bounds__(256) void tree_join_kernel(TreeParams p, int tile_rows) {
   constexpr int kLanes = kD / 8, kAtOnce = 64 / kLanes, kRound = 2;
@@ -753,7 +761,10 @@ struct TreeChoice {
   int rows() const { return 16 * tiles * row_groups; }
 };
 TreeChoice choose(int tokens, int rows, int hq, int hkv) {
-  // the smallest tile that holds a mean request's query rows
+  // The smallest tile that holds a mean request's query rows. A larger one computes rows that are not there, a smaller one reads keys
+  // again for each tile. us with tiles of 16 / 32 / 64 / 128 rows: one request of 16 rows over 2,048 keys 19.1 / 20.3 / 20.1 / 21.5; 32 of
+  // 64 over 32,768: 2,555 / 1,290 / 665 / 688; 16 of about 80 over 8,192: 295 / 184 / 131 / 107; 5 of about 480 over 12,001: 673 / 336 /
+  // 226 / 143. Up to 32 rows a wave holds them all and goes by itself, one workgroup a CU; with more, two workgroups a CU.
   const int64_t mean = (int64_t(tokens) + rows - 1) / rows * (hq / hkv);
   TreeChoice c{mean <= 16 ? 1 : 2, mean <= 32 ? 1 : mean <= 64 ? 2 : 4, 0, mean <= 128};
   c.groups = std::max(1, (c.row_groups == 1 ? 1 : 2) * kTreeGroups / hkv);
@@ -767,6 +778,7 @@ void launch(const TreeParams& p, TreeChoice c, hipStream_t s) {
   else if (c.row_groups == 2) tree_attention_kernel<kF16, kD, 2, 2, true><<<wgs, 256, 0, s>>>(p);
   else if (c.once) tree_attention_kernel<kF16, kD, 2, 4, true><<<wgs, 256, 0, s>>>(p);
   else tree_attention_kernel<kF16, kD, 2, 4, false><<<wgs, 256, 0, s>>>(p);
+  // two rows a wave where there are many: 16 trees of up to 40 tokens 106.3 us, with one 107.5, with four 108.6
   if (c.rows() <= 32) tree_join_kernel<kF16, kD, 1><<<dim3(wgs, c.rows() / 4), 256, 0, s>>>(p, c.rows());
   else tree_join_kernel<kF16, kD, 2><<<dim3(wgs, c.rows() / 8), 256, 0, s>>>(p, c.rows());
 }
