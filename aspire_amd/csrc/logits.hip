@@ -298,8 +298,7 @@ extern "C" int aspire_adjust_logits(const aspire_adjust_logits_args* a, void* st
   const bool bias = a->bias_indptr != nullptr && a->bias_entries > 0;
   // Chunks of 8,192 tokens, or 4,096 with two tables in LDS (four workgroups a CU either way) or while longer ones leave fewer than two
   // workgroups a CU; then a request's rows are shared by several, eight rows or more each, up to eight workgroups a CU (a history is
-  // counted once a workgroup: 16 trees of 1 to 24 tokens, 128,257 logits, took 54 us
-  // unshared and 59 shared by three when that was measured).
+  // counted once a workgroup: 16 trees of up to 24 tokens, 128,257 logits, took 54 us so, 59 with four rows or more each, in one build).
   LogitsLaunch l{counts && bias ? 1 : 2, counts, bias, dim3(), 0, static_cast<hipStream_t>(stream)};
   const auto chunk = [&] { return l.vectors * kVec * kLogitThreads; };
   const auto chunks = [&] { return (int64_t(a->vocab) + chunk() - 1) / chunk(); };
