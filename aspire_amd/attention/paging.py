@@ -108,7 +108,8 @@ class StepTables:
         new token of a tree, the index in its row of the token that it continues, -1 for a root: positions are then
         ``cached + depth``. Tokens behind the last row get position and slot -1 and no bits; a page that the table does not have
         is -1. Rows without new tokens list no pages. From the first row on that does not fit (``max_tokens``,
-        ``max_entries``, or more than ``64 * tree_words`` tokens) no row has tokens or pages."""
+        ``max_entries``, or more than ``64 * tree_words`` tokens, with ``parents`` and no masks more than 4,096) no row has
+        tokens or pages."""
         what = "StepTables.build"
         index = self._index
         if index < 0:

@@ -126,6 +126,7 @@ __global__ __launch_bounds__(kResizeThreads) void page_resize_kernel(aspire_page
 // Every workgroup takes the prefix sums of all rows for itself (a few thousand bytes from L2) instead of waiting for another
 // launch, then its share of the page entries and of the tokens.
 constexpr int kTableThreads = 256;
+constexpr int kLongestTree = 4096;
 constexpr int kParentWindow = 1024;  // parents before a workgroup's own tokens that are held in LDS
 
 __global__ __launch_bounds__(kTableThreads) void step_tables_kernel(aspire_step_tables_args a) {
@@ -150,6 +151,8 @@ __global__ __launch_bounds__(kTableThreads) void step_tables_kernel(aspire_step_
     sum.a += fresh;
     sum.b += pages_of(b, fresh);
   }
+  // a token walks up all its ancestors: without a mask's bound a tree's has one of its own
+  const int most = a.tree_words > 0 ? 64 * a.tree_words : a.parents != nullptr ? kLongestTree : 0x7fffffff;
   if (threadIdx.x == 0) first_out = a.rows;
   const Pair upto = block_scan<kTableThreads>(sum, sums, all);
   int64_t t = upto.a - sum.a, e = upto.b - sum.b;
@@ -160,7 +163,7 @@ __global__ __launch_bounds__(kTableThreads) void step_tables_kernel(aspire_step_
     pag[b] = int(min(e, int64_t(0x7fffffff)));
     t += fresh;
     e += pages_of(b, fresh);
-    if (t > a.max_tokens || e > a.max_entries || (a.tree_words > 0 && fresh > 64 * a.tree_words)) {
+    if (t > a.max_tokens || e > a.max_entries || fresh > most) {
       atomicMin(&first_out, b);
       for (int c = b + 1; c < row1; ++c) tok[c] = tok[b], pag[c] = pag[b];
       break;

@@ -667,8 +667,8 @@ int aspire_page_resize(const aspire_page_resize_args* args, void* stream);
  * page_size + offset of its place in the pages (-1 without a page). parents[t] is the index in its row of the
  * token that t continues, -1 (or any index that is not below t's own) for none; masks [max_tokens, tree_words] has bit j of a
  * token's words set for its row's token j among its ancestors and itself (NULL parents: a chain). Tokens behind the last
- * row have position and slot -1 and mask 0. From the first row on whose tokens pass max_tokens or 64 * tree_words, or
- * whose pages pass max_entries, no row has tokens or pages; totals = tokens and pages that all rows ask for, and that first
+ * row have position and slot -1 and mask 0. From the first row on whose tokens pass max_tokens or 64 * tree_words
+ * (with parents and no masks: that has more than 4,096), or whose pages pass max_entries, no row has tokens or pages; totals = tokens and pages that all rows ask for, and that first
  * row (rows: none). rows <= max_rows <= 4096, tree_words <= 64. */
 typedef struct {
   const int32_t* block_table; int64_t table_stride; const int32_t* cached; const int32_t* fresh; const int32_t* parents;

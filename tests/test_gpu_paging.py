@@ -133,6 +133,18 @@ def test_rows_that_do_not_fit(gpu):
     check_tables(t, table[:3], [0, 0, 0], [64, 65, 3], None)
 
 
+def test_longest_trees(gpu):
+    """A tree without masks has 4,096 tokens at most, a chain any number."""
+    say("tables of the longest trees")
+    table = dev(np.arange(2 * 600).reshape(2, 600), gpu)
+    for first, chain in ((4096, False), (4097, False), (4097, True)):
+        t = StepTables(2, 4400, 1200, 16, gpu)
+        parents = None if chain else np.r_[np.arange(-1, first - 1), [-1, 0, 0], np.zeros(4400 - first - 3, int)].astype(np.int32)
+        t.build(table, dev([5, 9], gpu), dev([first, 3], gpu), None if chain else dev(parents, gpu))
+        check_tables(t, table, [5, 9], [first, 3], parents)
+        assert int(t.totals[2]) == (0 if first > 4096 and not chain else 2)
+
+
 def test_odd_inputs(gpu):
     """Negative counts, sums past 2^31, tables that are too narrow or have holes, parents that are none."""
     say("tables of odd inputs")

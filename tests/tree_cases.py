@@ -125,9 +125,9 @@ def tables(table, cached, fresh, parents, page, max_rows, max_tokens, max_entrie
     need = [-(-(c + f) // page) if f else 0 for c, f in zip(cached, fresh)]
     qo, kvp, ids, last = [0], [0], [], [0] * max_rows
     positions, slots, masks = [-1] * max_tokens, [-1] * max_tokens, np.zeros((max_tokens, words), np.int64)
-    left = len(fresh)
+    left, most = len(fresh), 64 * words if words else 2 ** 31 if parents is None else 4096
     for b, (c, f, p) in enumerate(zip(cached, fresh, need)):
-        if left < b or qo[-1] + f > max_tokens or kvp[-1] + p > max_entries or (words and f > 64 * words):
+        if left < b or qo[-1] + f > max_tokens or kvp[-1] + p > max_entries or f > most:
             left = min(left, b)
             f = p = 0
         row = [table[b][i] if i < len(table[b]) else -1 for i in range(p)]
