@@ -159,7 +159,7 @@ struct TreeWave {
   f32x4 acc[kT][kJ];
   f32x4 sc[kT][2];
   uint4 pf[kT];
-  uint32_t vis[kT];
+  uint32_t vis[kT];  // of the present step, where it is masked (see) or has infinities or NaN to add (see_all)
 
   // LDS places: chunk c of a K row r is at c ^ swizzle_k(r), so that 16 rows' chunks c lie in different banks, and a V row's
   // where transpose reads of 4 rows do
@@ -205,6 +205,10 @@ struct TreeWave {
       }
       vis[t] = bits & limit;
     }
+  }
+  __device__ __forceinline__ void see_all() {
+#pragma unroll
+    for (int t = 0; t < kT; ++t) vis[t] = ~0u;
   }
   __device__ __forceinline__ void scores(const uint4* kb) {
 #pragma unroll
@@ -543,16 +547,18 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(kRW
           const int s = step_of(t);
           uint4* const kb = cur + kw * 4 * kHalf;
           const bool computes = s < end && has_rows;
-          bool bad = false;
+          bool bad = false, masked = false;
           if ((begin + (t + 1) * kKW) * kStepKeys > tree_start)  // every wave's: the stage reaches into the tree
             bad = __syncthreads_or(w.has_special(kb + 2 * kHalf)) != 0;
           if (computes) {
             const uint32_t mine = there >> (2 * (kStages - 1));
-            const bool masked = masked_step(s, mine & 1, mine & 2);
+            masked = masked_step(s, mine & 1, mine & 2);
             w.scores(kb);
             w.softmax(masked);
           }
           if (bad) {
+            // with two key groups one's step may lie in front of the tree that the stage reaches into: its rows see all of it
+            if (kKW > 1 && !masked) w.see_all();
             if (computes) w.add_special(kb + 2 * kHalf);
             __syncthreads();
             w.clear_special(kb + 2 * kHalf);  // (waves of a key group write the same)
