@@ -36,3 +36,20 @@ def same_attention(case, out, lse, scale=None):
         limit = np.where(blind[..., None], 0, attention_limit(ref, np.where(blind[..., None], 0, size), most, out.dtype, keys, ref.shape[2]))
         within(got, ref, limit, "out")
         within(got_lse, ref_lse, lse_limit(ref_lse, most, keys, ref.shape[2]), "lse")
+
+
+def same_logits(out, ref, touched, size, before):
+    """Adjusted logits against the definition (tree_cases.adjusted): half a step of the output's type, and 8 * 2^-24 of the largest
+    magnitude on the way (a quotient or product, the frequency's product and sum, presence and bias round once each); rows of no
+    request to the last bit. What is past the type's largest value is infinite, or that value where it lies that near."""
+    raw = lambda t: t.detach().contiguous().cpu().numpy() if t.dtype == torch.float32 else t.detach().contiguous().cpu().view(torch.int16).numpy()
+    assert np.array_equal(raw(out).view(np.uint8).reshape(*out.shape, -1)[~touched], raw(before).view(np.uint8).reshape(*out.shape, -1)[~touched])
+    got = out.detach().cpu().double().numpy()
+    big, half = float(torch.finfo(out.dtype).max), torch.finfo(out.dtype).eps / 2
+    ref, size = ref[touched], np.asarray(size)[touched]
+    with np.errstate(invalid="ignore"):
+        limit = half * np.abs(ref) + 8 * 2.0 ** -24 * size * (1 + half) + (2.0 ** -25 if out.dtype == torch.float16 else 0)
+    far = np.isfinite(ref) & (np.abs(ref) >= big * (1 - half))
+    got = got[touched]
+    got = np.where(far & np.isinf(got) & (np.sign(got) == np.sign(ref)), ref, got)
+    within(got, ref, limit, "logits")
