@@ -385,5 +385,11 @@ def dense(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
     return t if t.dtype == dtype and t.is_contiguous() else t.to(dtype).contiguous()
 
 
+def indices(t: torch.Tensor) -> torch.Tensor:
+    """Counts, lengths or indices as int32 in one piece. Of int64 ones those beyond int32 become its nearest value, which fits and
+    names nothing where they did not; their lower halves would be other, valid ones."""
+    return dense(t.clamp(-1 << 31, (1 << 31) - 1) if t.dtype is torch.int64 else t, torch.int32)
+
+
 def build_info() -> str:
     return lib().aspire_build_info().decode()

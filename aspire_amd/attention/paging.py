@@ -35,7 +35,7 @@ def _counts(t: torch.Tensor, length: int | None, index: int, what: str, name: st
     _lib.require_cuda(t, what=what)
     if t.dim() != 1 or t.dtype not in (torch.int32, torch.int64) or t.get_device() != index or (length is not None and t.shape[0] != length):
         raise ValueError(f"{what}: {name} must be int32 [{'requests' if length is None else length}] on cuda:{index}")
-    return _lib.dense(t, torch.int32)
+    return _lib.indices(t)
 
 
 class PagePool:

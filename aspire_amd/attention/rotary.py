@@ -167,7 +167,7 @@ class RotaryEmbedding:
         """An index array as int32 in one piece, and its length."""
         if t.dim() != 1 or t.get_device() != self._index or t.dtype not in _INTS:
             raise ValueError(f"{what}: the index arrays must be 1-D int32 on {self.device}")
-        t = _lib.dense(t, torch.int32)
+        t = _lib.indices(t)
         return t, t.shape[0]
 
     def _dtype(self, t: torch.Tensor, what: str) -> int:

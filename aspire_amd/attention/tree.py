@@ -33,7 +33,7 @@ def _list(t: torch.Tensor, index: int, what: str, name: str) -> torch.Tensor:
         return t
     if t.dim() != 1 or t.dtype not in (torch.int32, torch.int64) or t.get_device() != index:
         raise ValueError(f"{what}: {name} must be 1-D int32 on cuda:{index}")
-    return _lib.dense(t, torch.int32)
+    return _lib.indices(t)
 
 
 def _rows16(t: torch.Tensor):

@@ -117,7 +117,7 @@ def verify_tree_speculation(tree_tokens: torch.Tensor, parents: torch.Tensor, ta
                 _lib.require_cuda(t, what=what)
                 raise ValueError(f"{what}: {('tree_tokens', 'parents', 'target_ids', 'qo_indptr')[i]} must be 1-D int32 on "
                                  f"{tree_tokens.device}")
-            lists[i] = _lib.dense(t, torch.int32)
+            lists[i] = _lib.indices(t) if i in (1, 3) else _lib.dense(t, torch.int32)  # (ids of tokens lie below 2^31)
     tok, par, tgt, qo = lists
     tokens, rows = tok.shape[0], qo.shape[0] - 1
     if par.shape[0] < tokens or tgt.shape[0] < tokens:

@@ -183,7 +183,7 @@ def adjust_logits(logits: torch.Tensor, *, qo_indptr: torch.Tensor | None = None
         good = t.dim() == 1 and t.get_device() == index and (t.dtype == dtype or dtype is torch.int32 and t.dtype == torch.int64)
         if not good or length is not None and t.shape[0] != length or least is not None and t.shape[0] < least:
             raise ValueError(f"{what}: {name} must be {dtype} [{length if length is not None else f'at least {least or 0}'}] on {device}")
-        return _lib.dense(t, dtype)
+        return _lib.indices(t) if dtype is torch.int32 else _lib.dense(t, dtype)
 
     i32, f32 = torch.int32, torch.float32
     qo = vector(qo_indptr, "qo_indptr", i32, least=1)
