@@ -80,8 +80,9 @@ def tree_attention(q: torch.Tensor, kv_cache: torch.Tensor, qo_indptr: torch.Ten
     index, dtype, shape, cs = q.get_device(), q.dtype, q.shape, kv_cache.shape
     if index < 0:
         _lib.require_cuda(q, what=what)
-    if torch.is_grad_enabled() and (q.requires_grad or kv_cache.requires_grad) \
-            or forward_ad._current_level >= 0 and _lib.has_tangent(q, kv_cache, out):
+    if torch.is_grad_enabled() and (q.requires_grad or kv_cache.requires_grad or out is not None and out.requires_grad
+                                    or lse is not None and lse.requires_grad) \
+            or forward_ad._current_level >= 0 and _lib.has_tangent(q, kv_cache, out, lse):
         raise ValueError(f"{what}: not differentiable")
     code = _DTYPES.get(dtype)
     if code is None or len(shape) != 3 or shape[2] not in HEAD_DIMS or (qs := _rows16(q)) is None:

@@ -154,7 +154,9 @@ def adjust_logits(logits: torch.Tensor, *, qo_indptr: torch.Tensor | None = None
     index, shape, st, dtype = logits.get_device(), logits.shape, logits.stride(), logits.dtype
     if index < 0:
         _lib.require_cuda(logits, what=what)
-    if torch.is_grad_enabled() and logits.requires_grad or forward_ad._current_level >= 0 and _lib.has_tangent(logits, out):
+    floats = (logits, out, repetition, presence, frequency, None if bias is None else bias.values)
+    if torch.is_grad_enabled() and any([t is not None and t.requires_grad for t in floats]) \
+            or forward_ad._current_level >= 0 and _lib.has_tangent(*floats):
         raise ValueError(f"{what}: not differentiable")
     code = _LOGIT_DTYPES.get(dtype)
     if code is None or len(shape) != 2 or (shape[1] > 1 and st[1] != 1):
