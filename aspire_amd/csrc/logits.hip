@@ -52,6 +52,21 @@ template <> struct Pack<float> {
 // n values at any 2- or 4-byte aligned place, in one access
 template <typename R, int n> struct __attribute__((packed, aligned(sizeof(R)))) Vec { R v[n]; };
 
+// 1 / r = high + low: fma(x, high, x low) is x / r within half a step and 2^-46, for r from 2^-60 to 2^60 (beyond them, where the
+// parts leave the normal numbers, within a step, as the product with one rounded reciprocal is). high lies towards zero and low has its sign
+// and is not 0, so that infinite x stay so.
+// 16 trees over 128,257 logits, 64 requests over 151,936, us in a graph: one product 51.6 and 19.7, this 51.9 and 20.7, a division for each
+// value 56.6 and 20.4.
+__device__ __forceinline__ void reciprocal(float r, float& high, float& low) {
+  const float m = fabsf(r);
+  high = 1.f / m, low = m < __builtin_huge_valf() ? 0x1p-149f : 0.f;
+  if (m >= 0x1p-60f && m <= 0x1p60f) {
+    if (fmaf(-m, high, 1.f) < 0.f) high = __int_as_float(__float_as_int(high) - 1);
+    low = fmaxf(fmaf(-m, high, 1.f) * high, low);
+  }
+  high = copysignf(high, r), low = copysignf(low, r);
+}
+
 // A workgroup's chunk is kJ vectors a thread.
 template <typename T, int kJ, bool kCounts, bool kBias, bool kMask>
 __global__ __launch_bounds__(kLogitThreads, kJ == 1 || Pack<T>::kLean ? 8 : 6) void adjust_logits_kernel(LogitsParams p) {
@@ -103,12 +118,11 @@ __global__ __launch_bounds__(kLogitThreads, kJ == 1 || Pack<T>::kLean ? 8 : 6) v
   const bool tree = kCounts && a.tree_masks != nullptr;
   const int words = min(a.mask_words, (n + 63) / 64);  // of a row's mask that hold its request's tokens
   const bool listed = int64_t(row1 - row0) * words <= kTreeList;
-  float repetition = 1.f, inverse = 1.f, presence = 0.f, frequency = 0.f;
+  float repetition = 1.f, presence = 0.f, frequency = 0.f;
   if (kCounts) {
     if (a.repetition != nullptr) repetition = a.repetition[b];
     if (a.presence != nullptr) presence = a.presence[b];
     if (a.frequency != nullptr) frequency = a.frequency[b];
-    inverse = 1.f / repetition;  // (a product by it is off by one rounding more than the quotient)
     if (a.history != nullptr) {
       const int32_t* const history = a.history + b * a.history_stride;
       const int len = min(a.history_lens[b], a.history_len), told = a.prompt_lens != nullptr ? a.prompt_lens[b] : 0;
@@ -153,6 +167,8 @@ __global__ __launch_bounds__(kLogitThreads, kJ == 1 || Pack<T>::kLean ? 8 : 6) v
           paths[i] = uint64_t(a.tree_masks[(row0 + i / words) * a.mask_stride + i % words]);
     }
   }
+  float high = 1.f, low = 0.f;
+  if (kCounts) reciprocal(repetition, high, low);
   if (kBias) {
     const int last = min(a.bias_indptr[b + 1], a.bias_entries);
     for (int i = max(a.bias_indptr[b], 0) + threadIdx.x; i < last; i += kLogitThreads) {
@@ -161,7 +177,6 @@ __global__ __launch_bounds__(kLogitThreads, kJ == 1 || Pack<T>::kLean ? 8 : 6) v
     }
   }
   if (kCounts || kBias) __syncthreads();
-
   // the bits of word w of a row's path, and the drafted token of a node
   const auto path_word = [&](int row, int w) {
     const uint64_t bits = listed ? paths[(row - row0) * words + w] : uint64_t(a.tree_masks[row * a.mask_stride + w]);
@@ -186,7 +201,7 @@ __global__ __launch_bounds__(kLogitThreads, kJ == 1 || Pack<T>::kLean ? 8 : 6) v
   };
   const auto penalty = [&](float f, uint32_t c) {
     const uint32_t written = c & ~kPrompt;
-    const float seen = f * (f > 0.f ? inverse : repetition);
+    const float seen = f > 0.f ? fmaf(f, high, f * low) : f * repetition;
     f = c != 0 ? seen : f;
     return written != 0 ? (f - frequency * float(written)) - presence : f;
   };
