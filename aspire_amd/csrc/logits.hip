@@ -320,7 +320,8 @@ extern "C" int aspire_adjust_logits(const aspire_adjust_logits_args* a, void* st
   if (chunks() * a->requests < 512) l.vectors = 1;
   const int64_t wgs = chunks() * a->requests, mean = a->qo_indptr ? a->tokens / a->requests : 1;
   LogitsParams p{*a, static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({mean / 8, 2048 / wgs, 65535})))};
-  ASPIRE_CHECK_ARG(wgs <= (1 << 23), "vocabulary times requests too large");
+  // (a launch has less than 2^32 threads)
+  ASPIRE_CHECK_ARG(wgs < (int64_t(1) << 32) / kLogitThreads, "vocabulary times requests too large");
   l.grid = dim3(static_cast<uint32_t>(wgs), p.row_parts);
   l.lds = chunk() * 4 * ((counts ? 1 : 0) + (bias ? 1 : 0)) + (counts && a->tree_masks ? kTreeList * 12 : 0);
   if (a->dtype == 0) launch_logits<Bf16>(p, l);
