@@ -98,8 +98,8 @@ class StepTables:
         self.masks = torch.zeros(max_tokens, tree_words, **i64) if tree_words else None
         self.totals = torch.zeros(3, **i64)
         self.device, self._index = self.totals.device, self.totals.get_device()
-        self._outputs = tuple(_lib.ptr(t) or 0 for t in (self.qo_indptr, self.kv_indptr, self.kv_indices, self.last_page_len,
-                                                         self.positions, self.slots, self.masks, self.totals))
+        # the tensors, not their addresses: a copy of the object has its own
+        self._outputs = (self.qo_indptr, self.kv_indptr, self.kv_indices, self.last_page_len, self.positions, self.slots, self.masks, self.totals)
 
     def build(self, block_table: torch.Tensor, cached: torch.Tensor, new_tokens: torch.Tensor,
               parents: torch.Tensor | None = None) -> "StepTables":
@@ -131,7 +131,8 @@ class StepTables:
                 raise ValueError(f"{what}: parents needs {self.max_tokens} entries")
             at = parents.data_ptr()
         args = _TABLES.pack(block_table.data_ptr(), strides[0], cached.data_ptr(), new_tokens.data_ptr(), at, rows, shape[1],
-                            self.max_rows, self.max_tokens, self.max_entries, self.page_size, self.tree_words, 0, *self._outputs)
+                            self.max_rows, self.max_tokens, self.max_entries, self.page_size, self.tree_words, 0,
+                            *[0 if t is None else t.data_ptr() for t in self._outputs])
         _lib.launch(_lib.lib().aspire_step_tables, args, index, what)
         return self
 
