@@ -228,20 +228,27 @@ __global__ __launch_bounds__(kTableThreads) void step_tables_kernel(aspire_step_
         a.masks[int64_t(i) * a.tree_words + w] = bits == 64 ? ~int64_t(0) : (int64_t(1) << bits) - 1;
       }
     } else {
-      // up the ancestors, once for each word of the mask; an index that is not below its node's ends the walk
-      for (int w = 0; w < max(a.tree_words, 1); ++w) {
-        uint64_t bits = 0;
-        int up = node;
-        depth = -1;
-        while (up >= 0) {
-          ++depth;
-          if ((up >> 6) == w) bits |= uint64_t(1) << (up & 63);
-          const int j = tok[b] + up;
-          const int above = near ? window[j - first] : a.parents[j];
-          up = above < up ? above : -1;
-        }
-        if (w < a.tree_words) a.masks[int64_t(i) * a.tree_words + w] = int64_t(bits);
+      // Up the ancestors; an index that is not below its node's ends the walk. Indices fall on the way, so each word of the mask is
+      // written as the walk leaves it, zeros where it passes over one.
+      int64_t* const mask = a.tree_words > 0 ? a.masks + int64_t(i) * a.tree_words : nullptr;
+      int w = a.tree_words;  // words from here on are written, but for bits
+      uint64_t bits = 0;
+      const auto leave = [&](int to) {  // for word `to` (-1: the walk is over)
+        if (mask == nullptr) return;
+        if (w < a.tree_words) mask[w] = int64_t(bits);
+        for (int k = w - 1; k > to; --k) mask[k] = 0;
+        w = to, bits = 0;
+      };
+      depth = -1;
+      for (int up = node; up >= 0;) {
+        ++depth;
+        if ((up >> 6) != w) leave(up >> 6);
+        bits |= uint64_t(1) << (up & 63);
+        const int j = tok[b] + up;
+        const int above = near ? window[j - first] : a.parents[j];
+        up = above < up ? above : -1;
       }
+      leave(-1);
     }
     a.positions[i] = a.cached[b] + depth;
   }
