@@ -111,11 +111,14 @@ class LogitBias:
     def __init__(self, biases, device="cuda"):
         ids, values, ends = [], [], [0]
         for m in biases:
-            for token, value in sorted((m or {}).items()):
-                if not 0 <= int(token) < 1 << 31 or math.isnan(value):
-                    raise ValueError("LogitBias: tokens must be 0 to 2^31 - 1, values not NaN")
-                ids.append(int(token))
-                values.append(float(value))
+            start = len(ids)
+            for token, given, value in sorted(((int(t), t, float(v)) for t, v in (m or {}).items())):
+                if token != given or not 0 <= token < 1 << 31 or math.isnan(value):
+                    raise ValueError("LogitBias: tokens must be whole numbers from 0 to 2^31 - 1, values not NaN")
+                if len(ids) > start and ids[-1] == token:  # (keys that are not equal, tensors say, may name one token)
+                    raise ValueError(f"LogitBias: two values for token {token}")
+                ids.append(token)
+                values.append(value)
             ends.append(len(ids))
         self.requests = len(ends) - 1
         self.ids = torch.tensor(ids, dtype=torch.int32, device=device)
