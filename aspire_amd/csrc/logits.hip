@@ -112,7 +112,10 @@ __global__ __launch_bounds__(kLogitThreads, kJ == 1 || Pack<T>::kLean ? 8 : 6) v
   fetch(row0);
 
   if (kCounts || kBias) {
-    for (int i = threadIdx.x; i < (kChunk / 4) * ((kCounts ? 1 : 0) + (kBias ? 1 : 0)); i += kLogitThreads) logits_lds[i] = make_uint4(0, 0, 0, 0);
+    for (int i = threadIdx.x; i < (kChunk / 4) * ((kCounts ? 1 : 0) + (kBias ? 1 : 0)); i += kLogitThreads) {
+      const uint32_t none = kBias && i >= (kCounts ? kChunk / 4 : 0) ? 0x80000000u : 0u;  // a bias of -0 leaves every logit as it is
+      logits_lds[i] = make_uint4(none, none, none, none);
+    }
     __syncthreads();
   }
   const bool tree = kCounts && a.tree_masks != nullptr;
