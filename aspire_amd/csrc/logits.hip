@@ -55,14 +55,16 @@ template <typename R, int n> struct __attribute__((packed, aligned(sizeof(R)))) 
 // 1 / r = high + low: fma(x, high, x low) is x / r within half a step and 2^-46, for r from 2^-60 to 2^60 (beyond them, where the
 // parts leave the normal numbers, within a step, as the product with one rounded reciprocal is). high lies towards zero and low has its sign
 // and is not 0, so that infinite x stay so.
-// 16 trees over 128,257 logits, 64 requests over 151,936, us in a graph: one product 51.6 and 19.7, this 51.9 and 20.7, a division for each
+// 16 trees over 128,257 logits, 64 requests over 151,936, us in a graph: one product 51.6 and 19.8, this 51.6 and 20.6, a division for each
 // value 56.6 and 20.4.
 __device__ __forceinline__ void reciprocal(float r, float& high, float& low) {
   const float m = fabsf(r);
-  high = 1.f / m, low = m < __builtin_huge_valf() ? 0x1p-149f : 0.f;
   if (m >= 0x1p-60f && m <= 0x1p60f) {
-    if (fmaf(-m, high, 1.f) < 0.f) high = __int_as_float(__float_as_int(high) - 1);
-    low = fmaxf(fmaf(-m, high, 1.f) * high, low);
+    high = __builtin_amdgcn_rcpf(m);  // within a step: what it lacks is low's
+    if (fmaf(-m, high, 1.f) < 0.f) high = __int_as_float(__float_as_int(high) - 2);
+    low = fmaxf(fmaf(-m, high, 1.f) * high, 0x1p-149f);
+  } else {
+    high = 1.f / m, low = m < __builtin_huge_valf() ? 0x1p-149f : 0.f;
   }
   high = copysignf(high, r), low = copysignf(low, r);
 }
