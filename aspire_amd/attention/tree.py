@@ -72,10 +72,10 @@ def tree_attention(q: torch.Tensor, kv_cache: torch.Tensor, qo_indptr: torch.Ten
     the last one filled to ``kv_last_page_len[b]``; its last keys are its tokens'. ``tree_masks`` int64 ``[T, W]`` has bit ``j % 64`` of word ``j // 64``
     set where a token sees its row's token ``j`` (itself among them); all cached keys before the tree are seen.
 
-    Returns ``out`` (new, or the tensor given; apart from q and the cache), with ``return_lse`` and the base-2 ``lse`` fp32
-    ``[T, H_q]``. A token that sees no key gets zeros and ``-inf``. Keys that a token does not see do not touch it, whatever they
-    hold. Tokens of no row are left as they were. Sums and softmax are fp32; weights of keys are rounded to q's type for the
-    product with v. Not differentiable."""
+    Returns ``out``, with ``return_lse`` and the base-2 ``lse`` fp32 ``[T, H_q]``: new ones, or the tensors given, whose memory from
+    first to last value must lie apart from that of q, of the cache and of each other. A token that sees no key gets zeros and
+    ``-inf``. Keys that a token does not see do not touch it, whatever they hold. Tokens of no row are left as they were. Sums and
+    softmax are fp32; weights of keys are rounded to q's type for the product with v. Not differentiable."""
     what = "tree_attention"
     index, dtype, shape, cs = q.get_device(), q.dtype, q.shape, kv_cache.shape
     if index < 0:
@@ -118,6 +118,11 @@ def tree_attention(q: torch.Tensor, kv_cache: torch.Tensor, qo_indptr: torch.Ten
     if lse is not None:
         if lse.dtype is not torch.float32 or lse.shape != (tokens, hq) or lse.get_device() != index or not lse.is_contiguous():
             raise ValueError(f"{what}: lse must be a contiguous fp32 [T, H_q] tensor on {q.device}")
+        l0, l1 = _bytes(lse, lse.stride())
+        for t, st in ((q, qs), (kv_cache, c), (out, os)):
+            t0, t1 = _bytes(t, st)
+            if l0 < t1 and t0 < l1:
+                raise ValueError(f"{what}: lse must lie apart from q, the cache and out")
     elif return_lse:
         lse = torch.empty(tokens, hq, dtype=torch.float32, device=q.device)
     L, ws, at = _lib.lib(), None, 0
