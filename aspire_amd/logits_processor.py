@@ -232,6 +232,8 @@ def adjust_logits(logits: torch.Tensor, *, qo_indptr: torch.Tensor | None = None
     which = vector(grammar_rows, "grammar_rows", i32, least=tokens)
     if not 0 <= vocab_start <= (1 << 31) - vocab:
         raise ValueError(f"{what}: the shard's tokens must lie in 0 to 2^31 - 1")
+    if not words:  # no drafted token is on a path (and masks without words have no address)
+        tree = tree_masks = None
     at = lambda t: 0 if t is None else t.data_ptr()
     b = (None, None, None) if bias is None else (bias.ids, bias.values, bias.indptr)
     args = _ADJUST.pack(logits.data_ptr(), st[0], out.data_ptr(), os[0], at(qo), at(history), history_stride,
