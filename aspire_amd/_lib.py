@@ -348,28 +348,30 @@ def require_cuda(*tensors: torch.Tensor, what: str) -> None:
                                "there is no CPU implementation")
 
 
+def extent(t: torch.Tensor, strides) -> tuple[int, int]:
+    """First byte of a tensor of these strides and the one behind its last value."""
+    at, last = t.data_ptr(), 1
+    for n, s in zip(t.shape, strides):
+        if n == 0:
+            return at, at
+        last += (n - 1) * s
+    return at, at + last * t.element_size()
+
+
 def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Whether the bytes from a tensor's first to its last value meet the other's."""
-    def extent(t):
-        at, last = t.data_ptr(), 1
-        for n, s in zip(t.shape, t.stride()):
-            if n == 0:
-                return at, at
-            last += (n - 1) * s
-        return at, at + last * t.element_size()
-
-    (a0, a1), (b0, b1) = extent(a), extent(b)
+    (a0, a1), (b0, b1) = extent(a, a.stride()), extent(b, b.stride())
     return a0 < b1 and b0 < a1
 
 
-def launch(entry, args: bytes, index: int, what: str) -> None:
-    """``entry(args, stream)`` on the current stream of device ``index``, made current for the call."""
+def launch(entry, index: int, what: str, *args) -> None:
+    """``entry(*args, stream)`` on the current stream of device ``index``, made current for the call."""
     stream = torch._C._cuda_getCurrentRawStream(index)
     if torch._C._cuda_getDevice() == index:
-        rc = entry(args, stream)
+        rc = entry(*args, stream)
     else:
         with torch.cuda.device(index):
-            rc = entry(args, stream)
+            rc = entry(*args, stream)
     if rc:
         check(rc, what)
 

@@ -71,7 +71,7 @@ class PagePool:
         args = _RESIZE.pack(self.block_table.data_ptr(), self.held.data_ptr(), self.free.data_ptr(), self.free_count.data_ptr(),
                             self.shortage.data_ptr(), lengths.data_ptr(), self.max_requests, self.max_pages, self.num_pages,
                             self.page_size)
-        _lib.launch(_lib.lib().aspire_page_resize, args, self._index, what)
+        _lib.launch(_lib.lib().aspire_page_resize, self._index, what, args)
         return self.shortage
 
 
@@ -133,7 +133,7 @@ class StepTables:
         args = _TABLES.pack(block_table.data_ptr(), strides[0], cached.data_ptr(), new_tokens.data_ptr(), at, rows, shape[1],
                             self.max_rows, self.max_tokens, self.max_entries, self.page_size, self.tree_words, 0,
                             *[0 if t is None else t.data_ptr() for t in self._outputs])
-        _lib.launch(_lib.lib().aspire_step_tables, args, index, what)
+        _lib.launch(_lib.lib().aspire_step_tables, index, what, args)
         return self
 
 

@@ -52,16 +52,6 @@ def _rows16(t: torch.Tensor):
     return None if any(s % 8 for s in st[:-1]) else st
 
 
-def _bytes(t: torch.Tensor, st) -> tuple[int, int]:
-    """First byte of a tensor of these strides and the one behind its last."""
-    at, last = t.data_ptr(), 1
-    for n, s in zip(t.shape, st):
-        if n == 0:
-            return at, at
-        last += (n - 1) * s
-    return at, at + last * t.element_size()
-
-
 def tree_attention(q: torch.Tensor, kv_cache: torch.Tensor, qo_indptr: torch.Tensor, kv_page_indices: torch.Tensor,
                    kv_page_indptr: torch.Tensor, kv_last_page_len: torch.Tensor, tree_masks: torch.Tensor, page_size: int,
                    *, sm_scale: float | None = None, out: torch.Tensor | None = None, lse: torch.Tensor | None = None,
@@ -110,17 +100,17 @@ def tree_attention(q: torch.Tensor, kv_cache: torch.Tensor, qo_indptr: torch.Ten
     else:
         if tokens > 1 and os[0] == 0 or hq > 1 and os[1] == 0 or not (out.is_contiguous() or _apart(shape, os)):
             raise ValueError(f"{what}: the rows of out share memory")
-        o0, o1 = _bytes(out, os)
+        o0, o1 = _lib.extent(out, os)
         for t, st in ((q, qs), (kv_cache, c)):
-            t0, t1 = _bytes(t, st)
+            t0, t1 = _lib.extent(t, st)
             if o0 < t1 and t0 < o1:
                 raise ValueError(f"{what}: out must lie apart from q and the cache")
     if lse is not None:
         if lse.dtype is not torch.float32 or lse.shape != (tokens, hq) or lse.get_device() != index or not lse.is_contiguous():
             raise ValueError(f"{what}: lse must be a contiguous fp32 [T, H_q] tensor on {q.device}")
-        l0, l1 = _bytes(lse, lse.stride())
+        l0, l1 = _lib.extent(lse, lse.stride())
         for t, st in ((q, qs), (kv_cache, c), (out, os)):
-            t0, t1 = _bytes(t, st)
+            t0, t1 = _lib.extent(t, st)
             if l0 < t1 and t0 < l1:
                 raise ValueError(f"{what}: lse must lie apart from q, the cache and out")
     elif return_lse:
@@ -134,7 +124,7 @@ def tree_attention(q: torch.Tensor, kv_cache: torch.Tensor, qo_indptr: torch.Ten
                       ind.data_ptr(), ptr.data_ptr(), last.data_ptr(), tree_masks.data_ptr(), mst[0], out.data_ptr(), os[0], os[1],
                       0 if lse is None else lse.data_ptr(), tokens, rows, ms[1], hq, cs[3], dim, page_size, code,
                       dim ** -0.5 if sm_scale is None else float(sm_scale), 0, at, floats)
-    _lib.launch(L.aspire_tree_attention, args, index, what)
+    _lib.launch(L.aspire_tree_attention, index, what, args)
     return (out, lse) if return_lse else out
 
 
@@ -190,7 +180,7 @@ def compact_accepted(kv_caches, path: torch.Tensor, kept: torch.Tensor, qo_indpt
     args = _MOVE.pack(0 if table is None else ctypes.addressof(table), c.data_ptr(), step, st[0] * es, st[1] * es, st[2] * es, st[3] * es,
                       cs[0], path.data_ptr(), kept.data_ptr(), qo.data_ptr(), slots.data_ptr(), count, cs[3], cs[4] * es, cs[2], rows,
                       slots.shape[0], most, 0)
-    _lib.launch(_lib.lib().aspire_compact_accepted, args, index, what)
+    _lib.launch(_lib.lib().aspire_compact_accepted, index, what, args)
 
 
 def _apart(shape, strides) -> bool:

@@ -128,16 +128,8 @@ def verify_tree_speculation(tree_tokens: torch.Tensor, parents: torch.Tensor, ta
     output = torch.empty((rows, max_path), dtype=torch.int32, device=device)
     path = torch.empty((rows, max_path), dtype=torch.int32, device=device)
     kept = torch.empty(rows, dtype=torch.int32, device=device)
-    args = (tok.data_ptr(), par.data_ptr(), tgt.data_ptr(), qo.data_ptr(), tokens, rows, max_path, output.data_ptr(),
-            path.data_ptr(), kept.data_ptr())
-    stream, entry = torch._C._cuda_getCurrentRawStream(index), _lib.lib().aspire_verify_tree
-    if torch._C._cuda_getDevice() == index:
-        rc = entry(*args, stream)
-    else:
-        with torch.cuda.device(index):
-            rc = entry(*args, stream)
-    if rc:
-        _lib.check(rc, what)
+    _lib.launch(_lib.lib().aspire_verify_tree, index, what, tok.data_ptr(), par.data_ptr(), tgt.data_ptr(), qo.data_ptr(), tokens, rows,
+                max_path, output.data_ptr(), path.data_ptr(), kept.data_ptr())
     return output, path, kept
 
 

@@ -240,7 +240,7 @@ def adjust_logits(logits: torch.Tensor, *, qo_indptr: torch.Tensor | None = None
                         at(lens), at(told), at(rep), at(pres), at(freq), at(tree), at(tree_masks), mask_stride, at(b[0]), at(b[1]),
                         at(b[2]), at(grammar), grammar_stride, at(which), vocab_start, tokens, vocab, requests, code, history_len,
                         words, grammar_count, 0 if bias is None else bias.ids.shape[0])
-    _lib.launch(_lib.lib().aspire_adjust_logits, args, index, what)
+    _lib.launch(_lib.lib().aspire_adjust_logits, index, what, args)
     return out
 
 
