@@ -65,7 +65,10 @@ def tree_attention(q: torch.Tensor, kv_cache: torch.Tensor, qo_indptr: torch.Ten
     Returns ``out``, with ``return_lse`` and the base-2 ``lse`` fp32 ``[T, H_q]``: new ones, or the tensors given, whose memory from
     first to last value must lie apart from that of q, of the cache and of each other. A token that sees no key gets zeros and
     ``-inf``. Keys that a token does not see do not touch it, whatever they hold. Tokens of no row are left as they were. Sums and
-    softmax are fp32; weights of keys are rounded to q's type for the product with v. Not differentiable."""
+    softmax are fp32; weights of keys, up to 2^8 of the row's largest, are rounded to q's type for the product with v (values of v of
+    2^100 and more may overflow on the way). The launch goes by the mean tokens of a row: rows without tokens are better left out,
+    ``kv_last_page_len[:requests]``, where their number is known (32 requests of 16 tokens over 32,768 take twice as long with 32
+    empty rows behind them). Not differentiable."""
     what = "tree_attention"
     index, dtype, shape, cs = q.get_device(), q.dtype, q.shape, kv_cache.shape
     if index < 0:

@@ -7,7 +7,7 @@
 // meanwhile. (Counts and biases kept in registers over the rows take 121 VGPRs, half the waves, and as long.) A token that the
 // tree drafts is counted on a row's own path where it is met. Chunks of low tokens, which histories and trees meet most, start first.
 // HBM bounds it at batch sizes (logits once in, once out, and an eighth of a byte of mask a token); history is
-// read once a chunk, from L2. Measured: 64 x 151,936 bf16 logits with histories and masks 14 us = 2.9 TB/s, the history's chain (lengths,
+// read once a chunk, from L2. Measured: 64 x 151,936 bf16 logits with histories and masks 15 us = 2.8 TB/s, the history's chain (lengths,
 // tokens, LDS) before the first store; 16 trees of up to 24 tokens over 128,257 with 20,000 tokens of history and 100 biases 46 us = 3.1
 // TB/s, of which counting takes its part and rows whose trees draft tokens of the chunk theirs; one row of 32,000 4.3 us, latency.
 #include <algorithm>
@@ -316,9 +316,10 @@ extern "C" int aspire_adjust_logits(const aspire_adjust_logits_args* a, void* st
   ASPIRE_CHECK_ARG(!a->bias_indptr || a->bias_entries == 0 || (a->bias_ids && a->bias_values), "null biases");
   const bool counts = (a->history || a->tree_masks) && (a->repetition || a->presence || a->frequency);
   const bool bias = a->bias_indptr != nullptr && a->bias_entries > 0;
-  // Chunks of 8,192 tokens, or 4,096 with two tables in LDS (four workgroups a CU either way) or while longer ones leave fewer than two
-  // workgroups a CU; then a request's rows are shared by several, eight rows or more each, up to eight workgroups a CU (a history is
-  // counted once a workgroup: 16 trees of up to 24 tokens, 128,257 logits, took 54 us so, 59 with four rows or more each, in one build).
+  // Chunks of 8,192 tokens, or 4,096 with two tables in LDS (four workgroups a CU either way; three with 8,192 fp16 or fp32 logits, whose
+  // registers leave six waves a SIMD) or while longer ones leave fewer than two workgroups a CU; then a request's rows are shared by
+  // several, eight rows or more each, up to eight workgroups a CU (a history is counted once a workgroup: 16 trees of up to 24 tokens,
+  // 128,257 logits, took 54 us so, 59 with four rows or more each, in one build).
   LogitsLaunch l{counts && bias ? 1 : 2, counts, bias, dim3(), 0, static_cast<hipStream_t>(stream)};
   const auto chunk = [&] { return l.vectors * kVec * kLogitThreads; };
   const auto chunks = [&] { return (int64_t(a->vocab) + chunk() - 1) / chunk(); };

@@ -3,7 +3,7 @@
 // Both kernels are chains of a few memory round trips over some hundred to some hundred thousand bytes, so latency bounds
 // them: rows' counts are read once, prefix sums are taken by wave shuffles and held in LDS, and every page, entry
 // or token then finds its row there by a binary search (LDS reads, no further trip to memory). Measured, 4 / 64 rows of
-// long contexts: the pool 2.6 / 3.2 us, the tables 3.4 / 5.4.
+// long contexts: the pool 2.6 / 3.1 us, the tables 3.5 / 5.7.
 #include <algorithm>
 
 #include "common.h"

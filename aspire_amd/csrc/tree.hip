@@ -96,9 +96,8 @@ __device__ __forceinline__ int64_t wave_uniform64(int64_t v) {
   return int64_t((uint64_t(uint32_t(__builtin_amdgcn_readfirstlane(int(v >> 32)))) << 32) | uint32_t(__builtin_amdgcn_readfirstlane(int(v))));
 }
 
-// 16 bytes a lane from its offset into the buffer to the lane's place behind dst; once: keys that no other workgroup reads
-// (non-temporal: 32 requests of 32,768 keys 737 -> 665 us; the loads alone of tiles that share keys, seven to a request, 164 ->
-// 222).
+// 16 bytes a lane from its offset into the buffer to the lane's place behind dst; once: non-temporal, for keys that are mostly read by
+// one tile (choose has both sides).
 template <bool kOnce>
 __device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t rs, uint4* dst, int offset);
 template <>
@@ -272,6 +271,10 @@ struct TreeWave {
       }
       exponentials();
     }
+    // Weights go into the product with V rounded to V's type, as the matrix instruction takes them (their sum is of the fp32 ones).
+    // An output is off from 64 bits by 0.0020 of the rms of all (bf16, 16 tokens over 2,048 keys; fp16, heads of 64, 0.00029), its own
+    // rounding alone by 0.0017 (0.00021). In two parts, the second of what the first lacks, it is that, but 40 tokens over 8,192 keys take
+    // 113 us in place of 107 and 190 over 12,001 159 in place of 142, and an infinite V times a second part of 0 is NaN.
 #pragma unroll
     for (int t = 0; t < kT; ++t) {
       pf[t] = make_uint4(pack2<kF16>(pv[t][0], pv[t][1]), pack2<kF16>(pv[t][2], pv[t][3]), pack2<kF16>(pv[t][4], pv[t][5]),
@@ -771,6 +774,10 @@ TreeChoice choose(int tokens, int rows, int hq, int hkv) {
   // again for each tile. us with tiles of 16 / 32 / 64 / 128 rows: one request of 16 rows over 2,048 keys 19.1 / 20.3 / 20.1 / 21.5; 32 of
   // 64 over 32,768: 2,555 / 1,290 / 665 / 688; 16 of about 80 over 8,192: 295 / 184 / 131 / 107; 5 of about 480 over 12,001: 673 / 336 /
   // 226 / 143. Up to 32 rows a wave holds them all and goes by itself, one workgroup a CU; with more, two workgroups a CU.
+  // Rows without tokens count in the mean: the call is better made without them (5 of 480 rows with 59 empty ones 296 us in
+  // place of 141, 32 of 64 with 32 empty ones 1,286 in place of 663).
+  // Non-temporal loads where a mean request is one tile, us with / without: 32 of 64 rows over 32,768 keys 665 / 737, 16 of up to 160 (5
+  // of them two tiles) over 8,192 106 / 109; 5 of up to 950 over 12,001 148 / 142, 24 of up to 231 over 5,000, heads of 64, 41.6 / 40.3.
   const int64_t mean = (int64_t(tokens) + rows - 1) / rows * (hq / hkv);
   TreeChoice c{mean <= 16 ? 1 : 2, mean <= 32 ? 1 : mean <= 64 ? 2 : 4, 0, mean <= 128};
   c.groups = std::max(1, (c.row_groups == 1 ? 1 : 2) * kTreeGroups / hkv);
