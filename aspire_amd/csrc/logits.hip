@@ -52,20 +52,20 @@ template <> struct Pack<float> {
 // n values at any 2- or 4-byte aligned place, in one access
 template <typename R, int n> struct __attribute__((packed, aligned(sizeof(R)))) Vec { R v[n]; };
 
-// 1 / r = high + low: fma(x, high, x low) is x / r within half a step and 2^-46, for r from 2^-60 to 2^60 (beyond them, where the
-// parts leave the normal numbers, within a step, as the product with one rounded reciprocal is). high lies towards zero and low has its sign
-// and is not 0, so that infinite x stay so.
-// 16 trees over 128,257 logits, 64 requests over 151,936, us in a graph: one product 51.6 and 19.8, this 51.6 and 20.6, a division for each
-// value 56.6 and 20.4.
-__device__ __forceinline__ void reciprocal(float r, float& high, float& low) {
-  const float m = fabsf(r);
-  if (m >= 0x1p-60f && m <= 0x1p60f) {
-    high = __builtin_amdgcn_rcpf(m);  // within a step: what it lacks is low's
-    if (fmaf(-m, high, 1.f) < 0.f) high = __int_as_float(__float_as_int(high) - 2);
-    low = fmaxf(fmaf(-m, high, 1.f) * high, 0x1p-149f);
-  } else {
-    high = 1.f / m, low = m < __builtin_huge_valf() ? 0x1p-149f : 0.f;
-  }
+// 1 / r = (high + low) scale, scale a power of two: with m = |r| scale, fma(x, high, x low) is x / m within half a step and 2^-46, and times
+// scale x / r (rounded once more where that lies below the normal numbers). m is a normal number: as r is from 2^-60 to 2^60, past that 1 to
+// 2^68 and below 2^-60 to 2^-30, so that x / m only overflows where x / r does, and holds a small x's bits. high lies towards zero; low has
+// its sign and is not 0, so that infinite x stay so.
+// With two vectors a thread its three values leave the registers and each penalised logit is divided. 16 trees over 128,257 logits (one
+// vector) and 64 requests over 151,936 (two), us in a graph: one product by a rounded reciprocal 51.6 and 19.9; the parts 52.4 and 22.0;
+// divisions 56.6 and 20.6.
+__device__ __forceinline__ void reciprocal(float r, float& high, float& low, float& scale) {
+  float m = fabsf(r);
+  scale = m > 0x1p60f ? 0x1p-60f : m >= 0x1p-60f ? 1.f : m >= 0x1p-90f ? 0x1p30f : m >= 0x1p-120f ? 0x1p60f : 0x1p90f;
+  m *= scale;
+  high = __builtin_amdgcn_rcpf(m);  // within a step: what it lacks is low's
+  if (fmaf(-m, high, 1.f) < 0.f) high = __int_as_float(__float_as_int(high) - 2);
+  low = m < __builtin_huge_valf() ? fmaxf(fmaf(-m, high, 1.f) * high, 0x1p-149f) : 0.f;
   high = copysignf(high, r), low = copysignf(low, r);
 }
 
@@ -172,8 +172,8 @@ __global__ __launch_bounds__(kLogitThreads, kJ == 1 || Pack<T>::kLean ? 8 : 6) v
           paths[i] = uint64_t(a.tree_masks[(row0 + i / words) * a.mask_stride + i % words]);
     }
   }
-  float high = 1.f, low = 0.f;
-  if (kCounts) reciprocal(repetition, high, low);
+  float high = 1.f, low = 0.f, scale = 1.f;
+  if (kCounts && kJ == 1) reciprocal(repetition, high, low, scale);
   if (kBias) {
     const int last = min(a.bias_indptr[b + 1], a.bias_entries);
     for (int i = max(a.bias_indptr[b], 0) + threadIdx.x; i < last; i += kLogitThreads) {
@@ -206,8 +206,12 @@ __global__ __launch_bounds__(kLogitThreads, kJ == 1 || Pack<T>::kLean ? 8 : 6) v
   };
   const auto penalty = [&](float f, uint32_t c) {
     const uint32_t written = c & ~kPrompt;
-    const float seen = f > 0.f ? fmaf(f, high, f * low) : f * repetition;
-    f = c != 0 ? seen : f;
+    if constexpr (kJ == 1) {
+      const float seen = f > 0.f ? fmaf(f, high, f * low) * scale : f * repetition;
+      f = c != 0 ? seen : f;
+    } else if (c != 0) {
+      f = f > 0.f ? f / repetition : f * repetition;
+    }
     return written != 0 ? (f - frequency * float(written)) - presence : f;
   };
   for (int row = row0; row < row1; ++row) {

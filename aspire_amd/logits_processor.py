@@ -143,12 +143,11 @@ def adjust_logits(logits: torch.Tensor, *, qo_indptr: torch.Tensor | None = None
     Request ``b`` (of at most 65,535) has the rows ``qo_indptr[b]`` to ``qo_indptr[b + 1]`` (None: row ``b``, as many requests as
     rows); rows of no request are left as they were in ``out``. In this order, in fp32, rounded once:
 
-    * ``x / repetition`` for ``x > 0``, else ``x * repetition``, for every token of the request's prompt or output (penalties are normal
-      numbers; past 2^60 and below 2^-60 the quotient may be off by a step); then ``x - frequency * count - presence * (count > 0)``,
-      ``count`` its occurrences in the output (fp32 ``[B]`` each, None: 1, 0 and 0). ``history`` int32 ``[B, H]`` holds
-      ``history_lens[b]`` tokens, the first ``prompt_lens[b]`` the prompt's (None: none). With ``tree_tokens`` int32 ``[T]`` and
-      ``tree_masks`` int64 ``[T, W]`` (as ``tree_attention`` takes them) the drafted tokens that a row sees, itself among them, are
-      output too: they are then not in the history. Tokens outside the vocabulary do not count;
+    * ``x / repetition`` for ``x > 0``, else ``x * repetition``, for every token of the request's prompt or output; then
+      ``x - frequency * count - presence * (count > 0)``, ``count`` its occurrences in the output (fp32 ``[B]`` each, None: 1, 0
+      and 0). ``history`` int32 ``[B, H]`` holds ``history_lens[b]`` tokens, the first ``prompt_lens[b]`` the prompt's (None: none).
+      With ``tree_tokens`` int32 ``[T]`` and ``tree_masks`` int64 ``[T, W]`` (as ``tree_attention`` takes them) the drafted tokens
+      that a row sees, itself among them, are output too: they are then not in the history. Tokens outside the vocabulary do not count;
     * ``x + bias`` for the request's ``LogitBias`` entries;
     * ``-inf`` where the row's mask does not allow a token: bit ``i % 32`` of word ``i // 32`` of ``grammar`` int32 ``[G, ceil(V / 32)]``,
       row ``grammar_rows[t]`` (int32 ``[T]``; an index outside: no mask) or ``t``.
