@@ -182,6 +182,7 @@ __global__ __launch_bounds__(kLogitThreads, kJ == 1 || Pack<T>::kLean ? 8 : 6) v
     }
   }
   if (kCounts || kBias) __syncthreads();
+
   // the bits of word w of a row's path, and the drafted token of a node
   const auto path_word = [&](int row, int w) {
     const uint64_t bits = listed ? paths[(row - row0) * words + w] : uint64_t(a.tree_masks[row * a.mask_stride + w]);
